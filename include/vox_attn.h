@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define VOX_ABI_VERSION 13
+#define VOX_ABI_VERSION 14
 
 #define VOX_OK 0
 #define VOX_EINVAL 1 /* bad argument: shape, stride, alignment or null pointer (reference: the asserts of
@@ -254,6 +254,90 @@ size_t vox_prefill_int8_workspace_bytes(int64_t num_tokens, int batch, int max_s
  * Bit-exact. Entries that write a block another entry of the same call reads race, as in the reference. */
 int vox_copy_kv_block_prefix(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t per_token,
                              int elem_bytes, const int32_t* entries, int num_entries, int max_tokens, void* stream);
+
+/* ---- KV caches held in 4 bits. No reference counterpart (its caches are bf16): a step's bytes and a pool's size are 0.27
+ * of the bf16 cache's.
+ *
+ * The format is OCP MXFP4: every 32 channels of one token and kv head share a scale, a byte b that stands for
+ * 2^(b - 127) (255: not a number), and a value is one of 0, .5, 1, 1.5, 2, 3, 4, 6 times it, with a sign (codes 0-7, and
+ * 8-15 for the negatives; channel 2i in the low nibble of byte i). A plane is num_blocks blocks of block_size *
+ * num_kv_heads * 68 bytes; in a block the codes [block_size][num_kv_heads][64] come first, then the scales [block_size]
+ * [num_kv_heads][4]. Caches are 16-byte aligned, block_size a multiple of 64, head_dim 128, num_blocks * block_size
+ * below 2^31. */
+
+/* Quantises key / value rows (bf16 [num_tokens, num_kv_heads, head_dim], rows *_row_stride elements apart, heads
+ * contiguous) into their slots; slots outside [0, num_blocks * block_size) (-1: padding) store nothing. Of a group whose
+ * largest magnitude is amax the scale is the least power of two 2^e >= 2^-126 with amax <= 7 * 2^e; a value becomes the
+ * nearest one of the grid, ties to the even code, at most 6 * 2^e. A group that holds an infinity or NaN gets scale 255.
+ * The codes are a function of the row alone. Slots that occur twice in a call hold a mix of their rows. */
+int vox_store_kvcache_fp4(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride,
+                          void* k_cache, void* v_cache, int64_t num_blocks, int block_size, const int32_t* slot_mapping,
+                          int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
+
+/* The values held at slots as bf16 rows: key / value [num_tokens, num_kv_heads, head_dim], contiguous, 16-byte aligned.
+ * Exact; zeros for slots outside the cache. */
+int vox_load_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t num_blocks, int block_size,
+                         const int32_t* slots, int64_t num_tokens, int num_kv_heads, int head_dim, void* key,
+                         void* value, void* stream);
+
+/* vox_decode_attn over 4-bit caches: the attention over the values that the caches hold. Arguments, workspace and plans as
+ * vox_decode_attn's (records may not be shared with calls of other functions). */
+int vox_decode_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                        int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                        int max_blocks, const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
+                        int head_dim, float softmax_scale, int plan, void* workspace, size_t workspace_bytes,
+                        void* out, void* stream);
+
+/* vox_store_kvcache_fp4 of one row a sequence, then vox_decode_attn_fp4: the new tokens are attended over as the cache
+ * holds them. */
+int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                              int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping,
+                              void* k_cache, void* v_cache, int64_t num_blocks, int block_size,
+                              const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                              const int32_t* context_lens, int batch, int num_heads, int num_kv_heads, int head_dim,
+                              float softmax_scale, int plan, void* workspace, size_t workspace_bytes, void* out,
+                              void* stream);
+
+/* vox_prefill_attn over 4-bit caches through block tables, with cu_seqlens. num_tokens: the rows that q and out hold; rows
+ * at or past it are neither read nor written by the prefill kernel. plan, workspace: as vox_prefill_attn's (with the
+ * workspace the one-query sequences run on the decode kernels). num_heads / num_kv_heads divides 128. */
+int vox_prefill_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                         int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                         int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                         int max_seqlen_q, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                         float softmax_scale, int causal, void* out, int64_t out_row_stride, int plan, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ---- The care of a paged cache's blocks, in every plane at once. kv is [num_planes][num_blocks] blocks, one behind the
+ * other; a block is block_size slots of slot_bytes and behind them block_size slots of scale_bytes (a bf16 cache:
+ * num_kv_heads * 256 and 0; a 4-bit cache: num_kv_heads * 64 and num_kv_heads * 4). kv and both runs of a block are
+ * 16-byte aligned. */
+
+/* vox_copy_kv_block_prefix for caches of any slot: entries int32 [num_entries, 3] on the device: (src block, dst block, n),
+ * the first n slots copied. Entries that write a block another entry of the same call reads race. */
+int vox_copy_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                       int64_t scale_bytes, const int32_t* entries, int num_entries, void* stream);
+
+/* Forks sequences. Row p = parents[i] of block_tables (int32 [batch, bt_stride], the first max_blocks columns) with
+ * context_lens[p] tokens gets a child: it shares the parent's full blocks, and where the last block is partly filled its
+ * filled slots are copied to block new_blocks[i], which takes that block's place. child_tables int32 [num_forks,
+ * max_blocks] (-1 past the context), child_lens int32 [num_forks]. new_blocks must be blocks that no table names, no two
+ * the same; one whose parent ends with a full block is left alone. A parent outside [0, batch) gives an empty child; a
+ * last block or new block outside the cache copies nothing and leaves -1 in the child's table. */
+int vox_fork_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                       int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                       const int32_t* context_lens, int batch, const int32_t* parents, const int32_t* new_blocks,
+                       int num_forks, int32_t* child_tables, int32_t* child_lens, void* stream);
+
+/* Moves the live blocks (those that a row of block_tables names within its context) to the front of the cache: with L of
+ * them, those at or past L move to the dead blocks below L, the lowest to the lowest. Blocks shared by several rows move
+ * once. new_tables int32 [batch, max_blocks]: the tables with the new numbers (-1 past the context, entries outside the
+ * cache as they were); remap int32 [num_blocks]: each live block's new number, -1 for the dead; live int32 [1]: L. moves
+ * int32 [2 num_blocks + 1]: scratch. Blocks from L on are free afterwards; num_blocks at most 2^19. */
+int vox_compact_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                          int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                          const int32_t* context_lens, int batch, int32_t* new_tables, int32_t* remap, int32_t* live,
+                          int32_t* moves, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the library: shared HIP runti
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvoxattn.so")
 
 VOX_OK, VOX_EINVAL, VOX_EHIP = 0, 1, 2
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 PLAN_NONE, PLAN_RECORD, PLAN_REUSE = 0, 1, 2
 
@@ -41,6 +41,14 @@ EXPORTS = (
     "vox_prefill_attn_int8_store",
     "vox_prefill_int8_workspace_bytes",
     "vox_copy_kv_block_prefix",
+    "vox_store_kvcache_fp4",
+    "vox_load_kvcache_fp4",
+    "vox_decode_attn_fp4",
+    "vox_decode_attn_store_fp4",
+    "vox_prefill_attn_fp4",
+    "vox_copy_kv_blocks",
+    "vox_fork_kv_blocks",
+    "vox_compact_kv_blocks",
 )
 
 _c_void_p, _i32, _i64, _f32, _size = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -82,6 +90,24 @@ _SIGNATURES = {
                                      _i32, _i32, _f32, _i32, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
                                      _size, _c_void_p]),
     "vox_prefill_int8_workspace_bytes": (_size, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "vox_store_kvcache_fp4": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
+                                     _i64, _i32, _i32, _c_void_p]),
+    "vox_load_kvcache_fp4": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64, _i32, _i32, _c_void_p,
+                                    _c_void_p, _c_void_p]),
+    "vox_decode_attn_fp4": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64, _i32,
+                                   _c_void_p, _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p, _size, _c_void_p,
+                                   _c_void_p]),
+    "vox_decode_attn_store_fp4": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                         _c_void_p, _i64, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32, _i32, _i32,
+                                         _i32, _f32, _i32, _c_void_p, _size, _c_void_p, _c_void_p]),
+    "vox_prefill_attn_fp4": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64, _i32,
+                                    _c_void_p, _c_void_p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _c_void_p,
+                                    _i64, _i32, _c_void_p, _size, _c_void_p]),
+    "vox_copy_kv_blocks": (_i32, [_c_void_p, _i64, _i64, _i32, _i64, _i64, _c_void_p, _i32, _c_void_p]),
+    "vox_fork_kv_blocks": (_i32, [_c_void_p, _i64, _i64, _i32, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _i32,
+                                  _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p]),
+    "vox_compact_kv_blocks": (_i32, [_c_void_p, _i64, _i64, _i32, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _i32,
+                                     _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 

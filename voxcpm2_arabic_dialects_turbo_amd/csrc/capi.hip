@@ -120,7 +120,8 @@ vox::DecodeArgs with_workspace(const vox::DecodeArgs& a, int slice, int plan_mod
 }
 
 int launch_decode_slices(const vox::DecodeArgs& a, int batch, int num_kv_heads, int plan, void* workspace,
-                         hipStream_t stream) {
+                         hipStream_t stream,
+                         hipError_t (*launch)(const vox::DecodeArgs&, int, hipStream_t) = vox::launch_decode) {
   const int slice_max = batch < vox::kMaxSeqPerLaunch ? batch : vox::kMaxSeqPerLaunch;
   const vox::DecodeArgs base =
       with_workspace(a, slice_max, batch <= vox::kMaxSeqPerLaunch ? plan : vox::kPlanNone, workspace);
@@ -141,7 +142,7 @@ int launch_decode_slices(const vox::DecodeArgs& a, int batch, int num_kv_heads, 
         s.new_v = base.new_v + (int64_t)b0 * base.new_v_stride;
       }
     }
-    const int st = hip_status(vox::launch_decode(s, num_kv_heads, stream), "decode launch");
+    const int st = hip_status(launch(s, num_kv_heads, stream), "decode launch");
     if (st != VOX_OK) return st;
   }
   return VOX_OK;
@@ -789,6 +790,226 @@ int vox_copy_kv_block_prefix(void* kv, int64_t num_planes, int64_t num_blocks, i
   const bool vec16 = per_token % 8 == 0 && aligned16(kv);
   return hip_status(vox::launch_copy_block_prefix(a, max_tokens, vec16, (hipStream_t)stream),
                     "copy_kv_block_prefix launch");
+}
+
+}  // extern "C"
+
+// ---- 4-bit caches and the care of a cache's blocks
+
+namespace {
+// What every call over 4-bit caches needs of them.
+int fp4_cache(const char* fn, const void* k_cache, const void* v_cache, int64_t num_blocks, int block_size,
+              int num_kv_heads, int head_dim) {
+  if (!k_cache || !v_cache) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (head_dim != kHeadDim) return fail(VOX_EINVAL, "%s: head_dim %d unsupported (128 only)", fn, head_dim);
+  if (num_kv_heads <= 0 || num_kv_heads > 128) return fail(VOX_EINVAL, "%s: num_kv_heads %d", fn, num_kv_heads);
+  if (block_size <= 0 || block_size % 64)
+    return fail(VOX_EINVAL, "%s: block_size %d must be a positive multiple of 64", fn, block_size);
+  if (num_blocks <= 0) return fail(VOX_EINVAL, "%s: empty cache", fn);
+  // a block's byte offsets are 32-bit, its slots int32
+  if ((int64_t)block_size * num_kv_heads * 68 > (1 << 30) || num_blocks > INT32_MAX / block_size)
+    return fail(VOX_EINVAL, "%s: %lld blocks of %d slots are more than int32 slots reach", fn, (long long)num_blocks,
+                block_size);
+  if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(VOX_EINVAL, "%s: caches must be 16-byte aligned", fn);
+  return VOX_OK;
+}
+
+// A cache's planes as bytes; `what` is the name of the call.
+int pages_setup(const char* fn, void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                int64_t scale_bytes, vox::PagesArgs* out) {
+  if (!kv) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (num_planes <= 0 || num_planes > 65535) return fail(VOX_EINVAL, "%s: %lld planes", fn, (long long)num_planes);
+  if (num_blocks <= 0 || block_size <= 0 || slot_bytes <= 0 || scale_bytes < 0)
+    return fail(VOX_EINVAL, "%s: bad cache shape", fn);
+  if (num_blocks > INT32_MAX / block_size || slot_bytes > (1 << 20) || scale_bytes > (1 << 20) ||
+      (int64_t)block_size * (slot_bytes + scale_bytes) > (1 << 29))
+    return fail(VOX_EINVAL, "%s: cache shape out of range", fn);
+  if (!aligned16(kv) || (int64_t)block_size * slot_bytes % 16 || (int64_t)block_size * scale_bytes % 16)
+    return fail(VOX_EINVAL, "%s: the cache and the runs of a block must be 16-byte aligned", fn);
+  out->kv = (uint8_t*)kv;
+  out->num_planes = num_planes;
+  out->num_blocks = num_blocks;
+  out->block_size = block_size;
+  out->slot_bytes = slot_bytes;
+  out->scale_bytes = scale_bytes;
+  return VOX_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int vox_store_kvcache_fp4(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride,
+                          void* k_cache, void* v_cache, int64_t num_blocks, int block_size, const int32_t* slot_mapping,
+                          int64_t num_tokens, int num_kv_heads, int head_dim, void* stream) {
+  const char* fn = "store_kvcache_fp4";
+  if (num_tokens < 0) return fail(VOX_EINVAL, "%s: num_tokens %lld < 0", fn, (long long)num_tokens);
+  if (num_tokens == 0) return VOX_OK;
+  if (!key || !value || !slot_mapping) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  const int st = fp4_cache(fn, k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st != VOX_OK) return st;
+  const int64_t row = (int64_t)num_kv_heads * head_dim;
+  if (key_row_stride < row || value_row_stride < row)
+    return fail(VOX_EINVAL, "%s: row stride smaller than num_kv_heads * head_dim", fn);
+  const vox::Fp4RowsArgs a{(const uint16_t*)key, (const uint16_t*)value, key_row_stride, value_row_stride,
+                           (uint8_t*)k_cache, (uint8_t*)v_cache, num_blocks * block_size, block_size, num_kv_heads,
+                           slot_mapping, num_tokens};
+  const bool vec16 = key_row_stride % 8 == 0 && value_row_stride % 8 == 0 && aligned16(key) && aligned16(value);
+  return hip_status(vox::launch_store_fp4(a, vec16, (hipStream_t)stream), "store_kvcache_fp4 launch");
+}
+
+int vox_load_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t num_blocks, int block_size,
+                         const int32_t* slots, int64_t num_tokens, int num_kv_heads, int head_dim, void* key,
+                         void* value, void* stream) {
+  const char* fn = "load_kvcache_fp4";
+  if (num_tokens < 0) return fail(VOX_EINVAL, "%s: num_tokens %lld < 0", fn, (long long)num_tokens);
+  if (num_tokens == 0) return VOX_OK;
+  if (!key || !value || !slots) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  const int st = fp4_cache(fn, k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st != VOX_OK) return st;
+  if (!aligned16(key) || !aligned16(value)) return fail(VOX_EINVAL, "%s: key and value must be 16-byte aligned", fn);
+  const int64_t row = (int64_t)num_kv_heads * head_dim;
+  const vox::Fp4RowsArgs a{(const uint16_t*)key, (const uint16_t*)value, row, row, (uint8_t*)k_cache,
+                           (uint8_t*)v_cache, num_blocks * block_size, block_size, num_kv_heads, slots, num_tokens};
+  return hip_status(vox::launch_load_fp4(a, (hipStream_t)stream), "load_kvcache_fp4 launch");
+}
+
+int vox_decode_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                        int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                        int max_blocks, const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
+                        int head_dim, float softmax_scale, int plan, void* workspace, size_t workspace_bytes,
+                        void* out, void* stream) {
+  if (batch < 0) return fail(VOX_EINVAL, "decode_attn_fp4: batch < 0");
+  if (plan != VOX_PLAN_NONE && plan != VOX_PLAN_RECORD && plan != VOX_PLAN_REUSE)
+    return fail(VOX_EINVAL, "decode_attn_fp4: plan mode %d", plan);
+  if (batch == 0) return VOX_OK;
+  int st = fp4_cache("decode_attn_fp4", k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st != VOX_OK) return st;
+  vox::DecodeArgs a;
+  st = decode_setup(q, q_row_stride, k_cache, v_cache, num_blocks, block_size, block_tables, bt_stride, max_blocks,
+                    context_lens, batch, num_heads, num_kv_heads, head_dim, softmax_scale, workspace, workspace_bytes,
+                    out, &a);
+  if (st != VOX_OK) return st;
+  return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream, vox::launch_decode_fp4);
+}
+
+int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                              int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping,
+                              void* k_cache, void* v_cache, int64_t num_blocks, int block_size,
+                              const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                              const int32_t* context_lens, int batch, int num_heads, int num_kv_heads, int head_dim,
+                              float softmax_scale, int plan, void* workspace, size_t workspace_bytes, void* out,
+                              void* stream) {
+  if (batch < 0) return fail(VOX_EINVAL, "decode_attn_store_fp4: batch < 0");
+  if (plan != VOX_PLAN_NONE && plan != VOX_PLAN_RECORD && plan != VOX_PLAN_REUSE)
+    return fail(VOX_EINVAL, "decode_attn_store_fp4: plan mode %d", plan);
+  if (batch == 0) return VOX_OK;
+  if (!key || !value || !slot_mapping)
+    return fail(VOX_EINVAL, "decode_attn_store_fp4: null key, value or slot_mapping");
+  int st = fp4_cache("decode_attn_store_fp4", k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st != VOX_OK) return st;
+  const int64_t row = (int64_t)num_kv_heads * head_dim;
+  if (key_row_stride < row || value_row_stride < row)
+    return fail(VOX_EINVAL, "decode_attn_store_fp4: row stride smaller than num_kv_heads * head_dim");
+  // every argument is checked before anything is launched
+  vox::DecodeArgs a;
+  st = decode_setup(q, q_row_stride, k_cache, v_cache, num_blocks, block_size, block_tables, bt_stride, max_blocks,
+                    context_lens, batch, num_heads, num_kv_heads, head_dim, softmax_scale, workspace, workspace_bytes,
+                    out, &a);
+  if (st != VOX_OK) return st;
+  st = vox_store_kvcache_fp4(key, value, key_row_stride, value_row_stride, k_cache, v_cache, num_blocks, block_size,
+                             slot_mapping, batch, num_kv_heads, head_dim, stream);
+  if (st != VOX_OK) return st;
+  return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream, vox::launch_decode_fp4);
+}
+
+int vox_prefill_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                         int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                         int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                         int max_seqlen_q, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                         float softmax_scale, int causal, void* out, int64_t out_row_stride, int plan, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  const char* fn = "prefill_attn_fp4";
+  if (batch < 0 || max_seqlen_q < 0 || num_tokens < 0)
+    return fail(VOX_EINVAL, "%s: negative batch, max_seqlen_q or num_tokens", fn);
+  if (batch == 0 || max_seqlen_q == 0 || num_tokens == 0) return VOX_OK;
+  if (!block_tables || !cu_seqlens_q || !cu_seqlens_k || !out)
+    return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  int st = fp4_cache(fn, k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st != VOX_OK) return st;
+  if (out_row_stride < (int64_t)num_heads * head_dim || out_row_stride % 4 || ((uintptr_t)out & 7u))
+    return fail(VOX_EINVAL, "%s: bad out row stride or alignment", fn);
+  if (batch > 65535) return fail(VOX_EINVAL, "%s: more than 65535 sequences", fn);
+  if ((int64_t)max_blocks * block_size > (1 << 30)) return fail(VOX_EINVAL, "%s: block table too wide", fn);
+  vox::PrefillArgs a;
+  st = prefill_setup(fn, q, q_row_stride, nullptr, nullptr, 0, 0, k_cache, v_cache, num_blocks, block_size,
+                     block_tables, bt_stride, max_blocks, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, 0, 0,
+                     num_heads, num_kv_heads, head_dim, softmax_scale, causal, &a);
+  if (st != VOX_OK) return st;
+  a.out = (uint16_t*)out;
+  a.out_row_stride = out_row_stride;
+  a.row_limit = num_tokens;
+  const hipStream_t s = (hipStream_t)stream;
+  if (!varlen_decode_rows(a, workspace, num_kv_heads))
+    return hip_status(vox::launch_prefill_fp4(a, max_seqlen_q, s), "prefill_attn_fp4 launch");
+  // the one-query rows on the decode kernels, which spread a long context over every CU
+  st = check_varlen_workspace(fn, batch, plan, workspace, workspace_bytes);
+  if (st != VOX_OK) return st;
+  if (max_seqlen_q > 1) {
+    a.skip_single = 1;
+    st = hip_status(vox::launch_prefill_fp4(a, max_seqlen_q, s), "prefill_attn_fp4 launch");
+    if (st != VOX_OK) return st;
+  }
+  const vox::DecodeArgs d = varlen_decode_args(a, q_row_stride, num_blocks, num_heads, num_kv_heads);
+  return launch_decode_slices(d, batch, num_kv_heads, plan, workspace, s, vox::launch_decode_fp4);
+}
+
+int vox_copy_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                       int64_t scale_bytes, const int32_t* entries, int num_entries, void* stream) {
+  if (num_entries < 0) return fail(VOX_EINVAL, "copy_kv_blocks: negative count");
+  if (num_entries == 0) return VOX_OK;
+  if (!entries) return fail(VOX_EINVAL, "copy_kv_blocks: null pointer argument");
+  vox::PagesArgs a;
+  const int st = pages_setup("copy_kv_blocks", kv, num_planes, num_blocks, block_size, slot_bytes, scale_bytes, &a);
+  if (st != VOX_OK) return st;
+  return hip_status(vox::launch_copy_entries(a, entries, num_entries, (hipStream_t)stream), "copy_kv_blocks launch");
+}
+
+int vox_fork_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                       int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                       const int32_t* context_lens, int batch, const int32_t* parents, const int32_t* new_blocks,
+                       int num_forks, int32_t* child_tables, int32_t* child_lens, void* stream) {
+  const char* fn = "fork_kv_blocks";
+  if (num_forks < 0 || batch < 0) return fail(VOX_EINVAL, "%s: negative count", fn);
+  if (num_forks == 0) return VOX_OK;
+  if (!block_tables || !context_lens || !parents || !new_blocks || !child_tables || !child_lens)
+    return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (max_blocks <= 0 || bt_stride < max_blocks || (int64_t)max_blocks * block_size > (1 << 30))
+    return fail(VOX_EINVAL, "%s: bad block table shape", fn);
+  vox::PagesArgs a;
+  const int st = pages_setup(fn, kv, num_planes, num_blocks, block_size, slot_bytes, scale_bytes, &a);
+  if (st != VOX_OK) return st;
+  const vox::ForkArgs f{block_tables, bt_stride, max_blocks, context_lens, batch, parents, new_blocks, num_forks,
+                        child_tables, child_lens};
+  return hip_status(vox::launch_fork(a, f, (hipStream_t)stream), "fork_kv_blocks launch");
+}
+
+int vox_compact_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
+                          int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                          const int32_t* context_lens, int batch, int32_t* new_tables, int32_t* remap, int32_t* live,
+                          int32_t* moves, void* stream) {
+  const char* fn = "compact_kv_blocks";
+  if (batch < 0) return fail(VOX_EINVAL, "%s: batch < 0", fn);
+  if (!remap || !live || !moves || (batch > 0 && (!block_tables || !context_lens || !new_tables)))
+    return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (batch > 0 && (max_blocks <= 0 || bt_stride < max_blocks || (int64_t)max_blocks * block_size > (1 << 30)))
+    return fail(VOX_EINVAL, "%s: bad block table shape", fn);
+  vox::PagesArgs a;
+  const int st = pages_setup(fn, kv, num_planes, num_blocks, block_size, slot_bytes, scale_bytes, &a);
+  if (st != VOX_OK) return st;
+  if (num_blocks > (1 << 19))  // its bitmap of the blocks lives in 64 KiB of LDS
+    return fail(VOX_EINVAL, "%s: %lld blocks, %d at most", fn, (long long)num_blocks, 1 << 19);
+  const vox::CompactArgs c{block_tables, bt_stride, max_blocks > 0 ? max_blocks : 1, context_lens, batch, new_tables, remap, live, moves};
+  return hip_status(vox::launch_compact(a, c, (hipStream_t)stream), "compact_kv_blocks launch");
 }
 
 }  // extern "C"

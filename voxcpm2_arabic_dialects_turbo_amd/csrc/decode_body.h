@@ -185,6 +185,7 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // (147 KB, one workgroup per CU). The accessors fold to fixed LDS addresses once inlined.
 template <int HK, bool BTL>
 struct LdsOwn {
+  static constexpr bool kOwnWalk = false;
   static constexpr int kRoundSegs = 8;
   static constexpr int kSlots = kRoundSegs + kWaves - 1;
   static constexpr bool kBtl = BTL;
@@ -220,6 +221,7 @@ struct LdsOwn {
 // partials that leave the workgroup stay fp32), the block table read from memory, at most kSeqCap sequences.
 template <int HK>
 struct LdsBorrowed {
+  static constexpr bool kOwnWalk = false;
   static constexpr int kRoundSegs = 3;
   static constexpr int kSlots = kRoundSegs + kWaves - 1;
   static constexpr bool kBtl = false;
@@ -561,7 +563,21 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     const int R = re - rr;
     auto share_lo = [&](int ww) { return rr + (int)(((int64_t)R * ww) / kWaves); };
     const int t_lo = share_lo(w), t_hi = share_lo(w + 1);
-    if (t_lo < t_hi) {
+    if constexpr (LDS::kOwnWalk) {  // another cache format: the policy walks the share (decode_fp4.h)
+      if (t_lo < t_hi) {
+        struct Window {
+          int vst, ven, vctx, vrow;
+          __device__ __forceinline__ int st(int k) const { return __builtin_amdgcn_readlane(vst, k); }
+          __device__ __forceinline__ int en(int k) const { return __builtin_amdgcn_readlane(ven, k); }
+          __device__ __forceinline__ int ctx(int k) const { return __builtin_amdgcn_readlane(vctx, k); }
+          __device__ __forceinline__ int row(int k) const { return __builtin_amdgcn_readlane(vrow, k); }
+        };
+        const uint64_t hold = __builtin_amdgcn_ballot_w64(((segs >> lane) & 1ull) && w_st <= t_lo && t_lo < w_en);
+        const int k0 = __builtin_ctzll(hold);
+        L.walk(p, w, t_lo, t_hi, k0, __builtin_popcountll(segs & ((1ull << k0) - 1ull)), block_of, next_seg,
+               Window{w_st, w_en, w_ctx, w_row});
+      }
+    } else if (t_lo < t_hi) {
       // this wave's first tile: window lane kcur, round segment kc
       const uint64_t hold = __builtin_amdgcn_ballot_w64(((segs >> lane) & 1ull) && w_st <= t_lo && t_lo < w_en);
       int kcur = __builtin_ctzll(hold);

@@ -65,12 +65,20 @@ struct Entry<R (*)(A...)> {
   X(vox_decode_attn)                \
   X(vox_decode_attn_store)          \
   X(vox_decode_workgroups)          \
+  X(vox_decode_workspace_bytes)     \
   X(vox_prefill_attn)               \
   X(vox_prefill_attn_store)         \
   X(vox_prefill_attn_store_paged)   \
   X(vox_prefill_attn_int8)          \
   X(vox_prefill_attn_int8_store)    \
-  X(vox_prefill_int8_workspace_bytes)
+  X(vox_prefill_int8_workspace_bytes) \
+  X(vox_store_kvcache_fp4)          \
+  X(vox_load_kvcache_fp4)           \
+  X(vox_decode_attn_fp4)            \
+  X(vox_decode_attn_store_fp4)      \
+  X(vox_prefill_attn_fp4)           \
+  X(vox_fork_kv_blocks)             \
+  X(vox_compact_kv_blocks)
 
 #define VOX_DEFINE(name)                                                              \
   decltype(&name) g_##name = nullptr;                                                 \

@@ -121,6 +121,21 @@ struct PrefillArgs {
   int new_from_rows;
 };
 
+// Rows of a 4-bit cache (fp4_common.h has the format): quantised into their slots, or read back.
+struct Fp4RowsArgs {
+  const uint16_t* key;        // bf16 [num_tokens, HK, 128]; store: token rows *_row_stride apart, load: written, contiguous
+  const uint16_t* value;
+  int64_t key_row_stride;
+  int64_t value_row_stride;
+  uint8_t* k_cache;           // [num_blocks][block_size * HK * 68]
+  uint8_t* v_cache;
+  int64_t num_slots;          // num_blocks * block_size
+  int block_size;
+  int num_kv_heads;
+  const int32_t* slots;       // int32 [num_tokens]
+  int64_t num_tokens;
+};
+
 struct CopyArgs {
   void* kv;                   // [num_planes][num_blocks][block_size][per_token] elements, contiguous
   int64_t num_planes;         // layers x 2 (K, V)
@@ -131,15 +146,63 @@ struct CopyArgs {
   int num_entries;
 };
 
+// A paged cache's blocks as bytes (kv_pages.hip): kv[num_planes][num_blocks][block_size * (slot_bytes + scale_bytes)],
+// 16-byte aligned, as are a block and its first block_size * slot_bytes bytes.
+struct PagesArgs {
+  uint8_t* kv;
+  int64_t num_planes;
+  int64_t num_blocks;
+  int block_size;
+  int64_t slot_bytes;
+  int64_t scale_bytes;        // 0: slots only
+};
+
+struct ForkArgs {
+  const int32_t* block_tables;  // int32 [batch, bt_stride], first max_blocks columns used
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* context_lens;  // int32 [batch]
+  int batch;
+  const int32_t* parents;       // int32 [num_forks]: rows of block_tables
+  const int32_t* new_blocks;    // int32 [num_forks]
+  int num_forks;
+  int32_t* child_tables;        // int32 [num_forks, max_blocks]
+  int32_t* child_lens;          // int32 [num_forks]
+};
+
+struct CompactArgs {
+  const int32_t* block_tables;  // int32 [batch, bt_stride], first max_blocks columns used
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* context_lens;  // int32 [batch]
+  int batch;
+  int32_t* new_tables;          // int32 [batch, max_blocks]
+  int32_t* remap;               // int32 [num_blocks]
+  int32_t* live;                // int32 [1]
+  int32_t* moves;               // int32 [2 num_blocks + 1]: scratch
+};
+
+hipError_t launch_copy_entries(const PagesArgs& a, const int32_t* entries, int num_entries, hipStream_t stream);
+hipError_t launch_fork(const PagesArgs& a, const ForkArgs& f, hipStream_t stream);
+hipError_t launch_compact(const PagesArgs& a, const CompactArgs& c, hipStream_t stream);
+
 hipError_t launch_store_kvcache(const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
                                 void* k_cache, void* v_cache, int64_t num_slots, const int32_t* slot_mapping,
                                 int64_t n, int row_elems, bool vec16, hipStream_t stream);
 
+hipError_t launch_store_fp4(const Fp4RowsArgs& a, bool vec16, hipStream_t stream);
+hipError_t launch_load_fp4(const Fp4RowsArgs& a, hipStream_t stream);
+
 hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
+// The same over 4-bit caches (k_cache / v_cache are their bytes; no store mode).
+hipError_t launch_decode_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
 // The merge kernel alone (after a mixed launch whose decode workgroups left partials).
 hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t stream);
 
 hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
+
+// Varlen attention over 4-bit caches (paged keys, cu_seqlens; row_limit is the rows that q and out hold).
+hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 
 // A mixed prefill + decode step as one launch: the one-query rows on decode workgroups (d, its workspace set up),
 // the other rows on persistent prefill workgroups (a, persistent with skip_single) sharing the CUs, then the merge

@@ -13,6 +13,10 @@
 - causal decode: paged split-KV decode over ``context_lens`` / ``block_tables``; returns [B, 1, H, D];
 - non-causal: dense attention over [B, L, H, D] (LocEnc / LocDiT rows).
 
+Caches held in 4 bits (uint8 planes, see ops_fp4) take the same branches: the step's rows are quantised into them first, and
+decode steps and prefills through block tables attend over what the caches then hold (a prefill without block tables over
+the step's own rows).
+
 Every branch runs a HIP kernel of libvoxattn.so; nothing here synchronizes or allocates outside torch, so the
 module can be captured into HIP graphs exactly where the reference captures its decode step.
 """
@@ -28,6 +32,7 @@ from torch import nn
 from .context import get_context
 from .ops import (decode_attention, flash_attn_func, flash_attn_varlen_func, flash_attn_with_kvcache, planning,
                   prefill_attention_store, store_kvcache)
+from .ops_fp4 import decode_attention_fp4, is_fp4_cache
 
 __all__ = ["Attention", "store_kvcache"]
 
@@ -115,14 +120,19 @@ class Attention(nn.Module):
             context = get_context()
             k_cache, v_cache = self.k_cache, self.v_cache
             cached = bool(k_cache.numel() and v_cache.numel())
-            if cached and not context.is_prefill and _store_rides_in_decode(q, k, v, context.slot_mapping):
+            fp4 = cached and is_fp4_cache(k_cache)
+            if fp4 and not context.is_prefill and context.slot_mapping is not None and k.dim() == 3:
+                return decode_attention_fp4(q, k_cache, v_cache, context.context_lens, context.block_tables, self.scale,
+                                            key=k, value=v, slot_mapping=context.slot_mapping,
+                                            plan=_plan_key(context)).unsqueeze(1)
+            if cached and not fp4 and not context.is_prefill and _store_rides_in_decode(q, k, v, context.slot_mapping):
                 # decode step: the store rides in the decode call (one row per sequence, each writing the slot of
                 # its own newest token)
                 _check_riding_store(context, k_cache.shape[1], decode=True)
                 return decode_attention(q, k_cache, v_cache, context.context_lens, context.block_tables, self.scale,
                                         key=k, value=v, slot_mapping=context.slot_mapping,
                                         plan=_plan_key(context)).unsqueeze(1)
-            if cached and context.is_prefill and context.cu_seqlens_q is not None \
+            if cached and not fp4 and context.is_prefill and context.cu_seqlens_q is not None \
                     and _store_rides_in_prefill(k, v, context.slot_mapping):
                 # prefill: the store rides in the attention call. Over the step's own rows (no block table) the
                 # launch reads the packed rows; through the block tables (prefix cache, mixed steps) the launch reads

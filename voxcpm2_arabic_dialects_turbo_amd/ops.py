@@ -64,7 +64,12 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
                   slot_mapping: torch.Tensor) -> None:
     """Writes key[i] / value[i] ([N, HK, head_dim], token rows may be strided) to the cache slot slot_mapping[i];
     slot -1 is skipped. Caches are [num_blocks, block_size, HK, head_dim] (or any view whose slot rows are
-    HK * head_dim apart). Bit-exact. Reference: nanovllm_voxcpm/model/layers.py:290-305 (same asserts)."""
+    HK * head_dim apart). Bit-exact. Reference: nanovllm_voxcpm/model/layers.py:290-305 (same asserts). 4-bit caches
+    (ops_fp4) take the rows quantised."""
+    if k_cache.dtype == torch.uint8:
+        from .ops_fp4 import store_kvcache_fp4
+
+        return store_kvcache_fp4(key, value, k_cache, v_cache, slot_mapping)
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     _require(key.stride(-1) == 1 and value.stride(-1) == 1, "key/value: last dim must be contiguous")
@@ -474,10 +479,16 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
                            deterministic=False, return_attn_probs=False, block_table=None):
     """q [T, H, D]; k / v packed [Tk, HK, D], or the paged caches [num_blocks, block_size, HK, D] with
     block_table [B, max_blocks]. Returns o [T, H, D]. The kernel is deterministic whatever ``deterministic`` says.
-    (Reference call: nanovllm_voxcpm/model/layers.py:337-348.)"""
+    (Reference call: nanovllm_voxcpm/model/layers.py:337-348.) The paged caches may be 4-bit ones (ops_fp4)."""
     _unsupported("flash_attn_varlen_func", dropout_p=dropout_p, window_size=window_size, softcap=softcap,
                  alibi_slopes=alibi_slopes, return_attn_probs=return_attn_probs)
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    if block_table is not None and k.dtype == torch.uint8:
+        from .ops_fp4 import varlen_attention_fp4
+
+        return varlen_attention_fp4(q, k, v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
+                                    max_seqlen_q=max_seqlen_q, block_table=block_table, softmax_scale=scale,
+                                    causal=causal)
     if block_table is not None:
         return varlen_attention(q, None, None, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
                                 max_seqlen_q=max_seqlen_q, softmax_scale=scale, causal=causal,
@@ -493,7 +504,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     """q [B, Lq, H, D] over the paged caches; cache_seqlens (int32 [B], or one int for every sequence) counts every
     key; returns o [B, Lq, H, D]. Lq == 1 (the engine's decode) runs the split-KV decode kernel, which picks its
     own split (``num_splits`` is not used); Lq > 1 runs the varlen kernel with bottom-right causal alignment.
-    (Reference call: nanovllm_voxcpm/model/layers.py:350-358.)"""
+    (Reference call: nanovllm_voxcpm/model/layers.py:350-358.) The caches may be 4-bit ones (ops_fp4)."""
     _unsupported("flash_attn_with_kvcache", k=k, v=v, rotary_cos=rotary_cos, rotary_sin=rotary_sin,
                  cache_batch_idx=cache_batch_idx, cache_leftpad=cache_leftpad, window_size=window_size,
                  softcap=softcap, alibi_slopes=alibi_slopes, return_softmax_lse=return_softmax_lse)
@@ -503,6 +514,11 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     if isinstance(cache_seqlens, int):
         cache_seqlens = torch.full((B,), cache_seqlens, dtype=torch.int32, device=q.device)
     scale = D ** -0.5 if softmax_scale is None else softmax_scale
+    fp4 = k_cache.dtype == torch.uint8
+    if Lq == 1 and fp4:
+        from .ops_fp4 import decode_attention_fp4
+
+        return decode_attention_fp4(q[:, 0], k_cache, v_cache, cache_seqlens, block_table, scale).unsqueeze(1)
     if Lq == 1:
         return decode_attention(q[:, 0], k_cache, v_cache, cache_seqlens, block_table, scale).unsqueeze(1)
     lens = _as_i32(cache_seqlens.reshape(-1), "cache_seqlens")
@@ -510,6 +526,11 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     cu_k = torch.zeros(B + 1, dtype=torch.int32, device=q.device)
     torch.cumsum(lens, 0, out=cu_k[1:])
     q3 = q.reshape(B * Lq, H, D)
+    if fp4:
+        from .ops_fp4 import varlen_attention_fp4
+
+        return varlen_attention_fp4(q3, k_cache, v_cache, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=Lq,
+                                    block_table=block_table, softmax_scale=scale, causal=causal).view(B, Lq, H, D)
     o = varlen_attention(q3, None, None, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=Lq,
                          softmax_scale=scale, causal=causal, block_table=block_table, k_cache=k_cache,
                          v_cache=v_cache)

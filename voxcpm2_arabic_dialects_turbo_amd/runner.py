@@ -36,6 +36,8 @@ import torch
 
 from .context import get_context, set_context
 from .layers import Attention
+from .ops import HEAD_DIM
+from .ops_fp4 import ROW_BYTES
 
 
 @dataclass
@@ -273,9 +275,23 @@ def causal_attention_modules(model: torch.nn.Module) -> list[Attention]:
 
 
 def kv_cache_block_bytes(modules: Iterable[Attention], block_size: int, dtype=torch.bfloat16) -> int:
-    """Bytes one cache block takes across every causal layer, K and V (reference: model_runner.py:680-686)."""
-    itemsize = torch.empty(0, dtype=dtype).element_size()
-    return sum(2 * block_size * m.num_kv_heads * m.head_dim * itemsize for m in modules)
+    """Bytes one cache block takes across every causal layer, K and V (reference: model_runner.py:680-686).
+    ``dtype`` as allocate_kv_cache's."""
+    return sum(2 * block_size * m.num_kv_heads * _head_width(m.head_dim, dtype) * _held_as(dtype).itemsize
+               for m in modules)
+
+
+def _held_as(dtype: torch.dtype) -> torch.dtype:
+    return torch.uint8 if dtype == torch.float4_e2m1fn_x2 else dtype
+
+
+def _head_width(head_dim: int, dtype: torch.dtype) -> int:
+    """Elements of a token's head in the cache: head_dim, or a 4-bit head's bytes."""
+    if dtype != torch.float4_e2m1fn_x2:
+        return head_dim
+    if head_dim != HEAD_DIM:
+        raise ValueError(f"4-bit caches take head_dim {HEAD_DIM}, got {head_dim}")
+    return ROW_BYTES
 
 
 def allocate_kv_cache(model_or_modules, num_blocks: int, block_size: int, dtype=torch.bfloat16, device="cuda"
@@ -283,7 +299,9 @@ def allocate_kv_cache(model_or_modules, num_blocks: int, block_size: int, dtype=
     """Allocates the KV cache and assigns every causal Attention its per-layer views. One
     [layers, 2, num_blocks, block_size, HK, head_dim] tensor when all layers share a head shape (a block's KV across
     all layers is then reachable from one base pointer), else one pair of tensors per layer
-    (reference: nanovllm_voxcpm/engine/model_runner.py:726-751)."""
+    (reference: nanovllm_voxcpm/engine/model_runner.py:726-751).
+
+    ``dtype`` torch.float4_e2m1fn_x2 makes 4-bit caches (ops_fp4): uint8, with 68 in the place of head_dim."""
     if num_blocks <= 0:
         raise ValueError("num_blocks must be positive")
     if block_size % 256:
@@ -293,13 +311,15 @@ def allocate_kv_cache(model_or_modules, num_blocks: int, block_size: int, dtype=
     shapes = {(m.num_kv_heads, m.head_dim) for m in modules}
     if len(shapes) == 1:
         heads, dim = shapes.pop()
-        kv = torch.empty(len(modules), 2, num_blocks, block_size, heads, dim, dtype=dtype, device=device)
+        kv = torch.empty(len(modules), 2, num_blocks, block_size, heads, _head_width(dim, dtype), dtype=_held_as(dtype),
+                         device=device)
         for i, m in enumerate(modules):
             m.k_cache, m.v_cache = kv[i, 0], kv[i, 1]
         return kv
     for m in modules:
-        m.k_cache = torch.empty(num_blocks, block_size, m.num_kv_heads, m.head_dim, dtype=dtype, device=device)
-        m.v_cache = torch.empty(num_blocks, block_size, m.num_kv_heads, m.head_dim, dtype=dtype, device=device)
+        shape = (num_blocks, block_size, m.num_kv_heads, _head_width(m.head_dim, dtype))
+        m.k_cache = torch.empty(shape, dtype=_held_as(dtype), device=device)
+        m.v_cache = torch.empty(shape, dtype=_held_as(dtype), device=device)
     return None
 
 
