@@ -40,7 +40,7 @@ struct TileRegs {
 
 __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kBK * kVRow];
-  __shared__ uint8_t s_nan[2][kBK * 4];  // a tile's groups whose scale is not a number: [key][32-channel group]
+  __shared__ __attribute__((aligned(4))) uint8_t s_nan[2][kBK * 4];  // a tile's groups whose scale is not a number: [key][32-channel group]
   __shared__ int s_nan_at[2];            // the first key of the last tile that held any
   const int b = blockIdx.y, g = blockIdx.z;
   const int q0 = p.cu_q[b], nq = p.cu_q[b + 1] - q0;
@@ -71,9 +71,11 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   uint32_t qs;
   {
     u32x4 qv[8];
-    const uint16_t* qb = p.q + row * p.q_row_stride + (int64_t)head * kD + h * 16;
+    // (a row that is none reads the nearest one that q holds: its loads need no branches, its output is not written)
+    const int64_t qrow = max((int64_t)0, min(row, p.row_limit - 1));
+    const uint16_t* qb = p.q + qrow * p.q_row_stride + (int64_t)head * kD + h * 16;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) qv[i] = row_ok ? ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8) : zero4();
+    for (int i = 0; i < 8; ++i) qv[i] = ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8);
     uint32_t mb = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) mb = max(mb, fp4::max_bits(qv[i]));
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int vtr = (4 * h + ((lane & 15) >> 2)) * kVRow + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
 
   // Values that are not numbers stay out of the MFMAs, where a masked key's probability of 0 would not hide them: such a
-  // group is zeros in LDS, and mark_nan finds the rows that see it.
+  // group is zeros in LDS, and mark_nan finds the rows that see it (their outputs in the group are NaN).
   auto store_v = [&](const TileRegs& T, int kv0, int buf) {
     uint16_t* d = s_v[buf];
     const uint32_t b = T.ok && kv0 + (tid >> 2) < nk ? T.vs : 0u;
@@ -142,14 +144,10 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) *reinterpret_cast<u32x4*>(d + vst + q4 * 32) = fp4::values8(T.v[q4], sc);
   };
-  auto mark_nan = [&](int buf, int lim0) {  // lim0: the tile's keys that this lane's row sees
-    uint32_t hit = 0;  // byte c: the row sees such a key in group c
-    for (int j = 0; j < kBK; ++j) hit |= j < lim0 ? reinterpret_cast<const uint32_t*>(s_nan[buf])[j] : 0u;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if ((hit >> (8 * (i / 4))) & 1u) acc[dt][i] = __builtin_nanf("");
+  uint32_t nan_groups = 0;  // byte c, bit 0: the row has seen such a key in group c
+  auto mark_nan = [&](int buf, int seen) {  // seen: the tile's keys that this lane's row sees
+#pragma unroll 1
+    for (int j = 0; j < kBK; ++j) nan_groups |= j < seen ? reinterpret_cast<const uint32_t*>(s_nan[buf])[j] : 0u;
   };
   auto compute = [&](const TileRegs& T, int kv0, int buf, auto&& between) {
     const uint16_t* vt = s_v[buf];
@@ -242,10 +240,12 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // LDS column 32 dt + 8 i + 4 h + [0, 4): channels 32 i + 8 dt + 4 h + [0, 4)
+    for (int i = 0; i < 4; ++i) {  // LDS column 32 dt + 8 i + 4 h + [0, 4): channels 32 i + 8 dt + 4 h + [0, 4)
+      const float f = (nan_groups >> (8 * i)) & 1u ? __builtin_nanf("") : inv;
       *reinterpret_cast<u32x2*>(ob + i * 32 + dt * 8) =
-          u32x2{pack_bf16x2(acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv),
-                pack_bf16x2(acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv)};
+          u32x2{pack_bf16x2(acc[dt][4 * i] * f, acc[dt][4 * i + 1] * f),
+                pack_bf16x2(acc[dt][4 * i + 2] * f, acc[dt][4 * i + 3] * f)};
+    }
 }
 
 }  // namespace pf4
