@@ -157,15 +157,16 @@ __device__ __forceinline__ int64_t muldiv(int64_t a, int64_t b, int64_t c, int64
 //  * Beyond, ranges grow with the longest sequence (two steps for one of 800 tokens: 9.4 us, 10.0 in ranges of four), with
 //    four merging workgroups per sequence only up to four steps, a step for each wave, and from there on again at
 //    kMaxPiecesSplit pieces (one stream of 4000 tokens: 13.7 us with 32 pieces, 12.9 with 64).
+template <int kNW>
 __device__ __forceinline__ int active_workgroups(int grid, int64_t steps, int max_seq_steps, bool same, int batch) {
   if (max_seq_steps <= 0) return 1;
   int64_t cap;
-  if (same && max_seq_steps <= kWaves) {
+  if (same && max_seq_steps <= kNW) {
     cap = steps / max_seq_steps;
   } else {
     cap = min(steps, muldiv(kMaxPieces - 2, steps, 0, max_seq_steps));
     if (batch <= kMergeSplitBatch)
-      cap = max(cap, min((steps + kWaves - 1) / kWaves, muldiv(kMaxPiecesSplit - 2, steps, 0, max_seq_steps)));
+      cap = max(cap, min((steps + kNW - 1) / kNW, muldiv(kMaxPiecesSplit - 2, steps, 0, max_seq_steps)));
   }
   return (int)max((int64_t)1, min((int64_t)grid, cap));
 }
@@ -186,6 +187,8 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 template <int HK, bool BTL>
 struct LdsOwn {
   static constexpr bool kOwnWalk = false;
+  static constexpr int kNW = kWaves;
+  static constexpr int kGet = 2;  // 16-byte pieces of a slot that get() reads
   static constexpr int kRoundSegs = 8;
   static constexpr int kSlots = kRoundSegs + kWaves - 1;
   static constexpr bool kBtl = BTL;
@@ -222,6 +225,8 @@ struct LdsOwn {
 template <int HK>
 struct LdsBorrowed {
   static constexpr bool kOwnWalk = false;
+  static constexpr int kNW = kWaves;
+  static constexpr int kGet = 2;  // 16-byte pieces of a slot that get() reads
   static constexpr int kRoundSegs = 3;
   static constexpr int kSlots = kRoundSegs + kWaves - 1;
   static constexpr bool kBtl = false;
@@ -286,12 +291,14 @@ struct LdsBorrowed {
   }
 };
 
-// The split-KV decode work of workgroup g of `grid` (4 waves, kThreads threads), its LDS state in L.
+// The split-KV decode work of workgroup g of `grid` (LDS::kNW waves), its LDS state in L.
 template <int HK, class LDS>
 __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, const int grid, const LDS& L) {
   using TT = Tile<HK>;
   constexpr bool BTL = LDS::kBtl;
   constexpr int kRoundSegs = LDS::kRoundSegs;
+  constexpr int kNW = LDS::kNW;
+  constexpr int kNT = kNW * kWave;
   constexpr int VROW = TT::VROW;
   const int tid = threadIdx.x;
   const int w = tid >> 6;
@@ -316,8 +323,10 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
   // the window: lane k holds sequence wb + k (its steps [w_st, w_en), context, row, new-token slot)
   int w_st = 0, w_en = 0, w_ctx = 0, w_row = 0, w_snew = -1;
   if (p.plan_mode == kPlanReuse) {
-    const u32x4 v = ld_g16(p.plan + (int64_t)g * kPlanRecInts + tid * 4);
-    *reinterpret_cast<u32x4*>(&s_bt[tid * 4]) = v;
+    if (kNT * 4 == kPlanRecInts || tid < kPlanRecInts / 4) {
+      const u32x4 v = ld_g16(p.plan + (int64_t)g * kPlanRecInts + tid * 4);
+      *reinterpret_cast<u32x4*>(&s_bt[tid * 4]) = v;
+    }
     __syncthreads();
     r = s_bt[kRecR];
     r1 = s_bt[kRecR1];
@@ -394,8 +403,8 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
   };
   if (!use_rec) {
     // ---- block table into LDS and the step layout (a block-wide prefix sum over ceil(context / 16)). The lengths
-    // of the first kThreads sequences and every table entry a thread stages are loaded before any of them is waited
-    // for: one round trip (a load-then-store loop waits for each load in turn, one round trip per kThreads entries).
+    // of the first kNT sequences and every table entry a thread stages are loaded before any of them is waited
+    // for: one round trip (a load-then-store loop waits for each load in turn, one round trip per kNT entries).
     int l0 = 0, l1 = 0, l2 = 0, l3 = 0, slot_first = -1;
     if (tid < p.batch) {
       if (varlen) {
@@ -409,16 +418,16 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       if (store && !varlen) slot_first = p.slot_mapping[tid];  // (varlen mode finds the new token by position)
     }
     if constexpr (BTL) {
-      constexpr int kPer = (kBtLds + kThreads - 1) / kThreads;  // entries per thread at most
+      constexpr int kPer = (kBtLds + kNT - 1) / kNT;  // entries per thread at most
       const int nbt = p.batch * mb;
-      // entry i = tid + j kThreads sits at row i / mb, column i % mb; one step of kThreads entries moves the row by
-      // kThreads / mb and the column by kThreads % mb (with one carry at most)
-      const int dq = kThreads / mb, dr = kThreads % mb;
+      // entry i = tid + j kNT sits at row i / mb, column i % mb; one step of kNT entries moves the row by
+      // kNT / mb and the column by kNT % mb (with one carry at most)
+      const int dq = kNT / mb, dr = kNT % mb;
       int row = tid / mb, col = tid % mb;
       int vals[kPer];
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        vals[j] = tid + j * kThreads < nbt ? p.block_tables[(int64_t)row * p.bt_stride + col] : 0;
+        vals[j] = tid + j * kNT < nbt ? p.block_tables[(int64_t)row * p.bt_stride + col] : 0;
         row += dq;
         col += dr;
         if (col >= mb) {
@@ -428,13 +437,13 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       }
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
-        if (tid + j * kThreads < nbt) s_bt[tid + j * kThreads] = vals[j];
+        if (tid + j * kNT < nbt) s_bt[tid + j * kNT] = vals[j];
     }
     const int row_first = varlen ? l0 : tid;
     const int ctx_first = !varlen ? l2 : (l1 - l0 == 1 ? l3 - l2 : 0);
     int run = 0;
     int nmax = 0;  // most steps of one sequence
-    for (int base = 0; base < p.batch; base += kThreads) {
+    for (int base = 0; base < p.batch; base += kNT) {
       const int bb = base + tid;
       int row = row_first;
       const int raw = base == 0 ? ctx_first : (bb < p.batch ? seq_of(bb, row) : 0);
@@ -451,7 +460,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       __syncthreads();
       int before = 0, total = 0;
 #pragma unroll
-      for (int ww = 0; ww < kWaves; ++ww) {
+      for (int ww = 0; ww < kNW; ++ww) {
         before += ww < w ? L.wtot[ww] : 0;
         total += L.wtot[ww];
         nmax = max(nmax, L.wmax[ww]);
@@ -470,20 +479,23 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     S = uniform(run);
     nmax = uniform(nmax);
     bool same = false;  // every sequence that has steps has nmax of them (looked at where it matters)
-    if (nmax <= kWaves) {
+    if (nmax <= kNW) {
       bool other = false;
-      for (int bb = tid; bb < p.batch; bb += kThreads) {
+      for (int bb = tid; bb < p.batch; bb += kNT) {
         const int n = L.start[bb + 1] - L.start[bb];
         other = other || (n != 0 && n != nmax);
       }
       const uint64_t others = __builtin_amdgcn_ballot_w64(other);
       if (lane == 0) L.wmax[w] = others != 0;
       __syncthreads();
-      same = uniform(L.wmax[0] | L.wmax[1] | L.wmax[2] | L.wmax[3]) == 0;
+      int others_any = 0;
+#pragma unroll
+      for (int ww = 0; ww < kNW; ++ww) others_any |= L.wmax[ww];
+      same = uniform(others_any) == 0;
     }
-    G = active_workgroups(grid, S, nmax, same, p.batch);
+    G = active_workgroups<kNW>(grid, S, nmax, same, p.batch);
     if (g == 0) {  // the layout decode_merge_kernel reads, then the active workgroup count (a record keeps it)
-      for (int i = tid; i <= p.batch; i += kThreads) p.steps[i] = L.start[i];
+      for (int i = tid; i <= p.batch; i += kNT) p.steps[i] = L.start[i];
       if (tid == 0) p.steps[p.batch + 1] = G;
     }
     if (g < G) {
@@ -561,10 +573,10 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     const int k_last = 63 - __builtin_clzll(segs);
     const int re = min(r1, lane_val(w_en, k_last));
     const int R = re - rr;
-    auto share_lo = [&](int ww) { return rr + (int)(((int64_t)R * ww) / kWaves); };
+    auto share_lo = [&](int ww) { return rr + (int)(((int64_t)R * ww) / kNW); };
     const int t_lo = share_lo(w), t_hi = share_lo(w + 1);
     if constexpr (LDS::kOwnWalk) {  // another cache format: the policy walks the share (decode_fp4.h)
-      if (t_lo < t_hi) {
+      if (uniform(t_lo) < uniform(t_hi)) {
         struct Window {
           int vst, ven, vctx, vrow;
           __device__ __forceinline__ int st(int k) const { return __builtin_amdgcn_readlane(vst, k); }
@@ -572,9 +584,19 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
           __device__ __forceinline__ int ctx(int k) const { return __builtin_amdgcn_readlane(vctx, k); }
           __device__ __forceinline__ int row(int k) const { return __builtin_amdgcn_readlane(vrow, k); }
         };
+        // block_of, the table column known
+        auto block_at = [&](int k, int t, int col) -> int {
+          if (use_rec) return uniform(s_bt[kRecTileOff + (t - r)]);
+          const int bs = wb + k;
+          int blk;
+          if constexpr (BTL) blk = uniform(s_bt[bs * mb + col]);
+          else blk = p.block_tables[(int64_t)bs * p.bt_stride + col];
+          if (rec_write && lane == 0) L.rtiles[t - r] = blk;
+          return blk;
+        };
         const uint64_t hold = __builtin_amdgcn_ballot_w64(((segs >> lane) & 1ull) && w_st <= t_lo && t_lo < w_en);
         const int k0 = __builtin_ctzll(hold);
-        L.walk(p, w, t_lo, t_hi, k0, __builtin_popcountll(segs & ((1ull << k0) - 1ull)), block_of, next_seg,
+        L.walk(p, w, t_lo, t_hi, k0, __builtin_popcountll(segs & ((1ull << k0) - 1ull)), block_at, next_seg,
                Window{w_st, w_en, w_ctx, w_row});
       }
     } else if (t_lo < t_hi) {
@@ -706,9 +728,9 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     __syncthreads();  // every wave's partials of the round are in LDS
 
     // ---- merge the round's segments (fp32); thread (head hh, dims d0 .. d0 + kDpt) ----
-    constexpr int kDpt = kMaxHeads * kD / kThreads;  // output dims per thread
+    constexpr int kDpt = kMaxHeads * kD / kNT;  // output dims per thread
     constexpr int kTpr = kD / kDpt;                    // threads per head
-    static_assert(kDpt == 8, "a slot read covers 8 dims");
+    static_assert(kDpt == 4 * LDS::kGet, "a slot read covers a thread's dims");
     const int hh = tid / kTpr;
     const int d0 = (tid % kTpr) * kDpt;
     uint64_t rest = segs;
@@ -719,15 +741,16 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       const int sb = lane_val(w_st, kl), eb = lane_val(w_en, kl);
       const int a = max(rr, sb), e = min(re, eb);
       // the waves whose shares hold tiles of this segment, read in one pass (all loads before any use)
-      float mw[kWaves], lw[kWaves];
-      f32x4 ow[kWaves][kDpt / 4];
+      float mw[kNW], lw[kNW];
+      f32x4 ow[kNW][kDpt / 4];
 #pragma unroll
-      for (int ww = 0; ww < kWaves; ++ww) {
+      for (int ww = 0; ww < kNW; ++ww) {
         const bool touched = share_lo(ww) < e && share_lo(ww + 1) > a && share_lo(ww) < share_lo(ww + 1);
         // (a slot no wave wrote in this launch holds whatever LDS held: its values are selected away, never scaled)
-        f32x4 o2[2];
+        f32x4 o2[LDS::kGet];
         float m2, l2;
-        L.get(touched ? ww + k : k, hh, d0, o2, m2, l2);
+        if constexpr (LDS::kOwnWalk) L.get(ww, k, e >= share_lo(ww + 1), hh, d0, o2, m2, l2);
+        else L.get(touched ? ww + k : k, hh, d0, o2, m2, l2);
         mw[ww] = touched ? m2 : -INFINITY;
         lw[ww] = touched ? l2 : 0.f;
 #pragma unroll
@@ -735,14 +758,14 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       }
       float M = -INFINITY;
 #pragma unroll
-      for (int ww = 0; ww < kWaves; ++ww) M = fmaxf(M, mw[ww]);
+      for (int ww = 0; ww < kNW; ++ww) M = fmaxf(M, mw[ww]);
       const float Mu = M == -INFINITY ? 0.f : M;
       float Ls = 0.f;
       f32x4 o[kDpt / 4];
 #pragma unroll
       for (int i = 0; i < kDpt / 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ww = 0; ww < kWaves; ++ww) {
+      for (int ww = 0; ww < kNW; ++ww) {
         const float ew = fast_exp2(mw[ww] - Mu);  // 0 (and lw, ow 0) for the waves that did not touch the segment
         Ls += ew * lw[ww];
 #pragma unroll
@@ -773,7 +796,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
   if (p.plan_mode == kPlanRecord) {  // the record of this workgroup's range (tile ids collected behind the barrier)
     if (w == 0) write_record(rec_write);
     if (rec_write)
-      for (int i = tid; i < r1 - r; i += kThreads) rec[kRecTileOff + i] = L.rtiles[i];
+      for (int i = tid; i < r1 - r; i += kNT) rec[kRecTileOff + i] = L.rtiles[i];
   }
 }
 

@@ -6,13 +6,18 @@
 //    scale a lane), against the query in fp8. A query value needs two fp8 (mfma_scores16): with HK = 2 the 16 columns are
 //    the high parts of a kv head's 8 query heads and their low parts, one MFMA per kv head and step, and lane c adds
 //    column c ^ 8; with HK = 1 they are the 16 heads, high and low parts by an MFMA each. No conversion of K at all.
-//  * Values: a lane's 16 bytes are 32 channels of one token and share one scale: 16 conversions to bf16 (exact), then LDS.
-//    Piece w of chunk c of a row (8 channels) goes to 16-byte column w CPR + c, so that the lanes of one store write
-//    consecutive columns (in channel order they would be 64 bytes apart, a four-way bank conflict); the transposed reads
-//    then hand out the channels in that order, and put() writes them where they belong.
+//  * Values: a lane's 16 bytes are 32 channels of one token and kv head and share one scale: 16 conversions to bf16
+//    (exact), then LDS, one kv head at a time in the same tile. Piece w of group c of a row (8 channels) goes to 16-byte
+//    column 4 w + c, so that the four lanes of a token write consecutive columns (in channel order they would be 64 bytes
+//    apart, a four-way bank conflict); the transposed reads then hand out the channels in that order, and put() writes
+//    them where they belong.
 //  * O^T += V^T P^T by 16x16x32 MFMAs, both steps at once.
+// Eight waves a workgroup: one wave's conversions, LDS reads and MFMAs wait for each other most of the time (with four,
+// VALU and MFMA were busy for under a third of it each), and two to a SIMD fill each other's gaps.
+// The scales are loaded as words, four a lane, and shifted where they are used: a byte load's zero extension, an
+// instruction of its own, was put behind the loads of the next chunk and waited for all of them.
 // Loads are buffer loads whose descriptor ends with the cache block and is empty for a step that is not there: nothing
-// outside the block is read, and every chunk issues the same loads, so the waits count them exactly.
+// outside the block is read, and every chunk issues the same loads.
 #pragma once
 
 #include "decode_body.h"
@@ -29,29 +34,34 @@ constexpr int kSteps = 2;  // steps of a chunk
 template <int HK>
 struct Chunk {
   u32x4 k[kSteps][HK];      // codes: token r16 of the step, kv head g, channels 32 jq + [0, 32)
-  uint32_t ks[kSteps][HK];  // their scales
-  u32x4 v[kSteps][HK];      // codes: the step's 16-byte pieces i * 64 + lane
-  uint32_t vs[kSteps][HK];  // their scales
+  uint32_t ks[kSteps][HK];  // the token's four scales of kv head g, the lane's in byte jq
+  u32x4 v[kSteps][HK];      // codes: token lane / 4 of the step, kv head g, channels 32 (lane % 4) + [0, 32)
+  uint32_t vs[kSteps][HK];  // the token's four scales of kv head g, the lane's in byte lane % 4
   bool ok[kSteps];          // the step exists and its block is mapped
 };
 
 template <int HK, bool BTL>
 struct LdsFp4 {
   static constexpr bool kOwnWalk = true;
-  static constexpr int kRoundSegs = 5;
-  static constexpr int kSlots = kRoundSegs + kWaves - 1;
+  static constexpr int kNW = 8;
+  static constexpr int kGet = 1;
+  static constexpr int kRoundSegs = 6;
   static constexpr bool kBtl = BTL;
   static constexpr int kBtInts = BTL ? (kBtLds > kPlanRecInts ? kBtLds : kPlanRecInts) : kPlanRecInts;
-  static constexpr int CPR = HK * 4;  // 16-byte pieces of a token's codes: its groups of 32 channels
-  static constexpr int VROW = Tile<HK>::VROW;
+  static constexpr int VROW = kD + 32;  // elements of an LDS row: four rows' 64-byte runs, and the reads', in distinct banks
   static constexpr int kVt = kSteps * kTile * VROW;  // one wave's V tile
-  uint16_t* vt_all;  // [kWaves][kVt]
-  float* slots;      // [kSlots][kPartialFloats]
+  static_assert(kVt * 2 >= kPartialFloats * 4, "a V tile holds a partial");
+  uint16_t* vt_all;  // [kNW][kVt]
+  float* slots;      // [kRoundSegs - 1][kPartialFloats]
   int *ctx, *row, *snew, *start, *wtot, *wmax, *bt, *rtiles;
   __device__ __forceinline__ uint16_t* vt(int w) const { return vt_all + w * kVt; }
-  // head hh's part of a wave partial into slot si: accumulator a, rows jq*4 + [0, 4) are 4 channels from chan(a) on
-  __device__ __forceinline__ void put4(int si, int hh, int jq, const f32x4 (&acc)[8], float m, float l) const {
-    float* sl = slots + si * kPartialFloats;
+  // A wave's partial of segment k of the round: of its share's last segment in its V tile, which it has done with; of the
+  // others in slot k (a segment ends in one wave's share, so only that wave leaves it before its last).
+  __device__ __forceinline__ float* partial(int w, int k, bool last) const {
+    return last ? reinterpret_cast<float*>(vt(w)) : slots + k * kPartialFloats;
+  }
+  // head hh's part: accumulator a, rows jq*4 + [0, 4) are 4 channels
+  __device__ __forceinline__ void put4(float* sl, int hh, int jq, const f32x4 (&acc)[8], float m, float l) const {
 #pragma unroll
     for (int a = 0; a < 8; ++a)
       *reinterpret_cast<f32x4*>(&sl[hh * kD + (2 * (a & 1) + (jq >> 1)) * 32 + (a >> 1) * 8 + (jq & 1) * 4]) = acc[a];
@@ -60,54 +70,74 @@ struct LdsFp4 {
       sl[kLOff + hh] = l;
     }
   }
-  __device__ __forceinline__ void get(int si, int hh, int d0, f32x4 (&o)[2], float& m, float& l) const {
-    const float* sl = slots + si * kPartialFloats;
+  __device__ __forceinline__ void get(int w, int k, bool last, int hh, int d0, f32x4 (&o)[1], float& m, float& l) const {
+    const float* sl = partial(w, min(k, kRoundSegs - 2), last);  // (a pair that is none reads any slot: it is not used)
     m = sl[kMOff + hh];
     l = sl[kLOff + hh];
     o[0] = *reinterpret_cast<const f32x4*>(&sl[hh * kD + d0]);
-    o[1] = *reinterpret_cast<const f32x4*>(&sl[hh * kD + d0 + 4]);
   }
 
   // Wave w's share [t_lo, t_hi) of a round, from window lane k on, the kc-th segment of the round; a partial for each
-  // segment goes to slot w + its number. win: the window's values of a lane (st, en, ctx, row).
-  template <class BlockOf, class NextSeg, class Win>
-  __device__ __forceinline__ void walk(const DecodeArgs& p, int w, int t_lo, int t_hi, int k, int kc, BlockOf block_of,
-                                       NextSeg next_seg, Win win) const {
-    constexpr int kRing = 2;  // chunks in flight
+  // segment goes where partial() says. win: the window's values of a lane (st, en, ctx, row).
+  template <class BlockAt, class NextSeg, class Win>
+  __device__ __forceinline__ void walk(const DecodeArgs& p, int w_, int t_lo_, int t_hi_, int k_, int kc_,
+                                       BlockAt block_at, NextSeg next_seg, Win win) const {
+    // (in scalar registers: the descriptors of the loads are made from them)
+    const int w = uniform(w_), t_lo = uniform(t_lo_), t_hi = uniform(t_hi_);
+    int k = uniform(k_), kc = uniform(kc_);
     const int lane = threadIdx.x & 63;
     const int r16 = lane & 15;
     const int jq = lane >> 4;
     const int64_t bb = fp4::block_bytes(p.block_size, HK);
     const int scales = p.block_size * HK * fp4::kHeadCodes;  // where a block's scales start
-    const int kcode = r16 * CPR * 16 + jq * 16, kscale = r16 * CPR + jq;
+    const int kcode = r16 * HK * fp4::kHeadCodes + jq * 16, kscale = r16 * HK * fp4::kHeadScales;
+    const int vcode = (lane >> 2) * HK * fp4::kHeadCodes + (lane & 3) * 16, vscale = (lane >> 2) * HK * fp4::kHeadScales;
 
-    auto issue = [&](Chunk<HK>& T, bool any, int ks, int t) {
-      const int end = min(t_hi, any ? win.en(ks) : 0);
+    // ---- the next chunk to load: step ti of window lane ki, whose sequence ends (in this share) at step ei, at slot `in`
+    // of the block in table column `col`
+    int ki = k, ti = t_lo, ei = 0, col = 0, in = 0;
+    auto enter = [&]() {
+      ei = min(t_hi, win.en(ki));
+      const int tok = (ti - win.st(ki)) * kTile;
+      col = tok / p.block_size;
+      in = tok - col * p.block_size;
+    };
+    enter();
+    auto issue = [&](Chunk<HK>& T) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        const bool in = any && t + s < end;
-        const int64_t blk = in ? block_of(ks, t + s) : -1;
+        const bool there = ti < ei;
+        const int blk = there ? uniform((int)block_at(ki, ti, col)) : -1;
         T.ok[s] = blk >= 0 && blk < p.num_blocks;
-        const int tok = in ? ((t + s - win.st(ks)) * kTile) % p.block_size : 0;
         const int range = T.ok[s] ? (int)bb : 0;
         const int64_t at = T.ok[s] ? blk * bb : 0;
         const auto rk = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.k_cache) + at, (short)0, range,
                                                           fp4::kBufferWord3);
         const auto rv = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.v_cache) + at, (short)0, range,
                                                           fp4::kBufferWord3);
-        const int c0 = tok * HK * fp4::kHeadCodes, s0 = scales + tok * HK * fp4::kHeadScales;
+        const int c0 = in * HK * fp4::kHeadCodes, s0 = scales + in * HK * fp4::kHeadScales;
+        ti += there ? 1 : 0;
+        in += kTile;
+        if (in == p.block_size) {
+          in = 0;
+          ++col;
+        }
 #pragma unroll
         for (int g = 0; g < HK; ++g) {
           T.k[s][g] = __builtin_bit_cast(
               u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, kcode + g * fp4::kHeadCodes, c0, fp4::kStream));
-          T.ks[s][g] = __builtin_amdgcn_raw_buffer_load_b8(rk, kscale + g * fp4::kHeadScales, s0, fp4::kStream);
+          T.ks[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rk, kscale + g * fp4::kHeadScales, s0, fp4::kStream);
         }
 #pragma unroll
-        for (int i = 0; i < HK; ++i) {
-          T.v[s][i] = __builtin_bit_cast(
-              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (i * 64 + lane) * 16, c0, fp4::kStream));
-          T.vs[s][i] = __builtin_amdgcn_raw_buffer_load_b8(rv, i * 64 + lane, s0, fp4::kStream);
+        for (int g = 0; g < HK; ++g) {
+          T.v[s][g] = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, vcode + g * fp4::kHeadCodes, c0, fp4::kStream));
+          T.vs[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rv, vscale + g * fp4::kHeadScales, s0, fp4::kStream);
         }
+      }
+      if (ti == ei && ti < t_hi) {
+        ki = next_seg(ki);
+        enter();
       }
     };
 
@@ -160,58 +190,63 @@ struct LdsFp4 {
 #pragma unroll
     for (int a = 0; a < 8; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
     uint16_t* vt_w = vt(w);
-    uint16_t* vst = vt_w + (lane / CPR) * VROW + (lane % CPR) * 8;                      // stores
-    const uint16_t* vtr = vt_w + (jq * 4 + (r16 >> 2)) * VROW + 4 * (r16 & 3);          // transposed reads
+    uint16_t* vst = vt_w + (lane >> 2) * VROW + (lane & 3) * 8;                  // stores
+    const uint16_t* vtr = vt_w + (jq * 4 + (r16 >> 2)) * VROW + 4 * (r16 & 3);   // transposed reads
     const float c = p.scale_log2;
 
-    // Scores, online softmax and P V of a chunk whose first token is t0, of a sequence that ends at tok_end (as in
-    // decode_body.h: the running max moves when the chunk's exceeds it by more than 8 in log2 units).
+    // A chunk whose first token is t0, of a sequence that ends at tok_end: scores, online softmax (the running max moves
+    // when the chunk's exceeds it by more than 8 in log2 units, as in decode_body.h) and P V, one kv head after the other.
+    // `between`: called when the chunk's registers are free.
     auto compute = [&](const Chunk<HK>& T, int t0, int tok_end, auto&& between) {
-      const bool full = T.ok[0] && T.ok[1] && t0 + kSteps * kTile <= tok_end;  // wave-uniform
+      int lim[kSteps];  // tokens of each step that count
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) lim[s] = T.ok[s] ? tok_end - t0 - s * kTile : 0;
       float x[kSteps * 4];
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
         f32x4 y;
+        uint32_t sc[HK];
+#pragma unroll
+        for (int g = 0; g < HK; ++g) sc[g] = T.ks[s][g] >> (8 * jq);
         if constexpr (HK == 2) {
-          const f32x4 y0 = fp4::mfma_scores16(T.k[s][0], T.ks[s][0], qop[0], qs[0], z);
-          const f32x4 y1 = fp4::mfma_scores16(T.k[s][1], T.ks[s][1], qop[1], qs[1], z);
+          const f32x4 y0 = fp4::mfma_scores16(T.k[s][0], sc[0], qop[0], qs[0], z);
+          const f32x4 y1 = fp4::mfma_scores16(T.k[s][1], sc[1], qop[1], qs[1], z);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {  // lane c keeps kv head c / 8 and adds the other part, in lane c ^ 8
             const float give = r16 < 8 ? y1[i] : y0[i], keep = r16 < 8 ? y0[i] : y1[i];
             y[i] = keep + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0x128, 0xF, 0xF, false));
           }
         } else {
-          y = fp4::mfma_scores16(T.k[s][0], T.ks[s][0], qop[0], qs[0], z);
-          y = fp4::mfma_scores16(T.k[s][0], T.ks[s][0], qop[1], qs[0], y);
+          y = fp4::mfma_scores16(T.k[s][0], sc[0], qop[0], qs[0], z);
+          y = fp4::mfma_scores16(T.k[s][0], sc[0], qop[1], qs[0], y);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[s * 4 + i] = full || (T.ok[s] && t0 + s * kTile + jq * 4 + i < tok_end) ? y[i] : -INFINITY;
+        for (int i = 0; i < 4; ++i) x[s * 4 + i] = jq * 4 + i < lim[s] ? y[i] : -INFINITY;
       }
-      // V into LDS as bf16. Groups that are not numbers stay out of the MFMAs (the zeros that keep the kv heads apart
-      // would not hide them): the sequence's heads of that kv head are NaN in the group, which put() is told of.
+      // The values of kv head g into LDS as bf16. Groups that are not numbers stay out of the MFMAs (the zeros that keep the
+      // kv heads apart would not hide them): the sequence's heads of that kv head are NaN in the group.
+      auto store_v = [&](int g) {
+        uint32_t b[kSteps];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+        for (int s = 0; s < kSteps; ++s) b[s] = (lane >> 2) < lim[s] ? (T.vs[s][g] >> (8 * (lane & 3))) & 0xffu : 0u;
+        uint64_t bad = __builtin_amdgcn_ballot_w64(max(b[0], b[1]) == 255u);
+        if (__builtin_expect(bad != 0, 0)) {
 #pragma unroll
-        for (int i = 0; i < HK; ++i) {
-          const int tr = s * kTile + i * (64 / CPR);  // LDS row of the piece, less the lane's
-          const uint32_t b = full || (T.ok[s] && t0 + tr + lane / CPR < tok_end) ? T.vs[s][i] : 0u;
-          uint64_t bad = __builtin_amdgcn_ballot_w64(b == 255u);
-          if (__builtin_expect(bad != 0, 0)) {
-            bad |= bad >> 32;
-            bad |= bad >> 16;
-            bad |= bad >> 8;
-            if (CPR == 4) bad |= bad >> 4;
-            nan_groups |= (uint32_t)bad & ((1u << CPR) - 1u);
-          }
-          const float sc = fp4::scale_float(b == 255u ? 0u : b);
+          for (int i = 32; i >= 4; i >>= 1) bad |= bad >> i;
+          nan_groups |= ((uint32_t)bad & 15u) << (4 * g);
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) b[s] = b[s] == 255u ? 0u : b[s];
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
-            *reinterpret_cast<u32x4*>(vst + tr * VROW + q4 * CPR * 8) = fp4::values8(T.v[s][i][q4], sc);
-        }
-      wave_lds_sync();
-      between();  // the chunk's registers are free: the next one's loads go out
+            *reinterpret_cast<u32x4*>(vst + s * kTile * VROW + q4 * 32) =
+                fp4::values8(T.v[s][g][q4], fp4::scale_float(b[s]));
+        wave_lds_sync();
+      };
+      store_v(0);
 
       float tm = x[0];
 #pragma unroll
@@ -236,77 +271,56 @@ struct LdsFp4 {
 #pragma unroll
       for (int i = 0; i < 4; ++i) pv[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
 #pragma unroll
-      for (int gk = 0; gk < HK; ++gk) {
-        const u32x4 pb = HK == 1 || hg == gk ? pv : zero4();
+      for (int g = 0; g < HK; ++g) {
+        if (g > 0) store_v(g);
+        if (g == HK - 1) between();
+        const u32x4 pb = HK == 1 || hg == g ? pv : zero4();
 #pragma unroll
         for (int a = 0; a < 8; ++a) {
-          const int col = HK == 2 ? (a >> 1) * 4 + gk * 2 + (a & 1) : a;  // the 16 LDS columns of accumulator a
-          const s16x4 v0 = lds_read_tr16(vtr + col * 16);
-          const s16x4 v1 = lds_read_tr16(vtr + kTile * VROW + col * 16);
-          const u32x2 u0 = __builtin_bit_cast(u32x2, v0), u1 = __builtin_bit_cast(u32x2, v1);
+          const u32x2 u0 = __builtin_bit_cast(u32x2, lds_read_tr16(vtr + a * 16));
+          const u32x2 u1 = __builtin_bit_cast(u32x2, lds_read_tr16(vtr + kTile * VROW + a * 16));
           acc[a] = mfma_16x16x32(u32x4{u0[0], u0[1], u1[0], u1[1]}, pb, acc[a]);
         }
+        wave_lds_sync();
       }
-      wave_lds_sync();
     };
 
-    // ---- the ring: chunk registers T[u], refilled with the chunk kRing further on as soon as they are used
-    Chunk<HK> T[kRing];
+    // ---- one chunk in registers; the next one's loads go out as soon as they are free
+    Chunk<HK> T;
     u32x4 qv[HK][4];
     load_q(qv, k);
-    int ki = k, ti = t_lo;  // the next chunk to load
-    auto next = [&](Chunk<HK>& C) {
-      const bool any = ti < t_hi;
-      issue(C, any, ki, ti);
-      if (any) {
-        const int en = win.en(ki);
-        ti += kSteps;
-        if (ti >= en) {
-          ti = en;
-          if (ti < t_hi) ki = next_seg(ki);
-        }
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < kRing; ++u) next(T[u]);
+    issue(T);
     make_q(qv);
     int t = t_lo;
-    bool more = true;
-    while (more) {
-#pragma unroll
-      for (int u = 0; u < kRing; ++u) {
-        if (!more) break;
-        const int en = min(t_hi, win.en(k));
-        const bool last = t + kSteps >= en;
-        int kn = k;
-        if (last && en < t_hi) {
-          kn = next_seg(k);
-          load_q(qv, kn);
-        }
-        compute(T[u], (t - win.st(k)) * kTile, win.ctx(k), [&]() { next(T[u]); });
-        t = last ? en : t + kSteps;
-        if (last) {
-          const float l = col_sum4(lsum);
-          if (__builtin_expect(nan_groups != 0, 0)) {
-#pragma unroll
-            for (int a = 0; a < 8; ++a)
-              if ((nan_groups >> (hg * 4 + 2 * (a & 1) + (jq >> 1))) & 1u)
-                acc[a] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-          }
-          if (head_ok) put4(w + kc, head, jq, acc, m, l);
-          more = en < t_hi;
-          if (more) {
-            m = -INFINITY;
-            lsum = 0.f;
-            nan_groups = 0;
-#pragma unroll
-            for (int a = 0; a < 8; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-            make_q(qv);
-            k = kn;
-            ++kc;
-          }
-        }
+    for (;;) {
+      const int en = min(t_hi, win.en(k));
+      const bool last = t + kSteps >= en;  // of the segment
+      int kn = k;
+      if (last && en < t_hi) {
+        kn = next_seg(k);
+        load_q(qv, kn);
       }
+      compute(T, (t - win.st(k)) * kTile, win.ctx(k), [&]() { issue(T); });
+      t += kSteps;
+      if (!last) continue;
+      const float l = col_sum4(lsum);
+      if (__builtin_expect(nan_groups != 0, 0)) {
+#pragma unroll
+        for (int a = 0; a < 8; ++a)
+          if ((nan_groups >> (hg * 4 + 2 * (a & 1) + (jq >> 1))) & 1u)
+            acc[a] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+      }
+      if (head_ok) put4(partial(w, kc, en >= t_hi), head, jq, acc, m, l);
+      if (en >= t_hi) break;
+      m = -INFINITY;
+      lsum = 0.f;
+      nan_groups = 0;
+#pragma unroll
+      for (int a = 0; a < 8; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+      make_q(qv);
+      t = en;
+      k = kn;
+      ++kc;
     }
   }
 };
