@@ -66,34 +66,6 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int limit = p.causal ? min(nk, nk - nq + tq + 1) : nk;        // keys that this lane's row sees
   const int all_see = p.causal ? nk - nq + qt * bq + 1 : nk;          // keys that every row sees
 
-  // ---- the query in fp8 (fp4_common.h): operand ks holds channels 64 ks + 16 h + [0, 16) and 64 ks + 32 + 16 h + [0, 16)
-  fp4::i32x8 qhi[2], qlo[2];
-  uint32_t qs;
-  {
-    u32x4 qv[8];
-    // (a row that is none reads the nearest one that q holds: its loads need no branches, its output is not written)
-    const int64_t qrow = max((int64_t)0, min(row, p.row_limit - 1));
-    const uint16_t* qb = p.q + qrow * p.q_row_stride + (int64_t)head * kD + h * 16;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qv[i] = ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8);
-    uint32_t mb = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mb = max(mb, fp4::max_bits(qv[i]));
-    mb = __float_as_uint(xhalf_max(__uint_as_float(mb << 16))) >> 16;
-    qs = fp4::query_scale_byte(mb);
-    const float inv = fp4::query_inverse(qs);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t a = qv[ks * 4 + i / 2][(i & 1) * 2], c = qv[ks * 4 + i / 2][(i & 1) * 2 + 1];
-        const float x0 = __uint_as_float(a << 16) * inv, x1 = __uint_as_float(a & 0xffff0000u) * inv;
-        const float x2 = __uint_as_float(c << 16) * inv, x3 = __uint_as_float(c & 0xffff0000u) * inv;
-        qhi[ks][i] = fp4::query_part4(x0, x1, x2, x3, false);
-        qlo[ks][i] = fp4::query_part4(x0, x1, x2, x3, true);
-      }
-  }
-
   const int64_t bb = fp4::block_bytes(p.block_size, HK);
   const int crow = HK * fp4::kHeadCodes, srow = HK * fp4::kHeadScales;
   const int scales = p.block_size * crow;
@@ -120,6 +92,41 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     T.v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (tid >> 2) * crow + (tid & 3) * 16, c0, 0));
     T.vs = __builtin_amdgcn_raw_buffer_load_b8(rv, (tid >> 2) * srow + (tid & 3), s0, 0);
   };
+
+  // ---- the query's loads, then the first tiles': one round trip for both
+  u32x4 qv[8];
+  {
+    // (a row that is none reads the nearest one that q holds: its loads need no branches, its output is not written)
+    const int64_t qrow = max((int64_t)0, min(row, p.row_limit - 1));
+    const uint16_t* qb = p.q + qrow * p.q_row_stride + (int64_t)head * kD + h * 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qv[i] = ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8);
+  }
+  TileRegs T0, T1;
+  issue(T0, 0);
+  issue(T1, kBK);
+
+  // ---- the query in fp8 (fp4_common.h): operand ks holds channels 64 ks + 16 h + [0, 16) and 64 ks + 32 + 16 h + [0, 16)
+  fp4::i32x8 qhi[2], qlo[2];
+  uint32_t qs;
+  {
+    uint32_t mb = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mb = max(mb, fp4::max_bits(qv[i]));
+    mb = __float_as_uint(xhalf_max(__uint_as_float(mb << 16))) >> 16;
+    qs = fp4::query_scale_byte(mb);
+    const float inv = fp4::query_inverse(qs);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = qv[ks * 4 + i / 2][(i & 1) * 2], c = qv[ks * 4 + i / 2][(i & 1) * 2 + 1];
+        const float x0 = __uint_as_float(a << 16) * inv, x1 = __uint_as_float(a & 0xffff0000u) * inv;
+        const float x2 = __uint_as_float(c << 16) * inv, x3 = __uint_as_float(c & 0xffff0000u) * inv;
+        qhi[ks][i] = fp4::query_part4(x0, x1, x2, x3, false);
+        qlo[ks][i] = fp4::query_part4(x0, x1, x2, x3, true);
+      }
+  }
 
   float m = -INFINITY, lsum = 0.f;
   f32x16 acc[4];
@@ -210,13 +217,10 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_nan_at[buf]) == kv0, 0)) mark_nan(buf, limit - kv0);
   };
 
-  TileRegs T0, T1;
   if (kv_end > 0) {
-    issue(T0, 0);
     if (tid < 2) s_nan_at[tid] = -1;
     __syncthreads();
     store_v(T0, 0, 0);
-    issue(T1, kBK);
     __syncthreads();
     for (int kv0 = 0; kv0 < kv_end; kv0 += 2 * kBK) {
       compute(T0, kv0, 0, [&]() {
