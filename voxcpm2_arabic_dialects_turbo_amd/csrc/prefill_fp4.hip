@@ -6,14 +6,15 @@
 // A workgroup is four waves over 128 query rows (128 / G tokens x the G query heads of one kv head), a wave 32 of them,
 // and walks 64-key tiles (a tile lies inside one block: block_size is a multiple of 64).
 //  * S^T[64 keys x 32 rows] = K Q^T by 32x32x64 MFMAs on the codes as they are stored: a lane's 16 bytes are its
-//    operand and have one scale, so K needs no conversion and no LDS; each wave loads the tile's 4 KB for itself (three
-//    of the four from the CU's cache). The query is two fp8 parts, so the scores cost the MFMA time of bf16 ones.
+//    operand and have one scale, so K needs no conversion. The query is two fp8 parts, so the scores cost the MFMA time of
+//    bf16 ones.
 //  * V is converted once a workgroup (a thread 32 channels of a key: 16 exact conversions) into a bf16 LDS tile, double
 //    buffered, one barrier a tile. Column w * 4 + c of a row (16 bytes) holds piece w of the key's 32-channel group c, so
 //    that the four lanes of a key write consecutive columns.
 //  * O^T[128 x 32 rows] += V^T P^T by 32x32x16 MFMAs: P^T is in the B layout as the scores come, k-slot e of half h of
 //    step s being key 16 s + 8 (e / 4) + 4 h + e % 4, and the transposed reads gather the same keys.
-// The next tile's codes (20 registers a lane) are loaded while a tile is computed.
+// A tile's codes (8.5 KB, K and V) go from memory straight into LDS, a quarter by each wave. A tile's softmax and P V run
+// beside the next tile's scores and V conversion (step), while the codes of the tile after that are on their way.
 #include <climits>
 
 #include "fp4_common.h"
@@ -30,16 +31,16 @@ constexpr int kRows = 128;  // query rows of a workgroup
 constexpr int kBK = 64;     // keys of a tile
 constexpr int kVRow = kD + 16;  // elements of an LDS row: the four rows a transposed read touches lie in other banks
 
-struct TileRegs {
-  u32x4 k[2][2];    // keys 32 rt + l % 32, channels 64 ks + 32 (l / 32) + [0, 32)
-  uint32_t ks[2];   // their keys' four scales
-  u32x4 v;          // key tid / 4, channels 32 (tid % 4) + [0, 32)
-  uint32_t vs;      // their scale
-  bool ok;          // the tile's block is mapped
-};
+// A tile's codes as they come from memory: 64 keys x 64 bytes, then the keys' four scales. Of K's 16-byte pieces piece p of
+// key r lies in slot p ^ (r / 4 % 4): the eight lanes that an operand read serves at once then hit distinct banks.
+constexpr int kCodes = kBK * fp4::kHeadCodes;
+constexpr int kTileBytes = kCodes + kBK * fp4::kHeadScales;
+typedef __attribute__((address_space(3))) void lds_void;
 
 __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kBK * kVRow];
+  // (distinct arrays: the compiler can tell a tile's reads from the next one's transfers in flight)
+  __shared__ __attribute__((aligned(16))) uint8_t s_k0[kTileBytes], s_k1[kTileBytes], s_c0[kTileBytes], s_c1[kTileBytes];
   __shared__ __attribute__((aligned(4))) uint8_t s_nan[2][kBK * 4];  // a tile's groups whose scale is not a number: [key][32-channel group]
   __shared__ int s_nan_at[2];            // the first key of the last tile that held any
   const int b = blockIdx.y, g = blockIdx.z;
@@ -60,7 +61,6 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int tq = qt * bq + (rho >> gsh);
   const int head = (g << gsh) + (rho & (p.group - 1));
   const int64_t row = (int64_t)q0 + tq;
-  const bool row_ok = tq < nq && row >= 0 && row < p.row_limit;
   const int tq_last = min(nq, (qt + 1) * bq) - 1;
   const int kv_end = p.causal ? min(nk, nk - nq + tq_last + 1) : nk;  // keys that some row of the workgroup sees
   const int limit = p.causal ? min(nk, nk - nq + tq + 1) : nk;        // keys that this lane's row sees
@@ -70,27 +70,29 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int crow = HK * fp4::kHeadCodes, srow = HK * fp4::kHeadScales;
   const int scales = p.block_size * crow;
   const int32_t* bt = p.block_tables + (int64_t)b * p.bt_stride;
-  auto issue = [&](TileRegs& T, int kv0) {
+  // Tile kv0's codes from memory into LDS (K's to kd, V's to vd), a quarter of them by each wave; whether its block is mapped.
+  const int key16 = tid >> 2;  // the key of the 16-byte slot that this lane fills
+  const int kcode = key16 * crow + (((tid & 3) ^ ((key16 >> 2) & 3)) << 4), vcode = key16 * crow + ((tid & 3) << 4);
+  const int word = lane * srow;
+  auto issue = [&](uint8_t* kd, uint8_t* vd, int kv0) -> bool {
     const int blk = __builtin_amdgcn_readfirstlane(kv0 < kv_end ? bt[kv0 / p.block_size] : -1);
-    T.ok = blk >= 0 && blk < p.num_blocks;
-    const int tok = T.ok ? kv0 % p.block_size : 0;
-    const int64_t at = T.ok ? blk * bb : 0;
-    const int range = T.ok ? (int)bb : 0;
+    const bool ok = blk >= 0 && blk < p.num_blocks;
+    const int tok = ok ? kv0 % p.block_size : 0;
+    const int64_t at = ok ? blk * bb : 0;
+    const int range = ok ? (int)bb : 0;
     const auto rk = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.k_cache) + at, (short)0, range,
                                                       fp4::kBufferWord3);
     const auto rv = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.v_cache) + at, (short)0, range,
                                                       fp4::kBufferWord3);
     const int c0 = tok * crow + g * fp4::kHeadCodes, s0 = scales + tok * srow + g * fp4::kHeadScales;
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        T.k[rt][ks] = __builtin_bit_cast(
-            u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (rt * 32 + col) * crow + ks * 32 + h * 16, c0, 0));
-      T.ks[rt] = __builtin_amdgcn_raw_buffer_load_b32(rk, (rt * 32 + col) * srow, s0, 0);
-    }
-    T.v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (tid >> 2) * crow + (tid & 3) * 16, c0, 0));
-    T.vs = __builtin_amdgcn_raw_buffer_load_b8(rv, (tid >> 2) * srow + (tid & 3), s0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(kd + w * 1024), 16, kcode, c0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(vd + w * 1024), 16, vcode, c0, 0, 0);
+    // (the scales by two waves each: the same words)
+    if (w & 1)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(vd + kCodes), 4, word, s0, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(kd + kCodes), 4, word, s0, 0, 0);
+    return ok;
   };
 
   // ---- the query's loads, then the first tiles': one round trip for both
@@ -102,9 +104,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) qv[i] = ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8);
   }
-  TileRegs T0, T1;
-  issue(T0, 0);
-  issue(T1, kBK);
+  bool ok0 = issue(s_k0, s_c0, 0);
 
   // ---- the query in fp8 (fp4_common.h): operand ks holds channels 64 ks + 16 h + [0, 16) and 64 ks + 32 + 16 h + [0, 16)
   fp4::i32x8 qhi[2], qlo[2];
@@ -139,55 +139,75 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int vst = (tid >> 2) * kVRow + (tid & 3) * 8;
   const int vtr = (4 * h + ((lane & 15) >> 2)) * kVRow + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
 
-  // Values that are not numbers stay out of the MFMAs, where a masked key's probability of 0 would not hide them: such a
-  // group is zeros in LDS, and mark_nan finds the rows that see it (their outputs in the group are NaN).
-  auto store_v = [&](const TileRegs& T, int kv0, int buf) {
-    uint16_t* d = s_v[buf];
-    const uint32_t b = T.ok && kv0 + (tid >> 2) < nk ? T.vs : 0u;
+  // V of tile kv0 (in registers, `mapped`) into LDS buffer buf: the scale, then piece q4. Values that are not numbers stay
+  // out of the MFMAs, where a masked key's probability of 0 would not hide them: such a group is zeros in LDS, and mark_nan
+  // finds the rows that see it (their outputs in the group are NaN).
+  u32x4 vcodes;
+  float vscale = 0.f;
+  auto scale_v = [&](const uint8_t* vd, int kv0, bool mapped, int buf) {
+    vcodes = *reinterpret_cast<const u32x4*>(vd + tid * 16);
+    const uint32_t b = mapped && kv0 + (tid >> 2) < nk ? (uint32_t)vd[kCodes + tid] : 0u;
     const bool nan = b == 255u;
     s_nan[buf][tid] = nan;
     if (__builtin_amdgcn_ballot_w64(nan) != 0) s_nan_at[buf] = kv0;
-    const float sc = fp4::scale_float(nan ? 0u : b);
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) *reinterpret_cast<u32x4*>(d + vst + q4 * 32) = fp4::values8(T.v[q4], sc);
+    vscale = fp4::scale_float(nan ? 0u : b);
+  };
+  auto piece_v = [&](int q4, int buf) {
+    *reinterpret_cast<u32x4*>(s_v[buf] + vst + q4 * 32) = fp4::values8(vcodes[q4], vscale);
   };
   uint32_t nan_groups = 0;  // byte c, bit 0: the row has seen such a key in group c
   auto mark_nan = [&](int buf, int seen) {  // seen: the tile's keys that this lane's row sees
 #pragma unroll 1
     for (int j = 0; j < kBK; ++j) nan_groups |= j < seen ? reinterpret_cast<const uint32_t*>(s_nan[buf])[j] : 0u;
   };
-  auto compute = [&](const TileRegs& T, int kv0, int buf, auto&& between) {
-    const uint16_t* vt = s_v[buf];
-    f32x16 s[2];
+  // Score MFMA i of 8: channels 64 (i / 4) + [0, 64), the query's high or low parts (i / 2 % 2), key block i % 2. Its
+  // operand is piece 2 (i / 4) + h of key 32 (i % 2) + col.
+  u32x4 kf[2];
+  uint32_t ksc[2];
+  const int krow = col * fp4::kHeadCodes, kswz = (col >> 2) & 3;  // (32 keys on: the same swizzle)
+  auto read_k = [&](const uint8_t* kd, int ks) {
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
+    for (int rt = 0; rt < 2; ++rt)
+      kf[rt] = *reinterpret_cast<const u32x4*>(kd + rt * 32 * fp4::kHeadCodes + krow + (((2 * ks + h) ^ kswz) << 4));
+  };
+  auto read_scales = [&](const uint8_t* kd) {  // bytes 0 and 2: the scales of channels 32 h and 64 + 32 h on
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[rt][i] = 0.f;
-      const uint32_t ksc = T.ks[rt] >> (8 * h);  // bytes 0 and 2: the scales of channels 32 h and 64 + 32 h on
-      s[rt] = fp4::mfma_scores32<0>(T.k[rt][0], ksc, qhi[0], qs, s[rt]);
-      s[rt] = fp4::mfma_scores32<2>(T.k[rt][1], ksc, qhi[1], qs, s[rt]);
-      s[rt] = fp4::mfma_scores32<0>(T.k[rt][0], ksc, qlo[0], qs, s[rt]);
-      s[rt] = fp4::mfma_scores32<2>(T.k[rt][1], ksc, qlo[1], qs, s[rt]);
-    }
-    const bool full = T.ok && kv0 + kBK <= min(all_see, nk);  // workgroup-uniform
-    const int lim = T.ok ? limit - kv0 - 4 * h : INT_MIN;     // this half's keys below it are seen
-    between();  // the tile's registers are free
-    if (!full) {
+    for (int rt = 0; rt < 2; ++rt)
+      ksc[rt] = *reinterpret_cast<const uint32_t*>(kd + kCodes + (rt * 32 + col) * 4) >> (8 * h);
+  };
+  auto score = [&](int i, f32x16 (&s)[2]) {
+    const int rt = i & 1, ks = i >> 2;
+    const fp4::i32x8 q = i & 2 ? qlo[ks] : qhi[ks];
+    f32x16 z;
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[rt][i] = rt * 32 + 8 * (i / 4) + i % 4 < lim ? s[rt][i] : -INFINITY;
-    }
-    float tm = s[0][0];
+    for (int j = 0; j < 16; ++j) z[j] = 0.f;
+    const f32x16 in = i < 2 ? z : s[rt];
+    s[rt] = ks == 0 ? fp4::mfma_scores32<0>(kf[rt], ksc[rt], q, qs, in) : fp4::mfma_scores32<2>(kf[rt], ksc[rt], q, qs, in);
+  };
+  auto mask = [&](f32x16 (&s)[2], int kv0, bool mapped) -> bool {  // whether something was to be masked
+    if (mapped && kv0 + kBK <= min(all_see, nk)) return false;  // workgroup-uniform
+    const int lim = mapped ? limit - kv0 - 4 * h : INT_MIN;     // this half's keys below it are seen
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) tm = fmaxf(tm, s[rt][i]);
-    tm = xhalf_max(tm) * c;
+      for (int i = 0; i < 16; ++i) s[rt][i] = rt * 32 + 8 * (i / 4) + i % 4 < lim ? s[rt][i] : -INFINITY;
+    return true;
+  };
+  auto top_of = [&](const f32x16 (&s)[2]) {
+    float t = s[0][0];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t = fmaxf(t, s[rt][i]);
+    return t;
+  };
+  // The running max for scores whose largest (of this lane) is top: it moves where that exceeds it by more than 8 in log2
+  // units (p <= 256, exact after the final 1 / l).
+  auto raise = [&](float top) {
+    const float tm = xhalf_max(top) * c;
     const bool up = tm > m + 8.f;
-    if (__builtin_amdgcn_ballot_w64(up) != 0) {
-      const float alpha = up ? fast_exp2(m - tm) : 1.f;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(up) != 0, 0)) {
+      const float alpha = up ? fast_exp2(m - tm) : 1.f;  // exp2(-inf) = 0 on the first update
       m = up ? tm : m;
       lsum *= alpha;
 #pragma unroll
@@ -195,52 +215,120 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
     }
+  };
+  auto tile_barrier = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+  // One tile (kv0, its V in buffer buf; the next one's codes in kn, vn, the places kd, vd free): its softmax and P V beside the next tile's score MFMAs and V conversion, in this
+  // order, pinned: an MFMA leaves the wave's issue slots free, for about 2.3 elements' fma, exp, add and half a cvt (a score
+  // MFMA, 64 cycles) or 1.1 (a P V one, 32). Left to itself the compiler runs the MFMAs together and the softmax together.
+  auto step = [&](int kv0, int buf, f32x16 (&s)[2], f32x16 (&sn)[2], const uint8_t* kn, const uint8_t* vn, uint8_t* kd,
+                  uint8_t* vd, bool& okn, bool& okd) {
+    const bool more = kv0 + kBK < kv_end;
     const float mu = m == -INFINITY ? 0.f : m;
     u32x4 pb[4];
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = (st & 1) * 8 + 2 * e;
-        const float x0 = fast_exp2(fmaf(s[st >> 1][i], c, -mu)), x1 = fast_exp2(fmaf(s[st >> 1][i + 1], c, -mu));
-        lsum += x0 + x1;
-        pb[st][e] = pack_bf16x2(x0, x1);
+    float e[4];
+    float sum = 0.f;
+    auto element = [&](int x) {
+      e[x & 3] = fast_exp2(fmaf(s[x >> 4][x & 15], c, -mu));
+      if (x & 1) pb[x >> 3][(x >> 1) & 3] = pack_bf16x2(e[(x & 3) - 1], e[x & 3]);
+      if ((x & 3) == 3) {
+        sum += (e[0] + e[1]) + (e[2] + e[3]);
+        asm volatile("" : "+v"(sum));  // (here: sunk to the end of the tile, the adds would keep every e alive)
       }
+    };
+    const uint16_t* vt = s_v[buf] + vtr;
+    u32x4 vf[4];
+    auto read_v = [&](int i) {  // operand of P V MFMA i (16-key step i / 4, dims block i % 4)
+      const u32x2 u0 = __builtin_bit_cast(u32x2, lds_read_tr16(vt + (16 * (i >> 2)) * kVRow + (i & 3) * 32));
+      const u32x2 u1 = __builtin_bit_cast(u32x2, lds_read_tr16(vt + (16 * (i >> 2) + 8) * kVRow + (i & 3) * 32));
+      vf[i & 3] = u32x4{u0[0], u0[1], u1[0], u1[1]};
+    };
+    if (more) {
+      read_scales(kn);
+      read_k(kn, 0);
+      okd = issue(kd, vd, kv0 + 2 * kBK);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
+      for (int i = 0; i < 8; ++i) {
+        score(i, sn);
+        if (i == 0) scale_v(vn, kv0 + kBK, okn, buf ^ 1);
+        if (i == 3) read_k(kn, 1);
+        if (i >= 2 && i <= 5) piece_v(i - 2, buf ^ 1);
+        if (i >= 6) {
+          read_v(2 * (i - 6));
+          read_v(2 * (i - 6) + 1);
+        }
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt) {
-        const u32x2 u0 = __builtin_bit_cast(u32x2, lds_read_tr16(vt + vtr + (16 * st) * kVRow + dt * 32));
-        const u32x2 u1 = __builtin_bit_cast(u32x2, lds_read_tr16(vt + vtr + (16 * st + 8) * kVRow + dt * 32));
-        acc[dt] = mfma_32x32x16(u32x4{u0[0], u0[1], u1[0], u1[1]}, pb[st], acc[dt]);
+        for (int x = i * 18 / 8; x < (i + 1) * 18 / 8; ++x) element(x);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) read_v(i);
+#pragma unroll
+      for (int x = 0; x < 18; ++x) element(x);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      acc[i & 3] = mfma_32x32x16(vf[i & 3], pb[i >> 2], acc[i & 3]);
+      if (i + 4 < 16) read_v(i + 4);
+#pragma unroll
+      for (int x = 18 + i * 14 / 12; x < 18 + (i + 1) * 14 / 12 && x < 32; ++x) element(x);
+      if (more && i >= 12) {  // this lane's largest score of the next tile
+#pragma unroll
+        for (int x = 8 * (i - 12); x < 8 * (i - 11); ++x) top = fmaxf(top, sn[x >> 4][x & 15]);
+        asm volatile("" : "+v"(top));  // (here)
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    lsum += sum;
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_nan_at[buf]) == kv0, 0)) mark_nan(buf, limit - kv0);
+    if (more) {
+      if (mask(sn, kv0 + kBK, okn)) top = top_of(sn);
+      tile_barrier();
+      raise(top);
+    }
   };
 
   if (kv_end > 0) {
+    f32x16 sa[2], sb[2];
     if (tid < 2) s_nan_at[tid] = -1;
-    __syncthreads();
-    store_v(T0, 0, 0);
-    __syncthreads();
-    for (int kv0 = 0; kv0 < kv_end; kv0 += 2 * kBK) {
-      compute(T0, kv0, 0, [&]() {
-        store_v(T1, kv0 + kBK, 1);
-        issue(T0, kv0 + 2 * kBK);
-      });
-      __syncthreads();
-      if (kv0 + kBK >= kv_end) break;
-      compute(T1, kv0 + kBK, 1, [&]() {
-        store_v(T0, kv0 + 2 * kBK, 0);
-        issue(T1, kv0 + 3 * kBK);
-      });
-      __syncthreads();
+    tile_barrier();
+    bool ok1 = issue(s_k1, s_c1, kBK);
+    read_scales(s_k0);
+    scale_v(s_c0, 0, ok0, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i % 4 == 0) read_k(s_k0, i / 4);
+      score(i, sa);
+      if (i < 4) piece_v(i, 0);
     }
+    mask(sa, 0, ok0);
+    raise(top_of(sa));
+    tile_barrier();
+    for (int kv0 = 0;;) {
+      step(kv0, 0, sa, sb, s_k1, s_c1, s_k0, s_c0, ok1, ok0);
+      kv0 += kBK;
+      if (kv0 >= kv_end) break;
+      step(kv0, 1, sb, sa, s_k0, s_c0, s_k1, s_c1, ok0, ok1);
+      kv0 += kBK;
+      if (kv0 >= kv_end) break;
+    }
+  } else {
+    wait_vmem_all();  // (no transfer into LDS outlives the workgroup)
   }
 
   const float l = xhalf_sum(lsum);
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that sees no key: zeros
-  if (!row_ok) return;
-  uint16_t* ob = p.out + row * p.out_row_stride + (int64_t)head * kD + 4 * h;
+  // (the row again, from the thread's number: kept through the loop it would cost registers)
+  int id = tid;
+  asm volatile("" : "+v"(id));
+  const int orho = (id >> 6) * 32 + (id & 31);
+  const int otq = qt * bq + (orho >> gsh);
+  const int64_t orow = (int64_t)q0 + otq;
+  if (otq >= nq || orow < 0 || orow >= p.row_limit) return;
+  uint16_t* ob = p.out + orow * p.out_row_stride + (int64_t)((g << gsh) + (orho & (p.group - 1))) * kD + 4 * h;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
