@@ -70,14 +70,17 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int crow = HK * fp4::kHeadCodes, srow = HK * fp4::kHeadScales;
   const int scales = p.block_size * crow;
   const int32_t* bt = p.block_tables + (int64_t)b * p.bt_stride;
-  // Tile kv0's codes from memory into LDS (K's to kd, V's to vd), a quarter of them by each wave; whether its block is mapped.
+  // The next tile's codes from memory into LDS (K's to kd, V's to vd), a quarter of them by each wave; whether its block is
+  // mapped.
   const int key16 = tid >> 2;  // the key of the 16-byte slot that this lane fills
   const int kcode = key16 * crow + (((tid & 3) ^ ((key16 >> 2) & 3)) << 4), vcode = key16 * crow + ((tid & 3) << 4);
   const int word = lane * srow;
-  auto issue = [&](uint8_t* kd, uint8_t* vd, int kv0) -> bool {
-    const int blk = __builtin_amdgcn_readfirstlane(kv0 < kv_end ? bt[kv0 / p.block_size] : -1);
+  // the next tile: its first key, block (read a tile ahead) and place in the block
+  int next_kv = 0, next_col = 0, next_in = 0, next_blk = kv_end > 0 ? bt[0] : -1;
+  auto issue = [&](uint8_t* kd, uint8_t* vd) -> bool {
+    const int blk = __builtin_amdgcn_readfirstlane(next_blk);
     const bool ok = blk >= 0 && blk < p.num_blocks;
-    const int tok = ok ? kv0 % p.block_size : 0;
+    const int tok = next_in;
     const int64_t at = ok ? blk * bb : 0;
     const int range = ok ? (int)bb : 0;
     const auto rk = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.k_cache) + at, (short)0, range,
@@ -92,6 +95,13 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(vd + kCodes), 4, word, s0, 0, 0);
     else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(kd + kCodes), 4, word, s0, 0, 0);
+    next_kv += kBK;
+    next_in += kBK;
+    if (next_in == p.block_size) {
+      next_in = 0;
+      ++next_col;
+    }
+    next_blk = next_kv < kv_end ? bt[next_col] : -1;
     return ok;
   };
 
@@ -104,7 +114,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) qv[i] = ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8);
   }
-  bool ok0 = issue(s_k0, s_c0, 0);
+  bool ok0 = issue(s_k0, s_c0);
 
   // ---- the query in fp8 (fp4_common.h): operand ks holds channels 64 ks + 16 h + [0, 16) and 64 ks + 32 + 16 h + [0, 16)
   fp4::i32x8 qhi[2], qlo[2];
@@ -224,6 +234,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   auto step = [&](int kv0, int buf, f32x16 (&s)[2], f32x16 (&sn)[2], const uint8_t* kn, const uint8_t* vn, uint8_t* kd,
                   uint8_t* vd, bool& okn, bool& okd) {
     const bool more = kv0 + kBK < kv_end;
+    const int nan_at = s_nan_at[buf];
     const float mu = m == -INFINITY ? 0.f : m;
     u32x4 pb[4];
     float e[4];
@@ -246,7 +257,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     if (more) {
       read_scales(kn);
       read_k(kn, 0);
-      okd = issue(kd, vd, kv0 + 2 * kBK);
+      okd = issue(kd, vd);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -275,7 +286,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
       if (i + 4 < 16) read_v(i + 4);
 #pragma unroll
       for (int x = 18 + i * 14 / 12; x < 18 + (i + 1) * 14 / 12 && x < 32; ++x) element(x);
-      if (more && i >= 12) {  // this lane's largest score of the next tile
+      if (i >= 12) {  // this lane's largest score of the next tile
 #pragma unroll
         for (int x = 8 * (i - 12); x < 8 * (i - 11); ++x) top = fmaxf(top, sn[x >> 4][x & 15]);
         asm volatile("" : "+v"(top));  // (here)
@@ -283,19 +294,23 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
       __builtin_amdgcn_sched_barrier(0);
     }
     lsum += sum;
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_nan_at[buf]) == kv0, 0)) mark_nan(buf, limit - kv0);
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(nan_at) == kv0, 0)) mark_nan(buf, limit - kv0);
     if (more) {
       if (mask(sn, kv0 + kBK, okn)) top = top_of(sn);
-      tile_barrier();
       raise(top);
+      tile_barrier();
     }
   };
 
   if (kv_end > 0) {
     f32x16 sa[2], sb[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sb[rt][i] = 0.f;  // (read by the last tile's step, which has no next one)
     if (tid < 2) s_nan_at[tid] = -1;
     tile_barrier();
-    bool ok1 = issue(s_k1, s_c1, kBK);
+    bool ok1 = issue(s_k1, s_c1);
     read_scales(s_k0);
     scale_v(s_c0, 0, ok0, 0);
 #pragma unroll
