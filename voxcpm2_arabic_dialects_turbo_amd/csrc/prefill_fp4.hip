@@ -36,6 +36,7 @@ constexpr int kVRow = kD + 16;  // elements of an LDS row: the four rows a trans
 constexpr int kCodes = kBK * fp4::kHeadCodes;
 constexpr int kTileBytes = kCodes + kBK * fp4::kHeadScales;
 typedef __attribute__((address_space(3))) void lds_void;
+typedef u32x4 __attribute__((aligned(8))) u32x4_a8;  // output rows are 8-byte aligned
 
 __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kBK * kVRow];
@@ -336,23 +337,34 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 
   const float l = xhalf_sum(lsum);
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that sees no key: zeros
-  // (the row again, from the thread's number: kept through the loop it would cost registers)
-  int id = tid;
-  asm volatile("" : "+v"(id));
-  const int orho = (id >> 6) * 32 + (id & 31);
-  const int otq = qt * bq + (orho >> gsh);
-  const int64_t orow = (int64_t)q0 + otq;
-  if (otq >= nq || orow < 0 || orow >= p.row_limit) return;
-  uint16_t* ob = p.out + orow * p.out_row_stride + (int64_t)((g << gsh) + (orho & (p.group - 1))) * kD + 4 * h;
+  // O through LDS (each wave in a part of its own of the V tiles, which are done with), so that a row leaves in 16-byte
+  // pieces side by side: 8-byte stores straight from the accumulators, 32 rows apart, took a third of a short step's time
+  // (44 x 33-59 tokens over 50 cached: 16.0 us, 11.2 up to here).
+  constexpr int kORow = kD + 8;
+  static_assert(4 * 32 * kORow <= 2 * kBK * kVRow, "four waves' rows fit the V tiles");
+  __syncthreads();
+  uint16_t* const so = s_v[0] + w * 32 * kORow;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // LDS column 32 dt + 8 i + 4 h + [0, 4): channels 32 i + 8 dt + 4 h + [0, 4)
       const float f = (nan_groups >> (8 * i)) & 1u ? __builtin_nanf("") : inv;
-      *reinterpret_cast<u32x2*>(ob + i * 32 + dt * 8) =
+      *reinterpret_cast<u32x2*>(so + col * kORow + i * 32 + dt * 8 + 4 * h) =
           u32x2{pack_bf16x2(acc[dt][4 * i] * f, acc[dt][4 * i + 1] * f),
                 pack_bf16x2(acc[dt][4 * i + 2] * f, acc[dt][4 * i + 3] * f)};
     }
+  wave_lds_sync();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 4);
+    const int orho = w * 32 + r;
+    const int otq = qt * bq + (orho >> gsh);
+    const int64_t orow = (int64_t)q0 + otq;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(so + r * kORow + (lane & 15) * 8);
+    if (otq < nq && orow >= 0 && orow < p.row_limit)
+      *reinterpret_cast<u32x4_a8*>(p.out + orow * p.out_row_stride + (int64_t)((g << gsh) + (orho & (p.group - 1))) * kD +
+                                   (lane & 15) * 8) = x;
+  }
 }
 
 }  // namespace pf4
