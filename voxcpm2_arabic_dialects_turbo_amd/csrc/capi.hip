@@ -916,9 +916,18 @@ int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* k
                     context_lens, batch, num_heads, num_kv_heads, head_dim, softmax_scale, workspace, workspace_bytes,
                     out, &a);
   if (st != VOX_OK) return st;
-  st = vox_store_kvcache_fp4(key, value, key_row_stride, value_row_stride, k_cache, v_cache, num_blocks, block_size,
-                             slot_mapping, batch, num_kv_heads, head_dim, stream);
-  if (st != VOX_OK) return st;
+  if (key_row_stride % 8 || value_row_stride % 8 || !aligned16(key) || !aligned16(value)) {
+    // rows that the decode kernels' 16-byte loads cannot take: the two calls
+    st = vox_store_kvcache_fp4(key, value, key_row_stride, value_row_stride, k_cache, v_cache, num_blocks, block_size,
+                               slot_mapping, batch, num_kv_heads, head_dim, stream);
+    if (st != VOX_OK) return st;
+  } else {
+    a.slot_mapping = slot_mapping;
+    a.new_k = (const uint16_t*)key;
+    a.new_v = (const uint16_t*)value;
+    a.new_k_stride = key_row_stride;
+    a.new_v_stride = value_row_stride;
+  }
   return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream, vox::launch_decode_fp4);
 }
 

@@ -2,6 +2,7 @@
 // (decode_kernel, the work of decode_body.h's decode_split over its own LDS) and the merge of the sequences it cut
 // (decode_merge_kernel). The algorithm and its gfx950 mapping are described in decode_body.h.
 #include "decode_body.h"
+#include "fp4_common.h"
 
 namespace vox {
 
@@ -73,8 +74,9 @@ __device__ __forceinline__ void copy_new_rows(const DecodeArgs& p, int wid) {
 // workgroups touching b, g_first..g_last in merge_row, each left a partial at slot b + g. Online rescale over the
 // partials (fp32), the loads of kMergeBatch partials in flight together. Runs after decode_kernel on the same stream,
 // which makes the partials visible. In varlen store mode workgroups past the sequences copy the step's new rows into
-// the caches (copy_new_rows). PG workgroups per sequence, 16 / PG heads each (merge_row).
-template <int PG>
+// the caches (copy_new_rows). PG workgroups per sequence, 16 / PG heads each (merge_row). FP4: the caches are 4-bit ones, and
+// store mode quantises the row (as store_fp4_kernel does).
+template <int PG, bool FP4>
 __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs p) {
   __shared__ __attribute__((aligned(16))) float comb[PG > 1 ? PG - 1 : 1][kWave][12];
   const int b = blockIdx.x / PG, part = blockIdx.x % PG;
@@ -100,7 +102,25 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs p) {
   // (a non-temporal store: no later read of this step wants the row in L2)
   u32x4 kv_chunk = zero4();
   uint16_t* kv_dst = nullptr;
-  if (own_row) {
+  uint32_t fp4_codes = 0, fp4_scale = 0;
+  uint8_t *fp4_dst = nullptr, *fp4_scale_dst = nullptr;
+  if (FP4 && own_row) {
+    const int hk = p.num_heads / p.group;
+    const int64_t slot = slot32;
+    if (slot >= 0 && slot < p.num_blocks * p.block_size && tid < 32 * hk) {
+      const bool is_v = tid >= 16 * hk;
+      const int piece = is_v ? tid - 16 * hk : tid;  // 8 channels
+      const uint16_t* src = is_v ? p.new_v + (int64_t)b * p.new_v_stride : p.new_k + (int64_t)b * p.new_k_stride;
+      const u32x4 x = ld_g16(src + piece * 8);
+      fp4::quantise8(x, fp4_codes, fp4_scale);
+      const int64_t blk = slot / p.block_size, in = slot - blk * p.block_size;
+      uint8_t* base = reinterpret_cast<uint8_t*>(const_cast<uint16_t*>(is_v ? p.v_cache : p.k_cache)) +
+                      blk * fp4::block_bytes(p.block_size, hk);
+      fp4_dst = base + in * hk * fp4::kHeadCodes + piece * 4;
+      if ((piece & 3) == 0)
+        fp4_scale_dst = base + ((int64_t)p.block_size * fp4::kHeadCodes + in * fp4::kHeadScales) * hk + (piece >> 2);
+    }
+  } else if (own_row) {
     const int row_elems = p.group ? p.num_heads / p.group * kD : 0;  // HK x 128
     const int64_t slot = slot32;
     const int chunk = tid & 127;  // 16-byte chunk of the row: threads 0-127 K, 128-255 V
@@ -113,17 +133,33 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs p) {
   }
   merge_row<PG>(p, b, part, tid, s_tot, s_b, s_e, s_g, c0, c1, comb);
   if (kv_dst) __builtin_nontemporal_store(kv_chunk, reinterpret_cast<u32x4*>(kv_dst));
+  if constexpr (FP4) {
+    if (fp4_dst) *reinterpret_cast<uint32_t*>(fp4_dst) = fp4_codes;
+    if (fp4_scale_dst) *fp4_scale_dst = (uint8_t)fp4_scale;
+  }
 }
 
 }  // namespace
 
-hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t stream) {
+namespace {
+
+template <bool FP4>
+hipError_t launch_merge(const DecodeArgs& a, hipStream_t stream) {
   const int64_t copies = a.slot_mapping && a.cu_q && a.copy_rows > 0 ? a.copy_wgs : 0;
   if (a.batch <= kMergeSplitBatch)
-    decode_merge_kernel<4><<<dim3((unsigned)(4 * a.batch + copies)), dim3(256), 0, stream>>>(a);
+    decode_merge_kernel<4, FP4><<<dim3((unsigned)(4 * a.batch + copies)), dim3(256), 0, stream>>>(a);
   else
-    decode_merge_kernel<1><<<dim3((unsigned)(a.batch + copies)), dim3(256), 0, stream>>>(a);
+    decode_merge_kernel<1, FP4><<<dim3((unsigned)(a.batch + copies)), dim3(256), 0, stream>>>(a);
   return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t stream) { return launch_merge<false>(a, stream); }
+
+hipError_t launch_decode_merge_fp4(const DecodeArgs& a, hipStream_t stream) {
+  // (only the store knows the cache's format)
+  return a.slot_mapping ? launch_merge<true>(a, stream) : launch_merge<false>(a, stream);
 }
 
 hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stream) {

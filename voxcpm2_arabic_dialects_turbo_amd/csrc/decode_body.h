@@ -578,11 +578,12 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     if constexpr (LDS::kOwnWalk) {  // another cache format: the policy walks the share (decode_fp4.h)
       if (uniform(t_lo) < uniform(t_hi)) {
         struct Window {
-          int vst, ven, vctx, vrow;
+          int vst, ven, vctx, vrow, vsnew;
           __device__ __forceinline__ int st(int k) const { return __builtin_amdgcn_readlane(vst, k); }
           __device__ __forceinline__ int en(int k) const { return __builtin_amdgcn_readlane(ven, k); }
           __device__ __forceinline__ int ctx(int k) const { return __builtin_amdgcn_readlane(vctx, k); }
           __device__ __forceinline__ int row(int k) const { return __builtin_amdgcn_readlane(vrow, k); }
+          __device__ __forceinline__ int snew(int k) const { return __builtin_amdgcn_readlane(vsnew, k); }
         };
         // block_of, the table column known
         auto block_at = [&](int k, int t, int col) -> int {
@@ -597,7 +598,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
         const uint64_t hold = __builtin_amdgcn_ballot_w64(((segs >> lane) & 1ull) && w_st <= t_lo && t_lo < w_en);
         const int k0 = __builtin_ctzll(hold);
         L.walk(p, w, t_lo, t_hi, k0, __builtin_popcountll(segs & ((1ull << k0) - 1ull)), block_at, next_seg,
-               Window{w_st, w_en, w_ctx, w_row});
+               Window{w_st, w_en, w_ctx, w_row, w_snew});
       }
     } else if (t_lo < t_hi) {
       // this wave's first tile: window lane kcur, round segment kc

@@ -38,6 +38,8 @@ struct Chunk {
   u32x4 v[kSteps][HK];      // codes: token lane / 4 of the step, kv head g, channels 32 (lane % 4) + [0, 32)
   uint32_t vs[kSteps][HK];  // the token's four scales of kv head g, the lane's in byte lane % 4
   bool ok[kSteps];          // the step exists and its block is mapped
+  int fresh;                // store mode: the chunk's token that is the step's new one (-1: none), its row in `piece`
+  u32x4 piece;              // 8 channels: lanes [0, 16 HK) of its key row, [16 HK, 32 HK) of its value row
 };
 
 template <int HK, bool BTL>
@@ -93,6 +95,7 @@ struct LdsFp4 {
     const int kcode = r16 * HK * fp4::kHeadCodes + jq * 16, kscale = r16 * HK * fp4::kHeadScales;
     const int vcode = (lane >> 2) * HK * fp4::kHeadCodes + (lane & 3) * 16, vscale = (lane >> 2) * HK * fp4::kHeadScales;
 
+    const bool store = p.slot_mapping != nullptr;  // (never in varlen mode: slots are a row's own)
     // ---- the next chunk to load: step ti of window lane ki, whose sequence ends (in this share) at step ei, at slot `in`
     // of the block in table column `col`
     int ki = k, ti = t_lo, ei = 0, col = 0, in = 0;
@@ -104,11 +107,18 @@ struct LdsFp4 {
     };
     enter();
     auto issue = [&](Chunk<HK>& T) {
+      const int fresh_slot = store ? win.snew(ki) : -1;
+      T.fresh = -1;
+      const int64_t nrow = win.row(ki);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const bool there = ti < ei;
         const int blk = there ? uniform((int)block_at(ki, ti, col)) : -1;
         T.ok[s] = blk >= 0 && blk < p.num_blocks;
+        if (store) {
+          const int64_t d = (int64_t)fresh_slot - ((int64_t)blk * p.block_size + in);
+          if (T.ok[s] && d >= 0 && d < kTile) T.fresh = s * kTile + (int)d;
+        }
         const int range = T.ok[s] ? (int)bb : 0;
         const int64_t at = T.ok[s] ? blk * bb : 0;
         const auto rk = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.k_cache) + at, (short)0, range,
@@ -134,6 +144,10 @@ struct LdsFp4 {
               u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, vcode + g * fp4::kHeadCodes, c0, fp4::kStream));
           T.vs[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rv, vscale + g * fp4::kHeadScales, s0, fp4::kStream);
         }
+      }
+      if (T.fresh >= 0) {
+        const int at = (lane & (16 * HK - 1)) * 8;
+        T.piece = ld_g16((lane & (16 * HK) ? p.new_v + nrow * p.new_v_stride : p.new_k + nrow * p.new_k_stride) + at);
       }
       if (ti == ei && ti < t_hi) {
         ki = next_seg(ki);
@@ -194,10 +208,42 @@ struct LdsFp4 {
     const uint16_t* vtr = vt_w + (jq * 4 + (r16 >> 2)) * VROW + 4 * (r16 & 3);   // transposed reads
     const float c = p.scale_log2;
 
+    // Store mode: the new token as the cache will hold it, in the place of what was loaded for it (its row is stored by the
+    // merge kernel, after every read). The wave quantises the row once (a lane 8 channels, as store_fp4_kernel) and hands
+    // codes and scales out through its V tile.
+    auto take_fresh = [&](Chunk<HK>& T) {
+      uint32_t codes, b;
+      fp4::quantise8(T.piece, codes, b);
+      uint8_t* const s = reinterpret_cast<uint8_t*>(vt_w);
+      constexpr int kRow = HK * fp4::kHeadCodes, kScales = 2 * kRow;  // key codes, value codes, then their scales
+      if (lane < 32 * HK) {
+        *reinterpret_cast<uint32_t*>(s + lane * 4) = codes;
+        if ((lane & 3) == 0) s[kScales + (lane >> 2)] = (uint8_t)b;
+      }
+      wave_lds_sync();
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const int r = T.fresh - st * kTile;
+#pragma unroll
+        for (int g = 0; g < HK; ++g) {
+          const u32x4 kc = *reinterpret_cast<const u32x4*>(s + g * fp4::kHeadCodes + jq * 16);
+          const u32x4 vc = *reinterpret_cast<const u32x4*>(s + kRow + g * fp4::kHeadCodes + (lane & 3) * 16);
+          const uint32_t ks = *reinterpret_cast<const uint32_t*>(s + kScales + g * 4);
+          const uint32_t vs = *reinterpret_cast<const uint32_t*>(s + kScales + HK * 4 + g * 4);
+          T.k[st][g] = r16 == r ? kc : T.k[st][g];
+          T.ks[st][g] = r16 == r ? ks : T.ks[st][g];
+          T.v[st][g] = lane >> 2 == r ? vc : T.v[st][g];
+          T.vs[st][g] = lane >> 2 == r ? vs : T.vs[st][g];
+        }
+      }
+      wave_lds_sync();
+    };
+
     // A chunk whose first token is t0, of a sequence that ends at tok_end: scores, online softmax (the running max moves
     // when the chunk's exceeds it by more than 8 in log2 units, as in decode_body.h) and P V, one kv head after the other.
     // `between`: called when the chunk's registers are free.
-    auto compute = [&](const Chunk<HK>& T, int t0, int tok_end, auto&& between) {
+    auto compute = [&](Chunk<HK>& T, int t0, int tok_end, auto&& between) {
+      if (T.fresh >= 0) take_fresh(T);
       int lim[kSteps];  // tokens of each step that count
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) lim[s] = T.ok[s] ? tok_end - t0 - s * kTile : 0;

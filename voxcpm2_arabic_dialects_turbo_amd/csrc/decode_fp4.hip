@@ -1,5 +1,5 @@
 // Paged decode attention over a 4-bit KV cache: decode_split (decode_body.h) with the walk of decode_fp4.h, then the
-// merge of the sequences it cut (launch_decode_merge, the bf16 cache's: the partials are the same).
+// merge of the sequences it cut (decode_merge_kernel: the partials are the bf16 cache's).
 #include "decode_fp4.h"
 
 namespace vox {
@@ -42,7 +42,7 @@ hipError_t launch_decode_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t 
     decode_fp4_kernel<2, false><<<grid, dim3(kThreadsFp4), 0, stream>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  return launch_decode_merge(a, stream);
+  return launch_decode_merge_fp4(a, stream);
 }
 
 }  // namespace vox

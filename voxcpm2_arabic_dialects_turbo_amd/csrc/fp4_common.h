@@ -54,14 +54,6 @@ __device__ __forceinline__ uint32_t codes8(u32x4 x, float scale) {
   return r;
 }
 
-// 8 codes to 8 bf16 (packed): exact, a 2-bit significand and the scale's exponent.
-__device__ __forceinline__ u32x4 values8(uint32_t codes, float scale) {
-  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
-}
-
 // The largest magnitude of 8 packed bf16, as bits (so that infinity and NaN count as the largest).
 __device__ __forceinline__ uint32_t max_bits(u32x4 x) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -70,6 +62,23 @@ __device__ __forceinline__ uint32_t max_bits(u32x4 x) {
   for (int i = 1; i < 4; ++i)
     m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, (uint32_t)(x[i] & 0x7fff7fffu)));
   return max((uint32_t)m[0], (uint32_t)m[1]);
+}
+
+// 8 channels of a row by each of four neighbouring lanes, a group together: this lane's codes, the group's scale byte.
+__device__ __forceinline__ void quantise8(u32x4 x, uint32_t& codes, uint32_t& b) {
+  uint32_t m = max_bits(x);
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));  // quad_perm [2,3,0,1]
+  b = scale_byte(m);
+  codes = b == 255u ? 0u : codes8(x, scale_float(b));
+}
+
+// 8 codes to 8 bf16 (packed): exact, a 2-bit significand and the scale's exponent.
+__device__ __forceinline__ u32x4 values8(uint32_t codes, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
 }
 
 // The scores' MFMAs: D(fp32) += A(fp4 codes) B(fp8 e4m3), each 32 contraction elements with a scale byte of their own

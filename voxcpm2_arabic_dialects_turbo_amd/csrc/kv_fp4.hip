@@ -38,13 +38,10 @@ __global__ __launch_bounds__(kThreadsKv) void store_fp4_kernel(Fp4RowsArgs a) {
       for (int i = 0; i < 4; ++i) x[i] = (uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16);
     }
     const int64_t slot = a.slots[tok];
-    uint32_t m = fp4::max_bits(x);
-    // the four lanes of the group (idx is a multiple of 4 apart from the lane's place in it: pieces is one)
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));  // quad_perm [2,3,0,1]
+    // (the four lanes of the group: total is a multiple of 4, so they leave the loop together)
+    uint32_t codes, b;
+    fp4::quantise8(x, codes, b);
     if (slot < 0 || slot >= a.num_slots) continue;
-    const uint32_t b = fp4::scale_byte(m);
-    const uint32_t codes = b == 255u ? 0u : fp4::codes8(x, fp4::scale_float(b));
     const int64_t blk = slot / a.block_size;
     const int64_t in = slot - blk * a.block_size;
     uint8_t* base = (is_v ? a.v_cache : a.k_cache) + blk * fp4::block_bytes(a.block_size, a.num_kv_heads);

@@ -194,10 +194,11 @@ hipError_t launch_store_fp4(const Fp4RowsArgs& a, bool vec16, hipStream_t stream
 hipError_t launch_load_fp4(const Fp4RowsArgs& a, hipStream_t stream);
 
 hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
-// The same over 4-bit caches (k_cache / v_cache are their bytes; no store mode).
+// The same over 4-bit caches (k_cache / v_cache are their bytes; store mode: not with cu_q).
 hipError_t launch_decode_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
 // The merge kernel alone (after a mixed launch whose decode workgroups left partials).
 hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t stream);
+hipError_t launch_decode_merge_fp4(const DecodeArgs& a, hipStream_t stream);
 
 hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 

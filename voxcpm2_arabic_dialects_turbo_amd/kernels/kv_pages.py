@@ -34,8 +34,8 @@ def _context(kv: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.T
     dev = _check_cuda(kv, block_tables, context_lens, *more)
     if block_tables.dim() != 2 or block_tables.shape[0] < context_lens.numel():
         raise ValueError("block_tables must be [B, max_blocks] and context_lens [B]")
-    bt = _table(block_tables)
-    return dev, bt, max(bt.stride(0), bt.shape[1]), _as_i32(_flat(context_lens), "context_lens")
+    bt, bt_stride = _table(block_tables)
+    return dev, bt, bt_stride, _as_i32(_flat(context_lens), "context_lens")
 
 
 def fork_kv_blocks(kv: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, parents: torch.Tensor,

@@ -50,27 +50,34 @@ def fp4_parts(cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _cache_shape(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int]:
     """(num_blocks, block_size, HK) of a pair of 4-bit planes."""
+    shape = k_cache.shape
+    if len(shape) == 4 and shape[3] == ROW_BYTES and v_cache.shape == shape and k_cache.dtype == v_cache.dtype == torch.uint8 \
+            and k_cache.is_contiguous() and v_cache.is_contiguous():
+        return shape[0], shape[1], shape[2]
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise TypeError(f"4-bit caches are uint8, got {k_cache.dtype} and {v_cache.dtype}")
-    if k_cache.dim() != 4 or k_cache.shape[3] != ROW_BYTES or k_cache.shape != v_cache.shape:
+    if len(shape) != 4 or shape[3] != ROW_BYTES or v_cache.shape != shape:
         raise ValueError(f"4-bit caches must both be [num_blocks, block_size, HK, {ROW_BYTES}], got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError("4-bit caches must be contiguous")
-    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[2]
+    raise ValueError("4-bit caches must be contiguous")
 
 
-def _rows(fn: str, key: torch.Tensor, value: torch.Tensor, hk: int) -> None:
-    """Key and value rows [N, hk, 128] bf16 with heads contiguous; token rows may be strided."""
+def _rows(fn: str, key: torch.Tensor, value: torch.Tensor, hk: int) -> tuple[int, int, int]:
+    """Key and value rows [N, hk, 128] bf16 with heads contiguous; token rows may be strided. N and the row strides."""
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
         raise TypeError(f"{fn}: key and value must be bf16, got {key.dtype} and {value.dtype}")
-    if key.dim() != 3 or key.shape[1:] != (hk, HEAD_DIM) or key.shape != value.shape:
+    shape = key.shape
+    if len(shape) != 3 or shape[1] != hk or shape[2] != HEAD_DIM or shape != value.shape:
         raise ValueError(f"{fn}: key and value must be [N, {hk}, {HEAD_DIM}], got {tuple(key.shape)} and "
                          f"{tuple(value.shape)}")
-    for t in (key, value):
-        s = t.stride()
+    ks, vs = key.stride(), value.stride()
+    for s in (ks, vs):
         if s[2] != 1 or (s[1] != HEAD_DIM and hk > 1):
             raise ValueError(f"{fn}: key and value heads must be contiguous, got strides {s}")
+    n = shape[0]
+    if n == 1:  # (a single row's stride means nothing)
+        return 1, hk * HEAD_DIM, hk * HEAD_DIM
+    return n, ks[0], vs[0]
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -78,11 +85,14 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
-def _table(block_tables: torch.Tensor) -> torch.Tensor:
-    if block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.stride(1) == 1 \
-            and (block_tables.shape[0] == 1 or block_tables.stride(0) >= block_tables.shape[1]):
-        return block_tables
-    return _as_i32(block_tables, "block_tables").contiguous()
+def _table(block_tables: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """A block table as int32 with contiguous rows, and the elements between them."""
+    if block_tables.dtype == torch.int32:
+        stride, width = block_tables.stride(), block_tables.shape[1]
+        if stride[1] == 1 and stride[0] >= width:
+            return block_tables, stride[0]
+    bt = _as_i32(block_tables, "block_tables").contiguous()
+    return bt, bt.shape[1]
 
 
 def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -92,19 +102,19 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     at least) that leaves its largest magnitude at most 7 times it, and every value the nearest of the grid, ties to
     the even code, at most 6; a group that holds an infinity or NaN stands for NaN."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
-    _rows("store_kvcache_fp4", key, value, hk)
-    n = key.shape[0]
+    n, key_stride, value_stride = _rows("store_kvcache_fp4", key, value, hk)
     if slot_mapping.numel() != n:
         raise ValueError("store_kvcache_fp4: slot_mapping must hold one slot per token")
     if n == 0:
         return
     dev = _check_cuda(key, value, k_cache, v_cache, slot_mapping)
-    if n > 1 and (key.stride(0) == 0 or value.stride(0) == 0):  # one row for every token
+    if key_stride == 0 or value_stride == 0:  # one row for every token
         key, value = key.contiguous(), value.contiguous()
+        key_stride = value_stride = hk * HEAD_DIM
     slots = _as_i32(_flat(slot_mapping), "slot_mapping")
     lib = _lib.load()
     with _on(dev):
-        _lib.check(lib.vox_store_kvcache_fp4(key.data_ptr(), value.data_ptr(), _row_stride(key), _row_stride(value),
+        _lib.check(lib.vox_store_kvcache_fp4(key.data_ptr(), value.data_ptr(), key_stride, value_stride,
                                              k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, slots.data_ptr(), n,
                                              hk, HEAD_DIM, _lib.stream_handle(dev)), "store_kvcache_fp4")
 
@@ -117,8 +127,7 @@ def load_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.
     dev = _check_cuda(k_cache, v_cache, slots)
     at = _as_i32(_flat(slots), "slots")
     n = at.numel()
-    out = torch.empty(2, n, hk, HEAD_DIM, dtype=torch.bfloat16, device=dev)
-    key, value = out[0], out[1]
+    key, value = torch.empty(2, n, hk, HEAD_DIM, dtype=torch.bfloat16, device=dev).unbind(0)
     if n:
         lib = _lib.load()
         with _on(dev):
@@ -144,13 +153,15 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     sequence over its first context_lens[b] cached tokens; o [B, H, 128] bf16, zeros where context_lens[b] is 0. Up to 16
     query heads over 1 or 2 kv heads.
 
-    With key / value ([B, HK, 128]) and slot_mapping ([B]) the step's rows are stored first (``store_kvcache_fp4``) in the
-    same call. ``plan``: as decode_attention's; planned calls of one device share a workspace and must not overlap."""
+    With key / value ([B, HK, 128]) and slot_mapping ([B]) the step's rows are stored in the same call: the result (and the
+    caches afterwards) are those of ``store_kvcache_fp4`` followed by this attention, as long as no sequence's slot lies
+    inside another sequence's context. ``plan``: as decode_attention's; planned calls of one device share a workspace and must not overlap."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"decode_attention_fp4: q must be bf16 [B, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
     B, H, D = q.shape
-    if D != HEAD_DIM or q.stride(2) != 1 or (q.stride(1) != D and H > 1):
+    qs = q.stride()
+    if D != HEAD_DIM or qs[2] != 1 or (qs[1] != D and H > 1):
         raise ValueError(f"q must be [B, H, {HEAD_DIM}] with contiguous heads, got {tuple(q.shape)} {q.stride()}")
     if hk not in (1, 2) or H == 0 or H % hk or H > MAX_DECODE_HEADS:
         raise ValueError(f"decode supports H <= {MAX_DECODE_HEADS} query heads over 1 or 2 KV heads, got {H}/{hk}")
@@ -165,19 +176,19 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         if value is None or slot_mapping is None:
             raise ValueError("decode_attention_fp4: key, value and slot_mapping go together")
         _check_cuda(q, key, value, slot_mapping)
-        _rows("decode_attention_fp4", key, value, hk)
-        if key.shape[0] != B or slot_mapping.numel() != B:
+        rows, key_stride, value_stride = _rows("decode_attention_fp4", key, value, hk)
+        if rows != B or slot_mapping.numel() != B:
             raise ValueError(f"decode_attention_fp4: key, value and slot_mapping must hold {B} rows")
         slots = _as_i32(_flat(slot_mapping), "slot_mapping")
     elif value is not None or slot_mapping is not None:
         raise ValueError("decode_attention_fp4: key, value and slot_mapping go together")
     if B == 0:
         return out
-    if B > 1 and q.stride(0) == 0:
+    if qs[0] == 0:
         q = q.contiguous()
-    bt = _table(block_tables)
+    bt, bt_stride = _table(block_tables)
     lens = _as_i32(_flat(context_lens), "context_lens")
-    mb, bt_stride = bt.shape[1], max(bt.stride(0), bt.shape[1])
+    mb = bt.shape[1]
     lib = _lib.load()
     with _on(dev):
         ws, mode = _workspace(lib, dev, B, plan, "decode_fp4", B, mb, bt_stride, H, hk, bs)
@@ -187,10 +198,11 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                                                float(softmax_scale), mode, ws.data_ptr(), ws.numel(), out.data_ptr(),
                                                _lib.stream_handle(dev)), "decode_attn_fp4")
             return out
-        if B > 1 and (key.stride(0) == 0 or value.stride(0) == 0):
+        if key_stride == 0 or value_stride == 0:
             key, value = key.contiguous(), value.contiguous()
+            key_stride = value_stride = hk * D
         _lib.check(lib.vox_decode_attn_store_fp4(q.data_ptr(), _row_stride(q), key.data_ptr(), value.data_ptr(),
-                                                 _row_stride(key), _row_stride(value), slots.data_ptr(),
+                                                 key_stride, value_stride, slots.data_ptr(),
                                                  k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(),
                                                  bt_stride, mb, lens.data_ptr(), B, H, hk, D, float(softmax_scale), mode,
                                                  ws.data_ptr(), ws.numel(), out.data_ptr(), _lib.stream_handle(dev)),
@@ -209,7 +221,8 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"varlen_attention_fp4: q must be bf16 [T, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
     T, H, D = q.shape
-    if D != HEAD_DIM or q.stride(2) != 1 or (q.stride(1) != D and H > 1):
+    qs = q.stride()
+    if D != HEAD_DIM or qs[2] != 1 or (qs[1] != D and H > 1):
         raise ValueError(f"q must be [T, H, {HEAD_DIM}] with contiguous heads, got {tuple(q.shape)} {q.stride()}")
     if hk == 0 or H == 0 or H % hk:
         raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {hk}")
@@ -225,11 +238,11 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"out must be a bf16 [{T}, {H}, {D}] with contiguous heads on {dev}")
     if T == 0 or B <= 0 or max_seqlen_q <= 0:
         return out
-    if T > 1 and q.stride(0) == 0:
+    if qs[0] == 0:
         q = q.contiguous()
     cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
-    bt = _table(block_table)
-    mb, bt_stride = bt.shape[1], max(bt.stride(0), bt.shape[1])
+    bt, bt_stride = _table(block_table)
+    mb = bt.shape[1]
     lib = _lib.load()
     with _on(dev):
         ws, mode = None, _lib.PLAN_NONE
