@@ -430,6 +430,38 @@ def test_varlen_masks_unmapped_blocks_and_values_that_are_not_numbers():
     _check(torch.where(nan[100:], want.to(torch.bfloat16), o[100:]), want, tol + STEP * nan[100:])
 
 
+@pytest.mark.parametrize("heads,hk", [(16, 2), (3, 3), (64, 1), (128, 1)])
+@pytest.mark.parametrize("more", [0, 200])
+def test_varlen_of_few_and_many_workgroups(heads, hk, more):
+    """The same sequences alone and among so many others that a launch takes the variant for full chips: masks, blocks that
+    are none, values that are not numbers and rows without a key in both."""
+    gen = _gen(1000 + heads + more)
+    new, lens = [70, 37, 9, 100, 33], [200, 300, 4, 100, 0]
+    new, lens = new + [2] * more, lens + [2 + i for i in range(more)]
+    kc, vc, tables = _pool(gen, lens, hk, 64)
+    codes, scales = fp4.parts(vc)
+    scales[tables[0, 3], 0, hk - 1, 1] = 255  # position 192 of the first: its queries are 130 to 199
+    vc = fp4.plane(codes, scales)
+    bad = tables.clone()
+    bad[1, 1], bad[3, 1] = kc.shape[0], -5
+    q = randn(gen, sum(new), heads, D)
+    o = varlen_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), cu_seqlens_q=_cu(new), cu_seqlens_k=_cu(lens),
+                             max_seqlen_q=100, block_table=bad.to(DEV), softmax_scale=SCALE).cpu()
+    nan = torch.zeros(sum(new), heads, D, dtype=torch.bool)
+    nan[62:70, heads - heads // hk:, 32:64] = True
+    assert torch.equal(o.isnan(), nan)
+    kv, vv = fp4.cache_values(kc), fp4.cache_values(vc).nan_to_num(0.0)
+    want, tol = _varlen(q, kc, fp4.plane(codes, torch.where(scales == 255, 0, scales)), tables, new, lens)
+    # the second's keys without 64 to 127 (its queries 263 to 299 see all others before them), the fourth's first 64 only
+    k, v = (torch.cat([ref.gather_pages(c, tables[1], 300)[:64], ref.gather_pages(c, tables[1], 300)[128:]])
+            for c in (kv, vv))
+    want[70:107], tol[70:107] = _attend(q[70:107], k, v, True, SCALE)
+    k, v = (ref.gather_pages(c, tables[3], 64) for c in (kv, vv))
+    want[116:180], tol[116:180] = _attend(q[116:180], k, v, True, SCALE)
+    want[180:216], tol[180:216] = _attend(q[180:216], k, v, False, SCALE)
+    _check(torch.where(nan, want.to(torch.bfloat16), o), want, tol + STEP * nan * want.abs())
+
+
 def test_varlen_of_long_contexts():
     gen = _gen(34)
     new, lens = [40, 300], [9000, 4097]

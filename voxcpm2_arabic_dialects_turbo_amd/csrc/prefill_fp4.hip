@@ -3,8 +3,10 @@
 // keys sees keys j <= nk - nq + i (causal) or all nk; a row that sees no key gives zeros; keys of blocks outside the
 // cache have no weight. The format is in fp4_common.h.
 //
-// A workgroup is four waves over 128 query rows (128 / G tokens x the G query heads of one kv head), a wave 32 of them,
-// and walks 64-key tiles (a tile lies inside one block: block_size is a multiple of 64).
+// A workgroup is four waves over 128 / KS query rows (as many / G tokens x the G query heads of one kv head), and walks
+// 64-key tiles (a tile lies inside one block: block_size is a multiple of 64). With KS = 1 a wave has 32 of the rows and
+// every key; with KS = 2 two waves share 32 rows, each with half of every tile, and merge (O, m, l) at the end: half the
+// work a wave and tile, for grids so short that the chain of tiles is what takes the time (launch_prefill_fp4).
 //  * S^T[64 keys x 32 rows] = K Q^T by 32x32x64 MFMAs on the codes as they are stored: a lane's 16 bytes are its
 //    operand and have one scale, so K needs no conversion. The query is two fp8 parts, so the scores cost the MFMA time of
 //    bf16 ones.
@@ -14,7 +16,9 @@
 //  * O^T[128 x 32 rows] += V^T P^T by 32x32x16 MFMAs: P^T is in the B layout as the scores come, k-slot e of half h of
 //    step s being key 16 s + 8 (e / 4) + 4 h + e % 4, and the transposed reads gather the same keys.
 // A tile's codes (8.5 KB, K and V) go from memory straight into LDS, a quarter by each wave. A tile's softmax and P V run
-// beside the next tile's scores and V conversion (step), while the codes of the tile after that are on their way.
+// beside the next tile's scores and V conversion (step), while the codes of the tile after that are on their way (three
+// tiles ahead gave nothing: a tile's time is its instructions, about 1.1 us a wave alone with KS = 1, 0.87 with KS = 2).
+#include <algorithm>
 #include <climits>
 
 #include "fp4_common.h"
@@ -27,8 +31,8 @@ namespace {
 namespace pf4 {
 
 constexpr int kD = 128;
-constexpr int kRows = 128;  // query rows of a workgroup
-constexpr int kBK = 64;     // keys of a tile
+constexpr int kBK = 64;         // keys of a tile
+constexpr int kHalfChip = 128;  // half the compute units
 constexpr int kVRow = kD + 16;  // elements of an LDS row: the four rows a transposed read touches lie in other banks
 
 // A tile's codes as they come from memory: 64 keys x 64 bytes, then the keys' four scales. Of K's 16-byte pieces piece p of
@@ -36,19 +40,24 @@ constexpr int kVRow = kD + 16;  // elements of an LDS row: the four rows a trans
 constexpr int kCodes = kBK * fp4::kHeadCodes;
 constexpr int kTileBytes = kCodes + kBK * fp4::kHeadScales;
 typedef __attribute__((address_space(3))) void lds_void;
+// Read by scalar loads: as vector loads, behind the transfers into LDS, they could only be waited for with those.
+typedef const __attribute__((address_space(4))) int32_t* const_i32;
 typedef u32x4 __attribute__((aligned(8))) u32x4_a8;  // output rows are 8-byte aligned
 
+template <int KS>
 __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kBK * kVRow];
   // (distinct arrays: the compiler can tell a tile's reads from the next one's transfers in flight)
-  __shared__ __attribute__((aligned(16))) uint8_t s_k0[kTileBytes], s_k1[kTileBytes], s_c0[kTileBytes], s_c1[kTileBytes];
-  __shared__ __attribute__((aligned(4))) uint8_t s_nan[2][kBK * 4];  // a tile's groups whose scale is not a number: [key][32-channel group]
+  __shared__ __attribute__((aligned(16))) uint8_t s_t0[2 * kTileBytes], s_t1[2 * kTileBytes];  // K's, then V's
+  __shared__ __attribute__((aligned(4))) uint8_t s_nan[2][kBK * 4];  // [key][group]: a tile's scales that are not numbers
   __shared__ int s_nan_at[2];            // the first key of the last tile that held any
   const int b = blockIdx.y, g = blockIdx.z;
   const int q0 = p.cu_q[b], nq = p.cu_q[b + 1] - q0;
   const int HK = p.num_kv_heads;
   const int gsh = __builtin_ctz(p.group);  // the group divides 128: a power of two
-  const int bq = kRows >> gsh;             // query tokens of a workgroup
+  constexpr int ROWS = 128 / KS;           // query rows of the workgroup
+  constexpr int KT = 2 / KS;               // 32-key blocks of a tile that a wave takes
+  const int bq = ROWS >> gsh;              // query tokens of the workgroup
   const int qt = (int)gridDim.x - 1 - (int)blockIdx.x;  // the last tile has the most keys: first
   if (qt * bq >= nq || (p.skip_single && nq == 1)) return;  // (workgroup-uniform)
   const int nk = max(0, min(p.cu_k[b + 1] - p.cu_k[b], p.max_blocks * p.block_size));
@@ -58,7 +67,9 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int lane = tid & 63;
   const int col = lane & 31;
   const int h = lane >> 5;
-  const int rho = w * 32 + col;
+  const int rg = KS == 1 ? w : w & 1;      // rows 32 rg + [0, 32)
+  const int kh = KS == 1 ? 0 : w >> 1;     // keys 32 kh + [0, 32 KT) of every tile
+  const int rho = rg * 32 + col;
   const int tq = qt * bq + (rho >> gsh);
   const int head = (g << gsh) + (rho & (p.group - 1));
   const int64_t row = (int64_t)q0 + tq;
@@ -70,15 +81,15 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   const int64_t bb = fp4::block_bytes(p.block_size, HK);
   const int crow = HK * fp4::kHeadCodes, srow = HK * fp4::kHeadScales;
   const int scales = p.block_size * crow;
-  const int32_t* bt = p.block_tables + (int64_t)b * p.bt_stride;
-  // The next tile's codes from memory into LDS (K's to kd, V's to vd), a quarter of them by each wave; whether its block is
+  const const_i32 bt = (const_i32)(p.block_tables + (int64_t)b * p.bt_stride);
+  // The next tile's codes from memory into LDS at d, a quarter of them by each wave; whether its block is
   // mapped.
   const int key16 = tid >> 2;  // the key of the 16-byte slot that this lane fills
   const int kcode = key16 * crow + (((tid & 3) ^ ((key16 >> 2) & 3)) << 4), vcode = key16 * crow + ((tid & 3) << 4);
   const int word = lane * srow;
   // the next tile: its first key, block (read a tile ahead) and place in the block
   int next_kv = 0, next_col = 0, next_in = 0, next_blk = kv_end > 0 ? bt[0] : -1;
-  auto issue = [&](uint8_t* kd, uint8_t* vd) -> bool {
+  auto issue = [&](uint8_t* d) -> bool {
     const int blk = __builtin_amdgcn_readfirstlane(next_blk);
     const bool ok = blk >= 0 && blk < p.num_blocks;
     const int tok = next_in;
@@ -89,13 +100,13 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     const auto rv = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<uint16_t*>(p.v_cache) + at, (short)0, range,
                                                       fp4::kBufferWord3);
     const int c0 = tok * crow + g * fp4::kHeadCodes, s0 = scales + tok * srow + g * fp4::kHeadScales;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(kd + w * 1024), 16, kcode, c0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(vd + w * 1024), 16, vcode, c0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(d + w * 1024), 16, kcode, c0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(d + kTileBytes + w * 1024), 16, vcode, c0, 0, 0);
     // (the scales by two waves each: the same words)
     if (w & 1)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(vd + kCodes), 4, word, s0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(d + kTileBytes + kCodes), 4, word, s0, 0, 0);
     else
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(kd + kCodes), 4, word, s0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(d + kCodes), 4, word, s0, 0, 0);
     next_kv += kBK;
     next_in += kBK;
     if (next_in == p.block_size) {
@@ -115,7 +126,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) qv[i] = ld_g16(qb + (i >> 1) * 32 + (i & 1) * 8);
   }
-  bool ok0 = issue(s_k0, s_c0);
+  bool ok0 = issue(s_t0);
 
   // ---- the query in fp8 (fp4_common.h): operand ks holds channels 64 ks + 16 h + [0, 16) and 64 ks + 32 + 16 h + [0, 16)
   fp4::i32x8 qhi[2], qlo[2];
@@ -155,9 +166,9 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   // finds the rows that see it (their outputs in the group are NaN).
   u32x4 vcodes;
   float vscale = 0.f;
-  auto scale_v = [&](const uint8_t* vd, int kv0, bool mapped, int buf) {
-    vcodes = *reinterpret_cast<const u32x4*>(vd + tid * 16);
-    const uint32_t b = mapped && kv0 + (tid >> 2) < nk ? (uint32_t)vd[kCodes + tid] : 0u;
+  auto scale_v = [&](const uint8_t* d, int kv0, bool mapped, int buf) {
+    vcodes = *reinterpret_cast<const u32x4*>(d + kTileBytes + tid * 16);
+    const uint32_t b = mapped && kv0 + (tid >> 2) < nk ? (uint32_t)d[kTileBytes + kCodes + tid] : 0u;
     const bool nan = b == 255u;
     s_nan[buf][tid] = nan;
     if (__builtin_amdgcn_ballot_w64(nan) != 0) s_nan_at[buf] = kv0;
@@ -171,43 +182,43 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 #pragma unroll 1
     for (int j = 0; j < kBK; ++j) nan_groups |= j < seen ? reinterpret_cast<const uint32_t*>(s_nan[buf])[j] : 0u;
   };
-  // Score MFMA i of 8: channels 64 (i / 4) + [0, 64), the query's high or low parts (i / 2 % 2), key block i % 2. Its
-  // operand is piece 2 (i / 4) + h of key 32 (i % 2) + col.
-  u32x4 kf[2];
-  uint32_t ksc[2];
-  const int krow = col * fp4::kHeadCodes, kswz = (col >> 2) & 3;  // (32 keys on: the same swizzle)
+  // Score MFMA i of 4 KT: key block i % KT (of the wave's), the query's high or low parts (i / KT % 2), channels
+  // 64 (i / (2 KT)) + [0, 64). Its operand is piece 2 (i / (2 KT)) + h of key 32 (kh + i % KT) + col.
+  u32x4 kf[KT];
+  uint32_t ksc[KT];
+  const int krow = (kh * 32 + col) * fp4::kHeadCodes, kswz = (col >> 2) & 3;  // (32 keys on: the same swizzle)
   auto read_k = [&](const uint8_t* kd, int ks) {
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < KT; ++rt)
       kf[rt] = *reinterpret_cast<const u32x4*>(kd + rt * 32 * fp4::kHeadCodes + krow + (((2 * ks + h) ^ kswz) << 4));
   };
   auto read_scales = [&](const uint8_t* kd) {  // bytes 0 and 2: the scales of channels 32 h and 64 + 32 h on
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
-      ksc[rt] = *reinterpret_cast<const uint32_t*>(kd + kCodes + (rt * 32 + col) * 4) >> (8 * h);
+    for (int rt = 0; rt < KT; ++rt)
+      ksc[rt] = *reinterpret_cast<const uint32_t*>(kd + kCodes + ((kh + rt) * 32 + col) * 4) >> (8 * h);
   };
-  auto score = [&](int i, f32x16 (&s)[2]) {
-    const int rt = i & 1, ks = i >> 2;
-    const fp4::i32x8 q = i & 2 ? qlo[ks] : qhi[ks];
+  auto score = [&](int i, f32x16 (&s)[KT]) {
+    const int rt = i % KT, ks = i / (2 * KT);
+    const fp4::i32x8 q = (i / KT) & 1 ? qlo[ks] : qhi[ks];
     f32x16 z;
 #pragma unroll
     for (int j = 0; j < 16; ++j) z[j] = 0.f;
-    const f32x16 in = i < 2 ? z : s[rt];
+    const f32x16 in = i < KT ? z : s[rt];
     s[rt] = ks == 0 ? fp4::mfma_scores32<0>(kf[rt], ksc[rt], q, qs, in) : fp4::mfma_scores32<2>(kf[rt], ksc[rt], q, qs, in);
   };
-  auto mask = [&](f32x16 (&s)[2], int kv0, bool mapped) -> bool {  // whether something was to be masked
+  auto mask = [&](f32x16 (&s)[KT], int kv0, bool mapped) -> bool {  // whether something was to be masked
     if (mapped && kv0 + kBK <= min(all_see, nk)) return false;  // workgroup-uniform
-    const int lim = mapped ? limit - kv0 - 4 * h : INT_MIN;     // this half's keys below it are seen
+    const int lim = mapped ? limit - kv0 - 32 * kh - 4 * h : INT_MIN;  // this half's keys below it are seen
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < KT; ++rt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[rt][i] = rt * 32 + 8 * (i / 4) + i % 4 < lim ? s[rt][i] : -INFINITY;
     return true;
   };
-  auto top_of = [&](const f32x16 (&s)[2]) {
+  auto top_of = [&](const f32x16 (&s)[KT]) {
     float t = s[0][0];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < KT; ++rt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) t = fmaxf(t, s[rt][i]);
     return t;
@@ -229,15 +240,19 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   };
   auto tile_barrier = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-  // One tile (kv0, its V in buffer buf; the next one's codes in kn, vn, the places kd, vd free): its softmax and P V beside the next tile's score MFMAs and V conversion, in this
-  // order, pinned: an MFMA leaves the wave's issue slots free, for about 2.3 elements' fma, exp, add and half a cvt (a score
-  // MFMA, 64 cycles) or 1.1 (a P V one, 32). Left to itself the compiler runs the MFMAs together and the softmax together.
-  auto step = [&](int kv0, int buf, f32x16 (&s)[2], f32x16 (&sn)[2], const uint8_t* kn, const uint8_t* vn, uint8_t* kd,
-                  uint8_t* vd, bool& okn, bool& okd) {
+  // One tile (kv0, its V in buffer buf; the next one's codes at `next`, its own place free for the one after): its softmax
+  // and P V beside the next tile's score MFMAs and V conversion, in this order, pinned: an MFMA leaves the wave's issue slots
+  // free, for about 2.3 elements' fma, exp, add and half a cvt (a score MFMA, 64 cycles) or 1.1 (a P V one, 32). Left to
+  // itself the compiler runs the MFMAs together and the softmax together.
+  auto step = [&](int kv0, int buf, f32x16 (&s)[KT], f32x16 (&sn)[KT], const uint8_t* next, uint8_t* own, bool& okn,
+                  bool& okd) {
     const bool more = kv0 + kBK < kv_end;
     const int nan_at = s_nan_at[buf];
+    constexpr int NS = 4 * KT, NP = 8 * KT, NE = 16 * KT;  // score and P V MFMAs, elements of a lane
+    constexpr int E1 = KT == 2 ? 18 : 10;                  // elements beside the score MFMAs; the others ...
+    constexpr int SPAN = NP - 4;                           // ... beside the P V ones before the last 16 keys'
     const float mu = m == -INFINITY ? 0.f : m;
-    u32x4 pb[4];
+    u32x4 pb[2 * KT];
     float e[4];
     float sum = 0.f;
     auto element = [&](int x) {
@@ -248,7 +263,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
         asm volatile("" : "+v"(sum));  // (here: sunk to the end of the tile, the adds would keep every e alive)
       }
     };
-    const uint16_t* vt = s_v[buf] + vtr;
+    const uint16_t* vt = s_v[buf] + vtr + kh * 32 * kVRow;
     u32x4 vf[4];
     auto read_v = [&](int i) {  // operand of P V MFMA i (16-key step i / 4, dims block i % 4)
       const u32x2 u0 = __builtin_bit_cast(u32x2, lds_read_tr16(vt + (16 * (i >> 2)) * kVRow + (i & 3) * 32));
@@ -256,40 +271,42 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
       vf[i & 3] = u32x4{u0[0], u0[1], u1[0], u1[1]};
     };
     if (more) {
-      read_scales(kn);
-      read_k(kn, 0);
-      okd = issue(kd, vd);
+      read_scales(next);
+      read_k(next, 0);
+      okd = issue(own);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < NS; ++i) {
         score(i, sn);
-        if (i == 0) scale_v(vn, kv0 + kBK, okn, buf ^ 1);
-        if (i == 3) read_k(kn, 1);
-        if (i >= 2 && i <= 5) piece_v(i - 2, buf ^ 1);
-        if (i >= 6) {
-          read_v(2 * (i - 6));
-          read_v(2 * (i - 6) + 1);
+        if (i == 0) scale_v(next, kv0 + kBK, okn, buf ^ 1);
+        if (i == NS / 2 - 1) read_k(next, 1);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          if (i == (KT == 2 ? q4 + 2 : min(q4 + 1, 3))) piece_v(q4, buf ^ 1);
+        if (i >= NS - 2) {
+          read_v(2 * (i - (NS - 2)));
+          read_v(2 * (i - (NS - 2)) + 1);
         }
 #pragma unroll
-        for (int x = i * 18 / 8; x < (i + 1) * 18 / 8; ++x) element(x);
+        for (int x = i * E1 / NS; x < (i + 1) * E1 / NS; ++x) element(x);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) read_v(i);
 #pragma unroll
-      for (int x = 0; x < 18; ++x) element(x);
+      for (int x = 0; x < E1; ++x) element(x);
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < NP; ++i) {
       acc[i & 3] = mfma_32x32x16(vf[i & 3], pb[i >> 2], acc[i & 3]);
-      if (i + 4 < 16) read_v(i + 4);
+      if (i + 4 < NP) read_v(i + 4);
 #pragma unroll
-      for (int x = 18 + i * 14 / 12; x < 18 + (i + 1) * 14 / 12 && x < 32; ++x) element(x);
-      if (i >= 12) {  // this lane's largest score of the next tile
+      for (int x = E1 + i * (NE - E1) / SPAN; x < E1 + (i + 1) * (NE - E1) / SPAN && x < NE; ++x) element(x);
+      if (i >= NP - 4) {  // this lane's largest score of the next tile
 #pragma unroll
-        for (int x = 8 * (i - 12); x < 8 * (i - 11); ++x) top = fmaxf(top, sn[x >> 4][x & 15]);
+        for (int x = 4 * KT * (i - (NP - 4)); x < 4 * KT * (i - (NP - 5)); ++x) top = fmaxf(top, sn[x >> 4][x & 15]);
         asm volatile("" : "+v"(top));  // (here)
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -304,60 +321,90 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   };
 
   if (kv_end > 0) {
-    f32x16 sa[2], sb[2];
+    f32x16 sa[KT], sb[KT];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < KT; ++rt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) sb[rt][i] = 0.f;  // (read by the last tile's step, which has no next one)
     if (tid < 2) s_nan_at[tid] = -1;
     tile_barrier();
-    bool ok1 = issue(s_k1, s_c1);
-    read_scales(s_k0);
-    scale_v(s_c0, 0, ok0, 0);
+    bool ok1 = issue(s_t1);
+    read_scales(s_t0);
+    scale_v(s_t0, 0, ok0, 0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i % 4 == 0) read_k(s_k0, i / 4);
+    for (int i = 0; i < 4; ++i) piece_v(i, 0);
+#pragma unroll
+    for (int i = 0; i < 4 * KT; ++i) {
+      if (i % (2 * KT) == 0) read_k(s_t0, i / (2 * KT));
       score(i, sa);
-      if (i < 4) piece_v(i, 0);
     }
     mask(sa, 0, ok0);
     raise(top_of(sa));
     tile_barrier();
     for (int kv0 = 0;;) {
-      step(kv0, 0, sa, sb, s_k1, s_c1, s_k0, s_c0, ok1, ok0);
-      kv0 += kBK;
-      if (kv0 >= kv_end) break;
-      step(kv0, 1, sb, sa, s_k0, s_c0, s_k1, s_c1, ok0, ok1);
-      kv0 += kBK;
-      if (kv0 >= kv_end) break;
+      step(kv0, 0, sa, sb, s_t1, s_t0, ok1, ok0);
+      if ((kv0 += kBK) >= kv_end) break;
+      step(kv0, 1, sb, sa, s_t0, s_t1, ok0, ok1);
+      if ((kv0 += kBK) >= kv_end) break;
     }
-  } else {
-    wait_vmem_all();  // (no transfer into LDS outlives the workgroup)
   }
+  wait_vmem_all();  // (no transfer into LDS outlives the workgroup)
 
-  const float l = xhalf_sum(lsum);
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that sees no key: zeros
-  // O through LDS (each wave in a part of its own of the V tiles, which are done with), so that a row leaves in 16-byte
-  // pieces side by side: 8-byte stores straight from the accumulators, 32 rows apart, took a third of a short step's time
-  // (44 x 33-59 tokens over 50 cached: 16.0 us, 11.2 up to here).
+  // ---- O through LDS (in the V tiles, which are done with), so that a row leaves in 16-byte pieces side by side: 8-byte
+  // stores straight from the accumulators, 32 rows apart, took a third of a short step's time (44 x 33-59 tokens over 50
+  // cached: 16.0 us, 11.2 up to here). KS = 2: first the two waves of a row block trade halves: wave kh finishes the dims
+  // blocks 2 kh, 2 kh + 1.
+  float l = xhalf_sum(lsum);
+  constexpr int ND = 4 / KS;  // dims blocks a wave finishes
   constexpr int kORow = kD + 8;
-  static_assert(4 * 32 * kORow <= 2 * kBK * kVRow, "four waves' rows fit the V tiles");
+  static_assert(4 / KS * 32 * kORow <= 2 * kBK * kVRow && 4 * 64 * 36 * 2 <= 2 * kBK * kVRow, "they fit the V tiles");
   __syncthreads();
-  uint16_t* const so = s_v[0] + w * 32 * kORow;
+  if constexpr (KS == 2) {
+    float* const sx = reinterpret_cast<float*>(s_v[0]);  // [wave][piece of 4 or (m, l)][lane]
+    f32x4* const mine = reinterpret_cast<f32x4*>(sx + w * 64 * 36);
+    const f32x4* const theirs = reinterpret_cast<const f32x4*>(sx + (w ^ 2) * 64 * 36);
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // the blocks that the other wave finishes
+        const f32x16& o = kh == 0 ? acc[2 + dt] : acc[dt];
+        mine[(dt * 4 + i) * 64 + lane] = f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+      }
+    mine[8 * 64 + lane] = f32x4{m, l, __uint_as_float(nan_groups), 0.f};
+    __syncthreads();
+    const f32x4 x = theirs[8 * 64 + lane];
+    const float top = fmaxf(m, x[0]), mu = top == -INFINITY ? 0.f : top;
+    const float a0 = fast_exp2(m - mu), a1 = fast_exp2(x[0] - mu);
+    l = l * a0 + x[1] * a1;
+    nan_groups |= __float_as_uint(x[2]);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 y = theirs[(dt * 4 + i) * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[dt][4 * i + j] = (kh == 0 ? acc[dt][4 * i + j] : acc[2 + dt][4 * i + j]) * a0 + y[j] * a1;
+      }
+    __syncthreads();
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that sees no key: zeros
+  uint16_t* const so = s_v[0] + rg * 32 * kORow;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // LDS column 32 dt + 8 i + 4 h + [0, 4): channels 32 i + 8 dt + 4 h + [0, 4)
       const float f = (nan_groups >> (8 * i)) & 1u ? __builtin_nanf("") : inv;
-      *reinterpret_cast<u32x2*>(so + col * kORow + i * 32 + dt * 8 + 4 * h) =
+      *reinterpret_cast<u32x2*>(so + col * kORow + i * 32 + (kh * ND + dt) * 8 + 4 * h) =
           u32x2{pack_bf16x2(acc[dt][4 * i] * f, acc[dt][4 * i + 1] * f),
                 pack_bf16x2(acc[dt][4 * i + 2] * f, acc[dt][4 * i + 3] * f)};
     }
-  wave_lds_sync();
+  if constexpr (KS == 2) __syncthreads();
+  else wave_lds_sync();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 4);
-    const int orho = w * 32 + r;
+  for (int i = 0; i < 8 / KS; ++i) {
+    const int r = (kh * (8 / KS) + i) * 4 + (lane >> 4);
+    const int orho = rg * 32 + r;
     const int otq = qt * bq + (orho >> gsh);
     const int64_t orow = (int64_t)q0 + otq;
     const u32x4 x = *reinterpret_cast<const u32x4*>(so + r * kORow + (lane & 15) * 8);
@@ -372,9 +419,21 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
 }  // namespace
 
 hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream) {
-  const int bq = pf4::kRows / a.group;
-  const dim3 grid((unsigned)((max_seqlen_q + bq - 1) / bq), (unsigned)a.batch, (unsigned)a.num_kv_heads);
-  pf4::prefill_fp4_kernel<<<grid, dim3(256), 0, stream>>>(a);
+  // Two waves on the same rows where the launch is at most half a workgroup a compute unit: the chain of tiles is then the
+  // time (16 query heads of 2 kv heads, KS = 1 | 2: 1000 tokens over 2000 cached, 126 workgroups of 128 rows, 58.6 | 47.6 us;
+  // 4 x 200 over 2000, 104: 44.9 | 36.8; 100 over 300, 14: 13.4 | 11.9). From there on 64-row workgroups stage and convert
+  // every tile twice as often for more than they save (156 workgroups 19.5 | 20.8 us, 298: 12.7 | 16.4, 1134: 152 | 177).
+  // At most that many workgroups: every sequence's tiles, or one tile in part a sequence and the others full.
+  const int bq = 128 / a.group;
+  const int64_t tiles = std::min((int64_t)a.batch * ((max_seqlen_q + bq - 1) / bq), a.row_limit / bq + a.batch);
+  // (group 128: 64 rows would be half a token)
+  const bool two = a.group <= 64 && tiles * a.num_kv_heads <= pf4::kHalfChip;
+  const int bq_ks = two ? bq / 2 : bq;
+  const dim3 grid((unsigned)((max_seqlen_q + bq_ks - 1) / bq_ks), (unsigned)a.batch, (unsigned)a.num_kv_heads);
+  if (two)
+    pf4::prefill_fp4_kernel<2><<<grid, dim3(256), 0, stream>>>(a);
+  else
+    pf4::prefill_fp4_kernel<1><<<grid, dim3(256), 0, stream>>>(a);
   return hipGetLastError();
 }
 
