@@ -155,39 +155,47 @@ struct LdsFp4 {
       }
     };
 
+    // what lane c ^ 8 of the 16 gives
+    auto other_part = [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xF, 0xF, false); };
     // ---- the query of a sequence: column r16 of kv head g's operand is a part of head (HK == 2: g * group + r16 % 8)
-    auto load_q = [&](u32x4 (&qv)[HK][4], int ks) {
+    // With HK == 2 lanes c and c ^ 8 hold parts of the same values: each loads and splits half of them (channels 16 jq +
+    // [0, 16), or 64 on) and they trade.
+    constexpr int QL = HK == 2 ? 2 : 4;  // 16-byte loads of a lane
+    auto load_q = [&](u32x4 (&qv)[HK][QL], int ks) {
 #pragma unroll
       for (int g = 0; g < HK; ++g) {
         const int c = HK == 2 ? (r16 & 7) : r16;
         const int hd = HK == 2 ? g * p.group + (c < p.group ? c : 0) : (c < p.num_heads ? c : 0);
-        const uint16_t* qb = p.q + (int64_t)win.row(ks) * p.q_row_stride + (int64_t)hd * kD + jq * 16;
+        const uint16_t* qb = p.q + (int64_t)win.row(ks) * p.q_row_stride + (int64_t)hd * kD + jq * 16 +
+                             (HK == 2 ? (r16 >> 3) * 64 : 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qv[g][i] = ld_g16(qb + (i >> 1) * 64 + (i & 1) * 8);
+        for (int i = 0; i < QL; ++i) qv[g][i] = ld_g16(qb + (i >> 1) * 64 + (i & 1) * 8);
       }
     };
     // qop[g]: HK == 2: high parts of kv head g's heads in columns 0-7, low parts in 8-15; HK == 1: qop[0] high, qop[1] low
     fp4::i32x8 qop[2];
     uint32_t qs[HK];
-    auto make_q = [&](const u32x4 (&qv)[HK][4]) {
+    auto make_q = [&](const u32x4 (&qv)[HK][QL]) {
 #pragma unroll
       for (int g = 0; g < HK; ++g) {
         uint32_t mb = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mb = max(mb, fp4::max_bits(qv[g][i]));
-        mb = __float_as_uint(col_max4(__uint_as_float(mb << 16))) >> 16;  // the whole row: four lanes hold it
+        for (int i = 0; i < QL; ++i) mb = max(mb, fp4::max_bits(qv[g][i]));
+        if constexpr (HK == 2) mb = max(mb, (uint32_t)other_part((int)mb));
+        mb = __float_as_uint(col_max4(__uint_as_float(mb << 16))) >> 16;  // the whole row
         qs[g] = fp4::query_scale_byte(mb);
-        const float inv = fp4::query_inverse(qs[g]);
+        const float scale = fp4::scale_float(qs[g]), inv = fp4::query_inverse(qs[g]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t a = qv[g][i / 2][(i & 1) * 2], b = qv[g][i / 2][(i & 1) * 2 + 1];
-          const float x0 = __uint_as_float(a << 16) * inv, x1 = __uint_as_float(a & 0xffff0000u) * inv;
-          const float x2 = __uint_as_float(b << 16) * inv, x3 = __uint_as_float(b & 0xffff0000u) * inv;
+        for (int i = 0; i < 2 * QL; ++i) {
+          int hi, lo;
+          fp4::query_parts4(qv[g][i / 2][(i & 1) * 2], qv[g][i / 2][(i & 1) * 2 + 1], scale, inv, hi, lo);
           if constexpr (HK == 2) {
-            qop[g][i] = fp4::query_part4(x0, x1, x2, x3, r16 >= 8);
+            const int keep = r16 < 8 ? hi : lo, got = other_part(r16 < 8 ? lo : hi);
+            qop[g][i] = r16 < 8 ? keep : got;
+            qop[g][i + 4] = r16 < 8 ? got : keep;
           } else {
-            qop[0][i] = fp4::query_part4(x0, x1, x2, x3, false);
-            qop[1][i] = fp4::query_part4(x0, x1, x2, x3, true);
+            qop[0][i] = hi;
+            qop[1][i] = lo;
           }
         }
       }
@@ -261,7 +269,7 @@ struct LdsFp4 {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {  // lane c keeps kv head c / 8 and adds the other part, in lane c ^ 8
             const float give = r16 < 8 ? y1[i] : y0[i], keep = r16 < 8 ? y0[i] : y1[i];
-            y[i] = keep + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0x128, 0xF, 0xF, false));
+            y[i] = keep + __int_as_float(other_part(__float_as_int(give)));
           }
         } else {
           y = fp4::mfma_scores16(T.k[s][0], sc[0], qop[0], qs[0], z);
@@ -333,7 +341,7 @@ struct LdsFp4 {
 
     // ---- one chunk in registers; the next one's loads go out as soon as they are free
     Chunk<HK> T;
-    u32x4 qv[HK][4];
+    u32x4 qv[HK][QL];
     load_q(qv, k);
     issue(T);
     make_q(qv);

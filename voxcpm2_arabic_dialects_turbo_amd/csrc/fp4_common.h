@@ -109,15 +109,19 @@ __device__ __forceinline__ uint32_t query_scale_byte(uint32_t amax_bits) {
 // 1 / scale_float(b) for b in [1, 248]
 __device__ __forceinline__ float query_inverse(uint32_t b) { return __uint_as_float((254u - b) << 23); }
 
-// The hi (lo: the lo) parts of 4 values, as 4 packed bytes.
-__device__ __forceinline__ int query_part4(float x0, float x1, float x2, float x3, bool lo) {
-  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, hi, true);
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(x0 - __builtin_amdgcn_cvt_f32_fp8(hi, 0),
-                                          x1 - __builtin_amdgcn_cvt_f32_fp8(hi, 1), 0, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(x2 - __builtin_amdgcn_cvt_f32_fp8(hi, 2),
-                                      x3 - __builtin_amdgcn_cvt_f32_fp8(hi, 3), r, true);
-  return lo ? r : hi;
+// The parts of 4 values (packed bf16) as 4 packed bytes each: the high ones straight from bf16 under the scale 2^(e - 127),
+// the low ones from what those leave of x inv, inv = 2^(127 - e) (exact: a power of two, and hi is near).
+__device__ __forceinline__ void query_parts4(uint32_t a, uint32_t b, float scale, float inv, int& hi, int& lo) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  i16x2 h = {0, 0};
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2, a), scale, false);
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2, b), scale, true);
+  hi = __builtin_bit_cast(int, h);
+  const auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(fmaf(__uint_as_float(a << 16), inv, -y0[0]),
+                                       fmaf(__uint_as_float(a & 0xffff0000u), inv, -y0[1]), 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(fmaf(__uint_as_float(b << 16), inv, -y1[0]),
+                                       fmaf(__uint_as_float(b & 0xffff0000u), inv, -y1[1]), lo, true);
 }
 
 }  // namespace fp4

@@ -137,16 +137,16 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     for (int i = 0; i < 8; ++i) mb = max(mb, fp4::max_bits(qv[i]));
     mb = __float_as_uint(xhalf_max(__uint_as_float(mb << 16))) >> 16;
     qs = fp4::query_scale_byte(mb);
-    const float inv = fp4::query_inverse(qs);
+    const float scale = fp4::scale_float(qs), inv = fp4::query_inverse(qs);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t a = qv[ks * 4 + i / 2][(i & 1) * 2], c = qv[ks * 4 + i / 2][(i & 1) * 2 + 1];
-        const float x0 = __uint_as_float(a << 16) * inv, x1 = __uint_as_float(a & 0xffff0000u) * inv;
-        const float x2 = __uint_as_float(c << 16) * inv, x3 = __uint_as_float(c & 0xffff0000u) * inv;
-        qhi[ks][i] = fp4::query_part4(x0, x1, x2, x3, false);
-        qlo[ks][i] = fp4::query_part4(x0, x1, x2, x3, true);
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(&qv[ks * 4 + i / 2]) + (i & 1) * 2;
+        int hi, lo;
+        fp4::query_parts4(x[0], x[1], scale, inv, hi, lo);
+        qhi[ks][i] = hi;
+        qlo[ks][i] = lo;
       }
   }
 
