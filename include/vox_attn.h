@@ -281,7 +281,7 @@ int vox_load_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t num_b
                          void* value, void* stream);
 
 /* vox_decode_attn over 4-bit caches: the attention over the values that the caches hold. Arguments, workspace and plans as
- * vox_decode_attn's (records may not be shared with calls of other functions). */
+ * vox_decode_attn's (records may not be shared with calls of other functions). softmax_scale must be positive. */
 int vox_decode_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                         int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                         int max_blocks, const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
@@ -302,7 +302,8 @@ int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* k
 
 /* vox_prefill_attn over 4-bit caches through block tables, with cu_seqlens. num_tokens: the rows that q and out hold; rows
  * at or past it are neither read nor written by the prefill kernel. plan, workspace: as vox_prefill_attn's (with the
- * workspace the one-query sequences run on the decode kernels). num_heads / num_kv_heads divides 128. */
+ * workspace the one-query sequences run on the decode kernels). num_heads / num_kv_heads divides 128, softmax_scale is
+ * positive. */
 int vox_prefill_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                          int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                          int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
@@ -325,7 +326,8 @@ int vox_copy_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int blo
  * filled slots are copied to block new_blocks[i], which takes that block's place. child_tables int32 [num_forks,
  * max_blocks] (-1 past the context), child_lens int32 [num_forks]. new_blocks must be blocks that no table names, no two
  * the same; one whose parent ends with a full block is left alone. A parent outside [0, batch) gives an empty child; a
- * last block or new block outside the cache copies nothing and leaves -1 in the child's table. */
+ * last block or new block outside the cache copies nothing and leaves -1 in the child's table; a context past what
+ * max_blocks blocks hold counts as that. */
 int vox_fork_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
                        int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
                        const int32_t* context_lens, int batch, const int32_t* parents, const int32_t* new_blocks,
@@ -335,7 +337,7 @@ int vox_fork_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int blo
  * them, those at or past L move to the dead blocks below L, the lowest to the lowest. Blocks shared by several rows move
  * once. new_tables int32 [batch, max_blocks]: the tables with the new numbers (-1 past the context, entries outside the
  * cache as they were); remap int32 [num_blocks]: each live block's new number, -1 for the dead; live int32 [1]: L. moves
- * int32 [2 num_blocks + 1]: scratch. Blocks from L on are free afterwards; num_blocks at most 2^19. */
+ * int32 [2 num_blocks + 1]: scratch. Blocks from L on are free afterwards; num_blocks at most 2^18. */
 int vox_compact_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
                           int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
                           const int32_t* context_lens, int batch, int32_t* new_tables, int32_t* remap, int32_t* live,

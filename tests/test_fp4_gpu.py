@@ -167,6 +167,24 @@ def test_store_of_one_row_for_every_token_and_of_none():
     assert load_kvcache_fp4(*caches, slots[:0])[0].shape == (0, 2, D)
 
 
+def test_ids_past_int32_name_nothing():
+    """64-bit slots and block ids that int32 does not hold lie outside the cache, not where their low half points."""
+    gen = _gen(6)
+    kc, vc, tables = _pool(gen, [100, 100], 2)
+    row = randn(gen, 2, 2, D).to(DEV)
+    kd, vd = kc.to(DEV), vc.to(DEV)
+    store_kvcache_fp4(row, row, kd, vd, torch.tensor([2 ** 32 + 3, -2 ** 33], device=DEV))
+    assert torch.equal(kd.cpu(), kc) and torch.equal(vd.cpu(), vc)
+    assert not load_kvcache_fp4(kd, vd, torch.tensor([2 ** 32], device=DEV))[0].any()
+    wide = tables.long()
+    wide[1] += 2 ** 32
+    q = randn(gen, 2, 16, D)
+    o = decode_attention_fp4(q.to(DEV), kd, vd, torch.tensor([100, 100], device=DEV), wide.to(DEV), SCALE)
+    assert (o[1] == 0).all()
+    want, tol = _varlen(q, kc, vc, tables, [1, 1], [100, 100])
+    _check(o[:1], want[:1], tol[:1])
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # decode
 
@@ -459,6 +477,22 @@ def test_varlen_of_few_and_many_workgroups(heads, hk, more):
     k, v = (ref.gather_pages(c, tables[3], 64) for c in (kv, vv))
     want[116:180], tol[116:180] = _attend(q[116:180], k, v, True, SCALE)
     want[180:216], tol[180:216] = _attend(q[180:216], k, v, False, SCALE)
+    _check(torch.where(nan, want.to(torch.bfloat16), o), want, tol + STEP * nan * want.abs())
+
+
+@pytest.mark.parametrize("more", [0, 200])
+def test_varlen_of_queries_that_are_not_numbers(more):
+    gen = _gen(35 + more)
+    new, lens = [40, 30] + [2] * more, [200, 70] + [5] * more
+    kc, vc, tables = _pool(gen, lens, 2)
+    q = randn(gen, sum(new), 16, D)
+    want, tol = _varlen(q, kc, vc, tables, new, lens)
+    q[3, 2, 5], q[45, 15, 127] = float("nan"), float("-inf")
+    o = varlen_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), cu_seqlens_q=_cu(new), cu_seqlens_k=_cu(lens),
+                             max_seqlen_q=40, block_table=tables.to(DEV), softmax_scale=SCALE).cpu()
+    nan = torch.zeros(o.shape, dtype=torch.bool)
+    nan[3, 2], nan[45, 15] = True, True
+    assert torch.equal(o.isnan(), nan)
     _check(torch.where(nan, want.to(torch.bfloat16), o), want, tol + STEP * nan * want.abs())
 
 

@@ -13,6 +13,7 @@ from voxcpm2_arabic_dialects_turbo_amd import _lib, layers, ops, ops_fp4, runner
 from voxcpm2_arabic_dialects_turbo_amd.context import reset_context, set_context
 from voxcpm2_arabic_dialects_turbo_amd.kernels import kv_copy, kv_pages
 from voxcpm2_arabic_dialects_turbo_amd.layers import Attention
+from voxcpm2_arabic_dialects_turbo_amd.ops_fp4 import _ids, _table
 
 BF16, U8, I32 = torch.bfloat16, torch.uint8, torch.int32
 
@@ -242,6 +243,21 @@ def test_c_abi_rejects_bad_arguments_before_launching(name, args, over):
     assert _err()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-39, float("nan"), float("inf"), 3e38])
+@pytest.mark.parametrize("name,args", [("vox_decode_attn_fp4", DECODE), ("vox_decode_attn_store_fp4", STORES),
+                                       ("vox_prefill_attn_fp4", VARLEN)])
+def test_c_abi_takes_positive_softmax_scales(name, args, scale):
+    assert _call(name, args, dict(scale=scale)) == _lib.VOX_EINVAL
+    assert "softmax_scale" in _err()
+
+
+def test_ids_past_int32_are_outside_every_cache():
+    ids = torch.tensor([[0, 5, 2 ** 32 + 5], [-1, -2 ** 40, 2 ** 31]])
+    assert _ids(ids, "ids").tolist() == [0, 5, 2 ** 31 - 1, -1, -1, 2 ** 31 - 1]
+    table, stride = _table(ids)
+    assert table.tolist() == [[0, 5, 2 ** 31 - 1], [-1, -1, 2 ** 31 - 1]] and stride == 3 and table.dtype == torch.int32
+
+
 @pytest.mark.parametrize("name,args,over", [("vox_store_kvcache_fp4", STORE, dict(n=0)), ("vox_load_kvcache_fp4", LOAD, dict(n=0)),
                                             ("vox_decode_attn_fp4", DECODE, dict(batch=0)),
                                             ("vox_prefill_attn_fp4", VARLEN, dict(n=0)),
@@ -266,7 +282,7 @@ PAGES = [dict(kv=None), dict(planes=0), dict(planes=70000), dict(blocks=0), dict
         dict(mb=1 << 25, bts=1 << 25)]),
     *(("vox_compact_kv_blocks", COMPACT, o) for o in PAGES + [
         dict(batch=-1), dict(bt=None), dict(remap=None), dict(live=None), dict(moves=None), dict(mb=0), dict(bts=3),
-        dict(blocks=(1 << 19) + 1)]),
+        dict(blocks=(1 << 19) + 1), dict(blocks=(1 << 18) + 1)]),
 ])
 def test_c_abi_pages_reject_bad_arguments_before_launching(name, args, over):
     assert _call(name, args, over) == _lib.VOX_EINVAL

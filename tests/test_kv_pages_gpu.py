@@ -106,6 +106,32 @@ def test_compact_of_nothing_and_of_everything(fp4):
     assert int(live) == 1 and torch.equal(d.cpu(), kv)
 
 
+def test_compact_of_the_most_blocks():
+    """Live blocks at the end of a cache of 2^18 blocks, whose bitmap is the largest the plan takes."""
+    blocks = 1 << 18
+    bits = torch.arange(2 * blocks * 8).to(torch.int16).view(1, 2, blocks, 1, 1, 8)
+    d = bits.view(torch.bfloat16).to(DEV)
+    t, remap, live = compact_kv_blocks(d, _int([[blocks - 1, 7, blocks - 2], [1, blocks // 2, -1]]), _int([3, 2]))
+    _same(t, [[4, 0, 3], [1, 2, -1]])
+    _same(live, [5])
+    new = {1: 1, 7: 0, blocks // 2: 2, blocks - 2: 3, blocks - 1: 4}
+    want = torch.full((blocks,), -1, dtype=torch.int32)
+    for a, b in new.items():
+        want[a] = b
+        bits[:, :, b] = bits[:, :, a]
+    assert torch.equal(remap.cpu(), want)
+    assert torch.equal(d.cpu().view(torch.int16), bits)
+
+
+def test_fork_from_no_rows():
+    """Every parent is outside a batch of none: empty children."""
+    kv = torch.zeros(1, 2, 4, 64, 1, 68, dtype=torch.uint8, device=DEV)
+    tables, lens = fork_kv_blocks(kv, torch.empty(0, 3, dtype=torch.int32, device=DEV),
+                                  torch.empty(0, dtype=torch.int32, device=DEV), _int([0, 5]), _int([1, 2]))
+    _same(tables, [[-1, -1, -1], [-1, -1, -1]])
+    _same(lens, [0, 0])
+
+
 def test_copy_block_prefix_of_a_4_bit_cache():
     kv = _kv(torch.Generator().manual_seed(3), 5, 12, 256, 2, True)
     d = kv.to(DEV)

@@ -4,6 +4,7 @@
 // returns a status (VOX_OK, VOX_EINVAL, VOX_EHIP) instead of throwing; vox_last_error() gives the calling thread's
 // message for the last failure. Nothing here allocates, frees or synchronizes, so every call can be captured into
 // a HIP graph.
+#include <cfloat>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -814,7 +815,14 @@ int fp4_cache(const char* fn, const void* k_cache, const void* v_cache, int64_t 
   return VOX_OK;
 }
 
-// A cache's planes as bytes; `what` is the name of the call.
+// Of the attention calls: masked scores are -infinity before the scale, so it has to keep them there.
+int fp4_softmax(const char* fn, float softmax_scale) {
+  if (!(softmax_scale >= 2 * FLT_MIN && softmax_scale <= FLT_MAX / 2))
+    return fail(VOX_EINVAL, "%s: softmax_scale %g must be positive", fn, (double)softmax_scale);
+  return VOX_OK;
+}
+
+// A cache's planes as bytes, for the call fn.
 int pages_setup(const char* fn, void* kv, int64_t num_planes, int64_t num_blocks, int block_size, int64_t slot_bytes,
                 int64_t scale_bytes, vox::PagesArgs* out) {
   if (!kv) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
@@ -883,6 +891,7 @@ int vox_decode_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache
     return fail(VOX_EINVAL, "decode_attn_fp4: plan mode %d", plan);
   if (batch == 0) return VOX_OK;
   int st = fp4_cache("decode_attn_fp4", k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st == VOX_OK) st = fp4_softmax("decode_attn_fp4", softmax_scale);
   if (st != VOX_OK) return st;
   vox::DecodeArgs a;
   st = decode_setup(q, q_row_stride, k_cache, v_cache, num_blocks, block_size, block_tables, bt_stride, max_blocks,
@@ -906,6 +915,7 @@ int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* k
   if (!key || !value || !slot_mapping)
     return fail(VOX_EINVAL, "decode_attn_store_fp4: null key, value or slot_mapping");
   int st = fp4_cache("decode_attn_store_fp4", k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st == VOX_OK) st = fp4_softmax("decode_attn_store_fp4", softmax_scale);
   if (st != VOX_OK) return st;
   const int64_t row = (int64_t)num_kv_heads * head_dim;
   if (key_row_stride < row || value_row_stride < row)
@@ -944,6 +954,7 @@ int vox_prefill_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cach
   if (!block_tables || !cu_seqlens_q || !cu_seqlens_k || !out)
     return fail(VOX_EINVAL, "%s: null pointer argument", fn);
   int st = fp4_cache(fn, k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st == VOX_OK) st = fp4_softmax(fn, softmax_scale);
   if (st != VOX_OK) return st;
   if (out_row_stride < (int64_t)num_heads * head_dim || out_row_stride % 4 || ((uintptr_t)out & 7u))
     return fail(VOX_EINVAL, "%s: bad out row stride or alignment", fn);
@@ -990,7 +1001,7 @@ int vox_fork_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int blo
   const char* fn = "fork_kv_blocks";
   if (num_forks < 0 || batch < 0) return fail(VOX_EINVAL, "%s: negative count", fn);
   if (num_forks == 0) return VOX_OK;
-  if (!block_tables || !context_lens || !parents || !new_blocks || !child_tables || !child_lens)
+  if ((batch > 0 && (!block_tables || !context_lens)) || !parents || !new_blocks || !child_tables || !child_lens)
     return fail(VOX_EINVAL, "%s: null pointer argument", fn);
   if (max_blocks <= 0 || bt_stride < max_blocks || (int64_t)max_blocks * block_size > (1 << 30))
     return fail(VOX_EINVAL, "%s: bad block table shape", fn);
@@ -1015,9 +1026,10 @@ int vox_compact_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int 
   vox::PagesArgs a;
   const int st = pages_setup(fn, kv, num_planes, num_blocks, block_size, slot_bytes, scale_bytes, &a);
   if (st != VOX_OK) return st;
-  if (num_blocks > (1 << 19))  // its bitmap of the blocks lives in 64 KiB of LDS
-    return fail(VOX_EINVAL, "%s: %lld blocks, %d at most", fn, (long long)num_blocks, 1 << 19);
-  const vox::CompactArgs c{block_tables, bt_stride, max_blocks > 0 ? max_blocks : 1, context_lens, batch, new_tables, remap, live, moves};
+  if (num_blocks > (1 << 18))  // its bitmap of the blocks lives in 32 KiB of LDS
+    return fail(VOX_EINVAL, "%s: %lld blocks, %d at most", fn, (long long)num_blocks, 1 << 18);
+  const vox::CompactArgs c{block_tables, bt_stride, max_blocks > 0 ? max_blocks : 1, context_lens, batch, new_tables, remap, live,
+                           moves};
   return hip_status(vox::launch_compact(a, c, (hipStream_t)stream), "compact_kv_blocks launch");
 }
 

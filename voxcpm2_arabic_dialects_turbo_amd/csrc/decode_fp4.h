@@ -135,14 +135,14 @@ struct LdsFp4 {
 #pragma unroll
         for (int g = 0; g < HK; ++g) {
           T.k[s][g] = __builtin_bit_cast(
-              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, kcode + g * fp4::kHeadCodes, c0, fp4::kStream));
-          T.ks[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rk, kscale + g * fp4::kHeadScales, s0, fp4::kStream);
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, kcode + g * fp4::kHeadCodes, c0, 0));
+          T.ks[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rk, kscale + g * fp4::kHeadScales, s0, 0);
         }
 #pragma unroll
         for (int g = 0; g < HK; ++g) {
           T.v[s][g] = __builtin_bit_cast(
-              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, vcode + g * fp4::kHeadCodes, c0, fp4::kStream));
-          T.vs[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rv, vscale + g * fp4::kHeadScales, s0, fp4::kStream);
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, vcode + g * fp4::kHeadCodes, c0, 0));
+          T.vs[s][g] = __builtin_amdgcn_raw_buffer_load_b32(rv, vscale + g * fp4::kHeadScales, s0, 0);
         }
       }
       if (T.fresh >= 0) {

@@ -23,7 +23,6 @@ constexpr int kHeadScales = 4;   // bytes of a head's scales
 constexpr int kHeadBytes = kHeadCodes + kHeadScales;
 // word 3 of a raw buffer descriptor (32-bit data format; byte offsets, range-checked against num_records)
 constexpr int kBufferWord3 = 0x00020000;
-constexpr int kStream = 0;  // cache policy of a load: non-temporal
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

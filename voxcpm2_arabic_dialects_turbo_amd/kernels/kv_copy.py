@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from ..ops_fp4 import _on
 from .kv_pages import pages_of
 
 
@@ -34,8 +35,9 @@ def copy_kv_block_prefix(kv: torch.Tensor, entries: list[tuple[int, int, int]]) 
     pairs = torch.tensor(entries, dtype=torch.int32, pin_memory=True).to(kv.device, non_blocking=True)
     lib = _lib.load()
     if fp4:
-        _lib.check(lib.vox_copy_kv_blocks(kv.data_ptr(), *pages, pairs.data_ptr(), len(entries),
-                                          _lib.stream_handle(kv.device)), "copy_kv_block_prefix")
+        with _on(kv.device):
+            _lib.check(lib.vox_copy_kv_blocks(kv.data_ptr(), *pages, pairs.data_ptr(), len(entries),
+                                              _lib.stream_handle(kv.device)), "copy_kv_block_prefix")
         return
     _lib.check(lib.vox_copy_kv_block_prefix(kv.data_ptr(), layers * kvs, blocks, block_size, per_token, 2,
                                             pairs.data_ptr(), len(entries), max(n for _, _, n in entries),

@@ -13,7 +13,7 @@ import torch
 
 from .. import _lib
 from ..ops import _as_i32, _check_cuda, _flat
-from ..ops_fp4 import ROW_BYTES, _on, _table
+from ..ops_fp4 import ROW_BYTES, _ids, _on, _table
 
 
 def pages_of(kv: torch.Tensor) -> tuple[int, int, int, int, int]:
@@ -46,10 +46,11 @@ def fork_kv_blocks(kv: torch.Tensor, block_tables: torch.Tensor, context_lens: t
     lengths int32 [F].
 
     ``new_blocks`` ([F]) are blocks that no table names, no two the same; one whose parent ends with a full block stays
-    unused. A parent outside the batch gives an empty child."""
+    unused. A parent outside the batch gives an empty child; a partly filled block that is not in the cache, or a new block
+    that is not, leaves -1 in the child's table."""
     planes, blocks, bs, slot, scale = pages_of(kv)
     dev, bt, bt_stride, lens = _context(kv, block_tables, context_lens, parents, new_blocks)
-    who, fresh = _as_i32(_flat(parents), "parents"), _as_i32(_flat(new_blocks), "new_blocks")
+    who, fresh = _ids(parents, "parents"), _ids(new_blocks, "new_blocks")
     n, mb = who.numel(), bt.shape[1]
     if fresh.numel() != n:
         raise ValueError("fork_kv_blocks: one new block per parent")
@@ -74,7 +75,7 @@ def compact_kv_blocks(kv: torch.Tensor, block_tables: torch.Tensor, context_lens
     from L on are free.
 
     Returns the tables with the new numbers (int32 [B, max_blocks], -1 past the context, entries that name no block as
-    they were), the new number of every block (int32 [blocks], -1: dead), and L (int32 [1])."""
+    they were), the new number of every block (int32 [blocks], -1: dead), and L (int32 [1]). At most 2^18 blocks."""
     planes, blocks, bs, slot, scale = pages_of(kv)
     dev, bt, bt_stride, lens = _context(kv, block_tables, context_lens)
     batch, mb = lens.numel(), bt.shape[1]

@@ -85,13 +85,19 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
+def _ids(t: torch.Tensor, name: str) -> torch.Tensor:
+    """Slots or block ids as a flat int32 tensor; those that int32 does not hold become ids outside every cache."""
+    t = _flat(t)
+    return _as_i32(t.clamp(-1, 2 ** 31 - 1) if t.dtype == torch.int64 else t, name)
+
+
 def _table(block_tables: torch.Tensor) -> tuple[torch.Tensor, int]:
     """A block table as int32 with contiguous rows, and the elements between them."""
     if block_tables.dtype == torch.int32:
         stride, width = block_tables.stride(), block_tables.shape[1]
         if stride[1] == 1 and stride[0] >= width:
             return block_tables, stride[0]
-    bt = _as_i32(block_tables, "block_tables").contiguous()
+    bt = _ids(block_tables, "block_tables").view(block_tables.shape)
     return bt, bt.shape[1]
 
 
@@ -100,7 +106,8 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     """Quantises key[i] / value[i] ([N, HK, 128] bf16, token rows may be strided) into slot slot_mapping[i] of the 4-bit
     caches; slots outside them (-1: padding) store nothing. A group of 32 channels gets the least power of two (2^-126
     at least) that leaves its largest magnitude at most 7 times it, and every value the nearest of the grid, ties to
-    the even code, at most 6; a group that holds an infinity or NaN stands for NaN."""
+    the even code, at most 6; a group that holds an infinity or NaN stands for NaN. A slot that occurs twice holds a mix of
+    its rows."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     n, key_stride, value_stride = _rows("store_kvcache_fp4", key, value, hk)
     if slot_mapping.numel() != n:
@@ -111,7 +118,7 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     if key_stride == 0 or value_stride == 0:  # one row for every token
         key, value = key.contiguous(), value.contiguous()
         key_stride = value_stride = hk * HEAD_DIM
-    slots = _as_i32(_flat(slot_mapping), "slot_mapping")
+    slots = _ids(slot_mapping, "slot_mapping")
     lib = _lib.load()
     with _on(dev):
         _lib.check(lib.vox_store_kvcache_fp4(key.data_ptr(), value.data_ptr(), key_stride, value_stride,
@@ -125,7 +132,7 @@ def load_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.
     slots outside the cache."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     dev = _check_cuda(k_cache, v_cache, slots)
-    at = _as_i32(_flat(slots), "slots")
+    at = _ids(slots, "slots")
     n = at.numel()
     key, value = torch.empty(2, n, hk, HEAD_DIM, dtype=torch.bfloat16, device=dev).unbind(0)
     if n:
@@ -155,7 +162,8 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 
     With key / value ([B, HK, 128]) and slot_mapping ([B]) the step's rows are stored in the same call: the result (and the
     caches afterwards) are those of ``store_kvcache_fp4`` followed by this attention, as long as no sequence's slot lies
-    inside another sequence's context. ``plan``: as decode_attention's; planned calls of one device share a workspace and must not overlap."""
+    inside another sequence's context. ``softmax_scale`` is positive. ``plan``: as decode_attention's; planned calls of one
+    device share a workspace and must not overlap."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"decode_attention_fp4: q must be bf16 [B, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
@@ -179,7 +187,7 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         rows, key_stride, value_stride = _rows("decode_attention_fp4", key, value, hk)
         if rows != B or slot_mapping.numel() != B:
             raise ValueError(f"decode_attention_fp4: key, value and slot_mapping must hold {B} rows")
-        slots = _as_i32(_flat(slot_mapping), "slot_mapping")
+        slots = _ids(slot_mapping, "slot_mapping")
     elif value is not None or slot_mapping is not None:
         raise ValueError("decode_attention_fp4: key, value and slot_mapping go together")
     if B == 0:
@@ -216,7 +224,8 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """``ops.varlen_attention`` over 4-bit caches through a block table: q [T, H, 128] bf16 (token rows may be strided), the
     queries of sequence b the last of its cu_seqlens_k[b + 1] - cu_seqlens_k[b] cached tokens (bottom-right causal, or
     every key where ``causal`` is false); o [T, H, 128] bf16, zeros for a query that sees no key. H / HK divides 128.
-    One-query sequences run on the decode kernels where the call is mostly those. ``plan``: as decode_attention_fp4's."""
+    One-query sequences run on the decode kernels where the call is mostly those. ``softmax_scale`` and ``plan``: as
+    decode_attention_fp4's."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"varlen_attention_fp4: q must be bf16 [T, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
