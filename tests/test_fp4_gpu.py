@@ -189,25 +189,40 @@ def test_ids_past_int32_name_nothing():
 # decode
 
 
+def _reach(tables, wide, bs=BS):
+    """Tables on the GPU; wide: with columns behind them, so that they reach more than 8192 16-token steps, from where the
+    decode kernels have eight waves a workgroup instead of four."""
+    if wide:
+        cols = 8192 * 16 // (bs * len(tables)) + 1
+        tables = torch.nn.functional.pad(tables, (0, max(0, cols - tables.shape[1])), value=-1)
+    return tables.to(DEV)
+
+
+WIDE = pytest.mark.parametrize("wide", [False, True])
+
+
+@WIDE
 @pytest.mark.parametrize("heads,hk", [(16, 2), (8, 1), (16, 1), (1, 1), (2, 2), (6, 2), (5, 1)])
 @pytest.mark.parametrize("lens", [[1], [17, 0, 300], [15, 16, 31, 32, 33, 63, 64, 65, 255, 256, 257, 512, 0, 1]])
-def test_decode_matches_the_oracle(heads, hk, lens):
+def test_decode_matches_the_oracle(heads, hk, lens, wide):
     gen = _gen(heads * 100 + hk + len(lens))
     kc, vc, tables = _pool(gen, lens, hk, extra_cols=1)
     q = randn(gen, len(lens), heads, D)
     o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
-                             tables.to(DEV), SCALE)
+                             _reach(tables, wide), SCALE)
     _check(o, *_varlen(q, kc, vc, tables, [1] * len(lens), lens))
 
 
+@WIDE
 @pytest.mark.parametrize("bs", [64, 128, 192, 512])
 @pytest.mark.parametrize("batch,hi", [(3, 5000), (70, 700), (260, 90)])
-def test_decode_over_block_sizes_and_batches(bs, batch, hi):
+def test_decode_over_block_sizes_and_batches(bs, batch, hi, wide):
     gen = _gen(bs + batch)
     lens = torch.randint(1, hi, (batch,), generator=gen).tolist()
     kc, vc, tables = _pool(gen, lens, 2, bs)
     q = randn(gen, batch, 16, D)
-    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), tables.to(DEV), 0.05)
+    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV),
+                             _reach(tables, wide, bs), 0.05)
     _check(o, *_varlen(q, kc, vc, tables, [1] * batch, lens, scale=0.05))
 
 
@@ -220,14 +235,17 @@ def test_decode_of_more_sequences_than_a_launch_and_wide_tables():
     _check(o, *_varlen(q, kc, vc, tables, [1] * 700, lens))
 
 
-def test_decode_is_the_same_twice_and_with_any_workgroups():
+@WIDE
+def test_decode_is_the_same_twice_and_with_any_workgroups(wide):
     gen = _gen(8)
     lens = [3000, 40, 700, 1, 0, 2222]
     kc, vc, tables = _pool(gen, lens, 2)
     q = randn(gen, len(lens), 16, D)
-    args = (q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), tables.to(DEV), SCALE)
+    args = (q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), _reach(tables, wide), SCALE)
     a = decode_attention_fp4(*args)
     assert torch.equal(a, decode_attention_fp4(*args))
+    for plan in ("a", "a", "b", "a"):  # recorded, read back, recorded, recorded
+        assert torch.equal(a, decode_attention_fp4(*args, plan=plan))
     want = _varlen(q, kc, vc, tables, [1] * len(lens), lens)
     from voxcpm2_arabic_dialects_turbo_amd import _lib
     try:
@@ -238,7 +256,8 @@ def test_decode_is_the_same_twice_and_with_any_workgroups():
         _lib.load().vox_set_decode_workgroups(0)
 
 
-def test_decode_with_rising_scores_and_large_scales():
+@WIDE
+def test_decode_with_rising_scores_and_large_scales(wide):
     """Scores that rise along the context (the running maximum moves all the time), and values far from 1."""
     gen = _gen(9)
     lens = [900, 333]
@@ -252,11 +271,13 @@ def test_decode_with_rising_scores_and_large_scales():
     vcodes, vscales = fp4.parts(vc)
     vc = fp4.plane(vcodes, vscales + 80)  # 2^80
     q = randn(gen, 2, 16, D).abs()
-    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), tables.to(DEV), SCALE)
+    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV),
+                             _reach(tables, wide), SCALE)
     _check(o, *_varlen(q, kc, vc, tables, [1, 1], lens))
 
 
-def test_decode_masks_unmapped_blocks_and_what_lies_behind_the_context():
+@WIDE
+def test_decode_masks_unmapped_blocks_and_what_lies_behind_the_context(wide):
     """A block outside the cache has no weight; scales that are not numbers behind the context do not show."""
     gen = _gen(11)
     lens = [700, 500, 600]
@@ -270,7 +291,7 @@ def test_decode_masks_unmapped_blocks_and_what_lies_behind_the_context():
     bad = tables.clone()
     bad[0, 1], bad[1, 0], bad[2] = -1, 10 ** 6, -1
     q = randn(gen, 3, 16, D)
-    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), bad.to(DEV), SCALE)
+    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), _reach(bad, wide), SCALE)
     kv, vv = fp4.cache_values(kc), fp4.cache_values(vc)
     for b, keep in ((0, [*range(256), *range(512, 700)]), (1, [*range(256, 500)])):
         k, v = (ref.gather_pages(c, tables[b], lens[b])[keep] for c in (kv, vv))
@@ -279,8 +300,9 @@ def test_decode_masks_unmapped_blocks_and_what_lies_behind_the_context():
     assert (o[2] == 0).all()
 
 
+@WIDE
 @pytest.mark.parametrize("hk", [1, 2])
-def test_decode_with_values_that_are_not_numbers(hk):
+def test_decode_with_values_that_are_not_numbers(hk, wide):
     """A NaN group of a value row shows in its kv head's heads and its channels alone; one of a key row in its kv head's
     heads; a NaN query head in itself."""
     gen = _gen(12)
@@ -295,7 +317,8 @@ def test_decode_with_values_that_are_not_numbers(hk):
     q = randn(gen, 4, heads, D)
     q[2, 3, 77] = float("nan")
     q[3, 1, 0] = float("inf")
-    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV), tables.to(DEV), SCALE).cpu()
+    o = decode_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.tensor(lens, device=DEV),
+                             _reach(tables, wide), SCALE).cpu()
     want = torch.zeros(4, heads, D, dtype=torch.bool)
     want[0, 8 * (hk - 1):, 64:96] = True
     want[1, :8] = True
@@ -304,8 +327,9 @@ def test_decode_with_values_that_are_not_numbers(hk):
     assert torch.equal(o.isnan(), want)
 
 
+@WIDE
 @pytest.mark.parametrize("batch,hk", [(1, 2), (37, 2), (37, 1), (600, 2)])
-def test_decode_that_stores_is_store_then_decode(batch, hk):
+def test_decode_that_stores_is_store_then_decode(batch, hk, wide):
     gen = _gen(20 + batch + hk)
     lens = torch.randint(1, 600, (batch,), generator=gen).tolist()
     if batch > 3:
@@ -316,7 +340,7 @@ def test_decode_that_stores_is_store_then_decode(batch, hk):
     k, v = (rows[:, (8 + i) * hk * D:(9 + i) * hk * D].view(batch, hk, D) for i in (0, 1))
     slots = torch.tensor([ref.slot_of(tables[b], n - 1, BS) if n else -1 for b, n in enumerate(lens)], dtype=torch.int32)
     a, b = (kc.to(DEV), vc.to(DEV)), (kc.to(DEV), vc.to(DEV))
-    args = (torch.tensor(lens, dtype=torch.int32, device=DEV), tables.to(DEV), SCALE)
+    args = (torch.tensor(lens, dtype=torch.int32, device=DEV), _reach(tables, wide), SCALE)
     o = decode_attention_fp4(q, *a, *args, key=k, value=v, slot_mapping=slots.to(DEV))
     store_kvcache_fp4(k, v, *b, slots.to(DEV))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

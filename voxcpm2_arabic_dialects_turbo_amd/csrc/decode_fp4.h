@@ -12,8 +12,9 @@
 //    apart, a four-way bank conflict); the transposed reads then hand out the channels in that order, and put() writes
 //    them where they belong.
 //  * O^T += V^T P^T by 16x16x32 MFMAs, both steps at once.
-// Eight waves a workgroup: one wave's conversions, LDS reads and MFMAs wait for each other most of the time (with four,
-// VALU and MFMA were busy for under a third of it each), and two to a SIMD fill each other's gaps.
+// Eight waves a workgroup over long ranges (launch_split): one wave's conversions, LDS reads and MFMAs wait for each other
+// most of the time (with four, VALU and MFMA were busy for under a third of it each), and two to a SIMD fill each other's
+// gaps.
 // The scales are loaded as words, four a lane, and shifted where they are used: a byte load's zero extension, an
 // instruction of its own, was put behind the loads of the next chunk and waited for all of them.
 // Loads are buffer loads whose descriptor ends with the cache block and is empty for a step that is not there: nothing
@@ -42,11 +43,11 @@ struct Chunk {
   u32x4 piece;              // 8 channels: lanes [0, 16 HK) of its key row, [16 HK, 32 HK) of its value row
 };
 
-template <int HK, bool BTL>
+template <int HK, bool BTL, int NW>
 struct LdsFp4 {
   static constexpr bool kOwnWalk = true;
-  static constexpr int kNW = 8;
-  static constexpr int kGet = 1;
+  static constexpr int kNW = NW;
+  static constexpr int kGet = 8 / NW;
   static constexpr int kRoundSegs = 6;
   static constexpr bool kBtl = BTL;
   static constexpr int kBtInts = BTL ? (kBtLds > kPlanRecInts ? kBtLds : kPlanRecInts) : kPlanRecInts;
@@ -72,11 +73,13 @@ struct LdsFp4 {
       sl[kLOff + hh] = l;
     }
   }
-  __device__ __forceinline__ void get(int w, int k, bool last, int hh, int d0, f32x4 (&o)[1], float& m, float& l) const {
+  __device__ __forceinline__ void get(int w, int k, bool last, int hh, int d0, f32x4 (&o)[kGet], float& m,
+                                      float& l) const {
     const float* sl = partial(w, min(k, kRoundSegs - 2), last);  // (a pair that is none reads any slot: it is not used)
     m = sl[kMOff + hh];
     l = sl[kLOff + hh];
-    o[0] = *reinterpret_cast<const f32x4*>(&sl[hh * kD + d0]);
+#pragma unroll
+    for (int i = 0; i < kGet; ++i) o[i] = *reinterpret_cast<const f32x4*>(&sl[hh * kD + d0 + 4 * i]);
   }
 
   // Wave w's share [t_lo, t_hi) of a round, from window lane k on, the kc-th segment of the round; a partial for each

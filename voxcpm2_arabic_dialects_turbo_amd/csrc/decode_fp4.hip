@@ -8,11 +8,9 @@ namespace {
 
 using namespace dec;
 
-constexpr int kThreadsFp4 = LdsFp4<1, true>::kNW * kWave;
-
-template <int HK, bool BTL>
-__global__ __launch_bounds__(kThreadsFp4) void decode_fp4_kernel(DecodeArgs p) {
-  using LDS = LdsFp4<HK, BTL>;
+template <int HK, bool BTL, int NW>
+__global__ __launch_bounds__(NW * kWave) void decode_fp4_kernel(DecodeArgs p) {
+  using LDS = LdsFp4<HK, BTL, NW>;
   __shared__ __attribute__((aligned(16))) uint16_t s_vt[LDS::kNW * LDS::kVt];                  // per-wave V tiles (bf16)
   __shared__ __attribute__((aligned(16))) float s_slot[(LDS::kRoundSegs - 1) * kPartialFloats];  // segments' partials
   __shared__ int s_ctx[kMaxSeqPerLaunch];        // as in decode_kernel
@@ -27,19 +25,31 @@ __global__ __launch_bounds__(kThreadsFp4) void decode_fp4_kernel(DecodeArgs p) {
   decode_split<HK>(p, (int)blockIdx.x, (int)gridDim.x, L);
 }
 
+// Four waves a workgroup where the tables reach at most 8192 steps, 32 a compute unit: a short share is start-up, the
+// layout's scan and merges, and each costs less with half the waves. Beyond, eight keep the loads going (decode_fp4.h).
+// 16 query heads of 2 kv heads, four | eight waves with the merge, streams x tokens (steps the tables reach): 1 x 420 (32)
+// 11.8 | 12.7 us, 16 x 100-500 (512) 13.0 | 14.9, 64 x 500-1000 (4096) 16.6 | 18.9, 256 x 100-500 (8192) 18.8 | 20.6,
+// 16 x 4000-8000 (7936) 20.0 | 19.3, 64 x 1500-2500 (10240) 22.0 | 21.3, 150 x 1500-2500 (24000) 30.8 | 27.9,
+// 24 x 20000-32768 (49152) 48.2 | 39.0. The lengths are known on the device only. (A function of a plan's key: its record
+// and its reader take the same.)
+template <int HK, bool BTL>
+void launch_split(const DecodeArgs& a, hipStream_t stream) {
+  constexpr int kShort = 8192;
+  static_assert(kShort / (64 / kTile) <= kBtLds, "their block tables fit LDS");
+  if (BTL && (int64_t)a.batch * a.max_blocks * (a.block_size / kTile) <= kShort)
+    decode_fp4_kernel<HK, true, 4><<<dim3((unsigned)a.grid), dim3(4 * kWave), 0, stream>>>(a);
+  else
+    decode_fp4_kernel<HK, BTL, 8><<<dim3((unsigned)a.grid), dim3(8 * kWave), 0, stream>>>(a);
+}
+
 }  // namespace
 
 hipError_t launch_decode_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t stream) {
-  const dim3 grid((unsigned)a.grid);
   const bool btl = (int64_t)a.batch * a.max_blocks <= kBtLds;
-  if (num_kv_heads == 1 && btl)
-    decode_fp4_kernel<1, true><<<grid, dim3(kThreadsFp4), 0, stream>>>(a);
-  else if (num_kv_heads == 1)
-    decode_fp4_kernel<1, false><<<grid, dim3(kThreadsFp4), 0, stream>>>(a);
-  else if (btl)
-    decode_fp4_kernel<2, true><<<grid, dim3(kThreadsFp4), 0, stream>>>(a);
+  if (num_kv_heads == 1)
+    btl ? launch_split<1, true>(a, stream) : launch_split<1, false>(a, stream);
   else
-    decode_fp4_kernel<2, false><<<grid, dim3(kThreadsFp4), 0, stream>>>(a);
+    btl ? launch_split<2, true>(a, stream) : launch_split<2, false>(a, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   return launch_decode_merge_fp4(a, stream);
