@@ -443,6 +443,40 @@ def test_varlen_of_mixed_steps_takes_the_decode_kernels():
     _check(o, *_decode_ref(q[:62], kc, vc, tables, lens))
 
 
+@pytest.mark.parametrize("heads,hk", [(16, 2), (8, 1), (16, 1), (2, 1)])
+@pytest.mark.parametrize("prompts,decodes,hi", [(1, 10, 90), (2, 70, 300), (7, 200, 600), (4, 250, 330), (3, 300, 200)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_varlen_of_prompts_between_decode_rows(heads, hk, prompts, decodes, hi, causal):
+    """One launch for both kinds of rows (two past 256 sequences), few prompts and many: rows without a key, sequences
+    without a query, blocks that are none, and rows behind the last sequence, which stay as they were."""
+    gen = _gen(heads + decodes + hi)
+    n = prompts + decodes
+    new, lens = [1] * n, torch.randint(1, 500, (n,), generator=gen).tolist()
+    at = torch.randperm(n, generator=gen)[:prompts].tolist()
+    for i, b in enumerate(at):
+        new[b] = hi - 13 * i
+        lens[b] = new[b] + (0, 50, 700)[i % 3]
+    one = [b for b in range(n) if new[b] == 1]
+    lens[one[0]], new[one[1]] = 0, 0
+    kc, vc, tables = _pool(gen, lens, hk, 64)
+    bad = tables.clone()
+    bad[one[2], 0] = -1
+    lens[one[2]] = 60  # its only block is none
+    q = randn(gen, sum(new) + 5, heads, D)
+    want, tol = _varlen(q[:sum(new)], kc, vc, tables, new, lens, causal)
+    row = sum(new[:one[2]])
+    want[row] = tol[row] = 0.0
+    out = torch.full((sum(new) + 5, heads, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    assert 4 * len(q) <= n * hi  # the call is mostly decode rows
+    key = (heads, hk, n, hi, causal)
+    for plan in (None, key, key):
+        out.fill_(7.0)
+        varlen_attention_fp4(q.to(DEV), kc.to(DEV), vc.to(DEV), cu_seqlens_q=_cu(new), cu_seqlens_k=_cu(lens),
+                             max_seqlen_q=hi, block_table=bad.to(DEV), softmax_scale=SCALE, causal=causal, out=out, plan=plan)
+        _check(out[:sum(new)], want, tol)
+        assert (out[sum(new):] == 7).all()
+
+
 def test_varlen_masks_unmapped_blocks_and_values_that_are_not_numbers():
     """NaN groups show in the rows that see them, in their channels; not in rows before them, nor behind the sequence."""
     gen = _gen(33)

@@ -974,12 +974,15 @@ int vox_prefill_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cach
   // the one-query rows on the decode kernels, which spread a long context over every CU
   st = check_varlen_workspace(fn, batch, plan, workspace, workspace_bytes);
   if (st != VOX_OK) return st;
+  a.skip_single = 1;
+  const vox::DecodeArgs d = varlen_decode_args(a, q_row_stride, num_blocks, num_heads, num_kv_heads);
+  if (vox::mixed_fp4_fits(a, max_seqlen_q))
+    return hip_status(vox::launch_mixed_fp4(a, max_seqlen_q, with_workspace(d, batch, plan, workspace), s),
+                      "prefill_attn_fp4 mixed launch");
   if (max_seqlen_q > 1) {
-    a.skip_single = 1;
     st = hip_status(vox::launch_prefill_fp4(a, max_seqlen_q, s), "prefill_attn_fp4 launch");
     if (st != VOX_OK) return st;
   }
-  const vox::DecodeArgs d = varlen_decode_args(a, q_row_stride, num_blocks, num_heads, num_kv_heads);
   return launch_decode_slices(d, batch, num_kv_heads, plan, workspace, s, vox::launch_decode_fp4);
 }
 

@@ -43,12 +43,12 @@ struct Chunk {
   u32x4 piece;              // 8 channels: lanes [0, 16 HK) of its key row, [16 HK, 32 HK) of its value row
 };
 
-template <int HK, bool BTL, int NW>
+template <int HK, bool BTL, int NW, int SEGS = 6>
 struct LdsFp4 {
   static constexpr bool kOwnWalk = true;
   static constexpr int kNW = NW;
   static constexpr int kGet = 8 / NW;
-  static constexpr int kRoundSegs = 6;
+  static constexpr int kRoundSegs = SEGS;
   static constexpr bool kBtl = BTL;
   static constexpr int kBtInts = BTL ? (kBtLds > kPlanRecInts ? kBtLds : kPlanRecInts) : kPlanRecInts;
   static constexpr int VROW = kD + 32;  // elements of an LDS row: four rows' 64-byte runs, and the reads', in distinct banks

@@ -21,7 +21,7 @@
 #include <algorithm>
 #include <climits>
 
-#include "fp4_common.h"
+#include "decode_fp4.h"
 #include "vox_kernels.h"
 
 namespace vox {
@@ -44,21 +44,27 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(4))) int32_t* const_i32;
 typedef u32x4 __attribute__((aligned(8))) u32x4_a8;  // output rows are 8-byte aligned
 
+// A workgroup's LDS. s_t0 and s_t1 hold the codes of a tile each, K's, then V's (distinct arrays: the compiler can tell a
+// tile's reads from the next one's transfers in flight).
+struct Lds {
+  uint16_t* v;    // [2][kBK * kVRow]
+  uint8_t *t0, *t1;  // [2 * kTileBytes]
+  uint8_t* nan;   // [2][key][group]: a tile's scales that are not numbers
+  int* nan_at;    // [2]: the first key of the last tile that held any
+};
+
+// Query tile qt of sequence b and kv head g.
 template <int KS>
-__global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kBK * kVRow];
-  // (distinct arrays: the compiler can tell a tile's reads from the next one's transfers in flight)
-  __shared__ __attribute__((aligned(16))) uint8_t s_t0[2 * kTileBytes], s_t1[2 * kTileBytes];  // K's, then V's
-  __shared__ __attribute__((aligned(4))) uint8_t s_nan[2][kBK * 4];  // [key][group]: a tile's scales that are not numbers
-  __shared__ int s_nan_at[2];            // the first key of the last tile that held any
-  const int b = blockIdx.y, g = blockIdx.z;
+__device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g, int qt, const Lds& L) {
+  uint8_t* const s_t0 = L.t0;
+  uint8_t* const s_t1 = L.t1;
+  int* const s_nan_at = L.nan_at;
   const int q0 = p.cu_q[b], nq = p.cu_q[b + 1] - q0;
   const int HK = p.num_kv_heads;
   const int gsh = __builtin_ctz(p.group);  // the group divides 128: a power of two
   constexpr int ROWS = 128 / KS;           // query rows of the workgroup
   constexpr int KT = 2 / KS;               // 32-key blocks of a tile that a wave takes
   const int bq = ROWS >> gsh;              // query tokens of the workgroup
-  const int qt = (int)gridDim.x - 1 - (int)blockIdx.x;  // the last tile has the most keys: first
   if (qt * bq >= nq || (p.skip_single && nq == 1)) return;  // (workgroup-uniform)
   const int nk = max(0, min(p.cu_k[b + 1] - p.cu_k[b], p.max_blocks * p.block_size));
 
@@ -170,17 +176,17 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     vcodes = *reinterpret_cast<const u32x4*>(d + kTileBytes + tid * 16);
     const uint32_t b = mapped && kv0 + (tid >> 2) < nk ? (uint32_t)d[kTileBytes + kCodes + tid] : 0u;
     const bool nan = b == 255u;
-    s_nan[buf][tid] = nan;
+    L.nan[buf * (kBK * 4) + tid] = nan;
     if (__builtin_amdgcn_ballot_w64(nan) != 0) s_nan_at[buf] = kv0;
     vscale = fp4::scale_float(nan ? 0u : b);
   };
   auto piece_v = [&](int q4, int buf) {
-    *reinterpret_cast<u32x4*>(s_v[buf] + vst + q4 * 32) = fp4::values8(vcodes[q4], vscale);
+    *reinterpret_cast<u32x4*>(L.v + buf * (kBK * kVRow) + vst + q4 * 32) = fp4::values8(vcodes[q4], vscale);
   };
   uint32_t nan_groups = 0;  // byte c, bit 0: the row has seen such a key in group c
   auto mark_nan = [&](int buf, int seen) {  // seen: the tile's keys that this lane's row sees
 #pragma unroll 1
-    for (int j = 0; j < kBK; ++j) nan_groups |= j < seen ? reinterpret_cast<const uint32_t*>(s_nan[buf])[j] : 0u;
+    for (int j = 0; j < kBK; ++j) nan_groups |= j < seen ? reinterpret_cast<const uint32_t*>(L.nan + buf * (kBK * 4))[j] : 0u;
   };
   // Score MFMA i of 4 KT: key block i % KT (of the wave's), the query's high or low parts (i / KT % 2), channels
   // 64 (i / (2 KT)) + [0, 64). Its operand is piece 2 (i / (2 KT)) + h of key 32 (kh + i % KT) + col.
@@ -263,7 +269,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
         asm volatile("" : "+v"(sum));  // (here: sunk to the end of the tile, the adds would keep every e alive)
       }
     };
-    const uint16_t* vt = s_v[buf] + vtr + kh * 32 * kVRow;
+    const uint16_t* vt = L.v + buf * (kBK * kVRow) + vtr + kh * 32 * kVRow;
     u32x4 vf[4];
     auto read_v = [&](int i) {  // operand of P V MFMA i (16-key step i / 4, dims block i % 4)
       const u32x2 u0 = __builtin_bit_cast(u32x2, lds_read_tr16(vt + (16 * (i >> 2)) * kVRow + (i & 3) * 32));
@@ -360,7 +366,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   static_assert(4 / KS * 32 * kORow <= 2 * kBK * kVRow && 4 * 64 * 36 * 2 <= 2 * kBK * kVRow, "they fit the V tiles");
   __syncthreads();
   if constexpr (KS == 2) {
-    float* const sx = reinterpret_cast<float*>(s_v[0]);  // [wave][piece of 4 or (m, l)][lane]
+    float* const sx = reinterpret_cast<float*>(L.v);  // [wave][piece of 4 or (m, l)][lane]
     f32x4* const mine = reinterpret_cast<f32x4*>(sx + w * 64 * 36);
     const f32x4* const theirs = reinterpret_cast<const f32x4*>(sx + (w ^ 2) * 64 * 36);
 #pragma unroll
@@ -389,7 +395,7 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
     __syncthreads();
   }
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that sees no key: zeros
-  uint16_t* const so = s_v[0] + rg * 32 * kORow;
+  uint16_t* const so = L.v + rg * 32 * kORow;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -414,21 +420,128 @@ __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   }
 }
 
+template <int KS>
+__global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[2 * kBK * kVRow];
+  __shared__ __attribute__((aligned(16))) uint8_t s_t0[2 * kTileBytes], s_t1[2 * kTileBytes];
+  __shared__ __attribute__((aligned(4))) uint8_t s_nan[2 * kBK * 4];
+  __shared__ int s_nan_at[2];
+  // the last tile has the most keys: first
+  prefill_item<KS>(p, (int)blockIdx.y, (int)blockIdx.z, (int)gridDim.x - 1 - (int)blockIdx.x,
+                   Lds{s_v, s_t0, s_t1, s_nan, s_nan_at});
+}
+
+// ---- steps that mix prompts with decode rows, in one launch: workgroups [0, da.grid) are the decode split of the one-query
+// rows (decode_fp4.h, four waves), the others a prefill item each. The decode rows are a stream from memory, the prompts
+// chains of key tiles: side by side on a CU each has what the other leaves. Both fit a CU because the decode role's V tiles
+// lie where the prefill's do, its tables where the codes are. 16 query heads of 2 kv heads, with the merge, against a launch
+// of each: 6 prompts of 300-600 tokens and 120 decode rows over 128-1800 44.7 -> 28.5 us; 4 x 200-400 over 1000 cached and
+// 100 over 500-1500 61.0 -> 38.0; one of 40 and 8 over 100-500 18.5 -> 12.9.
+constexpr int kMixedSeqs = 256;
+
+// Item x of the launch: (sequence, kv head, query tile) in this order, the last tile of a sequence first; sequences of one
+// query have none. Every wave finds it by itself. Returns whether there is one.
+__device__ __forceinline__ bool find_item(const PrefillArgs& p, int x, int bq, int& b, int& g, int& qt) {
+  const int lane = threadIdx.x & 63;
+  int tiles[kMixedSeqs / 64];
+#pragma unroll
+  for (int i = 0; i < kMixedSeqs / 64; ++i) {
+    const int s = i * 64 + lane;
+    const int nq = s < p.batch ? p.cu_q[s + 1] - p.cu_q[s] : 0;
+    tiles[i] = nq > 1 ? (nq + bq - 1) / bq : 0;
+  }
+  const int hk = p.num_kv_heads;
+  g = x % hk;
+  int r = x / hk;  // tiles before it
+#pragma unroll
+  for (int i = 0; i < kMixedSeqs / 64; ++i) {
+    const int incl = wave_incl_scan(tiles[i], lane);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(incl > r);
+    if (past != 0) {
+      const int l = __builtin_ctzll(past);
+      b = i * 64 + l;
+      qt = __builtin_amdgcn_readlane(incl, l) - 1 - r;
+      return true;
+    }
+    r -= __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+template <int HK, int KS>
+__global__ __launch_bounds__(256, 2) void mixed_fp4_kernel(PrefillArgs pa, DecodeArgs da) {
+  using LD = dec::LdsFp4<HK, false, 4, 3>;
+  constexpr int kVs = LD::kNW * LD::kVt > 2 * kBK * kVRow ? LD::kNW * LD::kVt : 2 * kBK * kVRow;
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[kVs];
+  __shared__ __attribute__((aligned(16))) uint8_t s_t0[2 * kTileBytes], s_t1[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) float s_slot[(LD::kRoundSegs - 1) * kPartialFloats];
+  __shared__ __attribute__((aligned(4))) uint8_t s_nan[2 * kBK * 4];
+  __shared__ int s_nan_at[2];
+  static_assert((LD::kBtInts + dec::kRecTiles) * 4 <= sizeof(s_t0), "records and tile ids");
+  static_assert((4 * kMixedSeqs + 1 + 2 * LD::kNW) * 4 <= sizeof(s_t1), "the step's layout");
+  if ((int)blockIdx.x < da.grid) {
+    int* const i0 = reinterpret_cast<int*>(s_t0);
+    int* const i1 = reinterpret_cast<int*>(s_t1);
+    const LD L{s_v,
+               s_slot,
+               i1,
+               i1 + kMixedSeqs,
+               i1 + 2 * kMixedSeqs,
+               i1 + 3 * kMixedSeqs,
+               i1 + 4 * kMixedSeqs + 1,
+               i1 + 4 * kMixedSeqs + 1 + LD::kNW,
+               i0,
+               i0 + LD::kBtInts};
+    dec::decode_split<HK>(da, (int)blockIdx.x, da.grid, L);
+    return;
+  }
+  int b, g, qt;
+  if (!find_item(pa, (int)blockIdx.x - da.grid, 128 / KS / pa.group, b, g, qt)) return;
+  __builtin_amdgcn_s_setprio(1);  // the decode waves wait for memory anyway
+  prefill_item<KS>(pa, b, g, qt, Lds{s_v, s_t0, s_t1, s_nan, s_nan_at});
+}
+
+// Workgroups of `rows` query rows at most: every sequence's tiles, or one tile in part a sequence and the others full.
+int64_t most_items(const PrefillArgs& a, int max_seqlen_q, int rows) {
+  const int bq = rows / a.group;
+  return std::min((int64_t)a.batch * ((max_seqlen_q + bq - 1) / bq), a.row_limit / bq + a.batch) * a.num_kv_heads;
+}
+
 }  // namespace pf4
 
 }  // namespace
+
+bool mixed_fp4_fits(const PrefillArgs& a, int max_seqlen_q) {
+  return max_seqlen_q > 1 && a.batch <= pf4::kMixedSeqs && pf4::most_items(a, max_seqlen_q, 64) < (1 << 22);
+}
+
+hipError_t launch_mixed_fp4(const PrefillArgs& a, int max_seqlen_q, const DecodeArgs& d, hipStream_t stream) {
+  // Two waves on the same rows where the prompts (what is left of the rows without one a sequence: nearly all of these are
+  // decode rows) are at most half a workgroup a compute unit, as in launch_prefill_fp4. Prompts beside 60-100 decode rows,
+  // KS = 1 | 2, 8 query heads of one kv head: 2000 tokens (125 items) 46.3 | 39.5 us, 4 x 200-400 over 1000 (86) 36.1 |
+  // 31.4, 400 (25) 18.1 | 16.6, 3 x 1000-1500 (249) 38.0 | 46.8; 16 heads of two: 400 (50) 19.3 | 18.6, 6 x 300-600 (332)
+  // 28.5 | 35.7.
+  const bool two = a.group <= 64 && (a.row_limit - a.batch) * a.num_kv_heads <= (int64_t)pf4::kHalfChip * (128 / a.group);
+  const dim3 grid((unsigned)(d.grid + pf4::most_items(a, max_seqlen_q, two ? 64 : 128)));
+  if (a.num_kv_heads == 1)
+    two ? pf4::mixed_fp4_kernel<1, 2><<<grid, dim3(256), 0, stream>>>(a, d)
+        : pf4::mixed_fp4_kernel<1, 1><<<grid, dim3(256), 0, stream>>>(a, d);
+  else
+    two ? pf4::mixed_fp4_kernel<2, 2><<<grid, dim3(256), 0, stream>>>(a, d)
+        : pf4::mixed_fp4_kernel<2, 1><<<grid, dim3(256), 0, stream>>>(a, d);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  return launch_decode_merge_fp4(d, stream);
+}
 
 hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream) {
   // Two waves on the same rows where the launch is at most half a workgroup a compute unit: the chain of tiles is then the
   // time (16 query heads of 2 kv heads, KS = 1 | 2: 1000 tokens over 2000 cached, 126 workgroups of 128 rows, 58.6 | 47.6 us;
   // 4 x 200 over 2000, 104: 44.9 | 36.8; 100 over 300, 14: 13.4 | 11.9). From there on 64-row workgroups stage and convert
   // every tile twice as often for more than they save (156 workgroups 19.5 | 20.8 us, 298: 12.7 | 16.4, 1134: 152 | 177).
-  // At most that many workgroups: every sequence's tiles, or one tile in part a sequence and the others full.
-  const int bq = 128 / a.group;
-  const int64_t tiles = std::min((int64_t)a.batch * ((max_seqlen_q + bq - 1) / bq), a.row_limit / bq + a.batch);
   // (group 128: 64 rows would be half a token)
-  const bool two = a.group <= 64 && tiles * a.num_kv_heads <= pf4::kHalfChip;
-  const int bq_ks = two ? bq / 2 : bq;
+  const bool two = a.group <= 64 && pf4::most_items(a, max_seqlen_q, 128) <= pf4::kHalfChip;
+  const int bq_ks = (two ? 64 : 128) / a.group;
   const dim3 grid((unsigned)((max_seqlen_q + bq_ks - 1) / bq_ks), (unsigned)a.batch, (unsigned)a.num_kv_heads);
   if (two)
     pf4::prefill_fp4_kernel<2><<<grid, dim3(256), 0, stream>>>(a);

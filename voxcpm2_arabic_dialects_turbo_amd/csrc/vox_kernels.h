@@ -202,6 +202,9 @@ hipError_t launch_decode_merge_fp4(const DecodeArgs& a, hipStream_t stream);
 
 hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 
+// The same and the decode rows d of a mixed step (skip_single) in one launch, then their merge; up to 256 sequences.
+bool mixed_fp4_fits(const PrefillArgs& a, int max_seqlen_q);
+hipError_t launch_mixed_fp4(const PrefillArgs& a, int max_seqlen_q, const DecodeArgs& d, hipStream_t stream);
 // Varlen attention over 4-bit caches (paged keys, cu_seqlens; row_limit is the rows that q and out hold).
 hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 

@@ -258,7 +258,7 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         if hk <= 2 and H <= MAX_DECODE_HEADS and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q):
             if plan is None:
                 plan = getattr(_SCOPE, "key", None)
-            ws, mode = _workspace(lib, dev, B, plan, "varlen_fp4", B, mb, bt_stride, H, hk, bs)
+            ws, mode = _workspace(lib, dev, B, plan, "varlen_fp4", B, mb, bt_stride, H, hk, bs, max_seqlen_q > 1)
         _lib.check(lib.vox_prefill_attn_fp4(q.data_ptr(), _row_stride(q), k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs,
                                             bt.data_ptr(), bt_stride, mb, cu_q.data_ptr(), cu_k.data_ptr(), B,
                                             int(max_seqlen_q), T, H, hk, D, float(softmax_scale), 1 if causal else 0,
