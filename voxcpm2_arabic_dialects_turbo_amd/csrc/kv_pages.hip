@@ -4,7 +4,11 @@
 // lie one behind the other, kv[plane][block].
 //
 // Everything is a copy, bound by HBM (each byte read and written once) once it is more than a launch: a workgroup moves
-// 16 KB, each lane four 16-byte pieces whose loads are issued before the first store.
+// 16 KB, each lane four 16-byte pieces whose loads are issued before the first store, without a branch where the chunk is
+// whole. 12 layers of 2 kv heads in bf16, 604 MB moved by a compaction: 131 us with its plan (7 us), 4.9 TB/s, the rate of
+// a large copy; 156 us with branches around each piece and stores that stay in the caches. 28 layers, 32 children of 24
+// parents, 252 MB: 43.5 us (a parent's block is read from memory once for all its children), 59 us so. Two pieces a lane 45.0
+// us, eight 42.3; 4096 workgroups for the moves in place of 2048: the same.
 #include "vox_common.h"
 #include "vox_kernels.h"
 
@@ -20,35 +24,43 @@ __device__ __forceinline__ int64_t block_bytes(const PagesArgs& a) {
   return (int64_t)a.block_size * (a.slot_bytes + a.scale_bytes);
 }
 
-// Bytes [base, base + kChunkBytes) of the first `bytes` bytes of a run.
+// Bytes [base, base + kChunkBytes) of the first `bytes` bytes of a run. Non-temporal stores: they need not displace what
+// is in the caches (ONCE: nor do the loads, of blocks that nothing reads again).
+template <bool ONCE>
 __device__ __forceinline__ void copy_chunk(uint8_t* dst, const uint8_t* src, int64_t bytes, int64_t base) {
-  u32x4 v[kPerLanePages];
+  const auto load = [](const uint8_t* x) {
+    return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x)) : ld_g16(x);
+  };
+  const auto store = [](uint8_t* x, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(x)); };
+  const int at = (int)threadIdx.x * 16;
+  if (base + kChunkBytes <= bytes) {  // workgroup-uniform
+    u32x4 v[kPerLanePages];
 #pragma unroll
-  for (int i = 0; i < kPerLanePages; ++i) {
-    const int64_t off = base + (i * kThreadsPages + (int)threadIdx.x) * 16;
-    if (off + 16 <= bytes) v[i] = ld_g16(src + off);
+    for (int i = 0; i < kPerLanePages; ++i) v[i] = load(src + base + i * kThreadsPages * 16 + at);
+#pragma unroll
+    for (int i = 0; i < kPerLanePages; ++i) store(dst + base + i * kThreadsPages * 16 + at, v[i]);
+    return;
   }
-#pragma unroll
-  for (int i = 0; i < kPerLanePages; ++i) {
-    const int64_t off = base + (i * kThreadsPages + (int)threadIdx.x) * 16;
+  for (int64_t off = base + at; off < bytes; off += kThreadsPages * 16) {
     if (off + 16 <= bytes)
-      *reinterpret_cast<u32x4*>(dst + off) = v[i];
+      store(dst + off, load(src + off));
     else
-      for (int64_t k = off; k < bytes; ++k) dst[k] = src[k];  // a run's last bytes (off < bytes: one lane's)
+      for (int64_t k = off; k < bytes; ++k) dst[k] = src[k];  // a run's last bytes: one lane's
   }
 }
 
 // Chunk `chunk` of the first n slots of block src, to block dst: the slots' chunks first, then the scales'.
+template <bool ONCE>
 __device__ __forceinline__ void copy_slots(const PagesArgs& a, int64_t plane, int src, int dst, int n, int chunk) {
   const int64_t bb = block_bytes(a);
   const uint8_t* s = a.kv + (plane * a.num_blocks + src) * bb;
   uint8_t* d = a.kv + (plane * a.num_blocks + dst) * bb;
   const int slot_chunks = (int)(((int64_t)a.block_size * a.slot_bytes + kChunkBytes - 1) / kChunkBytes);
   if (chunk < slot_chunks) {
-    copy_chunk(d, s, (int64_t)n * a.slot_bytes, (int64_t)chunk * kChunkBytes);
+    copy_chunk<ONCE>(d, s, (int64_t)n * a.slot_bytes, (int64_t)chunk * kChunkBytes);
   } else {
     const int64_t at = (int64_t)a.block_size * a.slot_bytes;
-    copy_chunk(d + at, s + at, (int64_t)n * a.scale_bytes, (int64_t)(chunk - slot_chunks) * kChunkBytes);
+    copy_chunk<ONCE>(d + at, s + at, (int64_t)n * a.scale_bytes, (int64_t)(chunk - slot_chunks) * kChunkBytes);
   }
 }
 
@@ -64,7 +76,7 @@ __global__ __launch_bounds__(kThreadsPages) void copy_entries_kernel(PagesArgs a
   const int e = blockIdx.x;
   const int src = entries[3 * e], dst = entries[3 * e + 1], n = min(entries[3 * e + 2], a.block_size);
   if (n <= 0 || src < 0 || src >= a.num_blocks || dst < 0 || dst >= a.num_blocks) return;
-  copy_slots(a, blockIdx.y, src, dst, n, (int)blockIdx.z);
+  copy_slots<false>(a, blockIdx.y, src, dst, n, (int)blockIdx.z);
 }
 
 // Fork i: the child of row parents[i] shares its full blocks and has the copy new_blocks[i] of its last, partly filled
@@ -83,7 +95,7 @@ __global__ __launch_bounds__(kThreadsPages) void fork_kernel(PagesArgs a, ForkAr
       f.child_tables[(int64_t)i * f.max_blocks + c] = c < full ? row[c] : (c == full && copies ? fresh : -1);
     if (threadIdx.x == 0) f.child_lens[i] = len;
   }
-  if (copies && fresh != src) copy_slots(a, blockIdx.y, src, fresh, tail, (int)blockIdx.z);
+  if (copies && fresh != src) copy_slots<false>(a, blockIdx.y, src, fresh, tail, (int)blockIdx.z);
 }
 
 // ---- compaction
@@ -175,7 +187,7 @@ __global__ __launch_bounds__(kThreadsPages) void compact_copy_kernel(PagesArgs a
   for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
     const int64_t r = x / per, rest = x - r * per;
     const int64_t plane = rest / chunks;
-    copy_slots(a, plane, c.moves[1 + 2 * r], c.moves[2 + 2 * r], a.block_size, (int)(rest - plane * chunks));
+    copy_slots<true>(a, plane, c.moves[1 + 2 * r], c.moves[2 + 2 * r], a.block_size, (int)(rest - plane * chunks));
   }
 }
 
