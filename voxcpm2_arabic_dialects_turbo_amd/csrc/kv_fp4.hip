@@ -9,7 +9,8 @@
 // A thread takes 8 channels: one 16-byte load, so a wave reads 1 KB runs; the four lanes of a 32-channel group agree on
 // the largest magnitude by two DPP steps and each writes 4 bytes of codes (the lane that starts the group also its
 // scale). Flattened over (token, K / V, piece); bound by the launch at a step's rows and by HBM beyond: 512 HK bytes
-// read and 136 HK written a token.
+// read and 136 HK written a token. 8 rows of 2 kv heads: 2.0 us to store, 2.0 to load; 60001 rows (78 MB each way): 19.0 us
+// (4.1 TB/s) and 17.3 us (4.5 TB/s).
 #include "fp4_common.h"
 #include "vox_kernels.h"
 

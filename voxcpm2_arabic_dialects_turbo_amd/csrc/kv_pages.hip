@@ -5,8 +5,8 @@
 //
 // Everything is a copy, bound by HBM (each byte read and written once) once it is more than a launch: a workgroup moves
 // 16 KB, each lane four 16-byte pieces whose loads are issued before the first store, without a branch where the chunk is
-// whole. 12 layers of 2 kv heads in bf16, 604 MB moved by a compaction: 131 us with its plan (7 us), 4.9 TB/s, the rate of
-// a large copy; 156 us with branches around each piece and stores that stay in the caches. 28 layers, 32 children of 24
+// whole. 12 layers of 2 kv heads in bf16, 604 MB moved by a compaction: 126-131 us with its plan (6), 4.9-5.0 TB/s, the
+// rate of a large copy; 156 us with branches around each piece and stores that stay in the caches. 28 layers, 32 children of 24
 // parents, 252 MB: 43.5 us (a parent's block is read from memory once for all its children), 59 us so. Two pieces a lane 45.0
 // us, eight 42.3; 4096 workgroups for the moves in place of 2048: the same.
 #include "vox_common.h"
