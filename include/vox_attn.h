@@ -302,7 +302,8 @@ int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* k
 
 /* vox_prefill_attn over 4-bit caches through block tables, with cu_seqlens. num_tokens: the rows that q and out hold; rows
  * at or past it are neither read nor written by the prefill kernel. plan, workspace: as vox_prefill_attn's (with the
- * workspace the one-query sequences run on the decode kernels). num_heads / num_kv_heads divides 128, softmax_scale is
+ * workspace the one-query sequences run on the decode kernels, up to 256 sequences in the same launch). num_heads /
+ * num_kv_heads divides 128, softmax_scale is
  * positive. */
 int vox_prefill_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                          int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,

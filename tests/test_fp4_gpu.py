@@ -16,6 +16,7 @@ from oracle import fp4
 from tests._util import paged_pool, randn
 from voxcpm2_arabic_dialects_turbo_amd import ops, runner
 from voxcpm2_arabic_dialects_turbo_amd.context import reset_context
+from voxcpm2_arabic_dialects_turbo_amd.kernels import kv_pages
 from voxcpm2_arabic_dialects_turbo_amd.layers import Attention
 from voxcpm2_arabic_dialects_turbo_amd.ops_fp4 import (decode_attention_fp4, fp4_parts, load_kvcache_fp4,
                                                        store_kvcache_fp4, varlen_attention_fp4)
@@ -654,6 +655,67 @@ def test_engine_steps_through_attention_forward(hk):
                 assert (outs[i][2:] == 0).all()
     finally:
         reset_context()
+
+
+def test_streams_forked_and_compacted_between_steps():
+    """Two prompts stored in two layers, forked into takes, decode steps that store, a step that mixes a new prompt with
+    them, some takes freed and the pool compacted: every output against what the cache holds, the last step's again
+    bit for bit after the compaction."""
+    gen = _gen(51)
+    heads, hk, blocks, cols = 16, 2, 24, 6
+    layers = [Attention(heads, D, SCALE, hk) for _ in range(2)]
+    kv = runner.allocate_kv_cache(layers, blocks, BS, dtype=torch.float4_e2m1fn_x2, device=DEV)
+    kv.random_(0, 120)  # (no scale that is none)
+    tables = torch.full((2, cols), -1, dtype=torch.int32)
+    tables[0, :3], tables[1, :2] = torch.tensor([21, 4, 17]), torch.tensor([9, 23])
+    lens = [600, 300]
+
+    def rows(n):
+        x = randn(gen, 2, n, heads + 2 * hk, D).to(DEV)
+        return [(x[i, :, :heads], x[i, :, heads:heads + hk], x[i, :, heads + hk:]) for i in range(2)]
+
+    def slots(tables, new, lens):
+        return torch.tensor([ref.slot_of(tables[b], j, BS) for b, (n, m) in enumerate(zip(new, lens)) for j in range(m - n, m)],
+                            dtype=torch.int32, device=DEV)
+
+    def step(tables, new, lens, r):
+        outs = []
+        for i, (q, k, v) in enumerate(r):
+            kc, vc = kv[i, 0], kv[i, 1]
+            if max(new) == 1:
+                o = decode_attention_fp4(q, kc, vc, torch.tensor(lens, device=DEV), tables.to(DEV), SCALE, key=k, value=v,
+                                         slot_mapping=slots(tables, new, lens), plan=(*lens, *tables.flatten().tolist()))
+            else:
+                store_kvcache_fp4(k, v, kc, vc, slots(tables, new, lens))
+                o = varlen_attention_fp4(q, kc, vc, cu_seqlens_q=_cu(new), cu_seqlens_k=_cu(lens), max_seqlen_q=max(new),
+                                         block_table=tables.to(DEV), softmax_scale=SCALE)
+            _check(o, *_varlen(q.cpu(), kc.cpu(), vc.cpu(), tables, new, lens))
+            outs.append(o)
+        return outs
+
+    step(tables, lens, lens, rows(900))
+    ct, cl = kv_pages.fork_kv_blocks(kv, tables.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                     torch.tensor([0, 1, 0], device=DEV), torch.tensor([1, 2, 3], device=DEV))
+    assert cl.tolist() == [600, 300, 600]
+    tables, lens = torch.cat([tables, ct.cpu()]), lens + cl.tolist()
+    for _ in range(2):
+        lens = [n + 1 for n in lens]
+        step(tables, [1] * 5, lens, rows(5))
+    tables = torch.cat([tables, torch.tensor([[11, 12] + [-1] * (cols - 2)], dtype=torch.int32)])
+    lens = [n + 1 for n in lens] + [280]
+    assert 4 * 285 <= 6 * 280
+    step(tables, [1] * 5 + [280], lens, rows(285))
+    keep = [0, 2, 3, 5]
+    tables, lens = tables[keep], [lens[b] for b in keep]
+    lens = [n + 1 for n in lens]
+    r = rows(4)
+    before = step(tables, [1] * 4, lens, r)
+    moved, remap, live = kv_pages.compact_kv_blocks(kv, tables.to(DEV), torch.tensor(lens, device=DEV))
+    moved = moved.cpu()
+    assert int(live) == len({b for row in tables.tolist() for b in row if b >= 0}) == moved.max() + 1
+    assert ((moved < 0) == (tables < 0)).all() and torch.equal(moved[0, :2], moved[1, :2])  # (children share full blocks)
+    for a, b in zip(before, step(moved, [1] * 4, lens, r)):
+        assert torch.equal(a, b)
 
 
 def test_calls_on_two_streams_do_not_share_scratch():

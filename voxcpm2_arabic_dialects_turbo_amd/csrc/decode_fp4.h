@@ -327,7 +327,7 @@ struct LdsFp4 {
         x[i] = fast_exp2(fmaf(x[i], c, -mu));
         lsum += x[i];
       }
-      // P^T in bf16 (rounded by 2^-9, as the output is): k-slots 4 s + i = token 16 s + 4 jq + i
+      // P^T in bf16 (off by at most 2^-8 of each, as the output is): k-slots 4 s + i = token 16 s + 4 jq + i
       u32x4 pv;
 #pragma unroll
       for (int i = 0; i < 4; ++i) pv[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);

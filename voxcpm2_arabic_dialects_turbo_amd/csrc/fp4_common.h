@@ -88,7 +88,7 @@ __device__ __forceinline__ u32x4 values8(uint32_t codes, float scale) {
 //   32x32x64: A[l % 32][32 (l / 32) + [0, 32)]; B[16 (l / 32) + [0, 16)][l % 32] and B[32 + 16 (l / 32) + [0, 16)]. D as
 //   in mfma_32x32x16.
 // The products are exact and the sum is held in fp32; with a score's 128 terms it is off by 2^-18 of the score's size in
-// the mean (measured over normal q and K), where the bf16 probabilities are rounded by 2^-9.
+// the mean (measured over normal q and K), where the bf16 probabilities are off by up to 2^-8.
 __device__ __forceinline__ f32x4 mfma_scores16(u32x4 a, uint32_t sa, i32x8 b, uint32_t sb, f32x4 c) {
   const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, b, c, 4, 0, 0, (int)sa, 0, (int)sb);

@@ -17,8 +17,8 @@
 //    step s being key 16 s + 8 (e / 4) + 4 h + e % 4, and the transposed reads gather the same keys.
 // A tile's codes (8.5 KB, K and V) go from memory straight into LDS, a quarter by each wave. A tile's softmax and P V run
 // beside the next tile's scores and V conversion (step), while the codes of the tile after that are on their way (three
-// tiles ahead gave nothing). Probabilities are rounded to bf16 for the MFMA (by 2^-9 of each, as the output is); scores,
-// maxima, sums and O are fp32.
+// tiles ahead gave nothing). Probabilities are rounded to bf16 for the MFMA (off by at most 2^-8 of each, as the output
+// is); scores, maxima, sums and O are fp32.
 // A tile's time is its instructions: about 1.1 us for a wave alone on its SIMD with KS = 1, 0.87 with KS = 2, so short
 // prompts are bound by the chain of their tiles (44 x 33-59 tokens over 50 cached: 12.4 us), long ones by MFMA and VALU
 // issue: 16 query heads of 2 kv heads, 6 x 1000-2000 over 1500-2500 cached (0.214 PFLOP) 211-223 us, 0.96-1.02 PFLOP/s, where a
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void mixed_fp4_kernel(PrefillArgs pa, Decod
 
 // Workgroups of `rows` query rows at most: every sequence's tiles, or one tile in part a sequence and the others full.
 int64_t most_items(const PrefillArgs& a, int max_seqlen_q, int rows) {
-  const int bq = rows / a.group;
+  const int bq = std::max(1, rows / a.group);
   return std::min((int64_t)a.batch * ((max_seqlen_q + bq - 1) / bq), a.row_limit / bq + a.batch) * a.num_kv_heads;
 }
 
