@@ -405,17 +405,21 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     // ---- block table into LDS and the step layout (a block-wide prefix sum over ceil(context / 16)). The lengths
     // of the first kNT sequences and every table entry a thread stages are loaded before any of them is waited
     // for: one round trip (a load-then-store loop waits for each load in turn, one round trip per kNT entries).
+    // (kOwnWalk: up to 64 sequences every wave reads them all and lays them out by itself, without LDS; 4-bit caches, with
+    // the merge: one stream of 420 tokens 11.8 -> 11.2 us, 40 of 200-1500 14.5 -> 13.9, 24 of 20000-32768 40.8 -> 39.7)
+    const bool by_wave = LDS::kOwnWalk && p.batch <= kWave;
+    const int mine = by_wave ? lane : tid;
     int l0 = 0, l1 = 0, l2 = 0, l3 = 0, slot_first = -1;
-    if (tid < p.batch) {
+    if (mine < p.batch) {
       if (varlen) {
-        l0 = p.cu_q[tid];
-        l1 = p.cu_q[tid + 1];
-        l2 = p.cu_k[tid];
-        l3 = p.cu_k[tid + 1];
+        l0 = p.cu_q[mine];
+        l1 = p.cu_q[mine + 1];
+        l2 = p.cu_k[mine];
+        l3 = p.cu_k[mine + 1];
       } else {
-        l2 = p.context_lens[tid];
+        l2 = p.context_lens[mine];
       }
-      if (store && !varlen) slot_first = p.slot_mapping[tid];  // (varlen mode finds the new token by position)
+      if (store && !varlen) slot_first = p.slot_mapping[mine];  // (varlen mode finds the new token by position)
     }
     if constexpr (BTL) {
       constexpr int kPer = (kBtLds + kNT - 1) / kNT;  // entries per thread at most
@@ -439,70 +443,95 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       for (int j = 0; j < kPer; ++j)
         if (tid + j * kNT < nbt) s_bt[tid + j * kNT] = vals[j];
     }
-    const int row_first = varlen ? l0 : tid;
+    const int row_first = varlen ? l0 : mine;
     const int ctx_first = !varlen ? l2 : (l1 - l0 == 1 ? l3 - l2 : 0);
     int run = 0;
     int nmax = 0;  // most steps of one sequence
-    for (int base = 0; base < p.batch; base += kNT) {
-      const int bb = base + tid;
-      int row = row_first;
-      const int raw = base == 0 ? ctx_first : (bb < p.batch ? seq_of(bb, row) : 0);
-      const int ctx = bb < p.batch ? max(0, min(raw, max_ctx)) : 0;
-      const int n = (ctx + kTile - 1) / kTile;
-      const int incl = wave_incl_scan(n, lane);
-      int wmax = n;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) wmax = max(wmax, __shfl_xor(wmax, o, kWave));
-      if (lane == kWave - 1) {
-        L.wtot[w] = incl;
-        L.wmax[w] = wmax;
-      }
-      __syncthreads();
-      int before = 0, total = 0;
-#pragma unroll
-      for (int ww = 0; ww < kNW; ++ww) {
-        before += ww < w ? L.wtot[ww] : 0;
-        total += L.wtot[ww];
-        nmax = max(nmax, L.wmax[ww]);
-      }
-      if (bb < p.batch) {
-        L.ctx[bb] = ctx;
-        if (store) L.snew[bb] = varlen ? -1 : base == 0 ? slot_first : p.slot_mapping[bb];
-        L.row[bb] = row;
-        L.start[bb] = run + before + incl - n;
-      }
-      run += total;
-      __syncthreads();
-    }
-    if (tid == 0) L.start[p.batch] = run;
-    __syncthreads();
-    S = uniform(run);
-    nmax = uniform(nmax);
     bool same = false;  // every sequence that has steps has nmax of them (looked at where it matters)
-    if (nmax <= kNW) {
-      bool other = false;
-      for (int bb = tid; bb < p.batch; bb += kNT) {
-        const int n = L.start[bb + 1] - L.start[bb];
-        other = other || (n != 0 && n != nmax);
+    if (by_wave) {
+      w_ctx = max(0, min(ctx_first, max_ctx));
+      const int n = (w_ctx + kTile - 1) / kTile;
+      w_en = wave_incl_scan_dpp(n);
+      w_st = w_en - n;
+      w_row = row_first;
+      w_snew = slot_first;
+      S = lane_val(w_en, kWave - 1);
+      nmax = wave_max_dpp(n);
+      same = nmax <= kNW && __builtin_amdgcn_ballot_w64(n != 0 && n != nmax) == 0;
+      G = active_workgroups<kNW>(grid, S, nmax, same, p.batch);
+      if (g == 0 && w == 0) {
+        if (lane < p.batch) p.steps[lane] = w_st;
+        if (lane == 0) {
+          p.steps[p.batch] = S;
+          p.steps[p.batch + 1] = G;
+        }
       }
-      const uint64_t others = __builtin_amdgcn_ballot_w64(other);
-      if (lane == 0) L.wmax[w] = others != 0;
+      if (g < G) {
+        r1 = (int)muldiv(g + 1, S, 0, G);
+        r = (int)muldiv(g, S, 0, G);
+      }
+      if constexpr (BTL) __syncthreads();  // the block table
+    } else {
+      for (int base = 0; base < p.batch; base += kNT) {
+        const int bb = base + tid;
+        int row = row_first;
+        const int raw = base == 0 ? ctx_first : (bb < p.batch ? seq_of(bb, row) : 0);
+        const int ctx = bb < p.batch ? max(0, min(raw, max_ctx)) : 0;
+        const int n = (ctx + kTile - 1) / kTile;
+        const int incl = wave_incl_scan(n, lane);
+        int wmax = n;
+  #pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) wmax = max(wmax, __shfl_xor(wmax, o, kWave));
+        if (lane == kWave - 1) {
+          L.wtot[w] = incl;
+          L.wmax[w] = wmax;
+        }
+        __syncthreads();
+        int before = 0, total = 0;
+  #pragma unroll
+        for (int ww = 0; ww < kNW; ++ww) {
+          before += ww < w ? L.wtot[ww] : 0;
+          total += L.wtot[ww];
+          nmax = max(nmax, L.wmax[ww]);
+        }
+        if (bb < p.batch) {
+          L.ctx[bb] = ctx;
+          if (store) L.snew[bb] = varlen ? -1 : base == 0 ? slot_first : p.slot_mapping[bb];
+          L.row[bb] = row;
+          L.start[bb] = run + before + incl - n;
+        }
+        run += total;
+        __syncthreads();
+      }
+      if (tid == 0) L.start[p.batch] = run;
       __syncthreads();
-      int others_any = 0;
-#pragma unroll
-      for (int ww = 0; ww < kNW; ++ww) others_any |= L.wmax[ww];
-      same = uniform(others_any) == 0;
-    }
-    G = active_workgroups<kNW>(grid, S, nmax, same, p.batch);
-    if (g == 0) {  // the layout decode_merge_kernel reads, then the active workgroup count (a record keeps it)
-      for (int i = tid; i <= p.batch; i += kNT) p.steps[i] = L.start[i];
-      if (tid == 0) p.steps[p.batch + 1] = G;
-    }
-    if (g < G) {
-      r1 = (int)muldiv(g + 1, S, 0, G);
-      r = (int)muldiv(g, S, 0, G);
-      wb = seq_at(r);
-      load_window();
+      S = uniform(run);
+      nmax = uniform(nmax);
+      if (nmax <= kNW) {
+        bool other = false;
+        for (int bb = tid; bb < p.batch; bb += kNT) {
+          const int n = L.start[bb + 1] - L.start[bb];
+          other = other || (n != 0 && n != nmax);
+        }
+        const uint64_t others = __builtin_amdgcn_ballot_w64(other);
+        if (lane == 0) L.wmax[w] = others != 0;
+        __syncthreads();
+        int others_any = 0;
+  #pragma unroll
+        for (int ww = 0; ww < kNW; ++ww) others_any |= L.wmax[ww];
+        same = uniform(others_any) == 0;
+      }
+      G = active_workgroups<kNW>(grid, S, nmax, same, p.batch);
+      if (g == 0) {  // the layout decode_merge_kernel reads, then the active workgroup count (a record keeps it)
+        for (int i = tid; i <= p.batch; i += kNT) p.steps[i] = L.start[i];
+        if (tid == 0) p.steps[p.batch + 1] = G;
+      }
+      if (g < G) {
+        r1 = (int)muldiv(g + 1, S, 0, G);
+        r = (int)muldiv(g, S, 0, G);
+        wb = seq_at(r);
+        load_window();
+      }
     }
     // record mode: the record covers the range when the window reaches past it and the range's tiles fit. An active
     // workgroup collects its tiles' block ids in LDS and writes the record when its range is done: a global store
