@@ -478,17 +478,21 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
         const int raw = base == 0 ? ctx_first : (bb < p.batch ? seq_of(bb, row) : 0);
         const int ctx = bb < p.batch ? max(0, min(raw, max_ctx)) : 0;
         const int n = (ctx + kTile - 1) / kTile;
-        const int incl = wave_incl_scan(n, lane);
+        const int incl = LDS::kOwnWalk ? wave_incl_scan_dpp(n) : wave_incl_scan(n, lane);
         int wmax = n;
-  #pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) wmax = max(wmax, __shfl_xor(wmax, o, kWave));
+        if constexpr (LDS::kOwnWalk) {
+          wmax = wave_max_dpp(n);
+        } else {
+#pragma unroll
+          for (int o = 1; o < kWave; o <<= 1) wmax = max(wmax, __shfl_xor(wmax, o, kWave));
+        }
         if (lane == kWave - 1) {
           L.wtot[w] = incl;
           L.wmax[w] = wmax;
         }
         __syncthreads();
         int before = 0, total = 0;
-  #pragma unroll
+#pragma unroll
         for (int ww = 0; ww < kNW; ++ww) {
           before += ww < w ? L.wtot[ww] : 0;
           total += L.wtot[ww];
@@ -517,7 +521,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
         if (lane == 0) L.wmax[w] = others != 0;
         __syncthreads();
         int others_any = 0;
-  #pragma unroll
+#pragma unroll
         for (int ww = 0; ww < kNW; ++ww) others_any |= L.wmax[ww];
         same = uniform(others_any) == 0;
       }

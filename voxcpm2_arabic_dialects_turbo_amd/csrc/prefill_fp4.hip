@@ -460,7 +460,7 @@ __device__ __forceinline__ bool find_item(const PrefillArgs& p, int x, int bq, i
   int r = x / hk;  // tiles before it
 #pragma unroll
   for (int i = 0; i < kMixedSeqs / 64; ++i) {
-    const int incl = wave_incl_scan(tiles[i], lane);
+    const int incl = wave_incl_scan_dpp(tiles[i]);
     const uint64_t past = __builtin_amdgcn_ballot_w64(incl > r);
     if (past != 0) {
       const int l = __builtin_ctzll(past);
