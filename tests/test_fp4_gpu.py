@@ -204,7 +204,7 @@ WIDE = pytest.mark.parametrize("wide", [False, True])
 
 @WIDE
 @pytest.mark.parametrize("heads,hk", [(16, 2), (8, 1), (16, 1), (1, 1), (2, 2), (6, 2), (5, 1)])
-@pytest.mark.parametrize("lens", [[1], [17, 0, 300], [15, 16, 31, 32, 33, 63, 64, 65, 255, 256, 257, 512, 0, 1]])
+@pytest.mark.parametrize("lens", [[1], [0], [0, 0, 0], [17, 0, 300], [15, 16, 31, 32, 33, 63, 64, 65, 255, 256, 257, 512, 0, 1]])
 def test_decode_matches_the_oracle(heads, hk, lens, wide):
     gen = _gen(heads * 100 + hk + len(lens))
     kc, vc, tables = _pool(gen, lens, hk, extra_cols=1)

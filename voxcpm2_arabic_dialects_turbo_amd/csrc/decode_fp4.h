@@ -13,8 +13,8 @@
 //    them where they belong.
 //  * O^T += V^T P^T by 16x16x32 MFMAs, both steps at once.
 // 136 HK bytes a key: bound by HBM over long contexts (24 streams of 20000-32768 tokens, 177 MB: 36-40 us, 4.4-4.9 TB/s; the
-// bf16 cache's kernel takes 107 us), by the fixed costs over short ones (one of 420: 8.5 us, of which start and layout 4.4,
-// the first round trip 3, the merge of the waves 1.7; 150 of 256-2048, 46 MB: 22 us). A chunk's key loads sent ahead of its
+// bf16 cache's kernel takes 107 us), by fixed costs over short ones: start, layout, one round trip of loads and the merge of
+// the waves (one of 420: 7.9 us; 150 of 256-2048, 46 MB: 22 us). A chunk's key loads sent ahead of its
 // softmax, the values' one head at a time, in place of all at its end: 25.4 -> 26.3 us and 41 -> 42.7 with the merge.
 // Eight waves a workgroup over long ranges (launch_split): one wave's conversions, LDS reads and MFMAs wait for each other
 // most of the time (with four, VALU and MFMA were busy for under a third of it each), and two to a SIMD fill each other's

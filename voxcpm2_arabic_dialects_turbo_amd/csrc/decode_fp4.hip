@@ -28,9 +28,9 @@ __global__ __launch_bounds__(NW * kWave) void decode_fp4_kernel(DecodeArgs p) {
 // Four waves a workgroup where the tables reach at most 8192 steps, 32 a compute unit: a short share is start-up, the
 // layout's scan and merges, and each costs less with half the waves. Beyond, eight keep the loads going (decode_fp4.h).
 // 16 query heads of 2 kv heads, four | eight waves with the merge, streams x tokens (steps the tables reach): 1 x 420 (32)
-// 11.8 | 12.7 us, 16 x 100-500 (512) 13.0 | 14.9, 64 x 500-1000 (4096) 16.6 | 18.9, 256 x 100-500 (8192) 18.8 | 20.6,
-// 16 x 4000-8000 (7936) 20.0 | 19.3, 64 x 1500-2500 (10240) 22.0 | 21.3, 150 x 1500-2500 (24000) 30.8 | 27.9,
-// 24 x 20000-32768 (49152) 48.2 | 39.0. The lengths are known on the device only. (A function of a plan's key: its record
+// 11.2 | 11.9 us, 16 x 100-500 (512) 12.3 | 14.1, 64 x 500-1000 (4096) 15.8 | 18.1, 256 x 100-500 (8192) 18.9 | 20.3,
+// 16 x 4000-8000 (7936) 19.4 | 19.2, 64 x 1500-2500 (10240) 21.3 | 20.7, 150 x 1500-2500 (24000) 30.5 | 27.5,
+// 24 x 20000-32768 (49152) 47.5 | 38.4. The lengths are known on the device only. (A function of a plan's key: its record
 // and its reader take the same.)
 template <int HK, bool BTL>
 void launch_split(const DecodeArgs& a, hipStream_t stream) {
