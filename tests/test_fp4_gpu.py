@@ -718,6 +718,66 @@ def test_streams_forked_and_compacted_between_steps():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("seed", range(30))
+def test_random_steps(seed):
+    """Decode, prefill and mixed steps of random head layouts, block sizes, lengths, strides, unmapped blocks, table widths
+    and decode grids, planned or not, causal or not."""
+    from voxcpm2_arabic_dialects_turbo_amd import _lib
+    gen = _gen(7000 + seed)
+
+    def pick(*of):
+        return of[int(torch.randint(0, len(of), (1,), generator=gen))]
+
+    heads, hk = pick((16, 2), (8, 1), (16, 1), (4, 2), (2, 2), (1, 1), (8, 2))
+    bs, kind, wgs = pick(64, 128, 256, 320), pick("decode", "store", "varlen", "mixed"), pick(0, 0, 0, 3, 77, 1000)
+    n = pick(1, 2, 9, 33, 65, 130, 280)
+    top = pick(20, 90, 700, 3000) if n < 60 else pick(20, 90, 400)
+    lens = torch.randint(0, top + 1, (n,), generator=gen).tolist()
+    new = [1] * n
+    if kind == "varlen":
+        new = torch.randint(0, pick(3, 40, 200), (n,), generator=gen).tolist()
+    elif kind == "mixed":
+        new[int(torch.randint(0, n, (1,), generator=gen))] = pick(2, 31, 257)
+    if kind == "store" and heads // hk > 8:
+        kind = "decode"
+    lens = [max(a, b) if pick(True, True, False) or kind == "store" else b for a, b in zip(new, lens)]
+    kc, vc, tables = _pool(gen, lens, hk, bs, extra_cols=pick(0, 1, 40))
+    scale = pick(SCALE, 0.02, 0.3)
+    causal = pick(True, True, False) if kind in ("varlen", "mixed") else True
+    t = sum(new)
+    pad = pick(0, 3)
+    q = randn(gen, max(t, 1) + pad, heads * D + pick(0, 2 * hk * D))[:, :heads * D].unflatten(1, (heads, D))
+    qd, kd, vd = q.to(DEV), kc.to(DEV), vc.to(DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    plans = (None, ("random", seed), ("random", seed))
+    try:
+        if wgs:
+            _lib.load().vox_set_decode_workgroups(wgs)
+        for plan in plans:
+            if kind in ("decode", "store"):
+                kw = {}
+                if kind == "store":
+                    rows = randn(gen, n, 2 * hk * D).to(DEV)
+                    k, v = rows[:, :hk * D].unflatten(1, (hk, D)), rows[:, hk * D:].unflatten(1, (hk, D))
+                    slots = torch.tensor([ref.slot_of(tables[b], m - 1, bs) if m else -1 for b, m in enumerate(lens)],
+                                         dtype=torch.int32, device=DEV)
+                    kw = dict(key=k, value=v, slot_mapping=slots)
+                    want_k, want_v = kd.clone(), vd.clone()
+                    store_kvcache_fp4(k, v, want_k, want_v, slots)
+                o = decode_attention_fp4(qd[:n], kd, vd, lens_d, tables.to(DEV), scale, plan=plan, **kw)
+                if kind == "store":
+                    assert torch.equal(kd, want_k) and torch.equal(vd, want_v)
+                _check(o, *_varlen(q[:n], kd.cpu(), vd.cpu(), tables, new, lens, scale=scale), f"{kind}, plan {plan}")
+            else:
+                out = torch.full((len(q), heads, D), 7.0, dtype=torch.bfloat16, device=DEV)
+                varlen_attention_fp4(qd, kd, vd, cu_seqlens_q=_cu(new), cu_seqlens_k=_cu(lens), max_seqlen_q=max(new),
+                                     block_table=tables.to(DEV), softmax_scale=scale, causal=causal, out=out, plan=plan)
+                _check(out[:t], *_varlen(q[:t], kc, vc, tables, new, lens, causal, scale), f"{kind}, plan {plan}")
+                assert (out[t:] == 7).all()
+    finally:
+        _lib.load().vox_set_decode_workgroups(0)
+
+
 def test_calls_on_two_streams_do_not_share_scratch():
     gen = _gen(50)
     lens = [[4000, 30, 2500], [100, 3900, 1200]]

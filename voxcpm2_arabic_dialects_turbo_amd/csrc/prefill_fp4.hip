@@ -64,14 +64,21 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
   uint8_t* const s_t0 = L.t0;
   uint8_t* const s_t1 = L.t1;
   int* const s_nan_at = L.nan_at;
-  const int q0 = p.cu_q[b], nq = p.cu_q[b + 1] - q0;
+  // Scalar loads, all at once: the bounds and the first block, which every table row has (left to the compiler, each stands
+  // behind the branch before its use: a round trip each)
+  const const_i32 bt = (const_i32)(p.block_tables + (int64_t)b * p.bt_stride);
+  const const_i32 cu_q = (const_i32)(p.cu_q + b), cu_k = (const_i32)(p.cu_k + b);
+  const int q0 = cu_q[0], q1 = cu_q[1], k0 = cu_k[0], k1 = cu_k[1], blk0 = bt[0];
+  asm volatile("" ::"s"(q0), "s"(q1), "s"(k0), "s"(k1), "s"(blk0), "s"(p.skip_single), "s"(p.max_blocks), "s"(p.block_size),
+               "s"(p.num_blocks), "s"(p.row_limit), "s"(p.q), "s"(p.k_cache), "s"(p.v_cache));
+  const int nq = q1 - q0;
   const int HK = p.num_kv_heads;
   const int gsh = __builtin_ctz(p.group);  // the group divides 128: a power of two
   constexpr int ROWS = 128 / KS;           // query rows of the workgroup
   constexpr int KT = 2 / KS;               // 32-key blocks of a tile that a wave takes
   const int bq = ROWS >> gsh;              // query tokens of the workgroup
   if (qt * bq >= nq || (p.skip_single && nq == 1)) return;  // (workgroup-uniform)
-  const int nk = max(0, min(p.cu_k[b + 1] - p.cu_k[b], p.max_blocks * p.block_size));
+  const int nk = max(0, min(k1 - k0, p.max_blocks * p.block_size));
 
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -92,14 +99,13 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
   const int64_t bb = fp4::block_bytes(p.block_size, HK);
   const int crow = HK * fp4::kHeadCodes, srow = HK * fp4::kHeadScales;
   const int scales = p.block_size * crow;
-  const const_i32 bt = (const_i32)(p.block_tables + (int64_t)b * p.bt_stride);
   // The next tile's codes from memory into LDS at d, a quarter of them by each wave; whether its block is
   // mapped.
   const int key16 = tid >> 2;  // the key of the 16-byte slot that this lane fills
   const int kcode = key16 * crow + (((tid & 3) ^ ((key16 >> 2) & 3)) << 4), vcode = key16 * crow + ((tid & 3) << 4);
   const int word = lane * srow;
   // the next tile: its first key, block (read a tile ahead) and place in the block
-  int next_kv = 0, next_col = 0, next_in = 0, next_blk = kv_end > 0 ? bt[0] : -1;
+  int next_kv = 0, next_col = 0, next_in = 0, next_blk = kv_end > 0 ? blk0 : -1;
   auto issue = [&](uint8_t* d) -> bool {
     const int blk = __builtin_amdgcn_readfirstlane(next_blk);
     const bool ok = blk >= 0 && blk < p.num_blocks;
