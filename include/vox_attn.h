@@ -291,7 +291,8 @@ int vox_decode_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache
 /* vox_store_kvcache_fp4 of one row a sequence and vox_decode_attn_fp4 in one call: the new tokens are attended over as the
  * cache will hold them, and their rows stored behind the reads. Same results as the two calls when no slot_mapping[b] lies
  * inside another sequence's context, as vox_decode_attn_store's. Rows that are not 16-byte aligned with strides multiples of 8
- * take the two calls. */
+ * take the two calls. Plans: calls of either form may follow each other; a record made by one is not used by the other, which
+ * scans the layout. */
 int vox_decode_attn_store_fp4(const void* q, int64_t q_row_stride, const void* key, const void* value,
                               int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping,
                               void* k_cache, void* v_cache, int64_t num_blocks, int block_size,

@@ -1,0 +1,82 @@
+"""Planned calls over 4-bit caches against the calls they stand for, where a plan's calls differ in form, fail, or have other
+calls between them. Tolerances: test_fp4_gpu.py's, or none (the same kernels in the same order)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import attention as ref
+from tests._util import randn
+from tests.test_fp4_gpu import BS, D, DEV, SCALE, _check, _decode_ref, _gen, _pool
+from voxcpm2_arabic_dialects_turbo_amd import _lib, ops
+from voxcpm2_arabic_dialects_turbo_amd.ops_fp4 import decode_attention_fp4, store_kvcache_fp4
+
+pytestmark = pytest.mark.gpu
+H, HK = 16, 2
+
+
+@pytest.fixture(autouse=True)
+def _no_plans():
+    ops.forget_plans()
+    yield
+    ops.forget_plans()
+
+
+def _step(seed, lens):
+    """Caches, tables, lengths and slots of a decode step whose sequences end at a new token."""
+    gen = _gen(seed)
+    kc, vc, tables = _pool(gen, lens, HK)
+    slots = torch.tensor([ref.slot_of(tables[b], n - 1, BS) for b, n in enumerate(lens)], dtype=torch.int32)
+    return gen, kc, vc, tables, slots
+
+
+def _new_rows(gen, n, offset):
+    """Key and value rows [n, HK, 128], `offset` elements behind a 16-byte border."""
+    x = (4 * randn(gen, 2, n * HK * D + 8)).to(DEV)
+    return tuple(r[offset:offset + n * HK * D].view(n, HK, D) for r in x)
+
+
+LENS = [3000, 40, 700, 1, 16, 2222]  # (some cut over workgroups, so that a merge has partials to read)
+
+
+@pytest.mark.parametrize("forms", [(None, 0), (0, None, 0), (1, 0), (0, 1, 0, None, 0), (None, 1, 0, 0)])
+def test_calls_of_other_forms_under_one_plan(forms):
+    """Layers of one step under one plan, without rows (None) and with them at an element offset: each is its store followed
+    by its attention."""
+    gen, kc, vc, tables, slots = _step(900 + len(forms), LENS)
+    lens, bt, s = torch.tensor(LENS, dtype=torch.int32, device=DEV), tables.to(DEV), slots.to(DEV)
+    for i, form in enumerate(forms):
+        q = randn(gen, len(LENS), H, D)
+        a, b = (kc.to(DEV), vc.to(DEV)), (kc.to(DEV), vc.to(DEV))
+        kw = {}
+        if form is not None:
+            k, v = _new_rows(gen, len(LENS), form)
+            kw = dict(key=k, value=v, slot_mapping=s)
+            store_kvcache_fp4(k, v, *b, s)
+        o = decode_attention_fp4(q.to(DEV), *a, lens, bt, SCALE, plan="one step", **kw)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        _check(o, *_decode_ref(q, b[0].cpu(), b[1].cpu(), tables, LENS), f"layer {i} of {forms}")
+
+
+@pytest.mark.parametrize("first,second", [(1, 0), (0, 1), (1, 1), (0, 0)])
+def test_the_library_scans_anew_where_a_record_is_of_the_other_form(first, second):
+    """vox_decode_attn_store_fp4 recorded with unaligned rows (stored by a call of their own), then reused with aligned ones,
+    and the reverse: the caller cannot see which form a call took."""
+    lib = _lib.load()
+    gen, kc, vc, tables, slots = _step(950, LENS)
+    n = len(LENS)
+    lens, bt, s = torch.tensor(LENS, dtype=torch.int32, device=DEV), tables.to(DEV), slots.to(DEV)
+    ws = torch.zeros(lib.vox_decode_workspace_bytes(n), dtype=torch.uint8, device=DEV)
+    for plan, offset in ((_lib.PLAN_RECORD, first), (_lib.PLAN_REUSE, second)):
+        q = randn(gen, n, H, D)
+        k, v = _new_rows(gen, n, offset)
+        a, b, qd = (kc.to(DEV), vc.to(DEV)), (kc.to(DEV), vc.to(DEV)), q.to(DEV)
+        store_kvcache_fp4(k, v, *b, s)
+        o = torch.empty(n, H, D, dtype=torch.bfloat16, device=DEV)
+        _lib.check(lib.vox_decode_attn_store_fp4(
+            qd.data_ptr(), H * D, k.data_ptr(), v.data_ptr(), HK * D, HK * D, s.data_ptr(), a[0].data_ptr(), a[1].data_ptr(),
+            a[0].shape[0], BS, bt.data_ptr(), bt.shape[1], bt.shape[1], lens.data_ptr(), n, H, HK, D, SCALE, plan,
+            ws.data_ptr(), ws.numel(), o.data_ptr(), _lib.stream_handle(o.device)), "decode_attn_store_fp4")
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        _check(o, *_decode_ref(q, b[0].cpu(), b[1].cpu(), tables, LENS), f"plan mode {plan}")

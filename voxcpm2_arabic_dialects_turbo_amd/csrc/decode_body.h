@@ -77,6 +77,7 @@ __device__ __forceinline__ f32x4 mfma_16x16x16(s16x4 a, s16x4 b, f32x4 c) {
 
 // Plan record of one workgroup (int32 offsets). The window holds up to 64 consecutive sequences from wb on: their
 // first and end steps, context, q / output row and new-token slot; then the block id of every tile of the range.
+// kRecValid: 0 for a record that does not hold its range, else its form (decode_split's rec_form).
 constexpr int kRecValid = 0, kRecR = 1, kRecR1 = 2, kRecS = 3, kRecG = 4, kRecWb = 5, kRecBatch = 6, kRecGrid = 7;
 constexpr int kRecWin = 16;                       // [kRecWin + 64 a + k]: a = 0 st, 1 en, 2 ctx, 3 row, 4 snew
 constexpr int kRecTileOff = kRecWin + 5 * kWave;  // block id of range tile r + i
@@ -320,6 +321,9 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
   // ---- the layout: from this workgroup's plan record (reuse mode), or from a block-wide scan
   int S = 0, G = 1, r = 0, r1 = 0, wb = 0;
   bool use_rec = false;
+  // 4-bit caches: 2 where the record holds the new tokens' slots. A storing call may take either form (rows that cannot ride
+  // are stored by a call of their own), which its caller does not see: a record of the other form is not used.
+  const int rec_form = LDS::kOwnWalk && store ? 2 : 1;
   // the window: lane k holds sequence wb + k (its steps [w_st, w_en), context, row, new-token slot)
   int w_st = 0, w_en = 0, w_ctx = 0, w_row = 0, w_snew = -1;
   if (p.plan_mode == kPlanReuse) {
@@ -334,7 +338,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     G = s_bt[kRecG];
     wb = s_bt[kRecWb];
     // a record of this launch shape whose range fits it (the caller vouches for the rest: same lengths and tables)
-    use_rec = s_bt[kRecValid] == 1 && s_bt[kRecBatch] == p.batch && s_bt[kRecGrid] == grid && G >= 1 &&
+    use_rec = s_bt[kRecValid] == rec_form && s_bt[kRecBatch] == p.batch && s_bt[kRecGrid] == grid && G >= 1 &&
               G <= grid && 0 <= r && r <= r1 && r1 <= S && r1 - r <= kRecTiles &&
               (r == r1 || (0 <= wb && wb < p.batch));
     if (use_rec) {
@@ -394,7 +398,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
     rec[kRecWin + 3 * kWave + lane] = w_row;
     rec[kRecWin + 4 * kWave + lane] = w_snew;
     if (lane < 8) {
-      const int hdr[8] = {valid ? 1 : 0, r, r1, S, G, wb, p.batch, grid};
+      const int hdr[8] = {valid ? rec_form : 0, r, r1, S, G, wb, p.batch, grid};
       int v = hdr[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) v = lane == i ? hdr[i] : v;

@@ -190,6 +190,9 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         if rows != B or slot_mapping.numel() != B:
             raise ValueError(f"decode_attention_fp4: key, value and slot_mapping must hold {B} rows")
         slots = _ids(slot_mapping, "slot_mapping")
+        if key_stride == 0 or value_stride == 0:
+            key, value = key.contiguous(), value.contiguous()
+            key_stride = value_stride = hk * D
     elif value is not None or slot_mapping is not None:
         raise ValueError("decode_attention_fp4: key, value and slot_mapping go together")
     if B == 0:
@@ -201,16 +204,16 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     mb = bt.shape[1]
     lib = _lib.load()
     with _on(dev):
-        ws, mode = _workspace(lib, dev, B, plan, "decode_fp4", B, mb, bt_stride, H, hk, bs)
+        # a record holds the slots of rows that ride (the library stores others by a call of their own)
+        rides = plan is not None and key is not None and (key.data_ptr() | value.data_ptr()) % 16 == 0 \
+            and (key_stride | value_stride) % 8 == 0
+        ws, mode = _workspace(lib, dev, B, plan, "decode_fp4", rides, B, mb, bt_stride, H, hk, bs)
         if key is None:
             _lib.check(lib.vox_decode_attn_fp4(q.data_ptr(), _row_stride(q), k_cache.data_ptr(), v_cache.data_ptr(), blocks,
                                                bs, bt.data_ptr(), bt_stride, mb, lens.data_ptr(), B, H, hk, D,
                                                float(softmax_scale), mode, ws.data_ptr(), ws.numel(), out.data_ptr(),
                                                _lib.stream_handle(dev)), "decode_attn_fp4")
             return out
-        if key_stride == 0 or value_stride == 0:
-            key, value = key.contiguous(), value.contiguous()
-            key_stride = value_stride = hk * D
         _lib.check(lib.vox_decode_attn_store_fp4(q.data_ptr(), _row_stride(q), key.data_ptr(), value.data_ptr(),
                                                  key_stride, value_stride, slots.data_ptr(),
                                                  k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(),
