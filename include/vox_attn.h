@@ -267,8 +267,9 @@ int vox_copy_kv_block_prefix(void* kv, int64_t num_planes, int64_t num_blocks, i
 
 /* Quantises key / value rows (bf16 [num_tokens, num_kv_heads, head_dim], rows *_row_stride elements apart, heads
  * contiguous) into their slots; slots outside [0, num_blocks * block_size) (-1: padding) store nothing. Of a group whose
- * largest magnitude is amax the scale is the least power of two 2^e >= 2^-126 with amax <= 7 * 2^e; a value becomes the
- * nearest one of the grid, ties to the even code, at most 6 * 2^e. A group that holds an infinity or NaN gets scale 255.
+ * largest magnitude is amax the scale is the least power of two 2^e >= 2^-126 with amax <= 7 * 2^e, and 2^125 where that is
+ * more (6 * 2^125 is the largest that bf16 holds); a value becomes the nearest one of the grid, ties to the even code, at most
+ * 6 * 2^e. A group that holds an infinity or NaN gets scale 255.
  * The codes are a function of the row alone. Slots that occur twice in a call hold a mix of their rows. */
 int vox_store_kvcache_fp4(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride,
                           void* k_cache, void* v_cache, int64_t num_blocks, int block_size, const int32_t* slot_mapping,

@@ -20,7 +20,7 @@ def quantize_group(x) -> tuple[list[int], int]:
         return [0] * len(x), 255
     amax = max(abs(v) for v in x)
     e = -126
-    while amax > 7 * 2.0 ** e:
+    while amax > 7 * 2.0 ** e and e < 125:  # (6 x 2^125 is the last that bf16 holds)
         e += 1
     codes = []
     for v in x:

@@ -37,10 +37,11 @@ __device__ __forceinline__ float scale_float(uint32_t b) { return __uint_as_floa
 
 // The scale byte of a group whose largest magnitude has the bf16 bits `amax` (sign cleared): the least power of two that
 // leaves the largest value at most 7 times it, so it is off by at most half a step of its binade ([4, 6], where 7 is
-// held as 6); at least 2^-126, a normal float; 255 where the group holds an infinity or NaN.
+// held as 6); at least 2^-126, a normal float, and at most 2^125, whose 6 is the largest that bf16 holds (at 2^126 a 4 is
+// 2^128, an infinity); 255 where the group holds an infinity or NaN.
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
   const int e = (int)(amax >> 7) - 2 + ((amax & 0x7fu) > 0x60u ? 1 : 0);
-  return amax >= 0x7f80u ? 255u : (uint32_t)max(1, min(254, e));
+  return amax >= 0x7f80u ? 255u : (uint32_t)max(1, min(252, e));
 }
 
 // 8 bf16 (packed) to 8 codes: round to nearest, ties to the even code, saturating at 6.
