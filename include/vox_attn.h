@@ -276,13 +276,16 @@ int vox_store_kvcache_fp4(const void* key, const void* value, int64_t key_row_st
                           int64_t num_tokens, int num_kv_heads, int head_dim, void* stream);
 
 /* The values held at slots as bf16 rows: key / value [num_tokens, num_kv_heads, head_dim], contiguous, 16-byte aligned.
- * Exact; zeros for slots outside the cache. */
+ * Exact; zeros for slots outside the cache, infinities for what bf16 does not hold (no stored row: 4 and 6 times 2^126, 2 to 6
+ * times 2^127). */
 int vox_load_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t num_blocks, int block_size,
                          const int32_t* slots, int64_t num_tokens, int num_kv_heads, int head_dim, void* key,
                          void* value, void* stream);
 
-/* vox_decode_attn over 4-bit caches: the attention over the values that the caches hold. Arguments, workspace and plans as
- * vox_decode_attn's (records may not be shared with calls of other functions). softmax_scale must be positive. */
+/* vox_decode_attn over 4-bit caches: the attention over the values that the caches hold. Where a value row's group of 32 channels
+ * is not a number, or has a value past bf16's largest (no stored row), the outputs that see it are NaN in those channels.
+ * Arguments, workspace and plans as vox_decode_attn's (records may not be shared with calls of other functions). softmax_scale
+ * must be positive. */
 int vox_decode_attn_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                         int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                         int max_blocks, const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,

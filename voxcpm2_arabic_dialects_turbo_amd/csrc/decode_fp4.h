@@ -285,14 +285,16 @@ struct LdsFp4 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[s * 4 + i] = jq * 4 + i < lim[s] ? y[i] : -INFINITY;
       }
-      // The values of kv head g into LDS as bf16. Groups that are not numbers stay out of the MFMAs (the zeros that keep the
-      // kv heads apart would not hide them): the sequence's heads of that kv head are NaN in the group.
+      // The values of kv head g into LDS as bf16. Groups that are not numbers (or past bf16: held_scale) stay out of the MFMAs
+      // (the zeros that keep the kv heads apart would not hide them): the sequence's heads of that kv head are NaN in the group.
       auto store_v = [&](int g) {
         uint32_t b[kSteps];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) b[s] = (lane >> 2) < lim[s] ? (T.vs[s][g] >> (8 * (lane & 3))) & 0xffu : 0u;
-        uint64_t bad = __builtin_amdgcn_ballot_w64(max(b[0], b[1]) == 255u);
-        if (__builtin_expect(bad != 0, 0)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(max(b[0], b[1]) >= 253u) != 0, 0)) {
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) b[s] = fp4::held_scale(b[s], T.v[s][g]);
+          uint64_t bad = __builtin_amdgcn_ballot_w64(max(b[0], b[1]) == 255u);
 #pragma unroll
           for (int i = 32; i >= 4; i >>= 1) bad |= bad >> i;
           nan_groups |= ((uint32_t)bad & 15u) << (4 * g);

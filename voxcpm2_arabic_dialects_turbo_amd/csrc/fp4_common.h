@@ -81,6 +81,16 @@ __device__ __forceinline__ u32x4 values8(uint32_t codes, float scale) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
 }
 
+// The scale byte b of 32 codes as V's conversion to bf16 takes it: 255 too where they stand for more than bf16 holds, from
+// 2^128 on (a 4 at 2^126, a 2 at 2^127: planes that others have written, the store's scales end at 2^125). As an infinity such a
+// value would be NaN wherever it meets a probability of 0.
+__device__ __forceinline__ uint32_t held_scale(uint32_t b, u32x4 codes) {
+  uint32_t past = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) past |= (b == 253u ? codes[i] & (codes[i] << 1) : codes[i]) & 0x44444444u;
+  return b >= 253u && past != 0 ? 255u : b;
+}
+
 // The scores' MFMAs: D(fp32) += A(fp4 codes) B(fp8 e4m3), each 32 contraction elements with a scale byte of their own
 // (byte OP of the lane's register).
 //   16x16x128: lane l's codes are A[l % 16][32 (l / 16) + [0, 32)], its scale that block's; its B bytes 0-15 are

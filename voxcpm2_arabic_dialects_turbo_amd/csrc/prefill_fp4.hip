@@ -178,17 +178,20 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
   const int vst = (tid >> 2) * kVRow + (tid & 3) * 8;
   const int vtr = (4 * h + ((lane & 15) >> 2)) * kVRow + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
 
-  // V of tile kv0 (its codes at d, `mapped`) into LDS buffer buf: the scale, then piece q4. Values that are not numbers stay
-  // out of the MFMAs, where a masked key's probability of 0 would not hide them: such a group is zeros in LDS, and mark_nan
+  // V of tile kv0 (its codes at d, `mapped`) into LDS buffer buf: the scale, then piece q4. Values that are not numbers (or
+  // past bf16: held_scale) stay out of the MFMAs, where a masked key's probability of 0 would not hide them: such a group is zeros in LDS, and mark_nan
   // finds the rows that see it (their outputs in the group are NaN).
   u32x4 vcodes;
   float vscale = 0.f;
   auto scale_v = [&](const uint8_t* d, int kv0, bool mapped, int buf) {
     vcodes = *reinterpret_cast<const u32x4*>(d + kTileBytes + tid * 16);
-    const uint32_t b = mapped && kv0 + (tid >> 2) < nk ? (uint32_t)d[kTileBytes + kCodes + tid] : 0u;
+    uint32_t b = mapped && kv0 + (tid >> 2) < nk ? (uint32_t)d[kTileBytes + kCodes + tid] : 0u;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(b >= 253u) != 0, 0)) {
+      b = fp4::held_scale(b, vcodes);
+      if (__builtin_amdgcn_ballot_w64(b == 255u) != 0) s_nan_at[buf] = kv0;
+    }
     const bool nan = b == 255u;
     L.nan[buf * (kBK * 4) + tid] = nan;
-    if (__builtin_amdgcn_ballot_w64(nan) != 0) s_nan_at[buf] = kv0;
     vscale = fp4::scale_float(nan ? 0u : b);
   };
   auto piece_v = [&](int q4, int buf) {
