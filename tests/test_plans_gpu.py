@@ -7,10 +7,10 @@ import pytest
 import torch
 
 from oracle import attention as ref
-from tests._util import randn
-from tests.test_fp4_gpu import BS, D, DEV, SCALE, _check, _decode_ref, _gen, _pool
+from tests._util import paged_pool, randn
+from tests.test_fp4_gpu import BS, D, DEV, SCALE, _check, _cu, _decode_ref, _gen, _pool
 from voxcpm2_arabic_dialects_turbo_amd import _lib, ops
-from voxcpm2_arabic_dialects_turbo_amd.ops_fp4 import decode_attention_fp4, store_kvcache_fp4
+from voxcpm2_arabic_dialects_turbo_amd.ops_fp4 import decode_attention_fp4, store_kvcache_fp4, varlen_attention_fp4
 
 pytestmark = pytest.mark.gpu
 H, HK = 16, 2
@@ -80,3 +80,54 @@ def test_the_library_scans_anew_where_a_record_is_of_the_other_form(first, secon
             ws.data_ptr(), ws.numel(), o.data_ptr(), _lib.stream_handle(o.device)), "decode_attn_store_fp4")
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
         _check(o, *_decode_ref(q, b[0].cpu(), b[1].cpu(), tables, LENS), f"plan mode {plan}")
+
+
+OTHER = [700, 3000, 2222, 500, 1, 40]  # (another step of as many sequences)
+
+
+def _bf16_step(seed, lens):
+    gen = _gen(seed)
+    kc, vc, tables = paged_pool(gen, lens, sum(-(-n // BS) for n in lens) + 2)
+    return gen, kc, vc, tables
+
+
+def _call(fp4, step, lens, q, plan, scale=SCALE, out=None, varlen=False):
+    """One query per sequence of a step, over bf16 or 4-bit caches, as a decode or as a varlen call."""
+    kc, vc, bt = step[1].to(DEV), step[2].to(DEV), step[3].to(DEV)
+    if not varlen:
+        fn = decode_attention_fp4 if fp4 else ops.decode_attention
+        return fn(q, kc, vc, torch.tensor(lens, dtype=torch.int32, device=DEV), bt, scale, plan=plan, out=out)
+    kw = dict(cu_seqlens_q=_cu([1] * len(lens)), cu_seqlens_k=_cu(lens), max_seqlen_q=1, block_table=bt, softmax_scale=scale,
+              causal=True, plan=plan, out=out)
+    return varlen_attention_fp4(q, kc, vc, **kw) if fp4 else ops.varlen_attention(q, None, None, k_cache=kc, v_cache=vc, **kw)
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("varlen", [False, True])
+def test_a_plan_whose_first_call_was_refused(fp4, varlen):
+    """The workspace holds the records of another step of as many sequences; the refused call has made none."""
+    make = _step if fp4 else _bf16_step
+    before, now = make(960, OTHER), make(961, LENS)
+    q = randn(now[0], len(LENS), H, D).to(DEV)
+    want = _call(fp4, now, LENS, q, None, varlen=varlen)
+    _call(fp4, before, OTHER, q, "before", varlen=varlen)
+    with pytest.raises(ValueError):
+        _call(fp4, now, LENS, q, "now", scale=float("nan"), varlen=varlen)
+    for _ in range(2):
+        assert torch.equal(_call(fp4, now, LENS, q, "now", varlen=varlen), want)
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+def test_a_plan_whose_first_call_took_the_prefill_kernel(fp4):
+    """An output 8 bytes behind a 16-byte border is taken, by the kernel that makes no records."""
+    make = _step if fp4 else _bf16_step
+    before, now = make(970, OTHER), make(971, LENS)
+    q = randn(now[0], len(LENS), H, D).to(DEV)
+    want = _call(fp4, now, LENS, q, None, varlen=True)
+    _call(fp4, before, OTHER, q, "before", varlen=True)
+    out = torch.zeros(len(LENS) * H * D + 4, dtype=torch.bfloat16, device=DEV)[4:].view(len(LENS), H, D)
+    _call(fp4, now, LENS, q, "now", out=out, varlen=True)
+    for _ in range(2):
+        assert torch.equal(_call(fp4, now, LENS, q, "now", varlen=True), want)
+    # (the two kernels differ by the rounding of probabilities and outputs)
+    assert (out.float() - want.float()).abs().max() < 2e-2

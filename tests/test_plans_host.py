@@ -88,3 +88,78 @@ def test_one_row_for_every_sequence_rides(lib):
         _decode(True, "step", _rows(1).expand(B, HK, D))
     _decode(True, "step", _rows(B))
     assert lib.modes == [RECORD, REUSE, REUSE]
+
+
+def _varlen(fp4, plan, out=None, max_q=1, block_size=BS, hk=HK):
+    width = (68, U8) if fp4 else (D, BF16)
+    c = torch.zeros(4, block_size, hk, width[0], dtype=width[1])
+    cu, kw = torch.arange(B + 1, dtype=I32), dict(softmax_scale=0.1, causal=True, plan=plan, out=out, max_seqlen_q=max_q)
+    q, bt = torch.zeros(B, H, D, dtype=BF16), torch.zeros(B, 2, dtype=I32)
+    if fp4:
+        return ops_fp4.varlen_attention_fp4(q, c, c, cu_seqlens_q=cu, cu_seqlens_k=cu, block_table=bt, **kw)
+    return ops.varlen_attention(q, None, None, cu_seqlens_q=cu, cu_seqlens_k=cu, block_table=bt, k_cache=c, v_cache=c, **kw)
+
+
+def _prefill_store(_, plan, out=None):
+    c, cu, rows = _cache(False), torch.arange(B + 1, dtype=I32), _rows(B)
+    return ops.prefill_attention_store(torch.zeros(B, H, D, dtype=BF16), rows, rows, c, c, cu[:B], cu_seqlens_q=cu,
+                                       cu_seqlens_k=cu, max_seqlen_q=1, softmax_scale=0.1, plan=plan, out=out,
+                                       block_table=torch.zeros(B, 2, dtype=I32))
+
+
+CALLS = pytest.mark.parametrize("call,fp4", [(_decode, False), (_decode, True), (_varlen, False), (_varlen, True),
+                                             (_prefill_store, False)])
+VARLEN = pytest.mark.parametrize("call,fp4", [(_varlen, False), (_varlen, True), (_prefill_store, False)])
+
+
+@CALLS
+def test_a_refused_call_has_recorded_nothing(lib, call, fp4):
+    """The next call with its plan records: the workspace may hold another step's records."""
+    for status in (_lib.VOX_EINVAL, _lib.VOX_EHIP):
+        call(fp4, "before")
+        lib.status = status
+        with pytest.raises((ValueError, _lib.VoxAttnError)):
+            call(fp4, "step")
+        lib.status = _lib.VOX_OK
+        lib.modes.clear()
+        call(fp4, "step")
+        call(fp4, "step")
+        assert lib.modes == [RECORD, REUSE]
+
+
+@CALLS
+def test_a_refused_reuse_keeps_the_record(lib, call, fp4):
+    call(fp4, "step")
+    lib.status = _lib.VOX_EINVAL
+    with pytest.raises(ValueError):
+        call(fp4, "step")
+    lib.status = _lib.VOX_OK
+    call(fp4, "step")
+    assert lib.modes == [RECORD, REUSE, REUSE]
+
+
+@VARLEN
+def test_calls_whose_outputs_the_decode_kernels_cannot_write_record_nothing(lib, call, fp4):
+    """An output 8 bytes behind a 16-byte border, or with rows an odd number of 8 bytes apart, is the prefill kernel's in every
+    row: no plan, whatever the workspace holds, and none forgotten."""
+    call(fp4, "before")
+    for out in (torch.zeros(B * H * D + 4, dtype=BF16)[4:].view(B, H, D),
+                torch.zeros(B, H * D + 4, dtype=BF16)[:, :H * D].view(B, H, D)):
+        lib.modes.clear()
+        call(fp4, "step", out=out)
+        call(fp4, "before")
+        assert lib.modes == [NONE, REUSE]
+    lib.modes.clear()
+    call(fp4, "step", out=torch.zeros(B, H, D, dtype=BF16))
+    call(fp4, "step")
+    assert lib.modes == [RECORD, REUSE]
+
+
+def test_shapes_that_the_decode_kernels_do_not_take_record_nothing(lib):
+    for kw in (dict(block_size=48), dict(hk=4)):
+        lib.modes.clear()
+        _varlen(False, "before")
+        _varlen(False, "step", **kw)
+        _varlen(False, "before")
+        assert lib.modes == [RECORD, NONE, REUSE]
+        ops.forget_plans()

@@ -104,7 +104,7 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 # Plans: the layout of a decode step (which tiles each workgroup walks) is the same for every layer of the step.
 # Callers that know when a step's layout repeats pass a `plan` key (Attention.forward: the forward context, see
 # layers.py); the first call with a new key records the layout in the workspace, later calls with the same key reuse
-# it. The key also carries the graph capture in progress, so a capture always records its own plan in its first call.
+# it. A key counts once its call has succeeded. The key also carries the graph capture in progress, so a capture always records its own plan in its first call.
 
 _WS_LOCK = threading.Lock()
 _WORKSPACE: dict[tuple[int, int], torch.Tensor] = {}
@@ -128,18 +128,33 @@ def decode_workspace(dev: torch.device) -> torch.Tensor:
         return ws
 
 
-def _plan_mode(dev: torch.device, plan, *shape) -> int:
-    """The plan mode of a call with key `plan` (None: no plan) over launch shape `shape` on `dev`'s workspace."""
+def _plan_mode(dev: torch.device, plan, *shape) -> tuple[int, object]:
+    """The plan mode of a call with key `plan` (None: no plan) over launch shape `shape` on `dev`'s workspace, and what to
+    hand to `_plan_recorded` behind a call that records (None: nothing)."""
     if plan is None:
-        return _lib.PLAN_NONE
+        return _lib.PLAN_NONE, None
     lib = _lib.load()
     key = (plan, shape, int(lib.vox_decode_workgroups()), _lib.capture_id(_lib.stream_handle(dev)))
     idx = _device_index(dev)
     with _WS_LOCK:
         if _PLANNED.get(idx) == key:
-            return _lib.PLAN_REUSE
-        _PLANNED[idx] = key
-        return _lib.PLAN_RECORD
+            return _lib.PLAN_REUSE, None
+        _PLANNED.pop(idx, None)  # the call writes its own records, or, refused, none
+    return _lib.PLAN_RECORD, key
+
+
+def _plan_recorded(dev: torch.device, key) -> None:
+    """The call that `_plan_mode` gave `key` to has succeeded: its records are in the workspace."""
+    if key is not None:
+        with _WS_LOCK:
+            _PLANNED[_device_index(dev)] = key
+
+
+def _takes_decode_rows(H: int, HK: int, block_size: int, max_blocks: int, out: torch.Tensor, out_stride: int) -> bool:
+    """Whether the library runs the one-query rows of a paged varlen call of these shapes on the decode kernels: elsewhere
+    it takes no plan."""
+    return HK in (1, 2) and H <= MAX_DECODE_HEADS and block_size % 32 == 0 and max_blocks * block_size <= 1 << 30 \
+        and out_stride % 8 == 0 and out.data_ptr() % 16 == 0
 
 
 _SCOPE = threading.local()
@@ -217,13 +232,14 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     max_blocks = bt.shape[1]
     lib = _lib.load()
     ws = decode_workspace(dev)
-    mode = _plan_mode(dev, plan, "decode", key is not None, B, max_blocks, bt.stride(0), H, HK, block_size)
+    mode, recorded = _plan_mode(dev, plan, "decode", key is not None, B, max_blocks, bt.stride(0), H, HK, block_size)
     if key is None:
         _lib.check(lib.vox_decode_attn(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks,
                                        block_size, bt.data_ptr(), bt.stride(0), max_blocks, lens.data_ptr(), B, H, HK,
                                        D, float(softmax_scale), mode, ws.data_ptr(), ws.numel(), out.data_ptr(),
                                        _lib.stream_handle(dev)),
                    "decode_attn")
+        _plan_recorded(dev, recorded)
         return out
     _check_cuda(q, key, value, slot_mapping)
     if key.dtype != k_cache.dtype or value.dtype != v_cache.dtype:
@@ -241,6 +257,7 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                                          lens.data_ptr(), B, H, HK, D, float(softmax_scale), mode, ws.data_ptr(),
                                          ws.numel(), out.data_ptr(), _lib.stream_handle(dev)),
                "decode_attn_store")
+    _plan_recorded(dev, recorded)
     return out
 
 
@@ -340,12 +357,13 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | 
     # workspace. Passed when every row has one query, or when the (q tile, sequence) grid would be mostly empty
     # (T rows against B sequences of up to max_seqlen_q), which is what a few prefills beside many decode rows look
     # like; a dense prefill keeps the plain grid (a 44 x 46 paged step: 12.8 us there, 20.5 us persistent).
-    ws, mode = None, _lib.PLAN_NONE
-    if block_table is not None and cu_q is not None and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q):
+    ws, mode, recorded = None, _lib.PLAN_NONE, None
+    if block_table is not None and cu_q is not None and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) \
+            and _takes_decode_rows(H, HK, block_size, bt.shape[1], out, out.stride(0)):
         ws = decode_workspace(dev)
         if plan is None:
             plan = getattr(_SCOPE, "key", None)
-        mode = _plan_mode(dev, plan, "varlen", B, int(block_table.shape[1]), H, HK, int(k_cache.shape[1]))
+        mode, recorded = _plan_mode(dev, plan, "varlen", B, int(block_table.shape[1]), H, HK, int(k_cache.shape[1]))
     _lib.check(lib.vox_prefill_attn(q.data_ptr(), q.stride(0), *args,
                                     None if cu_q is None else cu_q.data_ptr(),
                                     None if cu_k is None else cu_k.data_ptr(), B, int(max_seqlen_q),
@@ -354,6 +372,7 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | 
                                     None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
                                     _lib.stream_handle(dev)),
                "prefill_attn")
+    _plan_recorded(dev, recorded)
     return out
 
 
@@ -431,18 +450,20 @@ def prefill_attention_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k
     if bt is not None:
         # the mixed launch (and with it the riding store) where varlen_attention would run the one-query rows on the
         # decode kernels
-        ws, mode = None, _lib.PLAN_NONE
-        if T and B > 0 and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q):
+        ws, mode, recorded = None, _lib.PLAN_NONE, None
+        if T and B > 0 and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) \
+                and _takes_decode_rows(H, HK, block_size, bt.shape[1], out, out.stride(0)):
             ws = decode_workspace(dev)
             if plan is None:
                 plan = getattr(_SCOPE, "key", None)
-            mode = _plan_mode(dev, plan, "varlen-store", B, int(bt.shape[1]), H, HK, int(block_size))
+            mode, recorded = _plan_mode(dev, plan, "varlen-store", B, int(bt.shape[1]), H, HK, int(block_size))
         _lib.check(lib.vox_prefill_attn_store_paged(
             q.data_ptr(), qs[0], k.data_ptr(), v.data_ptr(), ks[0], vs[0], slots.data_ptr(), N,
             k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, block_size, bt.data_ptr(), bt.stride(0), bt.shape[1],
             cu_q.data_ptr(), cu_k.data_ptr(), max(B, 0), int(max_seqlen_q) if T else 0, H, HK, D, float(softmax_scale),
             1 if causal else 0, out.data_ptr(), out.stride(0), mode, None if ws is None else ws.data_ptr(),
             0 if ws is None else ws.numel(), _lib.stream_handle(dev)), "prefill_attn_store_paged")
+        _plan_recorded(dev, recorded)
         return out
     _lib.check(lib.vox_prefill_attn_store(q.data_ptr(), qs[0], k.data_ptr(), v.data_ptr(), ks[0],
                                           vs[0], slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),

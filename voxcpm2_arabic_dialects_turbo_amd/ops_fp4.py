@@ -21,7 +21,8 @@ import contextlib
 import torch
 
 from . import _lib
-from .ops import (HEAD_DIM, MAX_DECODE_HEADS, _SCOPE, _as_i32, _check_cuda, _flat, _plan_mode, decode_workspace)
+from .ops import (HEAD_DIM, MAX_DECODE_HEADS, _SCOPE, _as_i32, _check_cuda, _flat, _plan_mode, _plan_recorded,
+                  _takes_decode_rows, decode_workspace)
 
 ROW_BYTES = 68  # of a token's head: 64 of codes, 4 of scales
 
@@ -146,12 +147,13 @@ def load_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.
     return key, value
 
 
-def _workspace(lib, dev: torch.device, batch: int, plan, *shape) -> tuple[torch.Tensor, int]:
-    """The scratch of a decode call over ``batch`` sequences and its plan mode. Without a plan it is the call's own (in a
-    captured graph, the graph's); with one it is the device's decode workspace, which keeps the records."""
+def _workspace(lib, dev: torch.device, batch: int, plan, *shape) -> tuple[torch.Tensor, int, object]:
+    """The scratch of a decode call over ``batch`` sequences, then its plan mode and key as ``_plan_mode`` gives them. Without a
+    plan the scratch is the call's own (in a captured graph, the graph's); with one it is the device's decode workspace, which
+    keeps the records."""
     if plan is None:
-        return torch.empty(lib.vox_decode_workspace_bytes(batch), dtype=torch.uint8, device=dev), _lib.PLAN_NONE
-    return decode_workspace(dev), _plan_mode(dev, plan, *shape)
+        return torch.empty(lib.vox_decode_workspace_bytes(batch), dtype=torch.uint8, device=dev), _lib.PLAN_NONE, None
+    return decode_workspace(dev), *_plan_mode(dev, plan, *shape)
 
 
 def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, context_lens: torch.Tensor,
@@ -207,12 +209,13 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         # a record holds the slots of rows that ride (the library stores others by a call of their own)
         rides = plan is not None and key is not None and (key.data_ptr() | value.data_ptr()) % 16 == 0 \
             and (key_stride | value_stride) % 8 == 0
-        ws, mode = _workspace(lib, dev, B, plan, "decode_fp4", rides, B, mb, bt_stride, H, hk, bs)
+        ws, mode, recorded = _workspace(lib, dev, B, plan, "decode_fp4", rides, B, mb, bt_stride, H, hk, bs)
         if key is None:
             _lib.check(lib.vox_decode_attn_fp4(q.data_ptr(), _row_stride(q), k_cache.data_ptr(), v_cache.data_ptr(), blocks,
                                                bs, bt.data_ptr(), bt_stride, mb, lens.data_ptr(), B, H, hk, D,
                                                float(softmax_scale), mode, ws.data_ptr(), ws.numel(), out.data_ptr(),
                                                _lib.stream_handle(dev)), "decode_attn_fp4")
+            _plan_recorded(dev, recorded)
             return out
         _lib.check(lib.vox_decode_attn_store_fp4(q.data_ptr(), _row_stride(q), key.data_ptr(), value.data_ptr(),
                                                  key_stride, value_stride, slots.data_ptr(),
@@ -220,6 +223,7 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                                                  bt_stride, mb, lens.data_ptr(), B, H, hk, D, float(softmax_scale), mode,
                                                  ws.data_ptr(), ws.numel(), out.data_ptr(), _lib.stream_handle(dev)),
                    "decode_attn_store_fp4")
+        _plan_recorded(dev, recorded)
     return out
 
 
@@ -259,15 +263,16 @@ def varlen_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     mb = bt.shape[1]
     lib = _lib.load()
     with _on(dev):
-        ws, mode = None, _lib.PLAN_NONE
-        if hk <= 2 and H <= MAX_DECODE_HEADS and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q):
+        ws, mode, recorded = None, _lib.PLAN_NONE, None
+        if (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) and _takes_decode_rows(H, hk, bs, mb, out, _row_stride(out)):
             if plan is None:
                 plan = getattr(_SCOPE, "key", None)
-            ws, mode = _workspace(lib, dev, B, plan, "varlen_fp4", B, mb, bt_stride, H, hk, bs, max_seqlen_q > 1)
+            ws, mode, recorded = _workspace(lib, dev, B, plan, "varlen_fp4", B, mb, bt_stride, H, hk, bs, max_seqlen_q > 1)
         _lib.check(lib.vox_prefill_attn_fp4(q.data_ptr(), _row_stride(q), k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs,
                                             bt.data_ptr(), bt_stride, mb, cu_q.data_ptr(), cu_k.data_ptr(), B,
                                             int(max_seqlen_q), T, H, hk, D, float(softmax_scale), 1 if causal else 0,
                                             out.data_ptr(), _row_stride(out), mode, None if ws is None else ws.data_ptr(),
                                             0 if ws is None else ws.numel(), _lib.stream_handle(dev)),
                    "prefill_attn_fp4")
+        _plan_recorded(dev, recorded)
     return out
