@@ -131,3 +131,19 @@ def test_a_plan_whose_first_call_took_the_prefill_kernel(fp4):
         assert torch.equal(_call(fp4, now, LENS, q, "now", varlen=True), want)
     # (the two kernels differ by the rounding of probabilities and outputs)
     assert (out.float() - want.float()).abs().max() < 2e-2
+
+
+@pytest.mark.parametrize("fp4,varlen", [(True, False), (True, True), (False, False), (False, True)])
+@pytest.mark.parametrize("others", [[700, 3000, 2222, 500, 1, 40], [900] * 150, [9, 20]])
+@pytest.mark.parametrize("other_varlen", [False, True])
+def test_unplanned_calls_between_planned_ones(fp4, varlen, others, other_varlen):
+    """Unplanned bf16 calls of as many and of other numbers of sequences between the layers of a planned step."""
+    step, between = (_step if fp4 else _bf16_step)(980, LENS), _bf16_step(981, others)
+    q, p = randn(step[0], len(LENS), H, D).to(DEV), randn(between[0], len(others), H, D).to(DEV)
+    want = _call(fp4, step, LENS, q, None, varlen=varlen)
+    first = _call(False, between, others, p, None, varlen=other_varlen)
+    for _ in range(3):
+        assert torch.equal(_call(fp4, step, LENS, q, "step", varlen=varlen), want)
+        assert torch.equal(_call(False, between, others, p, None, varlen=other_varlen), first)
+    assert torch.equal(_call(fp4, step, LENS, q, "step", varlen=varlen), want)
+    assert torch.equal(_call(fp4, step, LENS, q, "step", varlen=varlen), want)

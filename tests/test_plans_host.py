@@ -163,3 +163,23 @@ def test_shapes_that_the_decode_kernels_do_not_take_record_nothing(lib):
         _varlen(False, "before")
         assert lib.modes == [RECORD, NONE, REUSE]
         ops.forget_plans()
+
+
+@pytest.mark.parametrize("call,fp4", [(_decode, False), (_varlen, False), (_prefill_store, False)])
+@pytest.mark.parametrize("planned,fp4_planned", [(_decode, False), (_decode, True), (_varlen, False), (_varlen, True),
+                                                 (_prefill_store, False)])
+def test_an_unplanned_call_on_the_shared_workspace_ends_the_plan(lib, call, fp4, planned, fp4_planned):
+    """It writes its own step layout and partials where the records and layout of the plan are."""
+    planned(fp4_planned, "step")
+    call(fp4, None)
+    planned(fp4_planned, "step")
+    planned(fp4_planned, "step")
+    assert lib.modes == [RECORD, NONE, RECORD, REUSE]
+
+
+@pytest.mark.parametrize("call", [_decode, _varlen])
+def test_an_unplanned_4_bit_call_has_scratch_of_its_own(lib, call):
+    _decode(False, "step")
+    call(True, None)
+    _decode(False, "step")
+    assert lib.modes == [RECORD, NONE, REUSE]

@@ -104,7 +104,9 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 # Plans: the layout of a decode step (which tiles each workgroup walks) is the same for every layer of the step.
 # Callers that know when a step's layout repeats pass a `plan` key (Attention.forward: the forward context, see
 # layers.py); the first call with a new key records the layout in the workspace, later calls with the same key reuse
-# it. A key counts once its call has succeeded. The key also carries the graph capture in progress, so a capture always records its own plan in its first call.
+# it. A key counts once its call has succeeded, and until another call takes the workspace (a replayed graph that
+# does is not seen: forget_plans). The key also carries the graph capture in progress, so a capture always records its
+# own plan in its first call.
 
 _WS_LOCK = threading.Lock()
 _WORKSPACE: dict[tuple[int, int], torch.Tensor] = {}
@@ -131,11 +133,13 @@ def decode_workspace(dev: torch.device) -> torch.Tensor:
 def _plan_mode(dev: torch.device, plan, *shape) -> tuple[int, object]:
     """The plan mode of a call with key `plan` (None: no plan) over launch shape `shape` on `dev`'s workspace, and what to
     hand to `_plan_recorded` behind a call that records (None: nothing)."""
+    idx = _device_index(dev)
     if plan is None:
+        with _WS_LOCK:
+            _PLANNED.pop(idx, None)  # its layout and partials go where the recorded ones are
         return _lib.PLAN_NONE, None
     lib = _lib.load()
     key = (plan, shape, int(lib.vox_decode_workgroups()), _lib.capture_id(_lib.stream_handle(dev)))
-    idx = _device_index(dev)
     with _WS_LOCK:
         if _PLANNED.get(idx) == key:
             return _lib.PLAN_REUSE, None
