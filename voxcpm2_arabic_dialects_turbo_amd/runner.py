@@ -277,17 +277,21 @@ def causal_attention_modules(model: torch.nn.Module) -> list[Attention]:
 def kv_cache_block_bytes(modules: Iterable[Attention], block_size: int, dtype=torch.bfloat16) -> int:
     """Bytes one cache block takes across every causal layer, K and V (reference: model_runner.py:680-686).
     ``dtype`` as allocate_kv_cache's."""
-    return sum(2 * block_size * m.num_kv_heads * _head_width(m.head_dim, dtype) * _held_as(dtype).itemsize
-               for m in modules)
+    itemsize = torch.empty(0, dtype=_held_as(dtype)).element_size()
+    return sum(2 * block_size * m.num_kv_heads * _head_width(m.head_dim, dtype) * itemsize for m in modules)
 
 
-def _held_as(dtype: torch.dtype) -> torch.dtype:
-    return torch.uint8 if dtype == torch.float4_e2m1fn_x2 else dtype
+def _is_4_bit(dtype: torch.dtype | None) -> bool:
+    return dtype is not None and dtype == getattr(torch, "float4_e2m1fn_x2", None)  # (not every torch has the type)
 
 
-def _head_width(head_dim: int, dtype: torch.dtype) -> int:
+def _held_as(dtype: torch.dtype | None) -> torch.dtype | None:
+    return torch.uint8 if _is_4_bit(dtype) else dtype
+
+
+def _head_width(head_dim: int, dtype: torch.dtype | None) -> int:
     """Elements of a token's head in the cache: head_dim, or a 4-bit head's bytes."""
-    if dtype != torch.float4_e2m1fn_x2:
+    if not _is_4_bit(dtype):
         return head_dim
     if head_dim != HEAD_DIM:
         raise ValueError(f"4-bit caches take head_dim {HEAD_DIM}, got {head_dim}")
