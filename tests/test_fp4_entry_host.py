@@ -5,7 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from voxcpm2_arabic_dialects_turbo_amd import runner
+from voxcpm2_arabic_dialects_turbo_amd import layers, runner
+from voxcpm2_arabic_dialects_turbo_amd.context import reset_context, set_context
 from voxcpm2_arabic_dialects_turbo_amd.layers import Attention
 
 BF16, U8, I32 = torch.bfloat16, torch.uint8, torch.int32
@@ -21,3 +22,29 @@ def test_16_bit_caches_need_no_4_bit_type_of_torch(monkeypatch, dtype):
     assert runner.kv_cache_block_bytes(mods, 256, dtype) * 2 == kv.numel() * kv.element_size()
     assert runner.allocate_kv_cache([mods[0], Attention(8, 128, 0.1, 1)], 2, 256, dtype=dtype, device="cpu") is None
     assert mods[0].k_cache.shape == (2, 256, 2, 128)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float4_e2m1fn_x2])
+def test_decode_steps_with_more_rows_than_queries_store_then_attend(monkeypatch, dtype):
+    """Every row goes to its slot and the queries attend, over caches of either kind; with a row per query one call does both."""
+    calls = []
+    for name in ("decode_attention", "decode_attention_fp4", "store_kvcache", "flash_attn_with_kvcache"):
+        def fake(*args, _name=name, **kw):
+            calls.append((_name, args, kw))
+            return torch.zeros(args[0].shape, dtype=BF16)
+        monkeypatch.setattr(layers, name, fake)
+    m = Attention(16, 128, 0.1, 2)
+    runner.allocate_kv_cache([m], 4, 256, dtype=dtype, device="cpu")
+    q = torch.zeros(3, 16, 128, dtype=BF16)
+    lens, tables = torch.zeros(3, dtype=I32), torch.zeros(3, 1, dtype=I32)
+    try:
+        for rows, want in ((5, ["store_kvcache", "flash_attn_with_kvcache"]),
+                           (3, ["decode_attention" if dtype == BF16 else "decode_attention_fp4"])):
+            calls.clear()
+            k, slots = torch.zeros(rows, 2, 128, dtype=BF16), torch.zeros(rows, dtype=I32)
+            set_context(False, slot_mapping=slots, context_lens=lens, block_tables=tables)
+            assert m(q, k, k).shape == (3, 1, 16, 128)
+            assert [c[0] for c in calls] == want
+            assert rows == 3 or (calls[0][1][0] is k and calls[0][1][4] is slots and calls[1][1][1] is m.k_cache)
+    finally:
+        reset_context()

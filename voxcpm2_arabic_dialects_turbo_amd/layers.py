@@ -121,7 +121,8 @@ class Attention(nn.Module):
             k_cache, v_cache = self.k_cache, self.v_cache
             cached = bool(k_cache.numel() and v_cache.numel())
             fp4 = cached and is_fp4_cache(k_cache)
-            if fp4 and not context.is_prefill and context.slot_mapping is not None and k.dim() == 3:
+            if fp4 and not context.is_prefill and context.slot_mapping is not None and k.dim() == 3 \
+                    and k.shape[0] == q.shape[0]:
                 _check_riding_store(context, k_cache.shape[1], decode=True)
                 return decode_attention_fp4(q, k_cache, v_cache, context.context_lens, context.block_tables, self.scale,
                                             key=k, value=v, slot_mapping=context.slot_mapping,
