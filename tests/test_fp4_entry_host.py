@@ -7,6 +7,7 @@ import torch
 
 from voxcpm2_arabic_dialects_turbo_amd import layers, runner
 from voxcpm2_arabic_dialects_turbo_amd.context import reset_context, set_context
+from voxcpm2_arabic_dialects_turbo_amd.kernels import prefill_attn
 from voxcpm2_arabic_dialects_turbo_amd.layers import Attention
 
 BF16, U8, I32 = torch.bfloat16, torch.uint8, torch.int32
@@ -48,3 +49,17 @@ def test_decode_steps_with_more_rows_than_queries_store_then_attend(monkeypatch,
             assert rows == 3 or (calls[0][1][0] is k and calls[0][1][4] is slots and calls[1][1][1] is m.k_cache)
     finally:
         reset_context()
+
+
+def test_the_paged_prefill_wrapper_takes_4_bit_caches(monkeypatch):
+    calls = []
+    monkeypatch.setattr(prefill_attn, "varlen_attention_fp4", lambda *args, **kw: calls.append((args, kw)))
+    q, cu, bt = torch.zeros(5, 16, 128, dtype=BF16), torch.zeros(3, dtype=I32), torch.zeros(2, 1, dtype=I32)
+    kc, vc = (torch.zeros(2, 64, 2, 68, dtype=U8) for _ in range(2))
+    o = prefill_attn.paged_prefill_attention(q, kc, vc, bt, cu, cu, 3, 0.1)
+    ((args, kw),) = calls
+    assert o.shape == (5, 16 * 128) and o.dtype == BF16 and kw["out"].data_ptr() == o.data_ptr()
+    assert args[0] is q and args[1] is kc and args[2] is vc and kw["block_table"] is bt and kw["causal"]
+    assert kw["max_seqlen_q"] == 3 and kw["softmax_scale"] == 0.1
+    with pytest.raises(NotImplementedError, match="4-bit"):
+        prefill_attn.paged_prefill_attention(q, kc, vc, bt, cu, cu, 3, 0.1, quant=True)
