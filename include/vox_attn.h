@@ -35,7 +35,8 @@ extern "C" {
  *   VOX_PLAN_REUSE   the layout is read from the workspace, where the last VOX_PLAN_RECORD call on it recorded it;
  *                    the caller guarantees that call had the same batch, context lengths (varlen: cu_seqlens), block
  *                    tables, slots (store mode: reuse only after a store-mode record) and workgroup count. Parts of
- *                    the layout a record cannot hold are scanned again. Batches above 512 sequences run unplanned. */
+ *                    the layout a record cannot hold are scanned again. Batches above 512 sequences run unplanned.
+ * A call that fails records nothing, nor does a varlen call whose one-query rows the decode kernels do not take. */
 #define VOX_PLAN_NONE 0
 #define VOX_PLAN_RECORD 1
 #define VOX_PLAN_REUSE 2

@@ -8,7 +8,7 @@
 // whole. 12 layers of 2 kv heads in bf16, 604 MB moved by a compaction: 126-131 us with its plan (6), 4.9-5.0 TB/s, the
 // rate of a large copy; 156 us with branches around each piece and stores that stay in the caches. 28 layers, 32 children of 24
 // parents, 252 MB: 43.5 us (a parent's block is read from memory once for all its children), 59 us so. Two pieces a lane 45.0
-// us, eight 42.3; 4096 workgroups for the moves in place of 2048: the same.
+// us, eight 42.3; 4096 workgroups for the moves in place of 2048: the same. The same in 4 bits: 174 MB 42.8 us, 67 MB 16.2.
 #include "vox_common.h"
 #include "vox_kernels.h"
 

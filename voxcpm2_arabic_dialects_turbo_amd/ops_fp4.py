@@ -167,7 +167,7 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     With key / value ([B, HK, 128]) and slot_mapping ([B]) the step's rows are stored in the same call: the result (and the
     caches afterwards) are those of ``store_kvcache_fp4`` followed by this attention, as long as no sequence's slot lies
     inside another sequence's context. ``softmax_scale`` is positive. ``plan``: as decode_attention's; planned calls of one
-    device share a workspace and must not overlap."""
+    device share a workspace with each other and with unplanned calls over bf16 caches, and must not overlap those."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"decode_attention_fp4: q must be bf16 [B, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
