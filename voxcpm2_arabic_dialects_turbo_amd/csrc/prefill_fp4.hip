@@ -178,9 +178,9 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
   const int vst = (tid >> 2) * kVRow + (tid & 3) * 8;
   const int vtr = (4 * h + ((lane & 15) >> 2)) * kVRow + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
 
-  // V of tile kv0 (its codes at d, `mapped`) into LDS buffer buf: the scale, then piece q4. Values that are not numbers (or
-  // past bf16: held_scale) stay out of the MFMAs, where a masked key's probability of 0 would not hide them: such a group is zeros in LDS, and mark_nan
-  // finds the rows that see it (their outputs in the group are NaN).
+  // V of tile kv0 (its codes at d, `mapped`) into LDS buffer buf: the scale, then piece q4. Values that are not numbers (or past
+  // bf16: held_scale) stay out of the MFMAs, where a masked key's probability of 0 would not hide them: such a group is zeros in
+  // LDS, and mark_nan finds the rows that see it (their outputs in the group are NaN).
   u32x4 vcodes;
   float vscale = 0.f;
   auto scale_v = [&](const uint8_t* d, int kv0, bool mapped, int buf) {

@@ -109,8 +109,8 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     """Quantises key[i] / value[i] ([N, HK, 128] bf16, token rows may be strided) into slot slot_mapping[i] of the 4-bit
     caches; slots outside them (-1: padding) store nothing. A group of 32 channels gets the least power of two (2^-126
     at least, 2^125 at most: finite rows stay finite) that leaves its largest magnitude at most 7 times it, and every value
-    the nearest of the grid, ties to the even code, at most 6; a group that holds an infinity or NaN stands for NaN. A slot that occurs twice holds a mix of
-    its rows."""
+    the nearest of the grid, ties to the even code, at most 6; a group that holds an infinity or NaN stands for NaN. A slot
+    that occurs twice holds a mix of its rows."""
     blocks, bs, hk = _cache_shape(k_cache, v_cache)
     n, key_stride, value_stride = _rows("store_kvcache_fp4", key, value, hk)
     if slot_mapping.numel() != n:
