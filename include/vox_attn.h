@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define VOX_ABI_VERSION 14
+#define VOX_ABI_VERSION 15
 
 #define VOX_OK 0
 #define VOX_EINVAL 1 /* bad argument: shape, stride, alignment or null pointer (reference: the asserts of
@@ -349,6 +349,62 @@ int vox_compact_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int 
                           int64_t scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
                           const int32_t* context_lens, int batch, int32_t* new_tables, int32_t* remap, int32_t* live,
                           int32_t* moves, void* stream);
+
+/* ---- What each cached token receives of the attention, and its eviction. key_weights fp32 [num_weight_rows, num_kv_heads,
+ * weight_width] holds, for the sequence whose row it is (weight_rows int32 [batch] on the device, or NULL: sequence b's is row
+ * b; a row outside [0, num_weight_rows): none is kept) and each kv head, the sum of its cached tokens' probabilities over the
+ * kv head's query heads and every query so far. No two sequences of a call have the same row. softmax_scale is positive. */
+
+/* Scratch of vox_decode_attn_weights: the scores of every 16-token step that the tables allow. */
+size_t vox_decode_scores_bytes(int batch, int max_blocks, int block_size, int num_heads);
+
+/* vox_decode_attn, or with key (not NULL) vox_decode_attn_store, that also adds what every key received: a token before the
+ * last one of its context gets it on top of its weight, the last one's weight becomes it. Tokens at or past weight_width are
+ * left out. scores: vox_decode_scores_bytes bytes of scratch (16-byte aligned), the call's own. plan, workspace: as
+ * vox_decode_attn's. */
+int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                            int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping, void* k_cache,
+                            void* v_cache, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                            int64_t bt_stride, int max_blocks, const int32_t* context_lens, int batch, int num_heads,
+                            int num_kv_heads, int head_dim, float softmax_scale, float* key_weights,
+                            const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width, void* scores,
+                            size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
+                            void* stream);
+
+/* vox_prefill_attn with cu_seqlens, causal, that also adds what every key received: the last cu_seqlens_q[b + 1] -
+ * cu_seqlens_q[b] tokens of a sequence are the step's own, and their weights become it, the earlier ones' grow by it. A
+ * sequence without queries keeps its weights. max_seqlen_k: no sequence has more keys (further ones are left out of the
+ * weights). num_tokens: the rows that q and out hold. Paged blocks are a multiple of 64 tokens. lse: fp32 [num_tokens,
+ * num_heads], scratch of the call's own. */
+int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                             int64_t key_row_stride, int64_t value_row_stride, const void* k_cache, const void* v_cache,
+                             int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                             int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                             int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads, int num_kv_heads,
+                             int head_dim, float softmax_scale, float* key_weights, const int32_t* weight_rows,
+                             int64_t num_weight_rows, int64_t weight_width, float* lse, void* out,
+                             int64_t out_row_stride, void* stream);
+
+/* Drops tokens from sequences longer than `budget`: their first `sinks` and last `recent` tokens stay and, in every layer
+ * and kv head apart, the budget - sinks - recent heaviest of the others by key_weights (fp32 [num_layers, num_weight_rows,
+ * num_kv_heads, weight_width], weight_width >= max_blocks * block_size; of equal ones the earliest, NaN above every number).
+ * They move in their order to the first `budget` slots of the sequence, their weights to the first places of its row; what
+ * lies behind keeps what it held. A sequence within the budget, or without a row of weights, stays as it is.
+ *   kv           [num_layers][2][num_blocks] blocks: block_size slots of num_kv_heads * head_bytes, then block_size slots of
+ *                num_kv_heads * scale_bytes; head_bytes a multiple of 16, scale_bytes 0 or 4; num_blocks * block_size < 2^31
+ *   into         int32 [batch, into_stride] or NULL: where into[b][c] is not negative, block c of what sequence b keeps is
+ *                that one, which no table of the call names, in place of its own (which then stays as it was). Blocks that
+ *                several rows name need it in every row that is over the budget.
+ *   moves        int32 [num_layers, batch, num_kv_heads, min(budget, max_blocks * block_size)]: scratch
+ *   new_tables   int32 [batch, max_blocks]: the blocks still in use, -1 behind them; new_lens int32 [batch]
+ * A context past what max_blocks blocks hold counts as that. Tokens whose block, or whose new block, is not one of the cache
+ * are not moved: their new slots keep what they held. */
+int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_bytes,
+                        int scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                        const int32_t* context_lens, int batch, float* key_weights, const int32_t* weight_rows,
+                        int64_t num_weight_rows, int64_t weight_width, int budget, int sinks, int recent,
+                        const int32_t* into, int64_t into_stride, int32_t* moves, int32_t* new_tables, int32_t* new_lens,
+                        void* stream);
 
 #ifdef __cplusplus
 }

@@ -52,3 +52,14 @@ def compact(kv: torch.Tensor, tables, lens):
     new = [[remap[b] if 0 <= b < blocks else b for b in row] + [-1] * (len(full) - len(row))
            for row, full in zip(rows, tables)]
     return new, remap, len(live)
+
+
+def head_rows(kv: torch.Tensor):
+    """A token's head of every plane in one run: views [layers, 2, blocks, block_size, HK, ...] of kv's bytes, a 4-bit cache's
+    codes and scales apart."""
+    if kv.dtype != torch.uint8:
+        return [kv]
+    layers, two, blocks, bs, hk, width = kv.shape
+    flat = kv.view(layers, two, blocks, -1)
+    return [flat[..., :bs * hk * 64].view(layers, two, blocks, bs, hk, 64),
+            flat[..., bs * hk * 64:].view(layers, two, blocks, bs, hk, 4)]

@@ -12,6 +12,7 @@ from .layers import Attention
 from .ops import (flash_attn_func, flash_attn_varlen_func, flash_attn_with_kvcache, store_kvcache, decode_attention,
                   varlen_attention)
 from .ops_fp4 import (decode_attention_fp4, fp4_parts, load_kvcache_fp4, store_kvcache_fp4, varlen_attention_fp4)
+from .ops_weights import decode_attention_weights, varlen_attention_weights
 
 __all__ = [
     "Attention",
@@ -30,4 +31,6 @@ __all__ = [
     "decode_attention_fp4",
     "varlen_attention_fp4",
     "fp4_parts",
+    "decode_attention_weights",
+    "varlen_attention_weights",
 ]

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the library: shared HIP runti
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvoxattn.so")
 
 VOX_OK, VOX_EINVAL, VOX_EHIP = 0, 1, 2
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 PLAN_NONE, PLAN_RECORD, PLAN_REUSE = 0, 1, 2
 
@@ -49,6 +49,10 @@ EXPORTS = (
     "vox_copy_kv_blocks",
     "vox_fork_kv_blocks",
     "vox_compact_kv_blocks",
+    "vox_decode_scores_bytes",
+    "vox_decode_attn_weights",
+    "vox_prefill_attn_weights",
+    "vox_evict_kv_tokens",
 )
 
 _c_void_p, _i32, _i64, _f32, _size = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -108,6 +112,18 @@ _SIGNATURES = {
                                   _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p]),
     "vox_compact_kv_blocks": (_i32, [_c_void_p, _i64, _i64, _i32, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _i32,
                                      _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "vox_decode_scores_bytes": (_size, [_i32, _i32, _i32, _i32]),
+    "vox_decode_attn_weights": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                       _c_void_p, _i64, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32, _i32, _i32, _i32,
+                                       _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _i32, _c_void_p, _size,
+                                       _c_void_p, _c_void_p]),
+    "vox_prefill_attn_weights": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
+                                        _i32, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _i64,
+                                        _i32, _i32, _i32, _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                        _i64, _c_void_p]),
+    "vox_evict_kv_tokens": (_i32, [_c_void_p, _i64, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32,
+                                   _c_void_p, _c_void_p, _i64, _i64, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p,
+                                   _c_void_p, _c_void_p, _c_void_p]),
 }
 
 

@@ -25,7 +25,7 @@ BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_NAME = "libvoxattn.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["store_kvcache.hip", "decode_attn.hip", "prefill_attn.hip", "quantize_rows.hip", "kv_copy.hip", "kv_fp4.hip",
-           "decode_fp4.hip", "prefill_fp4.hip", "kv_pages.hip", "capi.hip"]
+           "decode_fp4.hip", "prefill_fp4.hip", "kv_pages.hip", "key_weights.hip", "kv_evict.hip", "capi.hip"]
 PROBE_PATH = os.path.join(PKG_DIR, "libvoxprobe.so")
 PROBE_SOURCES = ["bench_probe.hip"]
 # the CPython entry to the C ABI (host code only), for the interpreter that builds it

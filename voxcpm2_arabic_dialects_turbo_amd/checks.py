@@ -23,7 +23,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-__all__ = ["riding_store_violations"]
+__all__ = ["riding_store_violations", "eviction_violations"]
 
 
 def _host(t: torch.Tensor | None) -> np.ndarray | None:
@@ -91,3 +91,45 @@ def riding_store_violations(slot_mapping: torch.Tensor, block_tables: torch.Tens
                     return out
                 break
     return out
+
+
+def eviction_violations(block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int, budget: int, *,
+                        weight_rows: torch.Tensor | None = None, new_blocks: torch.Tensor | None = None,
+                        limit: int = 10) -> list[str]:
+    """What kernels.kv_evict.evict_kv_tokens assumes about a call and cannot see from the host (at most `limit` messages;
+    empty when all of it holds): no two sequences share a row of weights, and a block that a sequence over the budget is
+    brought down into is named by no other sequence and is no other's new block."""
+    tables, lens = _host(block_tables), _host(context_lens).reshape(-1)
+    if tables is None or tables.ndim != 2 or tables.shape[0] < lens.size:
+        return ["block_tables must be [B, max_blocks]"]
+    fresh = _host(new_blocks)
+    rows = np.arange(lens.size) if weight_rows is None else _host(weight_rows).reshape(-1)
+    out: list[str] = []
+    seen: dict[int, int] = {}
+    for b, r in enumerate(rows.tolist()):
+        if r >= 0 and r in seen:
+            out.append(f"sequences {seen[r]} and {b} share row {r} of the weights")
+        seen[r] = b
+    named: dict[int, set[int]] = {}
+    written: dict[int, int] = {}
+    for b, n in enumerate(lens.tolist()):
+        need = -(-min(max(n, 0), tables.shape[1] * block_size) // block_size)
+        for v in tables[b, :need].tolist():
+            if v >= 0:
+                named.setdefault(v, set()).add(b)
+    for b, n in enumerate(lens.tolist()):
+        if min(n, tables.shape[1] * block_size) <= budget or rows[b] < 0:
+            continue
+        for c in range(-(-budget // block_size)):
+            given = fresh is not None and fresh[b, c] >= 0
+            v = int(fresh[b, c]) if given else int(tables[b, c])
+            if v < 0:
+                continue
+            others = named.get(v, set()) - (set() if given else {b})
+            if others:
+                what = "new block" if given else "block"
+                out.append(f"sequence {b} is brought down into {what} {v}, which sequence {min(others)} names")
+            if v in written:
+                out.append(f"sequences {written[v]} and {b} are both brought down into block {v}")
+            written[v] = b
+    return out[:limit]

@@ -7,6 +7,8 @@ reset_context), so a runner that sets the context for the reference's Attention 
 - ``is_prefill`` bool; ``cu_seqlens_q`` / ``cu_seqlens_k`` int32 [B + 1]; ``max_seqlen_q`` / ``max_seqlen_k`` host ints;
 - ``slot_mapping`` int32 [N] (-1 = padded row); ``context_lens`` int32 [B]; ``block_tables`` int32 [B, max_blocks]
   (-1 padded);
+- ``weight_rows`` int32 [B] (no reference counterpart): the sequences' rows in the layers' ``key_weights``, None where the
+  step adds nothing to them;
 - ``first_patch``: carried for the reference's runner, not read by attention.
 
 The context is a module global read when ``Attention.forward`` runs: callers such as the reference's ``last_rows``
@@ -32,6 +34,7 @@ class Context:
     context_lens: torch.Tensor | None = None
     block_tables: torch.Tensor | None = None
     first_patch: bool = True
+    weight_rows: torch.Tensor | None = None
 
 
 _CONTEXT = Context()
@@ -50,6 +53,7 @@ def set_context(
     slot_mapping=None,
     context_lens=None,
     block_tables=None,
+    weight_rows=None,
 ):
     global _CONTEXT
     _CONTEXT = Context(
@@ -61,6 +65,7 @@ def set_context(
         slot_mapping,
         context_lens,
         block_tables,
+        weight_rows=weight_rows,
     )
 
 

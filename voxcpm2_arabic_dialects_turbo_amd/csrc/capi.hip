@@ -137,6 +137,8 @@ int launch_decode_slices(const vox::DecodeArgs& a, int batch, int num_kv_heads, 
       s.q = base.q + (int64_t)b0 * base.q_row_stride;
       s.context_lens = base.context_lens + b0;
       s.out = base.out + (int64_t)b0 * base.out_row_stride;
+      if (base.weight_rows) s.weight_rows = base.weight_rows + b0;
+      s.weight_row0 = base.weight_row0 + b0;
       if (base.slot_mapping) {
         s.slot_mapping = base.slot_mapping + b0;
         s.new_k = base.new_k + (int64_t)b0 * base.new_k_stride;
@@ -1034,6 +1036,174 @@ int vox_compact_kv_blocks(void* kv, int64_t num_planes, int64_t num_blocks, int 
   const vox::CompactArgs c{block_tables, bt_stride, max_blocks > 0 ? max_blocks : 1, context_lens, batch, new_tables, remap, live,
                            moves};
   return hip_status(vox::launch_compact(a, c, (hipStream_t)stream), "compact_kv_blocks launch");
+}
+
+}  // extern "C"
+
+// ---- what each key receives, and eviction by it
+
+namespace {
+int weights_setup(const char* fn, const float* key_weights, int64_t num_weight_rows, int64_t weight_width, float softmax_scale) {
+  if (!key_weights || ((uintptr_t)key_weights & 3u)) return fail(VOX_EINVAL, "%s: null or unaligned key_weights", fn);
+  if (num_weight_rows <= 0 || weight_width <= 0) return fail(VOX_EINVAL, "%s: empty key_weights", fn);
+  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return fail(VOX_EINVAL, "%s: softmax_scale %g must be positive and finite", fn, (double)softmax_scale);
+  return VOX_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t vox_decode_scores_bytes(int batch, int max_blocks, int block_size, int num_heads) {
+  if (batch <= 0 || max_blocks <= 0 || block_size <= 0 || num_heads <= 0) return 0;
+  const int slice = batch < vox::kMaxSeqPerLaunch ? batch : vox::kMaxSeqPerLaunch;
+  const size_t steps = ((size_t)max_blocks * block_size + 15) / 16;
+  return (size_t)slice * steps * num_heads * 16 * 4;
+}
+
+int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                            int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping, void* k_cache,
+                            void* v_cache, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                            int64_t bt_stride, int max_blocks, const int32_t* context_lens, int batch, int num_heads,
+                            int num_kv_heads, int head_dim, float softmax_scale, float* key_weights,
+                            const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width, void* scores,
+                            size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
+                            void* stream) {
+  const char* fn = "decode_attn_weights";
+  if (batch < 0) return fail(VOX_EINVAL, "%s: batch < 0", fn);
+  if (plan != VOX_PLAN_NONE && plan != VOX_PLAN_RECORD && plan != VOX_PLAN_REUSE)
+    return fail(VOX_EINVAL, "%s: plan mode %d", fn, plan);
+  if (batch == 0) return VOX_OK;
+  int st = weights_setup(fn, key_weights, num_weight_rows, weight_width, softmax_scale);
+  if (st != VOX_OK) return st;
+  if ((key == nullptr) != (value == nullptr) || (key == nullptr) != (slot_mapping == nullptr))
+    return fail(VOX_EINVAL, "%s: key, value and slot_mapping go together", fn);
+  const int64_t row = (int64_t)num_kv_heads * head_dim;
+  if (key && (key_row_stride < row || value_row_stride < row || key_row_stride % 8 || value_row_stride % 8 ||
+              !aligned16(key) || !aligned16(value)))
+    return fail(VOX_EINVAL, "%s: key / value rows must be 16-byte aligned, strides multiples of 8 elements and at least "
+                            "num_kv_heads * head_dim", fn);
+  vox::DecodeArgs a;
+  st = decode_setup(q, q_row_stride, k_cache, v_cache, num_blocks, block_size, block_tables, bt_stride, max_blocks,
+                    context_lens, batch, num_heads, num_kv_heads, head_dim, softmax_scale, workspace, workspace_bytes, out,
+                    &a);
+  if (st != VOX_OK) return st;
+  const size_t need = vox_decode_scores_bytes(batch, max_blocks, block_size, num_heads);
+  if (!scores || !aligned16(scores) || scores_bytes < need)
+    return fail(VOX_EINVAL, "%s: scores of %zu bytes (16-byte aligned), %zu needed", fn, scores_bytes, need);
+  if (key) {
+    a.slot_mapping = slot_mapping;
+    a.new_k = (const uint16_t*)key;
+    a.new_v = (const uint16_t*)value;
+    a.new_k_stride = key_row_stride;
+    a.new_v_stride = value_row_stride;
+  }
+  a.scores = (float*)scores;
+  a.weights = key_weights;
+  a.weight_rows = weight_rows;
+  a.weight_row_count = num_weight_rows;
+  a.weight_width = weight_width;
+  return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream, vox::launch_decode_weights);
+}
+
+int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                             int64_t key_row_stride, int64_t value_row_stride, const void* k_cache, const void* v_cache,
+                             int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                             int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                             int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads, int num_kv_heads,
+                             int head_dim, float softmax_scale, float* key_weights, const int32_t* weight_rows,
+                             int64_t num_weight_rows, int64_t weight_width, float* lse, void* out,
+                             int64_t out_row_stride, void* stream) {
+  const char* fn = "prefill_attn_weights";
+  if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_tokens < 0)
+    return fail(VOX_EINVAL, "%s: negative batch, max_seqlen_q, max_seqlen_k or num_tokens", fn);
+  if (batch == 0 || max_seqlen_q == 0 || num_tokens == 0) return VOX_OK;
+  if (!cu_seqlens_q || !cu_seqlens_k || !out || !lse) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  int st = weights_setup(fn, key_weights, num_weight_rows, weight_width, softmax_scale);
+  if (st != VOX_OK) return st;
+  if (out_row_stride < (int64_t)num_heads * head_dim || out_row_stride % 4 || ((uintptr_t)out & 7u))
+    return fail(VOX_EINVAL, "%s: bad out row stride or alignment", fn);
+  if (batch > 65535 || num_kv_heads > 65535) return fail(VOX_EINVAL, "%s: more than 65535 sequences or kv heads", fn);
+  if (block_tables && (block_size <= 0 || block_size % 64))
+    return fail(VOX_EINVAL, "%s: block_size %d must be a positive multiple of 64", fn, block_size);
+  if (block_tables && (int64_t)max_blocks * block_size > (1 << 30))
+    return fail(VOX_EINVAL, "%s: block table too wide", fn);
+  vox::KeyWeightsArgs k{};
+  st = prefill_setup(fn, q, q_row_stride, key, value, key_row_stride, value_row_stride, k_cache, v_cache, num_blocks,
+                     block_size, block_tables, bt_stride, max_blocks, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, 0, 0,
+                     num_heads, num_kv_heads, head_dim, softmax_scale, 1, &k.a);
+  if (st != VOX_OK) return st;
+  k.a.out = (uint16_t*)out;
+  k.a.out_row_stride = out_row_stride;
+  k.a.row_limit = num_tokens;
+  k.a.lse = lse;
+  k.weights = key_weights;
+  k.rows = weight_rows;
+  k.row_count = num_weight_rows;
+  k.width = weight_width;
+  st = hip_status(vox::launch_prefill_lse(k.a, max_seqlen_q, (hipStream_t)stream), "prefill_attn_weights launch");
+  if (st != VOX_OK) return st;
+  return hip_status(vox::launch_key_weights(k, max_seqlen_k, (hipStream_t)stream), "prefill_attn_weights sums launch");
+}
+
+int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_bytes,
+                        int scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                        const int32_t* context_lens, int batch, float* key_weights, const int32_t* weight_rows,
+                        int64_t num_weight_rows, int64_t weight_width, int budget, int sinks, int recent,
+                        const int32_t* into, int64_t into_stride, int32_t* moves, int32_t* new_tables, int32_t* new_lens,
+                        void* stream) {
+  const char* fn = "evict_kv_tokens";
+  if (batch < 0 || num_layers < 0) return fail(VOX_EINVAL, "%s: negative count", fn);
+  if (batch == 0 || num_layers == 0) return VOX_OK;
+  if (!kv || !block_tables || !context_lens || !key_weights || !moves || !new_tables || !new_lens)
+    return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (block_size <= 0 || num_blocks <= 0 || num_blocks > INT32_MAX / block_size)
+    return fail(VOX_EINVAL, "%s: cache of %lld blocks of %d tokens", fn, (long long)num_blocks, block_size);
+  if (num_kv_heads <= 0 || head_bytes <= 0 || head_bytes % 16 || head_bytes > 16 * 256 ||
+      (scale_bytes != 0 && scale_bytes != 4))
+    return fail(VOX_EINVAL, "%s: %d kv heads of %d and %d bytes (multiples of 16 up to 4096, and 0 or 4)", fn, num_kv_heads,
+                head_bytes, scale_bytes);
+  const int64_t block_bytes = (int64_t)block_size * num_kv_heads * (head_bytes + scale_bytes);
+  if (!aligned16(kv) || block_bytes % 16)
+    return fail(VOX_EINVAL, "%s: kv and its blocks must be 16-byte aligned", fn);
+  if (max_blocks <= 0 || bt_stride < max_blocks || (int64_t)max_blocks * block_size > (1 << 30))
+    return fail(VOX_EINVAL, "%s: bad block table shape", fn);
+  if (into && into_stride < max_blocks) return fail(VOX_EINVAL, "%s: bad shape of the new blocks' table", fn);
+  if (num_weight_rows <= 0 || weight_width < (int64_t)max_blocks * block_size)
+    return fail(VOX_EINVAL, "%s: key_weights of %lld rows of %lld, the tables reach %lld tokens", fn,
+                (long long)num_weight_rows, (long long)weight_width, (long long)max_blocks * block_size);
+  if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+    return fail(VOX_EINVAL, "%s: budget %d must be positive and hold sinks %d and recent %d", fn, budget, sinks, recent);
+  if (batch > 65535 || num_kv_heads > 65535 || num_layers > 32767)
+    return fail(VOX_EINVAL, "%s: at most 65535 sequences and kv heads and 32767 layers", fn);
+  const int64_t reach = (int64_t)max_blocks * block_size;
+  vox::EvictArgs a{};
+  a.kv = (uint8_t*)kv;
+  a.layers = (int)num_layers;
+  a.num_blocks = num_blocks;
+  a.block_size = block_size;
+  a.num_heads = num_kv_heads;
+  a.head_bytes = head_bytes;
+  a.scale_bytes = scale_bytes;
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.max_blocks = max_blocks;
+  a.context_lens = context_lens;
+  a.batch = batch;
+  a.weights = key_weights;
+  a.rows = weight_rows;
+  a.row_count = num_weight_rows;
+  a.width = weight_width;
+  a.budget = budget;
+  a.sinks = sinks;
+  a.recent = recent;
+  a.into = into;
+  a.into_stride = into_stride;
+  a.moves = moves;
+  a.kept = budget < reach ? budget : reach;
+  a.new_tables = new_tables;
+  a.new_lens = new_lens;
+  return hip_status(vox::launch_evict(a, (hipStream_t)stream), "evict_kv_tokens launch");
 }
 
 }  // extern "C"

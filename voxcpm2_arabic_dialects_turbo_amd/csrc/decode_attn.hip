@@ -10,7 +10,7 @@ namespace {
 
 using namespace dec;
 
-template <int HK, bool BTL>
+template <int HK, bool BTL, bool SCORES>
 __global__ __launch_bounds__(kThreads, 2) void decode_kernel(DecodeArgs p) {
   using LDS = LdsOwn<HK, BTL>;
   __shared__ __attribute__((aligned(16))) uint16_t s_vt[kWaves * kTile * Tile<HK>::VROW];  // per-wave V tiles
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(DecodeArgs p) {
   __shared__ __attribute__((aligned(16))) int s_bt[LDS::kBtInts];
   __shared__ int s_rtiles[kRecTiles];  // record mode: the block id of every tile of the range, for the record
   const LDS L{s_vt, s_slot, s_ctx, s_row, s_snew, s_start, s_wtot, s_wmax, s_bt, s_rtiles};
-  decode_split<HK>(p, (int)blockIdx.x, (int)gridDim.x, L);
+  decode_split<HK, LDS, SCORES>(p, (int)blockIdx.x, (int)gridDim.x, L);
 }
 
 // Varlen store mode: merge workgroup B + wid copies rows wid, wid + copy_wgs, ... of new_k / new_v (below copy_rows)
@@ -75,14 +75,22 @@ __device__ __forceinline__ void copy_new_rows(const DecodeArgs& p, int wid) {
 // partials (fp32), the loads of kMergeBatch partials in flight together. Runs after decode_kernel on the same stream,
 // which makes the partials visible. In varlen store mode workgroups past the sequences copy the step's new rows into
 // the caches (copy_new_rows). PG workgroups per sequence, 16 / PG heads each (merge_row). FP4: the caches are 4-bit ones, and
-// store mode quantises the row (as store_fp4_kernel does).
-template <int PG, bool FP4>
+// store mode quantises the row (as store_fp4_kernel does). WEIGHTS: the workgroups past the sequences add up what the keys
+// received (add_key_weights).
+template <int PG, bool FP4, bool WEIGHTS = false>
 __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs p) {
   __shared__ __attribute__((aligned(16))) float comb[PG > 1 ? PG - 1 : 1][kWave][12];
   const int b = blockIdx.x / PG, part = blockIdx.x % PG;
   const int tid = threadIdx.x;
-  if (b >= p.batch) {  // (workgroup-uniform) a copy workgroup of the varlen store mode
-    copy_new_rows(p, (int)blockIdx.x - PG * p.batch);
+  if (b >= p.batch) {  // (workgroup-uniform) a copy workgroup of the varlen store mode, or a weights workgroup
+    const int id = (int)blockIdx.x - PG * p.batch;
+    if constexpr (WEIGHTS) {
+      __shared__ float lse[4][kMaxHeads];
+      const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+      add_key_weights(p, 4 * id + w, 4 * p.weight_wgs, lse[w]);
+    } else {
+      copy_new_rows(p, id);
+    }
     return;
   }
   int s_tot = p.steps[p.batch], s_b = p.steps[b], s_e = p.steps[b + 1], s_g = p.steps[p.batch + 1];
@@ -162,20 +170,45 @@ hipError_t launch_decode_merge_fp4(const DecodeArgs& a, hipStream_t stream) {
   return a.slot_mapping ? launch_merge<true>(a, stream) : launch_merge<false>(a, stream);
 }
 
-hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stream) {
+namespace {
+
+template <bool SCORES>
+hipError_t launch_split(const DecodeArgs& a, int num_kv_heads, hipStream_t stream) {
   const dim3 grid((unsigned)a.grid);
   const bool btl = (int64_t)a.batch * a.max_blocks <= kBtLds;
   if (num_kv_heads == 1 && btl)
-    decode_kernel<1, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+    decode_kernel<1, true, SCORES><<<grid, dim3(kThreads), 0, stream>>>(a);
   else if (num_kv_heads == 1)
-    decode_kernel<1, false><<<grid, dim3(kThreads), 0, stream>>>(a);
+    decode_kernel<1, false, SCORES><<<grid, dim3(kThreads), 0, stream>>>(a);
   else if (btl)
-    decode_kernel<2, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+    decode_kernel<2, true, SCORES><<<grid, dim3(kThreads), 0, stream>>>(a);
   else
-    decode_kernel<2, false><<<grid, dim3(kThreads), 0, stream>>>(a);
-  const hipError_t e = hipGetLastError();
+    decode_kernel<2, false, SCORES><<<grid, dim3(kThreads), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stream) {
+  const hipError_t e = launch_split<false>(a, num_kv_heads, stream);
   if (e != hipSuccess) return e;
   return launch_decode_merge(a, stream);
+}
+
+hipError_t launch_decode_weights(const DecodeArgs& a0, int num_kv_heads, hipStream_t stream) {
+  if (!a0.scores || !a0.weights) return hipErrorInvalidValue;
+  DecodeArgs a = a0;
+  // a wave for every four steps (one round of add_key_weights) of the longest step the tables allow, up to two workgroups
+  // per CU
+  const int64_t steps = (int64_t)a.batch * (((int64_t)a.max_blocks * a.block_size + kTile - 1) / kTile);
+  a.weight_wgs = (int)min((int64_t)512, (steps + 15) / 16);
+  const hipError_t e = launch_split<true>(a, num_kv_heads, stream);
+  if (e != hipSuccess) return e;
+  if (a.batch <= kMergeSplitBatch)
+    decode_merge_kernel<4, false, true><<<dim3((unsigned)(4 * a.batch + a.weight_wgs)), dim3(256), 0, stream>>>(a);
+  else
+    decode_merge_kernel<1, false, true><<<dim3((unsigned)(a.batch + a.weight_wgs)), dim3(256), 0, stream>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace vox

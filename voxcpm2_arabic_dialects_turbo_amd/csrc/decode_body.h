@@ -292,8 +292,9 @@ struct LdsBorrowed {
   }
 };
 
-// The split-KV decode work of workgroup g of `grid` (LDS::kNW waves), its LDS state in L.
-template <int HK, class LDS>
+// The split-KV decode work of workgroup g of `grid` (LDS::kNW waves), its LDS state in L. SCORES: every tile's scores go to
+// p.scores, and (m, l) of a sequence that no range cuts to its partial's place, for add_key_weights.
+template <int HK, class LDS, bool SCORES = false>
 __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, const int grid, const LDS& L) {
   using TT = Tile<HK>;
   constexpr bool BTL = LDS::kBtl;
@@ -663,7 +664,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
       // scale goes into the exp2 argument (one FMA); the running max moves (rescaling acc and lsum) only when the
       // tile max exceeds it by more than 8 in log2 units (p <= 256, exact after the final 1 / l); the masks and zero
       // selects run only on a tile that is not fully valid.
-      auto compute = [&](const Tile<HK>& T, int t0, int tok_end, auto&& between) {
+      auto compute = [&](const Tile<HK>& T, int t, int t0, int tok_end, auto&& between) {
         f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < TT::KC; ++kk) s = mfma_16x16x32(T.k[kk], qop[kk], s);
@@ -673,6 +674,10 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
           x[q4] = full || (T.ok && (t0 + jq * 4 + q4) < tok_end) ? s[q4] : -INFINITY;
+        if constexpr (SCORES) {  // step t's scores [H][16 tokens], not scaled
+          if (h < H)
+            *reinterpret_cast<f32x4*>(p.scores + ((int64_t)t * H + h) * kTile + jq * 4) = f32x4{x[0], x[1], x[2], x[3]};
+        }
         // V tile -> LDS, row-major, 16-byte stores; rows of tokens past tok_end or of an unmapped block are zeroed
         // (they meet p = 0 in P V, and unwritten cache slots may hold any bit pattern)
         if (full) {
@@ -736,7 +741,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
           for (int kk = 0; kk < TT::KC; ++kk) qop[kk] = hg == kk / 4 ? qv[kk % 4] : zero4();
           fresh = false;
         }
-        compute(T, (t - lane_val(w_st, kcur)) * kTile, lane_val(w_ctx, kcur), [&]() {
+        compute(T, t, (t - lane_val(w_st, kcur)) * kTile, lane_val(w_ctx, kcur), [&]() {
           if (t + 1 < t_hi) {
             if (ki != kcur) load_q(qv, ki);
             issue(T, blk_pf, ki, t + 1);
@@ -817,6 +822,13 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
           for (int i = 0; i < kDpt / 4; ++i)
             *reinterpret_cast<u32x2*>(p.out + row * p.out_row_stride + (int64_t)hh * kD + d0 + 4 * i) =
                 u32x2{pack_bf16x2(o[i][0] * inv, o[i][1] * inv), pack_bf16x2(o[i][2] * inv, o[i][3] * inv)};
+        }
+        if constexpr (SCORES) {
+          float* part = p.partials + (int64_t)(bs + g) * kPartialFloats;
+          if (tid % kTpr == 0) {
+            part[kMOff + hh] = M;
+            part[kLOff + hh] = Ls;
+          }
         }
       } else {  // cut by a range boundary: partial for decode_merge_kernel, slot b + g
         float* part = p.partials + (int64_t)(bs + g) * kPartialFloats;
@@ -921,6 +933,80 @@ __device__ __forceinline__ void merge_row(const DecodeArgs& p, int b, int part, 
   *reinterpret_cast<u32x4*>(ob) =
       u32x4{pack_bf16x2(o2[0] * inv, o2[1] * inv), pack_bf16x2(o2[2] * inv, o2[3] * inv),
             pack_bf16x2(o2[4] * inv, o2[5] * inv), pack_bf16x2(o2[6] * inv, o2[7] * inv)};
+}
+
+// What the keys of the step layout's steps [W S / N, (W + 1) S / N) received, added to their weights, by wave W of
+// N = 4 weight_wgs (decode_merge_kernel; `lse` is the wave's own LDS). A key's weight at kv head g grows by the sum over
+// g's query heads h of exp2(s c - lse_h), the probabilities of the attention: s are the scores that the split kernel left,
+// lse_h comes from the partials' m and l, the same sum that the output is divided by. The newest token's weight is set: its
+// place may hold anything. Lane = (token, one of four steps), so a head's scores and a kv head's weights are read and
+// written side by side.
+__device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int N, float* lse) {
+  const int lane = threadIdx.x & 63;
+  const int r16 = lane & 15, sub = lane >> 4;
+  const int H = p.num_heads, HK = H / p.group;
+  const int64_t S = p.steps[p.batch], G = p.steps[p.batch + 1];
+  const int r0 = (int)muldiv(W, S, 0, N), r1 = (int)muldiv(W + 1, S, 0, N);
+  if (r0 >= r1) return;
+  // the sequence of step r0: the last that starts at or before it (an empty one shares its start with the next)
+  int b = -1;
+  for (int c = 0; c < p.batch; c += kWave) {
+    const bool at = c + lane < p.batch && p.steps[c + lane] <= r0;
+    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
+  }
+  for (int t = r0; t < r1; ++b) {
+    const int sb = p.steps[b], eb = p.steps[b + 1];
+    if (eb <= t) continue;
+    const int te = min(r1, eb);
+    // the sequence's pieces are those of merge_row; four at a time, head r16
+    const int g_first = (int)muldiv(sb + 1, G, S - 1, S) - 1;
+    const int g_last = (int)min(G - 1, muldiv(eb, G, S - 1, S) - 1);
+    float M = -INFINITY, L = 0.f;
+    for (int gg = g_first + sub; gg <= g_last; gg += 4) {
+      const float* pc = p.partials + (int64_t)(b + gg) * kPartialFloats;
+      const float mc = pc[kMOff + r16], lc = pc[kLOff + r16];
+      const float mn = fmaxf(M, mc);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      L = L * fast_exp2(M - mu) + lc * fast_exp2(mc - mu);
+      M = mn;
+    }
+    const float Mt = col_max4(M);
+    const float Lt = col_sum4(L * fast_exp2(M - (Mt == -INFINITY ? 0.f : Mt)));
+    // (a head without any key: exp2(s c - inf) = 0)
+    lse[r16] = Lt == 0.f ? INFINITY : Mt + __builtin_amdgcn_logf(Lt);
+    wave_lds_sync();
+    int len = 0;
+    if (p.cu_q)
+      len = p.cu_k[b + 1] - p.cu_k[b];
+    else
+      len = p.context_lens[b];
+    const int64_t reach = min((int64_t)len, p.weight_width);
+    const int64_t row = p.weight_rows ? (int64_t)p.weight_rows[b] : p.weight_row0 + b;
+    const bool mine = row >= 0 && row < p.weight_row_count;
+    for (int u = t; u < te; u += 4) {
+      const int step = u + sub;
+      const int64_t tok = (int64_t)(step - sb) * kTile + r16;
+      if (!mine || step >= te || tok >= reach) continue;
+      const float* s = p.scores + (int64_t)step * H * kTile + r16;
+      float* w = p.weights + row * HK * p.weight_width + tok;
+      float x[kMaxHeads];
+#pragma unroll
+      for (int hh = 0; hh < kMaxHeads; ++hh) x[hh] = hh < H ? s[hh * kTile] : -INFINITY;
+      const float w0 = w[0], w1 = HK == 2 ? w[p.weight_width] : 0.f;
+      float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+      for (int hh = 0; hh < kMaxHeads; ++hh) {
+        const float e = hh < H ? fast_exp2(fmaf(x[hh], p.scale_log2, -lse[hh])) : 0.f;
+        a0 += hh < p.group ? e : 0.f;
+        a1 += hh < p.group ? 0.f : e;
+      }
+      const bool fresh = tok == len - 1;
+      w[0] = fresh ? a0 : w0 + a0;
+      if (HK == 2) w[p.weight_width] = fresh ? a1 : w1 + a1;
+    }
+    wave_lds_sync();  // (lse is read before the next sequence's)
+    t = te;
+  }
 }
 
 }  // namespace dec

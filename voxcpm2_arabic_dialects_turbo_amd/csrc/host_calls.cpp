@@ -78,7 +78,11 @@ struct Entry<R (*)(A...)> {
   X(vox_decode_attn_store_fp4)      \
   X(vox_prefill_attn_fp4)           \
   X(vox_fork_kv_blocks)             \
-  X(vox_compact_kv_blocks)
+  X(vox_compact_kv_blocks)          \
+  X(vox_decode_scores_bytes)        \
+  X(vox_decode_attn_weights)        \
+  X(vox_prefill_attn_weights)       \
+  X(vox_evict_kv_tokens)
 
 #define VOX_DEFINE(name)                                                              \
   decltype(&name) g_##name = nullptr;                                                 \

@@ -54,7 +54,6 @@ constexpr int kKsStride = kD + 16;
 constexpr int kVsStride = kD + 24;
 // word 3 of a raw buffer descriptor (32-bit data format; offsets in bytes, range-checked against num_records)
 constexpr int kBufferWord3 = 0x00020000;
-constexpr unsigned kXcds = 8;                  // MI355X: workgroups are dealt round-robin over 8 XCDs
 constexpr unsigned kXcdOrderMinWorkgroups = 1024;
 // Paged caches of other block sizes: 128-row grids of up to this many workgroups take 8-wave workgroups (half of a wave's
 // work per key tile), larger ones 4 waves of 32 rows (fewer LDS reads per MFMA).
@@ -1017,23 +1016,6 @@ __device__ __forceinline__ void store_rows(const PrefillArgs& p, int wid) {
     for (int u = 0; u < kBatch; ++u)
       if (slot[u] >= 0 && slot[u] < p.store_num_slots)
         __builtin_nontemporal_store(val[u], reinterpret_cast<u32x4*>(dst[u] + slot[u] * row));
-  }
-}
-
-// The plain grid's work item of this workgroup (with xcd_order, its XCD's next one)
-__device__ __forceinline__ void grid_item(const PrefillArgs& p, int& qt, int& b, int& g) {
-  qt = blockIdx.x;
-  b = blockIdx.y;
-  g = blockIdx.z;
-  if (p.xcd_order) {
-    const unsigned nwg = gridDim.x * gridDim.y * gridDim.z;
-    const unsigned id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
-    const unsigned xq = nwg / kXcds, xr = nwg % kXcds, xcd = id % kXcds, loc = id / kXcds;
-    const unsigned work = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + loc;
-    qt = (int)(work % gridDim.x);
-    b = (int)((work / gridDim.x) % gridDim.y);
-    g = (int)(work / (gridDim.x * gridDim.y));
-    if (p.causal) qt = (int)gridDim.x - 1 - qt;  // heavy query tiles first
   }
 }
 

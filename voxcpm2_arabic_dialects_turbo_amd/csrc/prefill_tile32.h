@@ -61,7 +61,8 @@ struct Seq {
   int q0, nq, k0, nk, kn0, bid, bt_row;
 };
 
-template <int SRC, int RG, int KS>
+// LSE: every row's log2 of the sum its output is divided by goes to p.lse.
+template <int SRC, int RG, int KS, bool LSE = false>
 __device__ __forceinline__ void item(const PrefillArgs& p, const int qt, const int b, const int g, const Bufs& bufs,
                                      const Seq& seq) {
   constexpr int ROWS = 32 * RG;      // query rows of the item
@@ -507,8 +508,12 @@ __device__ __forceinline__ void item(const PrefillArgs& p, const int qt, const i
         for (int gp = 0; gp < 2; ++gp) *reinterpret_cast<u32x4_a8*>(op + (D0 + dt) * 32 + gp * 16) = o[dt][gp];
     }
   };
+  [[maybe_unused]] auto store_lse = [&](float sum, float max) {
+    if (h == 0 && row_ok) p.lse[((int64_t)q0 + tq) * p.num_heads + head] = sum == 0.f ? INFINITY : max + __builtin_amdgcn_logf(sum);
+  };
   using std::integral_constant;
   if constexpr (KS == 1) {
+    if constexpr (LSE) store_lse(L, m);
     store(integral_constant<int, 0>{}, integral_constant<int, 4>{}, L > 0.f ? 1.f / L : 0.f);
   } else {
     // the two waves of a row block hand each other half of their O: wave ks keeps dims [64 ks, 64 ks + 64)
@@ -535,11 +540,13 @@ __device__ __forceinline__ void item(const PrefillArgs& p, const int qt, const i
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = *reinterpret_cast<const f32x4*>(theirs + j * 1024 + lane * 16);
       float Ls = L;
+      [[maybe_unused]] float Mt = m;
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(m != mt) != 0, 0)) {
         const float M = fmaxf(m, mt);
         const float a = m == M ? 1.f : fast_exp2(m - M), at = mt == M ? 1.f : fast_exp2(mt - M);
         Ls *= a;
         Lt *= at;
+        Mt = M;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           y[j] *= at;
@@ -548,6 +555,7 @@ __device__ __forceinline__ void item(const PrefillArgs& p, const int qt, const i
         }
       }
       Ls += Lt;
+      if constexpr (LSE && OWN == 0) store_lse(Ls, Mt);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -561,7 +569,7 @@ __device__ __forceinline__ void item(const PrefillArgs& p, const int qt, const i
   }
 }
 
-template <int SRC, int RG, int KS>
+template <int SRC, int RG, int KS, bool LSE = false>
 __device__ __forceinline__ void tile(const PrefillArgs& p, const int qt, const int b, const int g, const Bufs& bufs) {
   constexpr int ROWS = 32 * RG;
   const int lane = threadIdx.x & 63;
@@ -600,14 +608,33 @@ __device__ __forceinline__ void tile(const PrefillArgs& p, const int qt, const i
     // source a tile. A layer of a step of 1 x 237 tokens 8.7 -> 7.6 us, 1 x 1500 31.7 -> 23.7, 5 x 1000 44.1 -> 38.2,
     // 2 x 4000 171 -> 146.
     if (kn0 == 0) {
-      item<kRows, RG, KS>(p, qt, b, g, bufs, Seq{q0, nq, q0, nk, 0, 0, -1});
+      item<kRows, RG, KS, LSE>(p, qt, b, g, bufs, Seq{q0, nq, q0, nk, 0, 0, -1});
       return;
     }
   }
-  item<SRC, RG, KS>(p, qt, b, g, bufs, Seq{q0, nq, k0, nk, kn0, bid, bt_row});
+  item<SRC, RG, KS, LSE>(p, qt, b, g, bufs, Seq{q0, nq, k0, nk, kn0, bid, bt_row});
 }
 
 }  // namespace pf32
+
+constexpr unsigned kXcds = 8;  // MI355X: workgroups are dealt round-robin over 8 XCDs
+
+// The plain grid's work item of this workgroup (with xcd_order, its XCD's next one)
+__device__ __forceinline__ void grid_item(const PrefillArgs& p, int& qt, int& b, int& g) {
+  qt = blockIdx.x;
+  b = blockIdx.y;
+  g = blockIdx.z;
+  if (p.xcd_order) {
+    const unsigned nwg = gridDim.x * gridDim.y * gridDim.z;
+    const unsigned id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+    const unsigned xq = nwg / kXcds, xr = nwg % kXcds, xcd = id % kXcds, loc = id / kXcds;
+    const unsigned work = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + loc;
+    qt = (int)(work % gridDim.x);
+    b = (int)((work / gridDim.x) % gridDim.y);
+    g = (int)(work / (gridDim.x * gridDim.y));
+    if (p.causal) qt = (int)gridDim.x - 1 - qt;  // heavy query tiles first
+  }
+}
 
 }  // namespace
 

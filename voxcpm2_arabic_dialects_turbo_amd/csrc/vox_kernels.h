@@ -61,6 +61,16 @@ struct DecodeArgs {
   int64_t new_v_stride;
   int64_t copy_rows;
   int copy_wgs;
+  // Weights mode (launch_decode_weights): what every key receives is added to row weight_rows[b] (weight_row0 + b where that
+  // is null; rows outside [0, weight_row_count): none) of weights fp32 [weight_row_count, HK, weight_width], by merge
+  // workgroups [merges, merges + weight_wgs); keys at or past weight_width: left out. scores: fp32 [steps, H, 16].
+  float* scores;
+  float* weights;
+  const int32_t* weight_rows;
+  int64_t weight_row0;
+  int64_t weight_row_count;
+  int64_t weight_width;
+  int weight_wgs;
 };
 
 struct PrefillArgs {
@@ -119,6 +129,44 @@ struct PrefillArgs {
   // nk - nq and later (its nq new tokens, stored by this launch's merge kernel) come from k_src / v_src rows
   // cu_q[b] + (position - (nk - nq)) instead of the cache; the earlier keys through the block table as usual
   int new_from_rows;
+  float* lse;                 // launch_prefill_lse: fp32 [rows, H], log2 of sum_j exp2(scaled score), +inf for a row without keys
+};
+
+// What the keys of a varlen call received (launch_key_weights), after launch_prefill_lse of the same call has left a.lse.
+struct KeyWeightsArgs {
+  PrefillArgs a;              // cu_q, cu_k; packed keys or paged ones
+  float* weights;             // fp32 [row_count, HK, width]
+  const int32_t* rows;        // int32 [batch], or null: row b (outside [0, row_count): none)
+  int64_t row_count;
+  int64_t width;              // keys at or past it: left out
+};
+
+// Tokens dropped from a paged cache (kv_evict.hip): of every sequence longer than `budget` its first `sinks`, last `recent`
+// and, for every layer and kv head, the budget - sinks - recent heaviest others, moved to the front in their order.
+struct EvictArgs {
+  uint8_t* kv;                  // [layers][2][num_blocks] blocks of block_size * num_heads * (head_bytes + scale_bytes) bytes
+  int layers;
+  int64_t num_blocks;
+  int block_size;
+  int num_heads;                // kv heads
+  int head_bytes;               // of a token's head: a multiple of 16
+  int scale_bytes;              // 0, or 4: a block's scales behind its slots
+  const int32_t* block_tables;  // int32 [batch, bt_stride], first max_blocks columns used
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* context_lens;  // int32 [batch]
+  int batch;
+  float* weights;               // fp32 [layers, row_count, num_heads, width]
+  const int32_t* rows;          // int32 [batch], or null: row b (outside [0, row_count): the sequence stays as it is)
+  int64_t row_count;
+  int64_t width;                // >= max_blocks * block_size
+  int budget, sinks, recent;    // budget > 0, sinks + recent <= budget
+  const int32_t* into;          // int32 [batch, into_stride], first max_blocks columns, or null: blocks that take the kept
+  int64_t into_stride;          // tokens in place of the table's own (-1: those)
+  int32_t* moves;               // int32 [layers, batch, num_heads, kept]: the slot that place j's token comes from, -1: it is
+  int64_t kept;                 // there; kept = min(budget, max_blocks * block_size)
+  int32_t* new_tables;          // int32 [batch, max_blocks]
+  int32_t* new_lens;            // int32 [batch]
 };
 
 // Rows of a 4-bit cache (fp4_common.h has the format): quantised into their slots, or read back.
@@ -200,7 +248,16 @@ hipError_t launch_decode_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t 
 hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t stream);
 hipError_t launch_decode_merge_fp4(const DecodeArgs& a, hipStream_t stream);
 
+// Decode in weights mode.
+hipError_t launch_decode_weights(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
+
 hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
+
+// Causal varlen attention that also leaves every row's a.lse, then what the keys received (key_weights.hip).
+hipError_t launch_prefill_lse(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
+hipError_t launch_key_weights(const KeyWeightsArgs& k, int max_seqlen_k, hipStream_t stream);
+
+hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 
 // The same and the decode rows d of a mixed step (skip_single) in one launch, then their merge; up to 256 sequences.
 bool mixed_fp4_fits(const PrefillArgs& a, int max_seqlen_q);

@@ -17,6 +17,10 @@ Caches held in 4 bits (uint8 planes, see ops_fp4) take the same branches: the st
 decode steps and prefills through block tables attend over what the caches then hold (a prefill without block tables over
 the step's own rows).
 
+A layer with ``key_weights`` (fp32 [rows, HK, width], see ops_weights; ``runner.allocate_key_weights`` sets them) adds to
+them what the step's attention gives every key, in every step whose context has ``weight_rows``; its bf16 caches and outputs
+are those of the step without (a step over 4-bit caches adds only in a prefill over its own rows, and is refused else).
+
 Every branch runs a HIP kernel of libvoxattn.so; nothing here synchronizes or allocates outside torch, so the
 module can be captured into HIP graphs exactly where the reference captures its decode step.
 """
@@ -33,6 +37,7 @@ from .context import get_context
 from .ops import (decode_attention, flash_attn_func, flash_attn_varlen_func, flash_attn_with_kvcache, planning,
                   prefill_attention_store, store_kvcache)
 from .ops_fp4 import decode_attention_fp4, is_fp4_cache
+from .ops_weights import decode_attention_weights, varlen_attention_weights
 
 __all__ = ["Attention", "store_kvcache"]
 
@@ -113,6 +118,7 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
+        self.key_weights = None
         self.is_causal = is_causal
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
@@ -120,6 +126,8 @@ class Attention(nn.Module):
             context = get_context()
             k_cache, v_cache = self.k_cache, self.v_cache
             cached = bool(k_cache.numel() and v_cache.numel())
+            if cached and self.key_weights is not None and context.weight_rows is not None:
+                return self._forward_weights(context, q, k, v)
             fp4 = cached and is_fp4_cache(k_cache)
             if fp4 and not context.is_prefill and context.slot_mapping is not None and k.dim() == 3 \
                     and k.shape[0] == q.shape[0]:
@@ -178,3 +186,19 @@ class Attention(nn.Module):
         else:  # non-causal, no KV cache
             o = flash_attn_func(q, k, v, softmax_scale=self.scale, causal=False)
         return o
+
+    def _forward_weights(self, context, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+        """A step that adds to key_weights."""
+        k_cache, v_cache, tables = self.k_cache, self.v_cache, context.block_tables
+        if not context.is_prefill:
+            _check_riding_store(context, k_cache.shape[1], decode=True)
+            return decode_attention_weights(q, k_cache, v_cache, context.context_lens, tables, self.scale,
+                                            self.key_weights, context.weight_rows, key=k, value=v,
+                                            slot_mapping=context.slot_mapping, plan=_plan_key(context)).unsqueeze(1)
+        if tables is not None and is_fp4_cache(k_cache):  # (refused before anything is stored)
+            raise TypeError("key_weights: attention through block tables takes bf16 caches")
+        store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
+        return varlen_attention_weights(q, k, v, self.key_weights, context.weight_rows, cu_seqlens_q=context.cu_seqlens_q,
+                                        cu_seqlens_k=context.cu_seqlens_k, max_seqlen_q=context.max_seqlen_q,
+                                        max_seqlen_k=context.max_seqlen_k, softmax_scale=self.scale, block_table=tables,
+                                        k_cache=k_cache, v_cache=v_cache)

@@ -1,0 +1,209 @@
+"""Attention that also adds up what every cached token receives of it, for eviction by that (kernels.kv_evict).
+
+``key_weights`` is fp32 [rows, HK, width], contiguous, one plane per layer: for the sequence whose row it is and each kv
+head, every cached token's sum of probabilities over the kv head's query heads and all queries so far, at the token's
+position. ``weight_rows`` (int [B]) says which row is whose, so that streams may come and go in any order; left out,
+sequence b has row b, and a row outside [0, rows) (-1) keeps none. No two sequences of a call share a row. The width covers
+what the block tables reach (packed keys: max_seqlen_k).
+
+A token that is new in a call starts with what it gets there, whatever its place held; the others get theirs on top. So a
+row needs no clearing between the sequences that have it in turn. ``runner.allocate_key_weights`` makes the planes, and
+``Attention.forward`` adds to its layer's.
+
+The attention itself is that of ``ops`` over bf16 caches. Like its operators these run on torch's current stream of the
+tensors' device, allocate with torch, never synchronize and can be captured into HIP graphs. head_dim 128, softmax_scale
+positive. No reference counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ops import HEAD_DIM, MAX_DECODE_HEADS, _as_i32, _check_cuda, _flat, _plan_recorded, store_kvcache
+from .ops_fp4 import _ids, _on, _row_stride, _table, _workspace
+
+
+def _weights(fn: str, key_weights: torch.Tensor, weight_rows: torch.Tensor | None, batch: int, hk: int, reach: int,
+             dev: torch.device) -> torch.Tensor | None:
+    """The checked ``weight_rows`` as int32 [batch], None where sequence b has row b."""
+    if key_weights.dtype != torch.float32:
+        raise TypeError(f"{fn}: key_weights must be fp32, got {key_weights.dtype}")
+    if key_weights.dim() != 3 or key_weights.shape[1] != hk or not key_weights.is_contiguous():
+        raise ValueError(f"{fn}: key_weights must be contiguous [rows, {hk}, width], got {tuple(key_weights.shape)}")
+    if key_weights.shape[2] < reach:
+        raise ValueError(f"{fn}: key_weights hold {key_weights.shape[2]} tokens a row, the keys may be {reach}")
+    if key_weights.device != dev:
+        raise ValueError(f"all tensors must be on the same GPU, got {key_weights.device} and {dev}")
+    if weight_rows is None:
+        if key_weights.shape[0] < batch:
+            raise ValueError(f"{fn}: key_weights have {key_weights.shape[0]} rows for {batch} sequences")
+        return None
+    if weight_rows.numel() != batch:
+        raise ValueError(f"{fn}: weight_rows must hold one row per sequence")
+    if key_weights.shape[0] == 0:
+        raise ValueError(f"{fn}: key_weights have no rows")
+    if weight_rows.device != dev:
+        raise ValueError(f"all tensors must be on the same GPU, got {weight_rows.device} and {dev}")
+    return _ids(weight_rows, "weight_rows")
+
+
+def _query(fn: str, q: torch.Tensor, out: torch.Tensor | None, dev: torch.device, contiguous: bool
+           ) -> tuple[torch.Tensor, torch.Tensor]:
+    """q with token rows apart from each other, and where the output goes."""
+    n, H, D = q.shape
+    if D != HEAD_DIM or q.stride(2) != 1 or (q.stride(1) != D and H > 1):
+        raise ValueError(f"{fn}: q must be [rows, H, {HEAD_DIM}] with contiguous heads, got {tuple(q.shape)} {q.stride()}")
+    if out is None:
+        out = torch.empty(n, H, D, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 or out.stride(1) != D \
+            or (contiguous and not out.is_contiguous()):
+        raise ValueError(f"{fn}: out must be a bf16 [{n}, {H}, {D}] with contiguous heads on {dev}")
+    return q.contiguous() if n > 1 and q.stride(0) < H * D else q, out
+
+
+def _caches(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int]:
+    """(num_blocks, block_size, HK) of a pair of bf16 caches."""
+    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+        raise TypeError(f"{fn} takes bf16 caches, got {k_cache.dtype} and {v_cache.dtype}")
+    if k_cache.dim() != 4 or k_cache.shape[3] != HEAD_DIM or v_cache.shape != k_cache.shape \
+            or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{fn}: caches must be contiguous [num_blocks, block_size, HK, {HEAD_DIM}] of one shape")
+    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[2]
+
+
+def _new_rows(fn: str, key: torch.Tensor, value: torch.Tensor, hk: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Key and value rows [N, hk, 128] bf16 with contiguous heads, token rows apart from each other."""
+    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+        raise TypeError(f"{fn}: key and value must be bf16, got {key.dtype} and {value.dtype}")
+    if key.dim() != 3 or key.shape[1:] != (hk, HEAD_DIM) or value.shape != key.shape:
+        raise ValueError(f"{fn}: key and value must be [N, {hk}, {HEAD_DIM}], got {tuple(key.shape)} and {tuple(value.shape)}")
+    for t in (key, value):
+        if t.stride(2) != 1 or (t.stride(1) != HEAD_DIM and hk > 1):
+            raise ValueError(f"{fn}: key and value heads must be contiguous, got strides {t.stride()}")
+    return tuple(t.contiguous() if t.shape[0] > 1 and t.stride(0) < hk * HEAD_DIM else t for t in (key, value))
+
+
+def _scale(fn: str, softmax_scale: float) -> float:
+    if not softmax_scale > 0:
+        raise ValueError(f"{fn}: softmax_scale must be positive, got {softmax_scale}")
+    return float(softmax_scale)
+
+
+def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, context_lens: torch.Tensor,
+                             block_tables: torch.Tensor, softmax_scale: float, key_weights: torch.Tensor,
+                             weight_rows: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                             key: torch.Tensor | None = None, value: torch.Tensor | None = None,
+                             slot_mapping: torch.Tensor | None = None, plan=None) -> torch.Tensor:
+    """``ops.decode_attention`` (one query per sequence over its first context_lens[b] cached tokens, with key / value /
+    slot_mapping the step's rows stored in the same call), adding to ``key_weights`` what every key received: for token j
+    and kv head g the sum of g's query heads' probabilities, on top of the weight for j < context_lens[b] - 1, in its place
+    for the newest. Returns o [B, H, 128] bf16, zeros where context_lens[b] is 0 (whose row is left alone).
+
+    The call takes scratch for the scores of every token that the tables reach, 4 H bytes a token. ``plan``: as
+    decode_attention's; planned calls share the device's decode workspace and must not overlap other calls on it."""
+    fn = "decode_attention_weights"
+    if q.dim() != 3 or q.dtype != torch.bfloat16:
+        raise TypeError(f"{fn}: q must be bf16 [B, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
+    blocks, bs, hk = _caches(fn, k_cache, v_cache)
+    B, H, D = q.shape
+    if hk not in (1, 2) or H == 0 or H % hk or H > MAX_DECODE_HEADS:
+        raise ValueError(f"decode supports H <= {MAX_DECODE_HEADS} query heads over 1 or 2 KV heads, got {H}/{hk}")
+    if context_lens.numel() != B or block_tables.dim() != 2 or block_tables.shape[0] < B:
+        raise ValueError("context_lens must be [B] and block_tables [B, max_blocks]")
+    scale = _scale(fn, softmax_scale)
+    dev = _check_cuda(q, k_cache, v_cache, context_lens, block_tables)
+    bt, bt_stride = _table(block_tables)
+    mb = bt.shape[1]
+    rows = _weights(fn, key_weights, weight_rows, B, hk, mb * bs, dev)
+    q, out = _query(fn, q, out, dev, True)
+    rides = False
+    if key is not None:
+        if value is None or slot_mapping is None:
+            raise ValueError(f"{fn}: key, value and slot_mapping go together")
+        _check_cuda(q, key, value, slot_mapping)
+        key, value = _new_rows(fn, key, value, hk)
+        if key.shape[0] != B or slot_mapping.numel() != B:
+            raise ValueError(f"{fn}: key, value and slot_mapping must hold {B} rows")
+        slots = _ids(slot_mapping, "slot_mapping")
+        # (rows that 16-byte loads cannot take are stored by a call of their own)
+        rides = (key.data_ptr() | value.data_ptr()) % 16 == 0 and (_row_stride(key) | _row_stride(value)) % 8 == 0
+    elif value is not None or slot_mapping is not None:
+        raise ValueError(f"{fn}: key, value and slot_mapping go together")
+    if B == 0:
+        return out
+    lens = _as_i32(_flat(context_lens), "context_lens")
+    lib = _lib.load()
+    with _on(dev):
+        if key is not None and not rides:
+            store_kvcache(key, value, k_cache, v_cache, slots)
+        ws, mode, recorded = _workspace(lib, dev, B, plan, "decode_weights", rides, B, mb, bt_stride, H, hk, bs)
+        scores = torch.empty(lib.vox_decode_scores_bytes(B, mb, bs, H), dtype=torch.uint8, device=dev)
+        _lib.check(lib.vox_decode_attn_weights(
+            q.data_ptr(), _row_stride(q), key.data_ptr() if rides else None, value.data_ptr() if rides else None,
+            _row_stride(key) if rides else 0, _row_stride(value) if rides else 0, slots.data_ptr() if rides else None,
+            k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, mb, lens.data_ptr(), B, H, hk, D,
+            scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), key_weights.shape[0],
+            key_weights.shape[2], scores.data_ptr(), scores.numel(), mode, ws.data_ptr(), ws.numel(), out.data_ptr(),
+            _lib.stream_handle(dev)), fn)
+    _plan_recorded(dev, recorded)
+    return out
+
+
+def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, key_weights: torch.Tensor,
+                             weight_rows: torch.Tensor | None = None, *, cu_seqlens_q: torch.Tensor,
+                             cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float,
+                             block_table: torch.Tensor | None = None, k_cache: torch.Tensor | None = None,
+                             v_cache: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``ops.varlen_attention`` (causal: sequence b's queries q [T, H, 128] are the last of its keys, from packed rows k / v
+    [Tk, HK, 128] or, with block_table, from the caches), adding to ``key_weights`` what every key received: for token j and
+    kv head g the sum of the probabilities of b's queries at g's query heads, in place of the weight for the step's own
+    tokens, the last cu_seqlens_q[b + 1] - cu_seqlens_q[b], on top of it for the earlier ones. Returns o [T, H, 128] bf16,
+    zeros for a query that sees no key. A sequence without queries keeps its weights.
+
+    No sequence has more than max_seqlen_q queries or max_seqlen_k keys (further ones are left out). H / HK divides 128, and
+    cache blocks are a multiple of 64 tokens."""
+    fn = "varlen_attention_weights"
+    if q.dim() != 3 or q.dtype != torch.bfloat16:
+        raise TypeError(f"{fn}: q must be bf16 [T, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
+    T, H, D = q.shape
+    B = cu_seqlens_q.numel() - 1
+    if cu_seqlens_k.numel() != B + 1:
+        raise ValueError("cu_seqlens_k must have as many entries as cu_seqlens_q")
+    scale = _scale(fn, softmax_scale)
+    dev = _check_cuda(q, cu_seqlens_q, cu_seqlens_k)
+    if block_table is not None:
+        if k_cache is None or v_cache is None:
+            raise ValueError(f"{fn}: block_table given without caches")
+        blocks, bs, hk = _caches(fn, k_cache, v_cache)
+        if bs % 64:
+            raise ValueError(f"{fn}: cache blocks must be a multiple of 64 tokens, got {bs}")
+        if block_table.dim() != 2 or block_table.shape[0] < B:
+            raise ValueError("block_table must be [B, max_blocks]")
+        _check_cuda(q, k_cache, v_cache, block_table)
+        bt, bt_stride = _table(block_table)
+        reach = min(int(max_seqlen_k), bt.shape[1] * bs)
+        keys = (None, None, 0, 0, k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, bt.shape[1])
+    else:
+        if k is None or v is None:
+            raise ValueError(f"{fn}: packed keys and values required without a block table")
+        _check_cuda(q, k, v)
+        hk = k.shape[1] if k.dim() == 3 else 0
+        k, v = _new_rows(fn, k, v, hk)
+        reach = int(max_seqlen_k)
+        keys = (k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), None, None, 0, 0, None, 0, 0)
+    if hk == 0 or H == 0 or H % hk:
+        raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {hk}")
+    rows = _weights(fn, key_weights, weight_rows, max(B, 0), hk, reach, dev)
+    q, out = _query(fn, q, out, dev, False)
+    if T == 0 or B <= 0 or max_seqlen_q <= 0:
+        return out
+    cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
+    lib = _lib.load()
+    with _on(dev):
+        lse = torch.empty(T, H, dtype=torch.float32, device=dev)
+        _lib.check(lib.vox_prefill_attn_weights(
+            q.data_ptr(), _row_stride(q), *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, int(max_seqlen_q), reach, T, H, hk, D,
+            scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), key_weights.shape[0],
+            key_weights.shape[2], lse.data_ptr(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
+    return out

@@ -215,10 +215,15 @@ def prefill_slots(batch: _Batch, block_size: int) -> np.ndarray:
 
 
 def prepare_prefill_context(seqs, block_size: int, device="cuda", graphs: bool = False,
-                            staging: StepStaging | None = None) -> torch.Tensor:
+                            staging: StepStaging | None = None, weight_rows: Sequence[int] | None = None,
+                            evicted: Sequence[int] | None = None) -> torch.Tensor:
     """Sets the prefill context of ``seqs`` and returns the positions of their uncached tokens (int64, on
     ``device``). Block tables are included when some sequence has a cached prefix or ``graphs`` is set (the
-    prefill graphs read every key through the tables) (reference: nanovllm_voxcpm/engine/model_runner.py:851-911)."""
+    prefill graphs read every key through the tables) (reference: nanovllm_voxcpm/engine/model_runner.py:851-911).
+
+    ``weight_rows``: every sequence's row in the layers' key_weights (-1: none), and the step adds to them. ``evicted``: how
+    many tokens each has lost (kernels.kv_evict): its lengths count what the cache holds, its positions go on behind the
+    text."""
     batch = _Batch.of(seqs)
     n = len(seqs)
     q = batch.length - batch.cached
@@ -230,8 +235,14 @@ def prepare_prefill_context(seqs, block_size: int, device="cuda", graphs: bool =
     specs = [(np.int64, (total_q,)), (np.int32, (n + 1,)), (np.int32, (n + 1,)), (np.int32, (slots.size,))]
     if with_tables:
         specs.append((np.int32, (n, int(batch.nblk.max(initial=0)))))
+    if weight_rows is not None:
+        specs.append((np.int32, (n,)))
     views = stage.layout(specs)
     np.add(np.repeat(batch.cached - (ends_q - q), q), np.arange(total_q), out=views[0])  # _runs(cached, q)
+    if evicted is not None:
+        views[0] += np.repeat(_per_sequence(evicted, n), q)
+    if weight_rows is not None:
+        views[-1][:] = _per_sequence(weight_rows, n)
     views[1][0] = views[2][0] = 0
     views[1][1:] = ends_q
     np.cumsum(batch.length, out=views[2][1:])
@@ -240,29 +251,45 @@ def prepare_prefill_context(seqs, block_size: int, device="cuda", graphs: bool =
         batch.padded_tables(views[4])
     dev = stage.upload()
     set_context(True, dev[1], dev[2], int(q.max(initial=0)), int(batch.length.max(initial=0)), dev[3], None,
-                dev[4] if with_tables else None)
+                dev[4] if with_tables else None, dev[-1] if weight_rows is not None else None)
     return dev[0]
 
 
-def prepare_decode_context(seqs, block_size: int, device="cuda", staging: StepStaging | None = None
+def _per_sequence(values: Sequence[int], n: int) -> np.ndarray:
+    out = np.asarray(values, dtype=np.int64).reshape(-1)
+    if out.size != n:
+        raise ValueError(f"one value per sequence: {out.size} for {n}")
+    return out
+
+
+def prepare_decode_context(seqs, block_size: int, device="cuda", staging: StepStaging | None = None,
+                           weight_rows: Sequence[int] | None = None, evicted: Sequence[int] | None = None
                            ) -> torch.Tensor:
     """Sets the decode context of ``seqs`` (one new token each, at position length - 1, stored in the table's last
-    block) and returns the positions (reference: nanovllm_voxcpm/engine/model_runner.py:913-938)."""
+    block) and returns the positions (reference: nanovllm_voxcpm/engine/model_runner.py:913-938). ``weight_rows`` and
+    ``evicted``: as prepare_prefill_context's."""
     batch = _Batch.of(seqs)
     n = len(seqs)
     if (batch.nblk == 0).any():
         raise ValueError("decode: every sequence needs a block for its new token")
     width = int(batch.nblk.max(initial=0))
     stage = staging or StepStaging(device)
-    pos, slot, lens, tables = stage.layout([(np.int64, (n,)), (np.int32, (n,)), (np.int32, (n,)),
-                                            (np.int32, (n, width))])
+    specs = [(np.int64, (n,)), (np.int32, (n,)), (np.int32, (n,)), (np.int32, (n, width))]
+    if weight_rows is not None:
+        specs.append((np.int32, (n,)))
+    pos, slot, lens, tables, *rows = stage.layout(specs)
     np.subtract(batch.length, 1, out=pos)
     last_entry = batch.flat[batch.row_start + batch.nblk - 1]
     slot[:] = last_entry * block_size + pos % block_size
     lens[:] = batch.length
     batch.padded_tables(tables)
+    if evicted is not None:  # (the slot is that of the length)
+        pos += _per_sequence(evicted, n)
+    if rows:
+        rows[0][:] = _per_sequence(weight_rows, n)
     dev = stage.upload()
-    set_context(False, slot_mapping=dev[1], context_lens=dev[2], block_tables=dev[3])
+    set_context(False, slot_mapping=dev[1], context_lens=dev[2], block_tables=dev[3],
+                weight_rows=dev[4] if rows else None)
     return dev[0]
 
 
@@ -327,20 +354,41 @@ def allocate_kv_cache(model_or_modules, num_blocks: int, block_size: int, dtype=
     return None
 
 
+def allocate_key_weights(model_or_modules, rows: int, max_tokens: int, device="cuda") -> torch.Tensor:
+    """Allocates what ``ops_weights`` adds up, zeros [layers, rows, HK, max_tokens] in fp32, and gives every causal
+    Attention its plane as ``key_weights``. A row for each sequence that may be served at once; max_tokens: what the widest
+    block table reaches. A sequence that takes over a row starts with the step's own tokens; one that starts behind tokens
+    cached for another (a shared prefix, a fork) copies the other's row, or clears it: ``weights[:, row] = ...``."""
+    if rows <= 0 or max_tokens <= 0:
+        raise ValueError("rows and max_tokens must be positive")
+    modules = causal_attention_modules(model_or_modules) if isinstance(model_or_modules, torch.nn.Module) \
+        else list(model_or_modules)
+    heads = {m.num_kv_heads for m in modules}
+    if len(heads) != 1:
+        raise ValueError(f"key weights take layers with one number of kv heads, got {sorted(heads)}")
+    weights = torch.zeros(len(modules), rows, heads.pop(), max_tokens, dtype=torch.float32, device=device)
+    for i, m in enumerate(modules):
+        m.key_weights = weights[i]
+    return weights
+
+
 class DecodeGraphBuffers:
     """Static decode-context buffers that a captured decode graph reads (reference:
-    nanovllm_voxcpm/engine/model_runner.py:1150-1152 allocation, :1558-1566 per-step load)."""
+    nanovllm_voxcpm/engine/model_runner.py:1150-1152 allocation, :1558-1566 per-step load). ``key_weights``: the graph adds
+    to the layers' key weights, and the buffers hold the step's rows too (-1 past the batch)."""
 
-    def __init__(self, max_bs: int, max_num_blocks: int, device="cuda"):
+    def __init__(self, max_bs: int, max_num_blocks: int, device="cuda", key_weights: bool = False):
         self.max_bs = max_bs
         self.slot_mapping = torch.zeros(max_bs, dtype=torch.int32, device=device)
         self.context_lens = torch.zeros(max_bs, dtype=torch.int32, device=device)
         self.block_tables = torch.zeros(max_bs, max_num_blocks, dtype=torch.int32, device=device)
+        self.weight_rows = torch.full((max_bs,), -1, dtype=torch.int32, device=device) if key_weights else None
 
     def bind(self, bs: int) -> None:
         """Sets the decode context to the first ``bs`` rows of the static buffers (done before capture)."""
         set_context(False, slot_mapping=self.slot_mapping[:bs], context_lens=self.context_lens[:bs],
-                    block_tables=self.block_tables[:bs])
+                    block_tables=self.block_tables[:bs],
+                    weight_rows=None if self.weight_rows is None else self.weight_rows[:bs])
 
     def load(self, bs: int | None = None) -> None:
         """Copies the current (eager-built) decode context into the static buffers, as run_model does."""
@@ -351,6 +399,10 @@ class DecodeGraphBuffers:
         self.context_lens.zero_()
         self.context_lens[:n] = ctx.context_lens
         self.block_tables[:n, :ctx.block_tables.size(1)] = ctx.block_tables
+        if self.weight_rows is not None:
+            self.weight_rows.fill_(-1)
+            if ctx.weight_rows is not None:
+                self.weight_rows[:n] = ctx.weight_rows
 
 
 def graph_batch_sizes(max_bs: int) -> list[int]:
