@@ -400,14 +400,15 @@ def test_c_scores_bytes():
 
 
 PREFILL_C = dict(q=P, qs=2048, key=P, value=P, ks=256, vs=256, kc=None, vc=None, blocks=0, bs=0, bt=None, bts=0, mb=0, cq=P,
-                 ck=P, batch=2, mq=4, mk=4, n=8, h=16, hk=2, d=128, scale=0.1, w=P, rows=None, n_rows=2, width=128, lse=P,
-                 out=P, outs=2048, stream=None)
+                 ck=P, batch=2, mq=4, mk=4, n=8, h=16, hk=2, d=128, scale=0.1, w=P, rows=None, n_rows=2, width=128,
+                 scratch=P, scratch_bytes=1 << 30, out=P, outs=2048, stream=None)
 PAGED = dict(key=None, value=None, ks=0, vs=0, kc=P, vc=P, blocks=4, bs=64, bt=P, bts=2, mb=2)
 
 
 @pytest.mark.parametrize("kw,match", [
     (dict(batch=-1), "negative"), (dict(mq=-1), "negative"), (dict(mk=-1), "negative"), (dict(n=-1), "negative"),
-    (dict(cq=None), "null"), (dict(lse=None), "null"), (dict(out=None), "null"), (dict(w=None), "key_weights"),
+    (dict(cq=None), "null"), (dict(out=None), "null"), (dict(scratch=None), "scratch"), (dict(scratch=P + 8), "scratch"),
+    (dict(scratch_bytes=8 * 16 * 4 - 1), "needed"), (dict(qs=1 << 24), "2^24"), (dict(w=None), "key_weights"),
     (dict(scale=-0.1), "positive"), (dict(outs=100), "out row stride"), (dict(out=P + 2), "alignment"),
     (dict(batch=70000), "65535"), (dict(key=None), "null key"), (dict(h=24, qs=3200, outs=3200), "divide 128"), (dict(d=64), "head_dim"),
     (dict(PAGED, bs=32), "multiple of 64"), (dict(PAGED, bs=0), "multiple of 64"), (dict(PAGED, mb=1 << 25, bts=1 << 25), "too wide"),

@@ -1106,24 +1106,52 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
   return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream, vox::launch_decode_weights);
 }
 
+namespace {
+// Scratch of a varlen call that adds to key weights, each part 256-byte aligned: lse [num_tokens, num_heads], then the parts'
+// sums [sequences of a launch, num_kv_heads, parts, max_k]
+struct WeightsScratch {
+  int part_rows, parts;
+  size_t partials, total;
+};
+WeightsScratch weights_scratch(int64_t num_tokens, int batch, int max_q, int max_k, int num_heads, int num_kv_heads) {
+  WeightsScratch s;
+  const int group = num_heads / num_kv_heads;
+  s.part_rows = vox::key_weights_part_rows(num_tokens, batch, max_q, max_k, group, num_kv_heads);
+  s.parts = (int)(((int64_t)max_q * group + s.part_rows - 1) / s.part_rows);
+  s.partials = round256((size_t)num_tokens * num_heads * 4);
+  const size_t slice = batch < vox::kMaxSeqPerLaunch ? batch : vox::kMaxSeqPerLaunch;
+  s.total = s.partials + (s.parts > 1 ? round256(slice * num_kv_heads * s.parts * (size_t)max_k * 4) : 0);
+  return s;
+}
+}  // namespace
+
+size_t vox_prefill_weights_bytes(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int num_heads,
+                                 int num_kv_heads) {
+  if (num_tokens <= 0 || batch <= 0 || max_seqlen_q <= 0 || max_seqlen_k < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads)
+    return 0;
+  return weights_scratch(num_tokens, batch, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads).total;
+}
+
 int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
                              int64_t key_row_stride, int64_t value_row_stride, const void* k_cache, const void* v_cache,
                              int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                              int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
                              int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads, int num_kv_heads,
                              int head_dim, float softmax_scale, float* key_weights, const int32_t* weight_rows,
-                             int64_t num_weight_rows, int64_t weight_width, float* lse, void* out,
-                             int64_t out_row_stride, void* stream) {
+                             int64_t num_weight_rows, int64_t weight_width, void* scratch,
+                             size_t scratch_bytes, void* out, int64_t out_row_stride, void* stream) {
   const char* fn = "prefill_attn_weights";
   if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_tokens < 0)
     return fail(VOX_EINVAL, "%s: negative batch, max_seqlen_q, max_seqlen_k or num_tokens", fn);
   if (batch == 0 || max_seqlen_q == 0 || num_tokens == 0) return VOX_OK;
-  if (!cu_seqlens_q || !cu_seqlens_k || !out || !lse) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (!cu_seqlens_q || !cu_seqlens_k || !out) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
   int st = weights_setup(fn, key_weights, num_weight_rows, weight_width, softmax_scale);
   if (st != VOX_OK) return st;
   if (out_row_stride < (int64_t)num_heads * head_dim || out_row_stride % 4 || ((uintptr_t)out & 7u))
     return fail(VOX_EINVAL, "%s: bad out row stride or alignment", fn);
   if (batch > 65535 || num_kv_heads > 65535) return fail(VOX_EINVAL, "%s: more than 65535 sequences or kv heads", fn);
+  if (q_row_stride >= (1 << 24)) return fail(VOX_EINVAL, "%s: q row stride must be below 2^24 elements", fn);
   if (block_tables && (block_size <= 0 || block_size % 64))
     return fail(VOX_EINVAL, "%s: block_size %d must be a positive multiple of 64", fn, block_size);
   if (block_tables && (int64_t)max_blocks * block_size > (1 << 30))
@@ -1136,14 +1164,21 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   k.a.out = (uint16_t*)out;
   k.a.out_row_stride = out_row_stride;
   k.a.row_limit = num_tokens;
-  k.a.lse = lse;
+  const WeightsScratch ws = weights_scratch(num_tokens, batch, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads);
+  if (!scratch || !aligned16(scratch) || scratch_bytes < ws.total)
+    return fail(VOX_EINVAL, "%s: scratch of %zu bytes (16-byte aligned), %zu needed", fn, scratch_bytes, ws.total);
+  k.a.lse = (float*)scratch;
   k.weights = key_weights;
   k.rows = weight_rows;
   k.row_count = num_weight_rows;
   k.width = weight_width;
+  k.max_k = max_seqlen_k;
+  k.part_rows = ws.part_rows;
+  k.max_parts = ws.parts;
+  k.partials = (float*)((char*)scratch + ws.partials);
   st = hip_status(vox::launch_prefill_lse(k.a, max_seqlen_q, (hipStream_t)stream), "prefill_attn_weights launch");
   if (st != VOX_OK) return st;
-  return hip_status(vox::launch_key_weights(k, max_seqlen_k, (hipStream_t)stream), "prefill_attn_weights sums launch");
+  return hip_status(vox::launch_key_weights(k, (hipStream_t)stream), "prefill_attn_weights sums launch");
 }
 
 int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_bytes,

@@ -9,6 +9,8 @@
 // (the A operand of the score MFMA) and takes the 32-row query tiles qw, qw + QW, ... from the first that sees its keys.
 // Rows are (token, query head of g), so S^T[32 keys x 32 rows] has a row's scores in one lane column and its lse in one
 // register; 16 fma, exp2 and adds a tile behind 8 MFMAs. The lanes' sums meet in LDS at the end.
+#include <type_traits>
+
 #include "prefill_tile32.h"
 #include "vox_common.h"
 #include "vox_kernels.h"
@@ -32,77 +34,304 @@ __global__ __launch_bounds__(64 * RG * KS, 2) void prefill32_lse_kernel(PrefillA
   pf32::tile<SRC, RG, KS, true>(p, qt, b, g, bufs);
 }
 
-template <int KW, int QW>
-__global__ __launch_bounds__(64 * KW * QW) void key_weights_kernel(KeyWeightsArgs k) {
+constexpr int kKwKeys = 128;  // keys of an item
+constexpr int kKwRows = 64;   // query rows of a tile
+
+// A sequence's items: query rows [0, n) in parts of k.part_rows, the cached keys `old` before its own, key blocks.
+struct KwSeq {
+  int q0, nq, k0, nk, old, n, parts;
+  int64_t row;
+  // key blocks that see a row of part x: those that start at or before the part's last token
+  __device__ __forceinline__ int blocks(const KeyWeightsArgs& k, int x, int gsh) const {
+    const int last = (min(n, (x + 1) * k.part_rows) - 1) >> gsh;
+    const int64_t end = min((int64_t)min(nk, old + last + 1), min(k.width, (int64_t)k.max_k));
+    return end <= 0 ? 0 : (int)((end + kKwKeys - 1) / kKwKeys);
+  }
+};
+__device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh) {
   const PrefillArgs& p = k.a;
-  __shared__ float sums[KW * QW][32][33];  // [wave][key][row column]
-  const int b = blockIdx.y, g = blockIdx.z;
-  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  KwSeq s;
+  s.q0 = p.cu_q[b];
+  s.nq = p.cu_q[b + 1] - s.q0;
+  s.k0 = p.cu_k[b];
+  s.nk = p.cu_k[b + 1] - s.k0;
+  s.old = s.nk - s.nq;
+  s.row = k.rows ? (int64_t)k.rows[b] : b + k.row0;
+  const bool mine = s.nq > 0 && s.nk > 0 && s.row >= 0 && s.row < k.row_count && !(p.skip_single && s.nq == 1);
+  if (p.row_limit > 0) s.nq = (int)max((int64_t)0, min((int64_t)s.nq, p.row_limit - s.q0));  // (rows that q holds)
+  s.n = mine ? s.nq << gsh : 0;
+  s.parts = (s.n + k.part_rows - 1) / k.part_rows;
+  return s;
+}
+
+// Persistent: the items (128 keys, a part of the query rows, kv head, sequence), the key blocks of a part side by side, are
+// dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2.
+__global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
+  constexpr int KW = 2, QW = 2, KT = 2;
+  constexpr int KEYS = 32 * KT;               // keys of a wave
+  constexpr int TILE = kKwRows * 256;
+  constexpr int BUF = QW * TILE + 4 * 256;    // a tile for each query wave, and each wave's copy of its rows' lse
+  const PrefillArgs& p = k.a;
+  // (distinct arrays, so the compiler can tell a tile's reads from the loads in flight)
+  __shared__ __attribute__((aligned(1024))) uint8_t buf0[BUF];
+  __shared__ __attribute__((aligned(1024))) uint8_t buf1[BUF];
+  __shared__ float sums[4][KEYS];
+  __shared__ int starts[kMaxSeqPerLaunch + 1];
+  __shared__ int wtot[4];
+  typedef __attribute__((address_space(3))) void lds_void;
+  using std::integral_constant;
+  const int tid = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kw = w % KW, qw = w / KW;
-  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  const int q0 = p.cu_q[b], nq = p.cu_q[b + 1] - q0;
-  const int k0 = p.cu_k[b], nk = p.cu_k[b + 1] - k0;
-  const int64_t row = k.rows ? (int64_t)k.rows[b] : b;
-  const int first = (int)blockIdx.x * (32 * KW);  // the workgroup's first key
-  if (nq <= 0 || first >= nk || first >= k.width || row < 0 || row >= k.row_count) return;
-
-  // ---- this wave's keys: key j = jb + col, dims 16 s + 8 h + [0, 8) in kf[s]; keys that do not count read row 0
-  const int jb = first + kw * 32, j = jb + col;
+  const int lane = tid & 63, col = lane & 31, h = lane >> 5, lr = lane >> 4;
+  const int gsh = __builtin_ctz(p.group), HK = p.num_kv_heads;
   const bool paged = p.block_tables != nullptr;
-  const uint16_t* kr = nullptr;
-  if (j < nk && !paged) {
-    kr = p.k_src + ((int64_t)k0 + j) * p.k_row_stride + g * kKwD;
-  } else if (j < nk && j < p.max_blocks * p.block_size) {
-    const int bid = p.block_tables[(int64_t)b * p.bt_stride + j / p.block_size];
-    if (bid >= 0 && bid < p.num_blocks)
-      kr = p.k_cache + (((int64_t)bid * p.block_size + j % p.block_size) * p.num_kv_heads + g) * kKwD;
-  }
-  const uint32_t counts = (uint32_t)__builtin_amdgcn_ballot_w64(kr != nullptr);  // bit: key jb + bit takes weight
-  u32x4 kf[8];
-#pragma unroll
-  for (int s = 0; s < 8; ++s) kf[s] = kr ? ld_g16(kr + 16 * s + 8 * h) : zero4();
+  const uint32_t qs = (uint32_t)p.q_row_stride * 2u;
+  const uint32_t lane_off = (uint32_t)(lr >> gsh) * qs + (uint32_t)((lr & (p.group - 1)) << 8);
+  const uint32_t lane_sw = (uint32_t)(((lane & 15) ^ lr) << 4);
 
-  // ---- the query tiles that see a key of the wave: token tq sees key j when j <= nk - nq + tq
-  const int gsh = __builtin_ctz(p.group), n = nq << gsh;
-  const int first_row = max(0, jb - (nk - nq)) << gsh;
-  float acc[16];
+  // k-step i of a query fragment (row col of a half, chunk 2 i + h) and the row's lse, in a buffer
+  uint32_t frag[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  const float c = p.scale_log2;
-  for (int r0 = (first_row & ~31) + 32 * qw; r0 < n; r0 += 32 * QW) {
-    const int rho = r0 + col, tq = rho >> gsh, head = (g << gsh) + (rho & (p.group - 1));
-    const bool ok = rho < n && (p.row_limit <= 0 || (int64_t)q0 + tq < p.row_limit);
-    u32x4 qf[8];
-    const uint16_t* qr = p.q + ((int64_t)q0 + (ok ? tq : 0)) * p.q_row_stride + head * kKwD + 8 * h;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) qf[s] = ok ? ld_g16(qr + 16 * s) : zero4();
-    const float lse = ok ? p.lse[((int64_t)q0 + tq) * p.num_heads + head] : INFINITY;
-    f32x16 sc;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) sc = mfma_32x32x16(kf[s], qf[s], sc);
-    // register i: key jb + 8 (i / 4) + 4 h + i % 4; the last key that the row sees, relative to jb + 4 h
-    const int last = ok ? min(nk - 1, nk - nq + tq) - jb - 4 * h : -1;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float e = fast_exp2(fmaf(sc[i], c, -lse));
-      acc[i] += 8 * (i >> 2) + (i & 3) <= last ? e : 0.f;
+  for (int i = 0; i < 8; ++i) frag[i] = (uint32_t)(qw * TILE + col * 256 + (((2 * i + h) ^ (col & 15)) << 4));
+  const uint32_t lse_at = (uint32_t)(QW * TILE + w * 256 + col * 4);
+
+  // ---- every sequence's first item
+  int total = 0;
+  for (int base = 0; base < p.batch; base += 256) {
+    const int b = base + tid;
+    int items = 0;
+    if (b < p.batch) {
+      const KwSeq s = kw_seq(k, b, gsh);
+      for (int x = 0; x < s.parts; ++x) items += s.blocks(k, x, gsh);
+      items *= HK;
     }
-  }
-
-  // ---- over the rows' lane columns and the workgroup's query waves
+    const int incl = wave_incl_scan_dpp(items);
+    if (lane == 63) wtot[w] = incl;
+    __syncthreads();
+    int before = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sums[w][8 * (i >> 2) + 4 * h + (i & 3)][col] = acc[i];
+    for (int x = 0; x < 4; ++x) before += x < w ? wtot[x] : 0;
+    if (b < p.batch) starts[b] = total + before + incl - items;
+    total += wtot[0] + wtot[1] + wtot[2] + wtot[3];
+    __syncthreads();
+  }
+  if (tid == 0) starts[p.batch] = total;
   __syncthreads();
-  if (qw != 0 || lane >= 32) return;
+  total = __builtin_amdgcn_readfirstlane(total);
+  const int xcd = blockIdx.x % kXcds, wgs = gridDim.x / kXcds;  // (the grid is a multiple of the XCDs)
+  const int hi = (int)((int64_t)total * (xcd + 1) / kXcds);
+
+  for (int item = (int)((int64_t)total * xcd / kXcds) + (int)(blockIdx.x / kXcds); item < hi; item += wgs) {
+    // ---- the item: the last sequence that starts at or before it, its part, kv head and key block
+    int b = -1;
+    for (int c = 0; c < p.batch; c += kWave) {
+      const int at = c + lane < p.batch ? starts[c + lane] : INT32_MAX;
+      b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at <= item));
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const KwSeq s = kw_seq(k, b, gsh);
+    int left = item - starts[b], x = 0, blocks = s.blocks(k, 0, gsh);
+    while (left >= blocks * HK) {
+      left -= blocks * HK;
+      blocks = s.blocks(k, ++x, gsh);
+    }
+    left = __builtin_amdgcn_readfirstlane(left);
+    x = __builtin_amdgcn_readfirstlane(x);
+    blocks = __builtin_amdgcn_readfirstlane(blocks);
+    const int g = left / blocks, first = (left % blocks) * kKwKeys;
+
+    // ---- this wave's keys: key j = jb + 32 kt + col, dims 16 s + 8 h + [0, 8) in kf[kt][s]; keys that do not count are zeros
+    const int jb = first + kw * KEYS;
+    u32x4 kf[KT][8];
+    uint64_t counts = 0;  // bit: key jb + bit takes weight
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int j = jb + 32 * kt + col;
+      bool ok = j < s.nk;
+      const uint16_t* kr;
+      if (!paged) {
+        kr = p.k_src + ((int64_t)s.k0 + (ok ? j : 0)) * p.k_row_stride + g * kKwD;
+      } else {
+        ok = ok && j < p.max_blocks * p.block_size;
+        const int bid = p.block_tables[(int64_t)b * p.bt_stride + (ok ? j / p.block_size : 0)];
+        ok = ok && bid >= 0 && bid < p.num_blocks;
+        kr = p.k_cache + (((int64_t)(ok ? bid : 0) * p.block_size + j % p.block_size) * HK + g) * kKwD;
+      }
+      counts |= (uint64_t)(uint32_t)__builtin_amdgcn_ballot_w64(ok) << (32 * kt);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32x4 v = ld_g16(kr + 16 * i + 8 * h);
+        kf[kt][i] = ok ? v : zero4();
+      }
+    }
+
+    // ---- the part's rows that see a key of the item: token tq sees key j when j <= old + tq. Query wave qw takes tiles qw,
+    // qw + QW, ... from row `begin` on; a tile is two halves of 32 rows.
+    const int end = min(s.n, (x + 1) * k.part_rows);
+    const int begin = max(x * k.part_rows, (max(0, first - s.old) << gsh) & ~31);
+    const int rounds = (end - begin + kKwRows * QW - 1) / (kKwRows * QW);
+    const uint16_t* const qb = p.q + (int64_t)s.q0 * p.q_row_stride + (g << gsh) * kKwD;
+    const float* const lb = p.lse + (int64_t)s.q0 * p.num_heads + (g << gsh);
+    auto buffer = [&](auto buf) -> uint8_t* { return decltype(buf)::value & 1 ? buf1 : buf0; };
+    auto row0 = [&](int t) { return begin + (t * QW + qw) * kKwRows; };
+    // Tile t into its buffer (t % 2): rows past the sequence's last read as zeros. A piece is four rows, which start at a
+    // multiple of four: its lanes' offsets are the same up to a uniform one, and the chunks' order (as prefill_tile32.h's).
+    const int r0 = row0(0) & (p.group - 1);  // every tile starts at this head of its first token
+    auto load = [&](int t, auto buf) {
+      const int tok0 = row0(t) >> gsh;
+      const uint32_t toks = (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(s.nq - tok0, kKwRows + 1)));
+      uint8_t* const to = buffer(buf) + qw * TILE;
+      const auto rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(qb + (int64_t)tok0 * p.q_row_stride), (short)0,
+                                                        toks * qs, 0x00020000);
+      uint32_t at = lane_off, sw = lane_sw;
+      asm volatile("" : "+v"(at), "+v"(sw));  // (the pieces' offsets made here, not held in registers over the loop)
+#pragma unroll
+      for (int i = 0; i < kKwRows / 4 / KW; ++i) {
+        const int rr = kw * (kKwRows / KW) + 4 * i, rho = r0 + rr;
+        const uint32_t piece = (uint32_t)(rho >> gsh) * qs + (uint32_t)((rho & (p.group - 1)) << 8);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lds_void*)(to + rr * 256), 16, piece + at + (sw ^ (uint32_t)((i & 3) << 6)),
+                                                 0, 0, 0);
+      }
+      const auto rl = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(lb + (int64_t)tok0 * p.num_heads), (short)0,
+                                                        toks * (uint32_t)p.num_heads * 4u, 0x00020000);
+      const int rho = r0 + lane;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rl, (lds_void*)(buffer(buf) + QW * TILE + w * 256), 4,
+          ((uint32_t)(rho >> gsh) * (uint32_t)p.num_heads + (uint32_t)(rho & (p.group - 1))) * 4u, 0, 0, 0);
+    };
+    auto arrive = [&]() {  // the tile on its way is there, and every wave has read the one before it
+      wait_vmem_all();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    const float c = p.scale_log2;
+    float acc[KT][16];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+    constexpr int NM = 8 * KT, NE = 16 * KT;
+    // the scores (into sn) of half `hn` of the tile in buffer `buf` beside the probabilities of the half before it, whose first
+    // row is r0
+    auto step = [&](auto masked, auto buf, auto hn, int r0, const f32x16 (&sc)[KT], f32x16 (&sn)[KT], float lse, float& lse_n) {
+      constexpr bool MASK = decltype(masked)::value;
+      constexpr int HN = decltype(hn)::value;
+      const uint8_t* tile = buffer(buf) + HN * 32 * 256;
+      u32x4 qf[4];  // (read four k-steps ahead)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const u32x4*>(tile + frag[i]);
+      lse_n = *reinterpret_cast<const float*>(buffer(buf) + lse_at + HN * 128);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sn[kt][i] = 0.f;
+      // register i: key jb + 32 kt + 8 (i / 4) + 4 h + i % 4; the last key that the row sees, relative to jb + 4 h
+      const int rho = r0 + col;
+      const int last = rho < end ? s.old + (rho >> gsh) - jb - 4 * h : -1;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        sn[i % KT] = mfma_32x32x16(kf[i % KT][i / KT], qf[i / KT % 4], sn[i % KT]);
+        if (i % KT == KT - 1 && i / KT + 4 < 8)
+          qf[i / KT % 4] = *reinterpret_cast<const u32x4*>(tile + frag[i / KT + 4]);
+#pragma unroll
+        for (int y = i * NE / NM; y < (i + 1) * NE / NM; ++y) {
+          const int kt = y >> 4, e = y & 15;
+          const float pr = fast_exp2(fmaf(sc[kt][e], c, -lse));
+          acc[kt][e] += !MASK || 32 * kt + 8 * (e >> 2) + (e & 3) <= last ? pr : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // step, masked where a row of the half before does not exist or does not see every key of the wave
+    auto half = [&](auto buf, auto hn, int r0, const f32x16 (&sc)[KT], f32x16 (&sn)[KT], float lse, float& lse_n) {
+      if (r0 + 32 <= end && s.old + (r0 >> gsh) >= jb + KEYS - 1)
+        step(std::false_type{}, buf, hn, r0, sc, sn, lse, lse_n);
+      else
+        step(std::true_type{}, buf, hn, r0, sc, sn, lse, lse_n);
+    };
+    using C0 = integral_constant<int, 0>;
+    using C1 = integral_constant<int, 1>;
+    f32x16 sa[KT], sb[KT];
+    float la, lx = 0.f;
+    load(0, C0{});
+    arrive();
+    load(1, C1{});
+    {
+      la = *reinterpret_cast<const float*>(buf0 + lse_at);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sa[kt][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32x4 qf = *reinterpret_cast<const u32x4*>(buf0 + frag[i]);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) sa[kt] = mfma_32x32x16(kf[kt][i], qf, sa[kt]);
+      }
+    }
+    // tile t: the scores of its second half, then those of the next tile's first, each beside the probabilities before them;
+    // the tile after next is loaded from where tile t is read, over the second of the two and the next tile's first
+    auto tile = [&](auto buf, auto other, int t) {
+      half(buf, C1{}, row0(t), sa, sb, la, lx);
+      arrive();
+      load(t + 2, buf);
+      half(other, C0{}, row0(t) + 32, sb, sa, lx, la);
+    };
+    for (int t = 0;;) {
+      tile(C0{}, C1{}, t);
+      if (++t >= rounds) break;
+      tile(C1{}, C0{}, t);
+      if (++t >= rounds) break;
+    }
+
+    // ---- over the rows' lane columns (the 32 lanes of a half) and the query waves
+    int lc = col;
+    asm volatile("" : "+v"(lc));  // (sixteen comparisons made here, not held in scalar registers over the loop)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      float mine = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float v = acc[kt][i];
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));  // row_ror:8, 4, 2, 1
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xF, 0xF, false));
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xF, 0xF, false));
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xF, 0xF, false));
+        v = xrow_sum(v);
+        mine = lc == i ? v : mine;
+      }
+      if (lc < 16) sums[w][32 * kt + 8 * (col >> 2) + 4 * h + (col & 3)] = mine;
+    }
+    wait_vmem_all();  // (tiles behind the last one)
+    __syncthreads();
+    const int j = jb + lane;
+    if (qw == 0 && j < s.nk && j < k.width) {
+      float got = sums[kw][lane] + sums[kw + KW][lane];
+      got = (counts >> lane) & 1u ? got : 0.f;
+      if (s.parts > 1) {
+        if (j < k.max_k) k.partials[(((int64_t)b * HK + g) * k.max_parts + x) * k.max_k + j] = got;
+      } else {
+        float* out = k.weights + (s.row * HK + g) * k.width + j;
+        *out = j >= s.old ? got : *out + got;
+      }
+    }
+    __syncthreads();  // (sums and tiles are free)
+  }
+}
+
+// The weights of the sequences in several parts: the sum of those whose rows see the key, in order.
+__global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) {
+  const int b = blockIdx.y, g = blockIdx.z, j = (int)(blockIdx.x * 256 + threadIdx.x);
+  const int gsh = __builtin_ctz(k.a.group);
+  const KwSeq s = kw_seq(k, b, gsh);
+  if (s.parts <= 1 || j >= s.nk || j >= k.width || j >= k.max_k) return;
+  const float* part = k.partials + ((int64_t)b * k.a.num_kv_heads + g) * k.max_parts * k.max_k + j;
   float got = 0.f;
-  for (int x = 0; x < QW; ++x)
-    for (int y = 0; y < 32; ++y) got += sums[kw + x * KW][col][y];
-  if (j >= nk || j >= k.width) return;
-  float* out = k.weights + (row * p.num_kv_heads + g) * k.width + j;
-  got = (counts >> col) & 1u ? got : 0.f;
-  *out = j >= nk - nq ? got : *out + got;
+  for (int x = 0; x < s.parts; ++x)
+    if (j < (int64_t)s.blocks(k, x, gsh) * kKwKeys) got += part[(int64_t)x * k.max_k];
+  float* out = k.weights + (s.row * k.a.num_kv_heads + g) * k.width + j;
+  *out = j >= s.old ? got : *out + got;
 }
 
 template <int RG, int KS>
@@ -131,13 +360,44 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
   return launch_lse<4, 1>(a, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
 }
 
-hipError_t launch_key_weights(const KeyWeightsArgs& k, int max_seqlen_k, hipStream_t stream) {
-  if (max_seqlen_k <= 0 || k.a.batch <= 0) return hipSuccess;
-  if (!k.a.lse || !k.weights || !k.a.cu_q || !k.a.cu_k) return hipErrorInvalidValue;
-  constexpr int KW = 2, QW = 4;
-  const dim3 grid((unsigned)((max_seqlen_k + 32 * KW - 1) / (32 * KW)), (unsigned)k.a.batch, (unsigned)k.a.num_kv_heads);
-  key_weights_kernel<KW, QW><<<grid, dim3(64 * KW * QW), 0, stream>>>(k);
-  return hipGetLastError();
+int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {
+  // about three items for each workgroup slot (two a CU), but no part of less than 512 rows nor more than eight of them
+  const int64_t blocks = ((int64_t)max_seqlen_k + kKwKeys - 1) / kKwKeys;
+  const int64_t want = num_tokens * group * num_kv_heads * blocks / 1536;
+  const int64_t least = ((int64_t)max_seqlen_q * group + 7) / 8;
+  const int64_t rows = want < 512 ? 512 : want > 4096 ? 4096 : want;
+  const int64_t r = ((rows > least ? rows : least) + 127) / 128 * 128;
+  return r > INT32_MAX / 2 ? INT32_MAX / 2 / 128 * 128 : (int)r;
+}
+
+hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
+  KeyWeightsArgs k = k0;
+  if (k.max_k <= 0 || k.a.batch <= 0) return hipSuccess;
+  if (!k.a.lse || !k.weights || !k.a.cu_q || !k.a.cu_k || k.part_rows <= 0 || k.part_rows % 128 ||
+      (k.max_parts > 1 && !k.partials))
+    return hipErrorInvalidValue;
+  const int batch = k0.a.batch;
+  for (int b0 = 0; b0 < batch; b0 += kMaxSeqPerLaunch) {  // (the sequences' items are laid out in LDS)
+    k.a.batch = batch - b0 < kMaxSeqPerLaunch ? batch - b0 : kMaxSeqPerLaunch;
+    k.a.cu_q = k0.a.cu_q + b0;
+    k.a.cu_k = k0.a.cu_k + b0;
+    if (k.a.block_tables) k.a.block_tables = k0.a.block_tables + (int64_t)b0 * k0.a.bt_stride;
+    if (k.rows)
+      k.rows = k0.rows + b0;
+    else
+      k.row0 = k0.row0 + b0;
+    const int64_t blocks = ((int64_t)k.max_k + kKwKeys - 1) / kKwKeys;
+    const int64_t items = blocks * k.max_parts * k.a.batch * k.a.num_kv_heads;
+    const int64_t most = 512;  // two workgroups a CU
+    const unsigned grid = (unsigned)(((items < most ? items : most) + kXcds - 1) / kXcds * kXcds);
+    key_weights_kernel<<<dim3(grid), dim3(256), 0, stream>>>(k);
+    if (k.max_parts > 1)
+      key_weights_sum_kernel<<<dim3((unsigned)((k.max_k + 255) / 256), (unsigned)k.a.batch, (unsigned)k.a.num_kv_heads),
+                               dim3(256), 0, stream>>>(k);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace vox

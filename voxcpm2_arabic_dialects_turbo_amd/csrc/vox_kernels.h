@@ -136,9 +136,14 @@ struct PrefillArgs {
 struct KeyWeightsArgs {
   PrefillArgs a;              // cu_q, cu_k; packed keys or paged ones
   float* weights;             // fp32 [row_count, HK, width]
-  const int32_t* rows;        // int32 [batch], or null: row b (outside [0, row_count): none)
+  const int32_t* rows;        // int32 [batch], or null: row b + row0 (outside [0, row_count): none)
+  int64_t row0;
   int64_t row_count;
-  int64_t width;              // keys at or past it: left out
+  int64_t width;              // keys at or past it, or at or past max_k: left out
+  int max_k;
+  int part_rows;              // a sequence's query rows (tokens x group) in parts of so many; a multiple of 128
+  int max_parts;              // of a sequence
+  float* partials;            // max_parts > 1: fp32 [a launch's sequences, HK, max_parts, max_k]
 };
 
 // Tokens dropped from a paged cache (kv_evict.hip): of every sequence longer than `budget` its first `sinks`, last `recent`
@@ -255,7 +260,8 @@ hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t st
 
 // Causal varlen attention that also leaves every row's a.lse, then what the keys received (key_weights.hip).
 hipError_t launch_prefill_lse(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
-hipError_t launch_key_weights(const KeyWeightsArgs& k, int max_seqlen_k, hipStream_t stream);
+hipError_t launch_key_weights(const KeyWeightsArgs& k, hipStream_t stream);
+int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads);
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 

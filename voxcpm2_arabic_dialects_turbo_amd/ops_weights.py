@@ -201,9 +201,10 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
     cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
     lib = _lib.load()
     with _on(dev):
-        lse = torch.empty(T, H, dtype=torch.float32, device=dev)
+        scratch = torch.empty(lib.vox_prefill_weights_bytes(T, B, int(max_seqlen_q), reach, H, hk), dtype=torch.uint8,
+                              device=dev)
         _lib.check(lib.vox_prefill_attn_weights(
             q.data_ptr(), _row_stride(q), *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, int(max_seqlen_q), reach, T, H, hk, D,
             scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), key_weights.shape[0],
-            key_weights.shape[2], lse.data_ptr(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
+            key_weights.shape[2], scratch.data_ptr(), scratch.numel(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
     return out
