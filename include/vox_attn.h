@@ -375,7 +375,9 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
  * cu_seqlens_q[b] tokens of a sequence are the step's own, and their weights become it, the earlier ones' grow by it. A
  * sequence without queries keeps its weights. max_seqlen_k: no sequence has more keys (further ones are left out of the
  * weights). num_tokens: the rows that q and out hold. Paged blocks are a multiple of 64 tokens. scratch:
- * vox_prefill_weights_bytes bytes (16-byte aligned), the call's own. */
+ * vox_prefill_weights_bytes bytes (16-byte aligned), the call's own. plan, workspace: as vox_prefill_attn's; with the workspace
+ * (NULL: none) the one-query sequences of a paged call run on the decode kernels, and scores is vox_decode_scores_bytes bytes
+ * of scratch. */
 size_t vox_prefill_weights_bytes(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int num_heads,
                                  int num_kv_heads);
 int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
@@ -385,7 +387,8 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
                              int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads, int num_kv_heads,
                              int head_dim, float softmax_scale, float* key_weights, const int32_t* weight_rows,
                              int64_t num_weight_rows, int64_t weight_width, void* scratch,
-                             size_t scratch_bytes, void* out, int64_t out_row_stride, void* stream);
+                             size_t scratch_bytes, void* scores, size_t scores_bytes, int plan, void* workspace,
+                             size_t workspace_bytes, void* out, int64_t out_row_stride, void* stream);
 
 /* Drops tokens from sequences longer than `budget`: their first `sinks` and last `recent` tokens stay and, in every layer
  * and kv head apart, the budget - sinks - recent heaviest of the others by key_weights (fp32 [num_layers, num_weight_rows,

@@ -442,3 +442,32 @@ def test_evict_nothing():
     kv, w = torch.zeros(1, 2, 4, 64, 1, 128, dtype=torch.bfloat16, device=DEV), torch.zeros(1, 4, 1, 256, device=DEV)
     t, n = evict_kv_tokens(kv, w, _i32([[1, 2]])[:0], _i32([]), 10)
     assert t.shape == (0, 2) and n.shape == (0,)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# steps that are mostly one-query rows
+
+
+@pytest.mark.parametrize("h,hk,bs", [(16, 2, 256), (8, 1, 64), (4, 4, 64), (32, 2, 64)])
+def test_chunk_mostly_one_query_rows(h, hk, bs):
+    """On the decode kernels where they take the heads; sequences without queries and prompts among them, rows of any order."""
+    seqs = [(1, 5 + 37 * i) for i in range(20)] + [(90, 90), (0, 50), (130, 400)] + [(1, 1), (1, 256)]
+    gen = torch.Generator().manual_seed(h)
+    rows = torch.randperm(len(seqs) + 3, generator=gen)[:len(seqs)].tolist()
+    rows[3], rows[20] = -1, -1
+    _varlen_case(30 + h, seqs, h, hk, bs, rows, extra_cols=1)
+
+
+@pytest.mark.parametrize("bs", [64, None])
+def test_chunk_more_sequences_than_a_launch_lays_out(bs):
+    """More than 512 sequences, long ones behind the first 512."""
+    _varlen_case(31, [(1 + i % 3, 1 + i % 3 + (i % 40 if bs else 0)) for i in range(700)] + [(100, 100), (1, 1)], 8, 1, bs)
+    _varlen_case(32, [(1, 1 + (i % 70 if bs else 0)) for i in range(600)], 8, 1, bs)
+
+
+def test_chunk_in_parts_of_its_rows():
+    """Long prompts whose query rows are summed in several parts, over caches and packed, one past eight parts of 512 rows."""
+    _varlen_case(33, [(700, 700), (65, 800), (64, 64)], 16, 2, 64)
+    _varlen_case(34, [(600, 600), (130, 130)], 64, 1)
+    _varlen_case(35, [(1300, 1300)], 8, 1)
+    _varlen_case(36, [(2100, 2100)], 2, 2)

@@ -401,7 +401,8 @@ def test_c_scores_bytes():
 
 PREFILL_C = dict(q=P, qs=2048, key=P, value=P, ks=256, vs=256, kc=None, vc=None, blocks=0, bs=0, bt=None, bts=0, mb=0, cq=P,
                  ck=P, batch=2, mq=4, mk=4, n=8, h=16, hk=2, d=128, scale=0.1, w=P, rows=None, n_rows=2, width=128,
-                 scratch=P, scratch_bytes=1 << 30, out=P, outs=2048, stream=None)
+                 scratch=P, scratch_bytes=1 << 30, scores=None, scores_bytes=0, plan=0, ws=None, ws_bytes=0, out=P, outs=2048,
+                 stream=None)
 PAGED = dict(key=None, value=None, ks=0, vs=0, kc=P, vc=P, blocks=4, bs=64, bt=P, bts=2, mb=2)
 
 
@@ -413,6 +414,9 @@ PAGED = dict(key=None, value=None, ks=0, vs=0, kc=P, vc=P, blocks=4, bs=64, bt=P
     (dict(batch=70000), "65535"), (dict(key=None), "null key"), (dict(h=24, qs=3200, outs=3200), "divide 128"), (dict(d=64), "head_dim"),
     (dict(PAGED, bs=32), "multiple of 64"), (dict(PAGED, bs=0), "multiple of 64"), (dict(PAGED, mb=1 << 25, bts=1 << 25), "too wide"),
     (dict(PAGED, kc=None), "without caches"), (dict(PAGED, bts=1), "bad block table"),
+    (dict(PAGED, ws=P, ws_bytes=10), "workspace"), (dict(PAGED, ws=P, ws_bytes=1 << 30, plan=5), "plan mode"),
+    (dict(PAGED, ws=P, ws_bytes=1 << 30), "scores"),
+    (dict(PAGED, ws=P, ws_bytes=1 << 30, scores=P, scores_bytes=2 * 8 * 16 * 16 * 4 - 1), "needed"),
 ])
 def test_c_prefill_refusals(kw, match):
     _einval(_lib.load().vox_prefill_attn_weights(*{**PREFILL_C, **kw}.values()), match)

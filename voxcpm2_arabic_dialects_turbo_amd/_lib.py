@@ -122,7 +122,7 @@ _SIGNATURES = {
     "vox_prefill_attn_weights": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
                                         _i32, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _i64,
                                         _i32, _i32, _i32, _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size,
-                                        _c_void_p, _i64, _c_void_p]),
+                                        _c_void_p, _size, _i32, _c_void_p, _size, _c_void_p, _i64, _c_void_p]),
     "vox_evict_kv_tokens": (_i32, [_c_void_p, _i64, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32,
                                    _c_void_p, _c_void_p, _i64, _i64, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p,
                                    _c_void_p, _c_void_p, _c_void_p]),

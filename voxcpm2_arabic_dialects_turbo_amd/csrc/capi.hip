@@ -130,6 +130,8 @@ int launch_decode_slices(const vox::DecodeArgs& a, int batch, int num_kv_heads, 
     vox::DecodeArgs s = base;
     s.batch = batch - b0 < vox::kMaxSeqPerLaunch ? batch - b0 : vox::kMaxSeqPerLaunch;
     s.block_tables = base.block_tables + (int64_t)b0 * base.bt_stride;
+    if (base.weight_rows) s.weight_rows = base.weight_rows + b0;
+    s.weight_row0 = base.weight_row0 + b0;
     if (base.cu_q) {  // varlen: rows are absolute (cu_seqlens_q), only the sequence arrays move
       s.cu_q = base.cu_q + b0;
       s.cu_k = base.cu_k + b0;
@@ -137,8 +139,6 @@ int launch_decode_slices(const vox::DecodeArgs& a, int batch, int num_kv_heads, 
       s.q = base.q + (int64_t)b0 * base.q_row_stride;
       s.context_lens = base.context_lens + b0;
       s.out = base.out + (int64_t)b0 * base.out_row_stride;
-      if (base.weight_rows) s.weight_rows = base.weight_rows + b0;
-      s.weight_row0 = base.weight_row0 + b0;
       if (base.slot_mapping) {
         s.slot_mapping = base.slot_mapping + b0;
         s.new_k = base.new_k + (int64_t)b0 * base.new_k_stride;
@@ -1140,7 +1140,8 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
                              int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads, int num_kv_heads,
                              int head_dim, float softmax_scale, float* key_weights, const int32_t* weight_rows,
                              int64_t num_weight_rows, int64_t weight_width, void* scratch,
-                             size_t scratch_bytes, void* out, int64_t out_row_stride, void* stream) {
+                             size_t scratch_bytes, void* scores, size_t scores_bytes, int plan, void* workspace,
+                             size_t workspace_bytes, void* out, int64_t out_row_stride, void* stream) {
   const char* fn = "prefill_attn_weights";
   if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_tokens < 0)
     return fail(VOX_EINVAL, "%s: negative batch, max_seqlen_q, max_seqlen_k or num_tokens", fn);
@@ -1176,9 +1177,30 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   k.part_rows = ws.part_rows;
   k.max_parts = ws.parts;
   k.partials = (float*)((char*)scratch + ws.partials);
-  st = hip_status(vox::launch_prefill_lse(k.a, max_seqlen_q, (hipStream_t)stream), "prefill_attn_weights launch");
-  if (st != VOX_OK) return st;
-  return hip_status(vox::launch_key_weights(k, (hipStream_t)stream), "prefill_attn_weights sums launch");
+  // with the workspace the one-query sequences run on the decode kernels, which spread a long context over every CU
+  const bool decodes = varlen_decode_rows(k.a, workspace, num_kv_heads);
+  vox::DecodeArgs d{};
+  if (decodes) {
+    st = check_varlen_workspace(fn, batch, plan, workspace, workspace_bytes);
+    if (st != VOX_OK) return st;
+    const size_t need = vox_decode_scores_bytes(batch, max_blocks, block_size, num_heads);
+    if (!scores || !aligned16(scores) || scores_bytes < need)
+      return fail(VOX_EINVAL, "%s: scores of %zu bytes (16-byte aligned), %zu needed", fn, scores_bytes, need);
+    k.a.skip_single = 1;
+    d = varlen_decode_args(k.a, q_row_stride, num_blocks, num_heads, num_kv_heads);
+    d.scores = (float*)scores;
+    d.weights = key_weights;
+    d.weight_rows = weight_rows;
+    d.weight_row_count = num_weight_rows;
+    d.weight_width = weight_width;
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  if (!decodes || max_seqlen_q > 1) {
+    st = hip_status(vox::launch_prefill_lse(k.a, max_seqlen_q, s), "prefill_attn_weights launch");
+    if (st == VOX_OK) st = hip_status(vox::launch_key_weights(k, s), "prefill_attn_weights sums launch");
+    if (st != VOX_OK) return st;
+  }
+  return decodes ? launch_decode_slices(d, batch, num_kv_heads, plan, workspace, s, vox::launch_decode_weights) : VOX_OK;
 }
 
 int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_bytes,

@@ -21,7 +21,43 @@ namespace {
 
 constexpr int kKwD = 128;
 
-template <int SRC, int RG, int KS>
+// Items numbered sequence by sequence: the first of each of `batch` <= kMaxSeqPerLaunch sequences, with items_of(b) of them,
+// into starts[0, batch] (LDS, with wtot[4]) by 256 threads; returns how many there are.
+template <typename F>
+__device__ __forceinline__ int number_items(int batch, int* starts, int* wtot, F&& items_of) {
+  const int tid = threadIdx.x, w = tid >> 6;
+  int total = 0;
+  for (int base = 0; base < batch; base += 256) {
+    const int b = base + tid;
+    const int items = b < batch ? items_of(b) : 0;
+    const int incl = wave_incl_scan_dpp(items);
+    if ((tid & 63) == 63) wtot[w] = incl;
+    __syncthreads();
+    int before = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) before += x < w ? wtot[x] : 0;
+    if (b < batch) starts[b] = total + before + incl - items;
+    total += wtot[0] + wtot[1] + wtot[2] + wtot[3];
+    __syncthreads();
+  }
+  if (tid == 0) starts[batch] = total;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(total);
+}
+// The sequence of an item: the last that starts at or before it (an empty one shares its start with the next).
+__device__ __forceinline__ int sequence_of(int item, int batch, const int* starts) {
+  int b = -1;
+  for (int c = 0; c < batch; c += kWave) {
+    const int lane = threadIdx.x & 63;
+    const int at = c + lane < batch ? starts[c + lane] : INT32_MAX;
+    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at <= item));
+  }
+  return __builtin_amdgcn_readfirstlane(b);
+}
+
+// WALK: for calls whose (q tile, sequence) grid would be mostly empty: a fixed grid walks the q tiles that there are, a
+// sequence's heaviest first.
+template <int SRC, int RG, int KS, bool WALK>
 __global__ __launch_bounds__(64 * RG * KS, 2) void prefill32_lse_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t kt0[pf32::kTB];
   __shared__ __attribute__((aligned(1024))) uint8_t kt1[pf32::kTB];
@@ -29,9 +65,25 @@ __global__ __launch_bounds__(64 * RG * KS, 2) void prefill32_lse_kernel(PrefillA
   __shared__ __attribute__((aligned(1024))) uint8_t vt1[pf32::kTB];
   __shared__ float red[KS == 2 ? 256 : 1];
   const pf32::Bufs bufs{kt0, kt1, vt0, vt1, red};
-  int qt, b, g;
-  grid_item(p, qt, b, g);
-  pf32::tile<SRC, RG, KS, true>(p, qt, b, g, bufs);
+  if constexpr (WALK) {
+    __shared__ int starts[kMaxSeqPerLaunch + 1];
+    __shared__ int wtot[4];
+    const int BQ = 32 * RG / p.group, HK = p.num_kv_heads;
+    const int total = number_items(p.batch, starts, wtot, [&](int b) {
+      const int nq = p.cu_q[b + 1] - p.cu_q[b];
+      return nq <= 0 || (p.skip_single && nq == 1) ? 0 : (nq + BQ - 1) / BQ * HK;
+    });
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+      const int b = sequence_of(item, p.batch, starts);
+      const int from = __builtin_amdgcn_readfirstlane(starts[b]), n = __builtin_amdgcn_readfirstlane(starts[b + 1]) - from;
+      pf32::tile<SRC, RG, KS, true>(p, (n - 1 - (item - from)) / HK, b, (item - from) % HK, bufs);
+      __syncthreads();  // the tiles are free
+    }
+  } else {
+    int qt, b, g;
+    grid_item(p, qt, b, g);
+    pf32::tile<SRC, RG, KS, true>(p, qt, b, g, bufs);
+  }
 }
 
 constexpr int kKwKeys = 128;  // keys of an item
@@ -97,39 +149,18 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   const uint32_t lse_at = (uint32_t)(QW * TILE + w * 256 + col * 4);
 
   // ---- every sequence's first item
-  int total = 0;
-  for (int base = 0; base < p.batch; base += 256) {
-    const int b = base + tid;
+  const int total = number_items(p.batch, starts, wtot, [&](int b) {
+    const KwSeq s = kw_seq(k, b, gsh);
     int items = 0;
-    if (b < p.batch) {
-      const KwSeq s = kw_seq(k, b, gsh);
-      for (int x = 0; x < s.parts; ++x) items += s.blocks(k, x, gsh);
-      items *= HK;
-    }
-    const int incl = wave_incl_scan_dpp(items);
-    if (lane == 63) wtot[w] = incl;
-    __syncthreads();
-    int before = 0;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) before += x < w ? wtot[x] : 0;
-    if (b < p.batch) starts[b] = total + before + incl - items;
-    total += wtot[0] + wtot[1] + wtot[2] + wtot[3];
-    __syncthreads();
-  }
-  if (tid == 0) starts[p.batch] = total;
-  __syncthreads();
-  total = __builtin_amdgcn_readfirstlane(total);
+    for (int x = 0; x < s.parts; ++x) items += s.blocks(k, x, gsh);
+    return items * HK;
+  });
   const int xcd = blockIdx.x % kXcds, wgs = gridDim.x / kXcds;  // (the grid is a multiple of the XCDs)
   const int hi = (int)((int64_t)total * (xcd + 1) / kXcds);
 
   for (int item = (int)((int64_t)total * xcd / kXcds) + (int)(blockIdx.x / kXcds); item < hi; item += wgs) {
-    // ---- the item: the last sequence that starts at or before it, its part, kv head and key block
-    int b = -1;
-    for (int c = 0; c < p.batch; c += kWave) {
-      const int at = c + lane < p.batch ? starts[c + lane] : INT32_MAX;
-      b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at <= item));
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
+    // ---- the item's sequence, part, kv head and key block
+    const int b = sequence_of(item, p.batch, starts);
     const KwSeq s = kw_seq(k, b, gsh);
     int left = item - starts[b], x = 0, blocks = s.blocks(k, 0, gsh);
     while (left >= blocks * HK) {
@@ -334,13 +365,13 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   *out = j >= s.old ? got : *out + got;
 }
 
-template <int RG, int KS>
+template <int RG, int KS, bool WALK>
 hipError_t launch_lse(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
   const dim3 block(64 * RG * KS);
   if (!a.block_tables)
-    prefill32_lse_kernel<pf32::kRows, RG, KS><<<grid, block, 0, stream>>>(a);
+    prefill32_lse_kernel<pf32::kRows, RG, KS, WALK><<<grid, block, 0, stream>>>(a);
   else
-    prefill32_lse_kernel<pf32::kCache, RG, KS><<<grid, block, 0, stream>>>(a);
+    prefill32_lse_kernel<pf32::kCache, RG, KS, WALK><<<grid, block, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -351,13 +382,26 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
   if (!a0.lse || !a0.cu_q || !a0.cu_k || !a0.causal || (a0.block_tables && a0.block_size % pf32::kBK) || 128 % a0.group)
     return hipErrorInvalidValue;
   PrefillArgs a = a0;
+  const int64_t tiles = ((int64_t)max_seqlen_q + 128 / a.group - 1) / (128 / a.group);
+  // T rows against the grid's: (row_limit is the rows that there are)
+  if (4 * a.row_limit <= (int64_t)max_seqlen_q * a.batch) {
+    for (int b0 = 0; b0 < a0.batch; b0 += kMaxSeqPerLaunch) {
+      a.batch = a0.batch - b0 < kMaxSeqPerLaunch ? a0.batch - b0 : kMaxSeqPerLaunch;
+      a.cu_q = a0.cu_q + b0;
+      a.cu_k = a0.cu_k + b0;
+      if (a.block_tables) a.block_tables = a0.block_tables + (int64_t)b0 * a0.bt_stride;
+      const int64_t items = tiles * a.batch * a.num_kv_heads;
+      const hipError_t e = launch_lse<4, 1, true>(a, dim3((unsigned)(items < 512 ? items : 512)), stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   const bool small = 64 % a.group == 0;
   const int64_t tiles64 = small ? ((int64_t)max_seqlen_q + 64 / a.group - 1) / (64 / a.group) : 0;
   if (small && tiles64 * a.batch * a.num_kv_heads <= 512)
-    return launch_lse<2, 2>(a, dim3((unsigned)tiles64, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
-  const int64_t tiles = ((int64_t)max_seqlen_q + 128 / a.group - 1) / (128 / a.group);
+    return launch_lse<2, 2, false>(a, dim3((unsigned)tiles64, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
   a.xcd_order = tiles * a.batch * a.num_kv_heads >= 1024;
-  return launch_lse<4, 1>(a, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
+  return launch_lse<4, 1, false>(a, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
 }
 
 int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {

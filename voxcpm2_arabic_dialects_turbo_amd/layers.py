@@ -201,4 +201,5 @@ class Attention(nn.Module):
         return varlen_attention_weights(q, k, v, self.key_weights, context.weight_rows, cu_seqlens_q=context.cu_seqlens_q,
                                         cu_seqlens_k=context.cu_seqlens_k, max_seqlen_q=context.max_seqlen_q,
                                         max_seqlen_k=context.max_seqlen_k, softmax_scale=self.scale, block_table=tables,
-                                        k_cache=k_cache, v_cache=v_cache)
+                                        k_cache=k_cache, v_cache=v_cache,
+                                        plan=_plan_key(context) if tables is not None else None)

@@ -20,7 +20,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import HEAD_DIM, MAX_DECODE_HEADS, _as_i32, _check_cuda, _flat, _plan_recorded, store_kvcache
+from .ops import (HEAD_DIM, MAX_DECODE_HEADS, _as_i32, _check_cuda, _flat, _plan_recorded, _takes_decode_rows,
+                  store_kvcache)
 from .ops_fp4 import _ids, _on, _row_stride, _table, _workspace
 
 
@@ -154,7 +155,8 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
                              weight_rows: torch.Tensor | None = None, *, cu_seqlens_q: torch.Tensor,
                              cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float,
                              block_table: torch.Tensor | None = None, k_cache: torch.Tensor | None = None,
-                             v_cache: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                             v_cache: torch.Tensor | None = None, out: torch.Tensor | None = None, plan=None
+                             ) -> torch.Tensor:
     """``ops.varlen_attention`` (causal: sequence b's queries q [T, H, 128] are the last of its keys, from packed rows k / v
     [Tk, HK, 128] or, with block_table, from the caches), adding to ``key_weights`` what every key received: for token j and
     kv head g the sum of the probabilities of b's queries at g's query heads, in place of the weight for the step's own
@@ -162,7 +164,8 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
     zeros for a query that sees no key. A sequence without queries keeps its weights.
 
     No sequence has more than max_seqlen_q queries or max_seqlen_k keys (further ones are left out). H / HK divides 128, and
-    cache blocks are a multiple of 64 tokens."""
+    cache blocks are a multiple of 64 tokens. One-query sequences run on the decode kernels where a call is mostly those, as
+    varlen_attention's do; ``plan``: as decode_attention_weights's, for these."""
     fn = "varlen_attention_weights"
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"{fn}: q must be bf16 [T, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
@@ -203,8 +206,16 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
     with _on(dev):
         scratch = torch.empty(lib.vox_prefill_weights_bytes(T, B, int(max_seqlen_q), reach, H, hk), dtype=torch.uint8,
                               device=dev)
+        ws, scores, mode, recorded = None, None, _lib.PLAN_NONE, None
+        if block_table is not None and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) \
+                and _takes_decode_rows(H, hk, bs, bt.shape[1], out, _row_stride(out)):
+            ws, mode, recorded = _workspace(lib, dev, B, plan, "varlen_weights", B, bt.shape[1], bt_stride, H, hk, bs)
+            scores = torch.empty(lib.vox_decode_scores_bytes(B, bt.shape[1], bs, H), dtype=torch.uint8, device=dev)
         _lib.check(lib.vox_prefill_attn_weights(
             q.data_ptr(), _row_stride(q), *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, int(max_seqlen_q), reach, T, H, hk, D,
             scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), key_weights.shape[0],
-            key_weights.shape[2], scratch.data_ptr(), scratch.numel(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
+            key_weights.shape[2], scratch.data_ptr(), scratch.numel(), None if scores is None else scores.data_ptr(),
+            0 if scores is None else scores.numel(), mode, None if ws is None else ws.data_ptr(),
+            0 if ws is None else ws.numel(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
+    _plan_recorded(dev, recorded)
     return out
