@@ -437,7 +437,7 @@ EVICT_C = dict(kv=P, layers=1, blocks=4, bs=64, hk=1, head=256, scale=0, bt=P, b
     (dict(tables=None), "null"), (dict(out_lens=None), "null"), (dict(w=None), "null"), (dict(blocks=0), "cache of"),
     (dict(bs=0), "cache of"), (dict(blocks=1 << 26), "cache of"), (dict(hk=0), "kv heads"), (dict(head=100), "multiples of 16"),
     (dict(head=0), "multiples of 16"), (dict(head=4112), "multiples of 16"), (dict(scale=8), "0 or 4"),
-    (dict(kv=P + 8), "aligned"), (dict(bs=1, head=16, scale=4), "aligned"), (dict(bts=1), "bad block table"),
+    (dict(kv=P + 8), "aligned"), (dict(moves=P + 4), "aligned"), (dict(bs=1, head=16, scale=4), "aligned"), (dict(bts=1), "bad block table"),
     (dict(mb=0), "bad block table"), (dict(into=P, into_s=1), "new blocks"), (dict(width=127), "the tables reach 128"),
     (dict(n_rows=0), "key_weights"), (dict(budget=0), "budget"), (dict(sinks=9), "budget"), (dict(recent=-1), "budget"),
     (dict(sinks=2**31 - 1, recent=2**31 - 1), "budget"), (dict(batch=70000), "65535"), (dict(layers=40000), "32767"),

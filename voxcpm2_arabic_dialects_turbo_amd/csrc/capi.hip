@@ -1221,8 +1221,8 @@ int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int bl
     return fail(VOX_EINVAL, "%s: %d kv heads of %d and %d bytes (multiples of 16 up to 4096, and 0 or 4)", fn, num_kv_heads,
                 head_bytes, scale_bytes);
   const int64_t block_bytes = (int64_t)block_size * num_kv_heads * (head_bytes + scale_bytes);
-  if (!aligned16(kv) || block_bytes % 16)
-    return fail(VOX_EINVAL, "%s: kv and its blocks must be 16-byte aligned", fn);
+  if (!aligned16(kv) || block_bytes % 16 || ((uintptr_t)moves & 7u))
+    return fail(VOX_EINVAL, "%s: kv and its blocks must be 16-byte aligned, moves 8-byte aligned", fn);
   if (max_blocks <= 0 || bt_stride < max_blocks || (int64_t)max_blocks * block_size > (1 << 30))
     return fail(VOX_EINVAL, "%s: bad block table shape", fn);
   if (into && into_stride < max_blocks) return fail(VOX_EINVAL, "%s: bad shape of the new blocks' table", fn);
@@ -1256,7 +1256,7 @@ int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int bl
   a.recent = recent;
   a.into = into;
   a.into_stride = into_stride;
-  a.moves = moves;
+  a.moves = (int2*)moves;
   a.kept = budget < reach ? budget : reach;
   a.new_tables = new_tables;
   a.new_lens = new_lens;

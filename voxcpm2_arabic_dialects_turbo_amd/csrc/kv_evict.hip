@@ -2,13 +2,15 @@
 // launches: which tokens stay (select_kernel), and their rows moved to the front of the sequence (move_kernel).
 //
 // select: a workgroup per (kv head, sequence, layer). Of the tokens [sinks, n - recent) the `want` heaviest stay, of equal
-// ones the earliest: the want-th largest weight T is found digit by digit, 8 bits a pass over the weights as ordered
-// integers (a histogram in LDS, the digit whose count reaches what is still wanted), then tokens above T stay, and the
-// first ones equal to T up to the number still wanted. One more pass in token order gives each kept token its place (the
-// count of kept ones before it), moves its weight there and leaves the slot it comes from for move_kernel.
+// ones the earliest. The want-th largest weight T is found over the weights as ordered integers (ordered): a histogram of
+// 2048 equal steps between the least and the largest (LDS), then of 2048 steps of the step that holds the want-th, until a
+// step is one integer, three rounds at most. Tokens above T stay, and of those equal to T the first ones that are still
+// wanted. Place j of a kept token at i is how many kept ones lie before it: (those above T or protected before i) + min(those
+// equal to T before i, still wanted), from ballots and one scan. Its weight moves there, and move_kernel gets the pair of
+// slots. Weights are held in registers (lane-contiguous rounds of the workgroup); rows longer than those are read again.
 //
-// Both passes that move work in place: place j takes token i_j >= j, a tile's reads are done before its writes, and a later
-// tile reads only behind them. So a sequence's tokens of one kv head are one workgroup's, tile after tile.
+// Both kernels work in place: place j takes token i_j >= j, a round's reads are done before its writes, and a later round
+// reads only behind them. So a sequence's tokens of one kv head (and of one slice of a row's bytes) are one workgroup's.
 #include "vox_common.h"
 #include "vox_kernels.h"
 
@@ -16,9 +18,9 @@ namespace vox {
 
 namespace {
 
-constexpr int kSelThreads = 256;
 constexpr int kMoveThreads = 256;
-constexpr int kMovePieces = 8;  // 16-byte pieces a lane keeps in flight
+constexpr int kMoveRows = 8;  // rows a lane keeps in flight, twice (a round's, and the next one's)
+constexpr int kBins = 2048;
 
 // Weights as integers of the same order: NaN above everything, the two zeros the same.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -28,7 +30,8 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// This thread's exclusive prefix of two counts over the workgroup, and their totals (scratch: 2 ints a wave).
+// This thread's exclusive prefixes of two counts over the workgroup of NW waves, and their totals.
+template <int NW>
 __device__ __forceinline__ void scan2(int a, int b, int (*scratch)[2], int& pa, int& pb, int& ta, int& tb) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int ia = wave_incl_scan_dpp(a), ib = wave_incl_scan_dpp(b);
@@ -41,7 +44,7 @@ __device__ __forceinline__ void scan2(int a, int b, int (*scratch)[2], int& pa, 
   pb = ib - b;
   ta = tb = 0;
 #pragma unroll
-  for (int x = 0; x < kSelThreads / kWave; ++x) {
+  for (int x = 0; x < NW; ++x) {
     const int va = scratch[x][0], vb = scratch[x][1];
     pa += x < w ? va : 0;
     pb += x < w ? vb : 0;
@@ -51,146 +54,281 @@ __device__ __forceinline__ void scan2(int a, int b, int (*scratch)[2], int& pa, 
   __syncthreads();
 }
 
-__global__ __launch_bounds__(kSelThreads) void select_kernel(EvictArgs p) {
-  __shared__ int hist[256];
-  __shared__ int scratch[kSelThreads / kWave][2];
-  __shared__ int s_digit, s_want;
+// NT threads, E weights each in registers.
+template <int NT, int E>
+__global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
+  constexpr int NW = NT / kWave, CHUNK = NT * E, PER = kBins / NT;
+  static_assert(E * NW <= NT && kBins % NT == 0, "a thread scans a count and its bins");
+  __shared__ int hist[kBins];
+  __shared__ int scratch[NW][2];
+  __shared__ uint32_t range[NW][2];
+  __shared__ int counts[E * NW][2];  // [round][wave]: tokens that stay for sure, and those equal to T
+  __shared__ int s_bin, s_want;
   const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
-  const int reach = p.max_blocks * p.block_size;
-  const int n = max(0, min(p.context_lens[b], reach));
+  const int lane = tid & 63, wv = tid >> 6;
+  const int bs = p.block_size;
+  const int n = max(0, min(p.context_lens[b], p.max_blocks * bs));
   const int64_t row = p.rows ? (int64_t)p.rows[b] : b;
   const bool drops = n > p.budget && row >= 0 && row < p.row_count;  // workgroup-uniform
-  const int left = drops ? p.budget : n;
   const int32_t* table = p.block_tables + (int64_t)b * p.bt_stride;
   const int32_t* into = p.into ? p.into + (int64_t)b * p.into_stride : nullptr;
   if (g == 0 && layer == 0) {
-    const int used = (left + p.block_size - 1) / p.block_size;
-    for (int c = tid; c < p.max_blocks; c += kSelThreads) {
+    const int left = drops ? p.budget : n, used = (left + bs - 1) / bs;
+    for (int c = tid; c < p.max_blocks; c += NT) {
       int blk = c < used ? table[c] : -1;
       if (drops && into && c < used && into[c] >= 0) blk = into[c];
       p.new_tables[(int64_t)b * p.max_blocks + c] = blk;
     }
     if (tid == 0) p.new_lens[b] = left;
   }
-  int32_t* moves = p.moves + (((int64_t)layer * p.batch + b) * p.num_heads + g) * p.kept;
-  if (!drops) {
-    for (int j = tid; j < left && j < p.kept; j += kSelThreads) moves[j] = -1;
-    return;
-  }
+  if (!drops) return;
   float* w = p.weights + (((int64_t)layer * p.row_count + row) * p.num_heads + g) * p.width;
+  int2* moves = p.moves + (((int64_t)layer * p.batch + b) * p.num_heads + g) * p.kept;
   const int lo = p.sinks, hi = n - p.recent;  // (n > budget >= sinks + recent)
   int want = p.budget - p.sinks - p.recent;
-  uint32_t top = 0;  // T's digits so far
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      hist[tid] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t key = ordered(w[i]);
-        if (shift == 24 || (key >> (shift + 8)) == (top >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+  const bool some = want > 0;
+  const int chunks = (n + CHUNK - 1) / CHUNK;
+
+  float x[E];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = c * CHUNK + e * NT + tid;
+      x[e] = i < n ? w[i] : 0.f;
+    }
+  };
+  load(0);
+  uint32_t top = 0;  // T
+  if (some) {
+    uint32_t least = 0xffffffffu, most = 0;
+    for (int c = 0; c < chunks; ++c) {
+      if (c > 0) load(c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = c * CHUNK + e * NT + tid;
+        const uint32_t key = ordered(x[e]);
+        least = min(least, i >= lo && i < hi ? key : 0xffffffffu);
+        most = max(most, i >= lo && i < hi ? key : 0u);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      least = min(least, (uint32_t)__shfl_xor((int)least, o, kWave));
+      most = max(most, (uint32_t)__shfl_xor((int)most, o, kWave));
+    }
+    if (lane == 0) {
+      range[wv][0] = least;
+      range[wv][1] = most;
+    }
+    for (int i = tid; i < kBins; i += NT) hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      least = min(least, range[i][0]);
+      most = max(most, range[i][1]);
+    }
+    uint32_t span = most - least;  // the want-th lies in [least, least + span]
+    for (;;) {
+      const int shift = max(0, 32 - __builtin_clz(span | 1u) - 11);
+      for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) load(c);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = c * CHUNK + e * NT + tid;
+          const uint32_t at = ordered(x[e]) - least;
+          if (i >= lo && i < hi && at <= span) atomicAdd(&hist[at >> shift], 1);
+        }
       }
       __syncthreads();
-      // digit d holds the want-th largest when fewer than `want` lie in the digits above it and at least as many with it
-      const int d = 255 - tid, mine = hist[d];
-      int before, unused, total, total2;
-      scan2(mine, 0, scratch, before, unused, total, total2);
+      // the bin that holds the want-th: fewer than `want` lie in the bins above it, and not fewer with it. Thread t has
+      // bins kBins - 1 - (PER t + [0, PER))
+      int mine = 0, cnt[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        cnt[i] = hist[kBins - 1 - (tid * PER + i)];
+        mine += cnt[i];
+      }
+      int before, none, total, none2;
+      scan2<NW>(mine, 0, scratch, before, none, total, none2);
       if (before < want && before + mine >= want) {
-        s_digit = d;
-        s_want = want - before;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          if (before < want && before + cnt[i] >= want) {
+            s_bin = kBins - 1 - (tid * PER + i);
+            s_want = want - before;
+          }
+          before += cnt[i];
+        }
       }
+      for (int i = tid; i < kBins; i += NT) hist[i] = 0;
       __syncthreads();
-      top |= (uint32_t)s_digit << shift;
+      least += (uint32_t)s_bin << shift;
       want = s_want;
-      __syncthreads();
+      if (shift == 0) break;
+      span = (1u << shift) - 1u;
     }
+    top = least;
+    if (chunks > 1) load(0);
   }
-  // want: how many of those equal to T stay
-  int done = 0, ties = 0;  // kept, and equal ones met, before this tile
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + tid;
-    const float x = i < n ? w[i] : 0.f;
-    const uint32_t key = ordered(x);
-    const bool mid = i >= lo && i < hi;
-    const bool tie = mid && p.budget > p.sinks + p.recent && key == top;
-    bool keep = i < n && (!mid || (p.budget > p.sinks + p.recent && key > top));
-    int before, ties_before, kept, met;
-    scan2(0, tie, scratch, before, ties_before, kept, met);
-    keep = keep || (tie && ties + ties_before < want);
-    ties += met;
-    scan2(keep, 0, scratch, before, ties_before, kept, met);  // (every read of the tile lies before its barriers)
-    if (keep) {
-      const int j = done + before;
-      w[j] = x;
-      const int src = table[i / p.block_size];
-      int dst = table[j / p.block_size];
-      if (into && into[j / p.block_size] >= 0) dst = into[j / p.block_size];
-      const bool there = src >= 0 && src < p.num_blocks && dst >= 0 && dst < p.num_blocks;
-      const int64_t from = (int64_t)src * p.block_size + i % p.block_size;
-      moves[j] = there && from != (int64_t)dst * p.block_size + j % p.block_size ? (int)from : -1;
-    }
-    done += kept;
-    __syncthreads();
-  }
-}
-
-// Workgroup (sequence, plane = layer and K / V, kv head): rows of PIECES units of type V, `head_run` bytes a head, `slot_run`
-// a slot, from `at` bytes into the block on.
-template <typename V>
-__device__ __forceinline__ void move_rows(const EvictArgs& p, const int32_t* moves, int left, uint8_t* plane,
-                                          int64_t block_bytes, int64_t at, int64_t slot_run, int pieces,
-                                          const int32_t* table, const int32_t* into) {
-  const int rows = kMoveThreads * kMovePieces / pieces;  // a tile's
-  for (int base = 0; base < left; base += rows) {
-    V v[kMovePieces];
-    uint8_t* dst[kMovePieces];
+  // `want`: how many of those equal to T stay
+  int sure0 = 0, ties0 = 0;  // of the chunks before
+  for (int c = 0; c < chunks; ++c) {
+    if (c > 0) load(c);
+    auto kind = [&](int e, bool& sure, bool& tie) {
+      const int i = c * CHUNK + e * NT + tid;
+      const bool mid = i >= lo && i < hi;
+      const uint32_t key = ordered(x[e]);
+      sure = i < n && (!mid || (some && key > top));
+      tie = mid && some && key == top;
+    };
 #pragma unroll
-    for (int u = 0; u < kMovePieces; ++u) {
-      const int idx = u * kMoveThreads + (int)threadIdx.x;
-      const int j = base + idx / pieces, piece = idx % pieces;
-      const int from = idx / pieces < rows && j < left ? moves[j] : -1;
-      dst[u] = nullptr;
-      if (from >= 0) {
-        int blk = table[j / p.block_size];
-        if (into && into[j / p.block_size] >= 0) blk = into[j / p.block_size];
-        const int64_t src = (int64_t)(from / p.block_size) * block_bytes + at + (from % p.block_size) * slot_run;
-        dst[u] = plane + (int64_t)blk * block_bytes + at + (j % p.block_size) * slot_run + piece * (int)sizeof(V);
-        v[u] = *reinterpret_cast<const V*>(plane + src + piece * (int)sizeof(V));
+    for (int e = 0; e < E; ++e) {
+      bool sure, tie;
+      kind(e, sure, tie);
+      const int a = __builtin_popcountll(__builtin_amdgcn_ballot_w64(sure)), z = __builtin_popcountll(__builtin_amdgcn_ballot_w64(tie));
+      if (lane == 0) {
+        counts[e * NW + wv][0] = a;
+        counts[e * NW + wv][1] = z;
       }
     }
-    wait_vmem_all();  // every read of the tile before its first write
     __syncthreads();
+    int pa, pb, ta, tb;
+    const bool in = tid < E * NW;
+    scan2<NW>(in ? counts[tid][0] : 0, in ? counts[tid][1] : 0, scratch, pa, pb, ta, tb);
+    if (in) {
+      counts[tid][0] = sure0 + pa;
+      counts[tid][1] = ties0 + pb;
+    }
+    __syncthreads();  // (and every read of the chunk lies before this)
+    sure0 += ta;
+    ties0 += tb;
 #pragma unroll
-    for (int u = 0; u < kMovePieces; ++u)
-      if (dst[u]) *reinterpret_cast<V*>(dst[u]) = v[u];
+    for (int e = 0; e < E; ++e) {
+      bool sure, tie;
+      kind(e, sure, tie);
+      const uint64_t a = __builtin_amdgcn_ballot_w64(sure), z = __builtin_amdgcn_ballot_w64(tie);
+      const int before = counts[e * NW + wv][0] + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
+      const int ties = counts[e * NW + wv][1] + __builtin_amdgcn_mbcnt_hi((uint32_t)(z >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)z, 0));
+      if (sure || (tie && ties < want)) {
+        const int i = c * CHUNK + e * NT + tid, j = before + min(ties, want);
+        w[j] = x[e];
+        const int src = table[i / bs];
+        int dst = table[j / bs];
+        if (into && into[j / bs] >= 0) dst = into[j / bs];
+        const bool there = src >= 0 && src < p.num_blocks && dst >= 0 && dst < p.num_blocks;
+        const int from = there ? src * bs + i % bs : -1, to = there ? dst * bs + j % bs : -1;
+        moves[j] = make_int2(from == to ? -1 : from, to);
+      }
+    }
+    __syncthreads();
   }
 }
 
+// The rows of one (plane, sequence, kv head) moved: units of V, `pieces` a row, from byte `at` of a block on, a slot's
+// `slot_run` bytes apart; idle: a slot of the sequence's. LINEAR: the cache's slots are evenly spaced (no scales behind a block's slots).
+template <typename V, bool LINEAR>
+__device__ __forceinline__ void move_rows(const EvictArgs& p, const int2* moves, uint8_t* plane, int64_t block_bytes, int64_t at,
+                                          int64_t slot_run, int pieces, int idle) {
+  const int per = kMoveThreads / pieces;  // rows a step of the workgroup moves
+  const int r = (int)threadIdx.x / pieces, piece = (int)threadIdx.x % pieces;
+  const bool on = r < per;
+  uint8_t* const base = plane + at + piece * (int)sizeof(V);
+  auto place = [&](int slot) -> V* {
+    if constexpr (LINEAR) return reinterpret_cast<V*>(base + (int64_t)slot * slot_run);
+    const int blk = slot / p.block_size;
+    return reinterpret_cast<V*>(base + blk * block_bytes + (int64_t)(slot - blk * p.block_size) * slot_run);
+  };
+  const int left = p.budget, round = per * kMoveRows;
+  auto pairs = [&](int j0, int2 (&m)[kMoveRows]) {
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      const int j = j0 + u * per + r;
+      m[u] = moves[min(j, left - 1)];
+      if (!on || j >= left) m[u].x = -1;
+    }
+  };
+  // (rows that stay read the sequence's first slot, a line for them all, and store nothing: loads behind branches would have
+  // every wait for an earlier round wait for all)
+  auto rows = [&](const int2 (&m)[kMoveRows], V (&v)[kMoveRows]) {
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) v[u] = __builtin_nontemporal_load(place(m[u].x >= 0 ? m[u].x : idle));
+  };
+  auto write = [&](const int2 (&m)[kMoveRows], V (&v)[kMoveRows]) {
+    // every wave's reads of the round before its first write; the next round's, already on their way, lie behind them
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) asm volatile("" : "+v"(v[u]));
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u)
+      if (m[u].x >= 0) __builtin_nontemporal_store(v[u], place(m[u].y));
+  };
+  int2 ma[kMoveRows], mb[kMoveRows];
+  V va[kMoveRows], vb[kMoveRows];
+  const int rounds = (left + round - 1) / round;
+  pairs(0, ma);
+  rows(ma, va);
+  pairs(round, mb);
+  int t = 0;
+  for (; t + 2 < rounds; t += 2) {  // two rounds a turn, without copies of the registers
+    rows(mb, vb);
+    write(ma, va);
+    pairs((t + 2) * round, ma);
+    rows(ma, va);
+    write(mb, vb);
+    pairs((t + 3) * round, mb);
+  }
+  if (t + 1 < rounds) {
+    rows(mb, vb);
+    write(ma, va);
+    write(mb, vb);
+  } else {
+    write(ma, va);
+  }
+}
+
+// Workgroup (sequence, plane = layer and K / V, kv head x part): part x of p.parts slices of a row's bytes, or the scales.
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs p) {
-  const int b = blockIdx.x, plane = blockIdx.y, g = blockIdx.z;
+  const int b = blockIdx.x, plane = blockIdx.y, parts = p.parts + (p.scale_bytes ? 1 : 0);
+  const int g = blockIdx.z / parts, x = blockIdx.z % parts;
   const int n = max(0, min(p.context_lens[b], p.max_blocks * p.block_size));
   const int64_t row = p.rows ? (int64_t)p.rows[b] : b;
   if (n <= p.budget || row < 0 || row >= p.row_count) return;
-  const int32_t* moves = p.moves + (((int64_t)(plane >> 1) * p.batch + b) * p.num_heads + g) * p.kept;
-  const int32_t* table = p.block_tables + (int64_t)b * p.bt_stride;
-  const int32_t* into = p.into ? p.into + (int64_t)b * p.into_stride : nullptr;
+  const int2* moves = p.moves + (((int64_t)(plane >> 1) * p.batch + b) * p.num_heads + g) * p.kept;
   const int64_t block_bytes = (int64_t)p.block_size * p.num_heads * (p.head_bytes + p.scale_bytes);
+  const int64_t run = (int64_t)p.num_heads * p.head_bytes;
   uint8_t* base = p.kv + (int64_t)plane * p.num_blocks * block_bytes;
-  move_rows<u32x4>(p, moves, p.budget, base, block_bytes, (int64_t)g * p.head_bytes, (int64_t)p.num_heads * p.head_bytes,
-                   p.head_bytes / 16, table, into);
-  if (p.scale_bytes)
-    move_rows<uint32_t>(p, moves, p.budget, base, block_bytes,
-                        (int64_t)p.block_size * p.num_heads * p.head_bytes + (int64_t)g * p.scale_bytes,
-                        (int64_t)p.num_heads * p.scale_bytes, p.scale_bytes / 4, table, into);
+  const int blk0 = p.block_tables[(int64_t)b * p.bt_stride], idle = blk0 >= 0 && blk0 < p.num_blocks ? blk0 * p.block_size : 0;
+  const int bytes = p.head_bytes / p.parts;
+  const int64_t at = (int64_t)g * p.head_bytes + x * bytes;
+  if (!p.scale_bytes)
+    move_rows<u32x4, true>(p, moves, base, block_bytes, at, run, bytes / 16, idle);
+  else if (x < p.parts)
+    move_rows<u32x4, false>(p, moves, base, block_bytes, at, run, bytes / 16, idle);
+  else
+    move_rows<uint32_t, false>(p, moves, base, block_bytes, (int64_t)p.block_size * run + (int64_t)g * p.scale_bytes,
+                               (int64_t)p.num_heads * p.scale_bytes, p.scale_bytes / 4, idle);
 }
 
 }  // namespace
 
-hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
+hipError_t launch_evict(const EvictArgs& a0, hipStream_t stream) {
+  EvictArgs a = a0;
   if (a.batch <= 0 || a.layers <= 0 || a.num_heads <= 0) return hipSuccess;
-  select_kernel<<<dim3((unsigned)a.num_heads, (unsigned)a.batch, (unsigned)a.layers), dim3(kSelThreads), 0, stream>>>(a);
+  const dim3 grid((unsigned)a.num_heads, (unsigned)a.batch, (unsigned)a.layers);
+  // sequences that the tables let grow past 2048 tokens: 16 waves with 32 weights a lane (32768 tokens)
+  if ((int64_t)a.max_blocks * a.block_size <= 2048)
+    select_kernel<256, 8><<<grid, dim3(256), 0, stream>>>(a);
+  else
+    select_kernel<1024, 32><<<grid, dim3(1024), 0, stream>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  move_kernel<<<dim3((unsigned)a.batch, (unsigned)(2 * a.layers), (unsigned)a.num_heads), dim3(kMoveThreads), 0, stream>>>(a);
+  // slices of a row of 64 bytes or more, until there are two workgroups a CU
+  a.parts = 1;
+  while (a.parts < 4 && a.head_bytes % (a.parts * 128) == 0 &&
+         (int64_t)a.batch * 2 * a.layers * a.num_heads * a.parts < 512)
+    a.parts *= 2;
+  move_kernel<<<dim3((unsigned)a.batch, (unsigned)(2 * a.layers), (unsigned)(a.num_heads * (a.parts + (a.scale_bytes ? 1 : 0)))),
+                dim3(kMoveThreads), 0, stream>>>(a);
   return hipGetLastError();
 }
 
