@@ -471,3 +471,17 @@ def test_chunk_in_parts_of_its_rows():
     _varlen_case(34, [(600, 600), (130, 130)], 64, 1)
     _varlen_case(35, [(1300, 1300)], 8, 1)
     _varlen_case(36, [(2100, 2100)], 2, 2)
+
+
+def test_evict_with_tables_wider_than_a_workgroup_holds():
+    """Blocks of 16 tokens: 600 columns, with and without new blocks; a block size that is no power of two."""
+    gen = torch.Generator().manual_seed(41)
+    for bs, n, budget in ((16, 9500, 700), (48, 3000, 1111)):
+        cols = -(-n // bs) + 5
+        need = -(-n // bs)
+        tables, rest = _tables(gen, [n, 40], need + 3 + -(-budget // bs) + 4, bs, cols)
+        weights = torch.rand(1, 2, 2, cols * bs, generator=gen)
+        kv = _kv(gen, 1, need + 3 + -(-budget // bs) + 4, bs, 2, "narrow")
+        _evict_case(kv.clone(), weights.clone(), tables, [n, 40], budget, 3, 100)
+        new = [rest[:-(-budget // bs)] + [-1] * (cols - -(-budget // bs)), [-1] * cols]
+        _evict_case(kv, weights, tables, [n, 40], budget, 3, 100, None, new)

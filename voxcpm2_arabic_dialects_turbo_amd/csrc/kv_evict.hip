@@ -2,9 +2,8 @@
 // launches: which tokens stay (select_kernel), and their rows moved to the front of the sequence (move_kernel).
 //
 // select: a workgroup per (kv head, sequence, layer). Of the tokens [sinks, n - recent) the `want` heaviest stay, of equal
-// ones the earliest. The want-th largest weight T is found over the weights as ordered integers (ordered): a histogram of
-// 2048 equal steps between the least and the largest (LDS), then of 2048 steps of the step that holds the want-th, until a
-// step is one integer, three rounds at most. Tokens above T stay, and of those equal to T the first ones that are still
+// ones the earliest. The want-th largest weight T is found digit by digit over the weights as ordered integers (ordered), 11,
+// 11 and 10 bits, each digit from a histogram in LDS of the weights that share the ones before it. Tokens above T stay, and of those equal to T the first ones that are still
 // wanted. Place j of a kept token at i is how many kept ones lie before it: (those above T or protected before i) + min(those
 // equal to T before i, still wanted), from ballots and one scan. Its weight moves there, and move_kernel gets the pair of
 // slots. Weights are held in registers (lane-contiguous rounds of the workgroup); rows longer than those are read again.
@@ -21,6 +20,7 @@ namespace {
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 8;  // rows a lane keeps in flight, twice (a round's, and the next one's)
 constexpr int kBins = 2048;
+constexpr int kTable = 512;  // blocks of a sequence that a workgroup holds in LDS
 
 // Weights as integers of the same order: NaN above everything, the two zeros the same.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -61,9 +61,9 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
   static_assert(E * NW <= NT && kBins % NT == 0, "a thread scans a count and its bins");
   __shared__ int hist[kBins];
   __shared__ int scratch[NW][2];
-  __shared__ uint32_t range[NW][2];
   __shared__ int counts[E * NW][2];  // [round][wave]: tokens that stay for sure, and those equal to T
   __shared__ int s_bin, s_want;
+  __shared__ int s_from[kTable], s_to[kTable];  // the blocks of the sequence, and those that take what it keeps
   const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
   const int lane = tid & 63, wv = tid >> 6;
   const int bs = p.block_size;
@@ -86,57 +86,49 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
   int2* moves = p.moves + (((int64_t)layer * p.batch + b) * p.num_heads + g) * p.kept;
   const int lo = p.sinks, hi = n - p.recent;  // (n > budget >= sinks + recent)
   int want = p.budget - p.sinks - p.recent;
-  const bool some = want > 0;
   const int chunks = (n + CHUNK - 1) / CHUNK;
 
+  const bool held = p.max_blocks <= kTable;
+  for (int c = tid; held && c < p.max_blocks; c += NT) {
+    const int blk = table[c];
+    s_from[c] = blk;
+    s_to[c] = into && into[c] >= 0 ? into[c] : blk;
+  }
+  const int* const from_block = held ? s_from : table;  // (read behind the barriers below)
+  const int* const to_block = held ? s_to : table;
+
+  // a lane's weights, and as ordered integers; 0, which none has, for the tokens that are not among the `mid` ones
   float x[E];
+  uint32_t key[E];
   auto load = [&](int c) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = c * CHUNK + e * NT + tid;
-      x[e] = i < n ? w[i] : 0.f;
+      x[e] = w[min(i, n - 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = c * CHUNK + e * NT + tid;
+      key[e] = i >= lo && i < hi ? ordered(x[e]) : 0u;
     }
   };
   load(0);
-  uint32_t top = 0;  // T
-  if (some) {
-    uint32_t least = 0xffffffffu, most = 0;
-    for (int c = 0; c < chunks; ++c) {
-      if (c > 0) load(c);
+  uint32_t top = 0xffffffffu;  // T; where none of the mid ones stays, none is above it, and of those equal to it none is wanted
+  if (want > 0) {
+    top = 0;
+    // T's digits of 11, 11 and 10 bits, each from a histogram of the weights that have the digits before it
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = c * CHUNK + e * NT + tid;
-        const uint32_t key = ordered(x[e]);
-        least = min(least, i >= lo && i < hi ? key : 0xffffffffu);
-        most = max(most, i >= lo && i < hi ? key : 0u);
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      least = min(least, (uint32_t)__shfl_xor((int)least, o, kWave));
-      most = max(most, (uint32_t)__shfl_xor((int)most, o, kWave));
-    }
-    if (lane == 0) {
-      range[wv][0] = least;
-      range[wv][1] = most;
-    }
-    for (int i = tid; i < kBins; i += NT) hist[i] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      least = min(least, range[i][0]);
-      most = max(most, range[i][1]);
-    }
-    uint32_t span = most - least;  // the want-th lies in [least, least + span]
-    for (;;) {
-      const int shift = max(0, 32 - __builtin_clz(span | 1u) - 11);
+    for (int level = 0; level < 3; ++level) {
+      const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
+      const uint32_t span = level == 0 ? 0xffffffffu : level == 1 ? 0x1fffffu : 0x3ffu;
+      for (int i = tid; i < kBins; i += NT) hist[i] = 0;
+      __syncthreads();
       for (int c = 0; c < chunks; ++c) {
         if (chunks > 1) load(c);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int i = c * CHUNK + e * NT + tid;
-          const uint32_t at = ordered(x[e]) - least;
-          if (i >= lo && i < hi && at <= span) atomicAdd(&hist[at >> shift], 1);
+          const uint32_t at = key[e] - top;
+          if (level == 0 ? key[e] != 0 : at <= span) atomicAdd(&hist[at >> shift], 1);
         }
       }
       __syncthreads();
@@ -160,14 +152,10 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
           before += cnt[i];
         }
       }
-      for (int i = tid; i < kBins; i += NT) hist[i] = 0;
       __syncthreads();
-      least += (uint32_t)s_bin << shift;
+      top += (uint32_t)s_bin << shift;
       want = s_want;
-      if (shift == 0) break;
-      span = (1u << shift) - 1u;
     }
-    top = least;
     if (chunks > 1) load(0);
   }
   // `want`: how many of those equal to T stay
@@ -176,10 +164,8 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
     if (c > 0) load(c);
     auto kind = [&](int e, bool& sure, bool& tie) {
       const int i = c * CHUNK + e * NT + tid;
-      const bool mid = i >= lo && i < hi;
-      const uint32_t key = ordered(x[e]);
-      sure = i < n && (!mid || (some && key > top));
-      tie = mid && some && key == top;
+      sure = key[e] > top || (key[e] == 0 && i < n);
+      tie = key[e] == top;
     };
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -202,23 +188,31 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
     __syncthreads();  // (and every read of the chunk lies before this)
     sure0 += ta;
     ties0 += tb;
+    auto put = [&](auto block_of) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      bool sure, tie;
-      kind(e, sure, tie);
-      const uint64_t a = __builtin_amdgcn_ballot_w64(sure), z = __builtin_amdgcn_ballot_w64(tie);
-      const int before = counts[e * NW + wv][0] + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
-      const int ties = counts[e * NW + wv][1] + __builtin_amdgcn_mbcnt_hi((uint32_t)(z >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)z, 0));
-      if (sure || (tie && ties < want)) {
-        const int i = c * CHUNK + e * NT + tid, j = before + min(ties, want);
-        w[j] = x[e];
-        const int src = table[i / bs];
-        int dst = table[j / bs];
-        if (into && into[j / bs] >= 0) dst = into[j / bs];
-        const bool there = src >= 0 && src < p.num_blocks && dst >= 0 && dst < p.num_blocks;
-        const int from = there ? src * bs + i % bs : -1, to = there ? dst * bs + j % bs : -1;
-        moves[j] = make_int2(from == to ? -1 : from, to);
+      for (int e = 0; e < E; ++e) {
+        bool sure, tie;
+        kind(e, sure, tie);
+        const uint64_t a = __builtin_amdgcn_ballot_w64(sure), z = __builtin_amdgcn_ballot_w64(tie);
+        const int before = counts[e * NW + wv][0] + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
+        const int ties = counts[e * NW + wv][1] + __builtin_amdgcn_mbcnt_hi((uint32_t)(z >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)z, 0));
+        if (sure || (tie && ties < want)) {
+          const int i = c * CHUNK + e * NT + tid, j = before + min(ties, want);
+          w[j] = x[e];
+          const int ci = block_of(i), cj = block_of(j), src = from_block[ci];
+          int dst = to_block[cj];
+          if (!held && into && into[cj] >= 0) dst = into[cj];
+          const bool there = src >= 0 && src < p.num_blocks && dst >= 0 && dst < p.num_blocks;
+          const int from = there ? src * bs + i - ci * bs : -1, to = there ? dst * bs + j - cj * bs : -1;
+          moves[j] = make_int2(from == to ? -1 : from, to);
+        }
       }
+    };
+    if ((bs & (bs - 1)) == 0) {  // (a division is some twenty instructions)
+      const int sh = __builtin_ctz(bs);
+      put([&](int i) { return i >> sh; });
+    } else {
+      put([&](int i) { return i / bs; });
     }
     __syncthreads();
   }
