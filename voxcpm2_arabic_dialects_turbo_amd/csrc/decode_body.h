@@ -674,10 +674,6 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
           x[q4] = full || (T.ok && (t0 + jq * 4 + q4) < tok_end) ? s[q4] : -INFINITY;
-        if constexpr (SCORES) {  // step t's scores [H][16 tokens], not scaled
-          if (h < H)
-            *reinterpret_cast<f32x4*>(p.scores + ((int64_t)t * H + h) * kTile + jq * 4) = f32x4{x[0], x[1], x[2], x[3]};
-        }
         // V tile -> LDS, row-major, 16-byte stores; rows of tokens past tok_end or of an unmapped block are zeroed
         // (they meet p = 0 in P V, and unwritten cache slots may hold any bit pattern)
         if (full) {
@@ -696,6 +692,12 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& p, const int g, c
         }
         wave_lds_sync();
         between();  // the tile's registers are free: the next tile's loads go out before the softmax and P V
+        if constexpr (SCORES) {
+          // step t's scores [H][16 tokens], not scaled; behind the loads, whose waits would else wait for the store too (24
+          // of 20000-32768 tokens 152 -> 143 us)
+          if (h < H)
+            *reinterpret_cast<f32x4*>(p.scores + ((int64_t)t * H + h) * kTile + jq * 4) = f32x4{x[0], x[1], x[2], x[3]};
+        }
 
         const float tm = col_max4(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) * c;
         const bool up = tm > m + 8.f;
@@ -945,54 +947,84 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
   const int lane = threadIdx.x & 63;
   const int r16 = lane & 15, sub = lane >> 4;
   const int H = p.num_heads, HK = H / p.group;
-  const int64_t S = p.steps[p.batch], G = p.steps[p.batch + 1];
+  // lane k: sequence base + k's first and end steps, context and row
+  int base = 0, st = 0, en = 0, len = 0, row = 0;
+  auto window = [&](int at) {
+    base = at;
+    const int b = min(at + lane, p.batch - 1);
+    st = p.steps[b];
+    en = p.steps[b + 1];
+    len = p.cu_q ? p.cu_k[b + 1] - p.cu_k[b] : p.context_lens[b];
+    row = p.weight_rows ? p.weight_rows[b] : (int)p.weight_row0 + b;
+  };
+  int s_tot = p.steps[p.batch], s_g = p.steps[p.batch + 1];
+  window(0);
+  // (one round trip: left to itself the compiler loads each where it is first used)
+  asm volatile("" ::"s"(s_tot), "s"(s_g), "v"(st), "v"(en), "v"(len), "v"(row));
+  const int64_t S = s_tot, G = s_g;
   const int r0 = (int)muldiv(W, S, 0, N), r1 = (int)muldiv(W + 1, S, 0, N);
   if (r0 >= r1) return;
   // the sequence of step r0: the last that starts at or before it (an empty one shares its start with the next)
-  int b = -1;
-  for (int c = 0; c < p.batch; c += kWave) {
-    const bool at = c + lane < p.batch && p.steps[c + lane] <= r0;
-    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
+  int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < p.batch && st <= r0)) - 1;
+  if (b == kWave - 1) {
+    for (int c = kWave; c < p.batch; c += kWave) {
+      const bool at = c + lane < p.batch && p.steps[min(c + lane, p.batch)] <= r0;
+      b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at));
+    }
+    window(b / kWave * kWave);
   }
   for (int t = r0; t < r1; ++b) {
-    const int sb = p.steps[b], eb = p.steps[b + 1];
+    if (b - base >= kWave) window(b);
+    const int k = b - base;
+    const int sb = __builtin_amdgcn_readlane(st, k), eb = __builtin_amdgcn_readlane(en, k);
     if (eb <= t) continue;
     const int te = min(r1, eb);
+    const int n = __builtin_amdgcn_readlane(len, k);
+    const int64_t wr = __builtin_amdgcn_readlane(row, k), reach = min((int64_t)n, p.weight_width);
+    const bool mine = wr >= 0 && wr < p.weight_row_count;
+    float* const wb = p.weights + wr * HK * p.weight_width;
+    // steps u to u + 3: the scores of every head and the weights
+    float x[kMaxHeads], w0 = 0.f, w1 = 0.f;
+    auto live = [&](int u) { return mine && u + sub < te && (int64_t)(u + sub - sb) * kTile + r16 < reach; };
+    auto fetch = [&](int u) {
+      const int64_t tok = (int64_t)(u + sub - sb) * kTile + r16;
+      const float* s = p.scores + (int64_t)(u + sub) * H * kTile + r16;
+      if (live(u)) {
+#pragma unroll
+        for (int hh = 0; hh < kMaxHeads; ++hh) x[hh] = hh < H ? s[hh * kTile] : -INFINITY;
+        w0 = wb[tok];
+        w1 = HK == 2 ? wb[p.weight_width + tok] : 0.f;
+      }
+    };
+    fetch(t);
     // the sequence's pieces are those of merge_row; four at a time, head r16
     const int g_first = (int)muldiv(sb + 1, G, S - 1, S) - 1;
     const int g_last = (int)min(G - 1, muldiv(eb, G, S - 1, S) - 1);
     float M = -INFINITY, L = 0.f;
-    for (int gg = g_first + sub; gg <= g_last; gg += 4) {
-      const float* pc = p.partials + (int64_t)(b + gg) * kPartialFloats;
-      const float mc = pc[kMOff + r16], lc = pc[kLOff + r16];
-      const float mn = fmaxf(M, mc);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      L = L * fast_exp2(M - mu) + lc * fast_exp2(mc - mu);
-      M = mn;
+    constexpr int kPieces = 8;  // of a lane's loads in flight
+    for (int g0 = g_first + sub; g0 - sub <= g_last; g0 += 4 * kPieces) {
+      float mc[kPieces], lc[kPieces];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const float* pc = p.partials + (int64_t)(b + min(g0 + 4 * i, g_last)) * kPartialFloats;
+        mc[i] = pc[kMOff + r16];
+        lc[i] = pc[kLOff + r16];
+      }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const bool in = g0 + 4 * i <= g_last;
+        const float mn = fmaxf(M, in ? mc[i] : -INFINITY);
+        const float mu = mn == -INFINITY ? 0.f : mn;
+        L = L * fast_exp2(M - mu) + (in ? lc[i] * fast_exp2(mc[i] - mu) : 0.f);
+        M = mn;
+      }
     }
     const float Mt = col_max4(M);
     const float Lt = col_sum4(L * fast_exp2(M - (Mt == -INFINITY ? 0.f : Mt)));
     // (a head without any key: exp2(s c - inf) = 0)
     lse[r16] = Lt == 0.f ? INFINITY : Mt + __builtin_amdgcn_logf(Lt);
     wave_lds_sync();
-    int len = 0;
-    if (p.cu_q)
-      len = p.cu_k[b + 1] - p.cu_k[b];
-    else
-      len = p.context_lens[b];
-    const int64_t reach = min((int64_t)len, p.weight_width);
-    const int64_t row = p.weight_rows ? (int64_t)p.weight_rows[b] : p.weight_row0 + b;
-    const bool mine = row >= 0 && row < p.weight_row_count;
     for (int u = t; u < te; u += 4) {
-      const int step = u + sub;
-      const int64_t tok = (int64_t)(step - sb) * kTile + r16;
-      if (!mine || step >= te || tok >= reach) continue;
-      const float* s = p.scores + (int64_t)step * H * kTile + r16;
-      float* w = p.weights + row * HK * p.weight_width + tok;
-      float x[kMaxHeads];
-#pragma unroll
-      for (int hh = 0; hh < kMaxHeads; ++hh) x[hh] = hh < H ? s[hh * kTile] : -INFINITY;
-      const float w0 = w[0], w1 = HK == 2 ? w[p.weight_width] : 0.f;
       float a0 = 0.f, a1 = 0.f;
 #pragma unroll
       for (int hh = 0; hh < kMaxHeads; ++hh) {
@@ -1000,9 +1032,13 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
         a0 += hh < p.group ? e : 0.f;
         a1 += hh < p.group ? 0.f : e;
       }
-      const bool fresh = tok == len - 1;
-      w[0] = fresh ? a0 : w0 + a0;
-      if (HK == 2) w[p.weight_width] = fresh ? a1 : w1 + a1;
+      if (live(u)) {
+        const int64_t tok = (int64_t)(u + sub - sb) * kTile + r16;
+        const bool fresh = tok == n - 1;
+        wb[tok] = fresh ? a0 : w0 + a0;
+        if (HK == 2) wb[p.weight_width + tok] = fresh ? a1 : w1 + a1;
+      }
+      if (u + 4 < te) fetch(u + 4);
     }
     wave_lds_sync();  // (lse is read before the next sequence's)
     t = te;
