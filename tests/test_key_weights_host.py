@@ -269,7 +269,7 @@ def test_weights_refusals(kw, error, match):
     a = dict(key_weights=torch.zeros(2, 2, 128), weight_rows=None)
     a.update(kw)
     with pytest.raises(error, match=match):
-        ops_weights._weights("f", a["key_weights"], a["weight_rows"], 2, 2, 128, torch.device("cpu"))
+        ops_weights._weights("f", a["key_weights"], a["weight_rows"], 2, 2, 128, -1)
 
 
 def test_decode_rows_refusals(monkeypatch):

@@ -26,51 +26,57 @@ from .ops_fp4 import _ids, _on, _row_stride, _table, _workspace
 
 
 def _weights(fn: str, key_weights: torch.Tensor, weight_rows: torch.Tensor | None, batch: int, hk: int, reach: int,
-             dev: torch.device) -> torch.Tensor | None:
-    """The checked ``weight_rows`` as int32 [batch], None where sequence b has row b."""
+             index: int) -> tuple[int, int, torch.Tensor | None]:
+    """The rows and width of key_weights, and weight_rows as int32 [batch], None where sequence b has row b."""
     if key_weights.dtype != torch.float32:
         raise TypeError(f"{fn}: key_weights must be fp32, got {key_weights.dtype}")
-    if key_weights.dim() != 3 or key_weights.shape[1] != hk or not key_weights.is_contiguous():
-        raise ValueError(f"{fn}: key_weights must be contiguous [rows, {hk}, width], got {tuple(key_weights.shape)}")
-    if key_weights.shape[2] < reach:
-        raise ValueError(f"{fn}: key_weights hold {key_weights.shape[2]} tokens a row, the keys may be {reach}")
-    if key_weights.device != dev:
-        raise ValueError(f"all tensors must be on the same GPU, got {key_weights.device} and {dev}")
+    shape = key_weights.shape
+    if len(shape) != 3 or shape[1] != hk or not key_weights.is_contiguous():
+        raise ValueError(f"{fn}: key_weights must be contiguous [rows, {hk}, width], got {tuple(shape)}")
+    rows, _, width = shape
+    if width < reach:
+        raise ValueError(f"{fn}: key_weights hold {width} tokens a row, the keys may be {reach}")
+    if key_weights.get_device() != index or (weight_rows is not None and weight_rows.get_device() != index):
+        raise ValueError(f"{fn}: key_weights and weight_rows must be on the other tensors' GPU")
     if weight_rows is None:
-        if key_weights.shape[0] < batch:
-            raise ValueError(f"{fn}: key_weights have {key_weights.shape[0]} rows for {batch} sequences")
-        return None
+        if rows < batch:
+            raise ValueError(f"{fn}: key_weights have {rows} rows for {batch} sequences")
+        return rows, width, None
     if weight_rows.numel() != batch:
         raise ValueError(f"{fn}: weight_rows must hold one row per sequence")
-    if key_weights.shape[0] == 0:
+    if rows == 0:
         raise ValueError(f"{fn}: key_weights have no rows")
-    if weight_rows.device != dev:
-        raise ValueError(f"all tensors must be on the same GPU, got {weight_rows.device} and {dev}")
-    return _ids(weight_rows, "weight_rows")
+    if weight_rows.dtype == torch.int32 and weight_rows.is_contiguous():
+        return rows, width, weight_rows
+    return rows, width, _ids(weight_rows, "weight_rows")
 
 
 def _query(fn: str, q: torch.Tensor, out: torch.Tensor | None, dev: torch.device, contiguous: bool
-           ) -> tuple[torch.Tensor, torch.Tensor]:
-    """q with token rows apart from each other, and where the output goes."""
+           ) -> tuple[torch.Tensor, int, torch.Tensor]:
+    """q with token rows apart from each other, the elements between them, and where the output goes."""
     n, H, D = q.shape
-    if D != HEAD_DIM or q.stride(2) != 1 or (q.stride(1) != D and H > 1):
+    s0, s1, s2 = q.stride()
+    if D != HEAD_DIM or s2 != 1 or (s1 != D and H > 1):
         raise ValueError(f"{fn}: q must be [rows, H, {HEAD_DIM}] with contiguous heads, got {tuple(q.shape)} {q.stride()}")
     if out is None:
-        out = torch.empty(n, H, D, dtype=q.dtype, device=dev)
+        out = torch.empty((n, H, D), dtype=torch.bfloat16, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 or out.stride(1) != D \
             or (contiguous and not out.is_contiguous()):
         raise ValueError(f"{fn}: out must be a bf16 [{n}, {H}, {D}] with contiguous heads on {dev}")
-    return q.contiguous() if n > 1 and q.stride(0) < H * D else q, out
+    if n == 1:  # (a single row's stride means nothing)
+        return q, H * D, out
+    return (q, s0, out) if s0 >= H * D else (q.contiguous(), H * D, out)
 
 
 def _caches(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int]:
     """(num_blocks, block_size, HK) of a pair of bf16 caches."""
+    shape = k_cache.shape
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         raise TypeError(f"{fn} takes bf16 caches, got {k_cache.dtype} and {v_cache.dtype}")
-    if k_cache.dim() != 4 or k_cache.shape[3] != HEAD_DIM or v_cache.shape != k_cache.shape \
-            or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v_cache.shape != shape or not (k_cache.is_contiguous()
+                                                                                and v_cache.is_contiguous()):
         raise ValueError(f"{fn}: caches must be contiguous [num_blocks, block_size, HK, {HEAD_DIM}] of one shape")
-    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[2]
+    return shape[0], shape[1], shape[2]
 
 
 def _new_rows(fn: str, key: torch.Tensor, value: torch.Tensor, hk: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -116,9 +122,9 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     dev = _check_cuda(q, k_cache, v_cache, context_lens, block_tables)
     bt, bt_stride = _table(block_tables)
     mb = bt.shape[1]
-    rows = _weights(fn, key_weights, weight_rows, B, hk, mb * bs, dev)
-    q, out = _query(fn, q, out, dev, True)
-    rides = False
+    n_rows, width, rows = _weights(fn, key_weights, weight_rows, B, hk, mb * bs, q.get_device())
+    q, q_stride, out = _query(fn, q, out, dev, True)
+    ride = (None, None, 0, 0, None)
     if key is not None:
         if value is None or slot_mapping is None:
             raise ValueError(f"{fn}: key, value and slot_mapping go together")
@@ -126,9 +132,10 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         key, value = _new_rows(fn, key, value, hk)
         if key.shape[0] != B or slot_mapping.numel() != B:
             raise ValueError(f"{fn}: key, value and slot_mapping must hold {B} rows")
-        slots = _ids(slot_mapping, "slot_mapping")
+        slots, ks, vs = _ids(slot_mapping, "slot_mapping"), _row_stride(key), _row_stride(value)
         # (rows that 16-byte loads cannot take are stored by a call of their own)
-        rides = (key.data_ptr() | value.data_ptr()) % 16 == 0 and (_row_stride(key) | _row_stride(value)) % 8 == 0
+        if (key.data_ptr() | value.data_ptr()) % 16 == 0 and (ks | vs) % 8 == 0:
+            ride = (key.data_ptr(), value.data_ptr(), ks, vs, slots.data_ptr())
     elif value is not None or slot_mapping is not None:
         raise ValueError(f"{fn}: key, value and slot_mapping go together")
     if B == 0:
@@ -136,18 +143,27 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     lens = _as_i32(_flat(context_lens), "context_lens")
     lib = _lib.load()
     with _on(dev):
-        if key is not None and not rides:
+        if key is not None and ride[0] is None:
             store_kvcache(key, value, k_cache, v_cache, slots)
-        ws, mode, recorded = _workspace(lib, dev, B, plan, "decode_weights", rides, B, mb, bt_stride, H, hk, bs)
-        scores = torch.empty(lib.vox_decode_scores_bytes(B, mb, bs, H), dtype=torch.uint8, device=dev)
+        need = lib.vox_decode_scores_bytes(B, mb, bs, H)
+        mode, recorded = _lib.PLAN_NONE, None
+        if plan is None:  # all scratch in one piece: the call's own
+            ws_bytes = lib.vox_decode_workspace_bytes(B)
+            scratch = torch.empty((ws_bytes + need,), dtype=torch.uint8, device=dev)
+            ws = scratch.data_ptr()
+            scores = ws + ws_bytes
+        else:
+            scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
+            scores = scratch.data_ptr()
+            kept, mode, recorded = _workspace(lib, dev, B, plan, "decode_weights", ride[0] is not None, B, mb, bt_stride, H,
+                                              hk, bs)
+            ws, ws_bytes = kept.data_ptr(), kept.numel()
         _lib.check(lib.vox_decode_attn_weights(
-            q.data_ptr(), _row_stride(q), key.data_ptr() if rides else None, value.data_ptr() if rides else None,
-            _row_stride(key) if rides else 0, _row_stride(value) if rides else 0, slots.data_ptr() if rides else None,
-            k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, mb, lens.data_ptr(), B, H, hk, D,
-            scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), key_weights.shape[0],
-            key_weights.shape[2], scores.data_ptr(), scores.numel(), mode, ws.data_ptr(), ws.numel(), out.data_ptr(),
-            _lib.stream_handle(dev)), fn)
-    _plan_recorded(dev, recorded)
+            q.data_ptr(), q_stride, *ride, k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, mb,
+            lens.data_ptr(), B, H, hk, D, scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), n_rows,
+            width, scores, need, mode, ws, ws_bytes, out.data_ptr(), _lib.stream_handle(dev)), fn)
+    if recorded is not None:
+        _plan_recorded(dev, recorded)
     return out
 
 
@@ -197,25 +213,26 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         keys = (k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), None, None, 0, 0, None, 0, 0)
     if hk == 0 or H == 0 or H % hk:
         raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {hk}")
-    rows = _weights(fn, key_weights, weight_rows, max(B, 0), hk, reach, dev)
-    q, out = _query(fn, q, out, dev, False)
+    n_rows, width, rows = _weights(fn, key_weights, weight_rows, max(B, 0), hk, reach, q.get_device())
+    q, q_stride, out = _query(fn, q, out, dev, False)
     if T == 0 or B <= 0 or max_seqlen_q <= 0:
         return out
     cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
     lib = _lib.load()
     with _on(dev):
-        scratch = torch.empty(lib.vox_prefill_weights_bytes(T, B, int(max_seqlen_q), reach, H, hk), dtype=torch.uint8,
-                              device=dev)
-        ws, scores, mode, recorded = None, None, _lib.PLAN_NONE, None
+        need = lib.vox_prefill_weights_bytes(T, B, int(max_seqlen_q), reach, H, hk)
+        scores_at = (need + 255) // 256 * 256
+        ws, scores_bytes, mode, recorded = None, 0, _lib.PLAN_NONE, None
         if block_table is not None and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) \
                 and _takes_decode_rows(H, hk, bs, bt.shape[1], out, _row_stride(out)):
             ws, mode, recorded = _workspace(lib, dev, B, plan, "varlen_weights", B, bt.shape[1], bt_stride, H, hk, bs)
-            scores = torch.empty(lib.vox_decode_scores_bytes(B, bt.shape[1], bs, H), dtype=torch.uint8, device=dev)
+            scores_bytes = lib.vox_decode_scores_bytes(B, bt.shape[1], bs, H)
+        scratch = torch.empty((scores_at + scores_bytes,), dtype=torch.uint8, device=dev)
+        at = scratch.data_ptr()
         _lib.check(lib.vox_prefill_attn_weights(
-            q.data_ptr(), _row_stride(q), *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, int(max_seqlen_q), reach, T, H, hk, D,
-            scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), key_weights.shape[0],
-            key_weights.shape[2], scratch.data_ptr(), scratch.numel(), None if scores is None else scores.data_ptr(),
-            0 if scores is None else scores.numel(), mode, None if ws is None else ws.data_ptr(),
+            q.data_ptr(), q_stride, *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, int(max_seqlen_q), reach, T, H, hk, D,
+            scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), n_rows, width, at, need,
+            at + scores_at if scores_bytes else None, scores_bytes, mode, None if ws is None else ws.data_ptr(),
             0 if ws is None else ws.numel(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
     _plan_recorded(dev, recorded)
     return out
