@@ -117,7 +117,9 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
 }
 
 // Persistent: the items (128 keys, a part of the query rows, kv head, sequence), the key blocks of a part side by side, are
-// dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2.
+// dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2. DIRECT, where the grid of
+// all there may be is at most two workgroups a CU: a workgroup for each, without the items' layout.
+template <bool DIRECT>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   constexpr int KW = 2, QW = 2, KT = 2;
   constexpr int KEYS = 32 * KT;               // keys of a wave
@@ -128,8 +130,8 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   __shared__ __attribute__((aligned(1024))) uint8_t buf0[BUF];
   __shared__ __attribute__((aligned(1024))) uint8_t buf1[BUF];
   __shared__ float sums[4][KEYS];
-  __shared__ int starts[kMaxSeqPerLaunch + 1];
-  __shared__ int wtot[4];
+  __shared__ int starts[DIRECT ? 1 : kMaxSeqPerLaunch + 1];
+  __shared__ int wtot[DIRECT ? 1 : 4];
   typedef __attribute__((address_space(3))) void lds_void;
   using std::integral_constant;
   const int tid = threadIdx.x;
@@ -148,55 +150,52 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   for (int i = 0; i < 8; ++i) frag[i] = (uint32_t)(qw * TILE + col * 256 + (((2 * i + h) ^ (col & 15)) << 4));
   const uint32_t lse_at = (uint32_t)(QW * TILE + w * 256 + col * 4);
 
-  // ---- every sequence's first item
-  const int total = number_items(p.batch, starts, wtot, [&](int b) {
-    const KwSeq s = kw_seq(k, b, gsh);
-    int items = 0;
-    for (int x = 0; x < s.parts; ++x) items += s.blocks(k, x, gsh);
-    return items * HK;
-  });
-  const int xcd = blockIdx.x % kXcds, wgs = gridDim.x / kXcds;  // (the grid is a multiple of the XCDs)
-  const int hi = (int)((int64_t)total * (xcd + 1) / kXcds);
+  // ---- every sequence's first item, and this workgroup's items
+  int item = (int)blockIdx.x, step = 1, hi = item + 1;
+  if constexpr (!DIRECT) {
+    const int total = number_items(p.batch, starts, wtot, [&](int b) {
+      const KwSeq s = kw_seq(k, b, gsh);
+      int items = 0;
+      for (int x = 0; x < s.parts; ++x) items += s.blocks(k, x, gsh);
+      return items * HK;
+    });
+    const int xcd = blockIdx.x % kXcds;
+    step = gridDim.x / kXcds;  // (the grid is a multiple of the XCDs)
+    item = (int)((int64_t)total * xcd / kXcds) + (int)(blockIdx.x / kXcds);
+    hi = (int)((int64_t)total * (xcd + 1) / kXcds);
+  }
 
-  for (int item = (int)((int64_t)total * xcd / kXcds) + (int)(blockIdx.x / kXcds); item < hi; item += wgs) {
+  for (; item < hi; item += step) {
     // ---- the item's sequence, part, kv head and key block
-    const int b = sequence_of(item, p.batch, starts);
-    const KwSeq s = kw_seq(k, b, gsh);
-    int left = item - starts[b], x = 0, blocks = s.blocks(k, 0, gsh);
-    while (left >= blocks * HK) {
-      left -= blocks * HK;
-      blocks = s.blocks(k, ++x, gsh);
+    int b, x, g, first;
+    KwSeq s;
+    if constexpr (DIRECT) {
+      const int blocks = (k.max_k + kKwKeys - 1) / kKwKeys;
+      first = item % blocks * kKwKeys;
+      x = item / blocks % k.max_parts;
+      g = item / blocks / k.max_parts % HK;
+      b = item / blocks / k.max_parts / HK;
+      s = kw_seq(k, b, gsh);
+      if (x >= s.parts || first >= s.blocks(k, x, gsh) * kKwKeys) return;
+    } else {
+      b = sequence_of(item, p.batch, starts);
+      s = kw_seq(k, b, gsh);
+      int left = item - starts[b], blocks = s.blocks(k, 0, gsh);
+      x = 0;
+      while (left >= blocks * HK) {
+        left -= blocks * HK;
+        blocks = s.blocks(k, ++x, gsh);
+      }
+      left = __builtin_amdgcn_readfirstlane(left);
+      x = __builtin_amdgcn_readfirstlane(x);
+      blocks = __builtin_amdgcn_readfirstlane(blocks);
+      g = left / blocks;
+      first = left % blocks * kKwKeys;
     }
-    left = __builtin_amdgcn_readfirstlane(left);
-    x = __builtin_amdgcn_readfirstlane(x);
-    blocks = __builtin_amdgcn_readfirstlane(blocks);
-    const int g = left / blocks, first = (left % blocks) * kKwKeys;
 
-    // ---- this wave's keys: key j = jb + 32 kt + col, dims 16 s + 8 h + [0, 8) in kf[kt][s]; keys that do not count are zeros
-    const int jb = first + kw * KEYS;
+    const int jb = first + kw * KEYS;  // this wave's first key
     u32x4 kf[KT][8];
     uint64_t counts = 0;  // bit: key jb + bit takes weight
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const int j = jb + 32 * kt + col;
-      bool ok = j < s.nk;
-      const uint16_t* kr;
-      if (!paged) {
-        kr = p.k_src + ((int64_t)s.k0 + (ok ? j : 0)) * p.k_row_stride + g * kKwD;
-      } else {
-        ok = ok && j < p.max_blocks * p.block_size;
-        const int bid = p.block_tables[(int64_t)b * p.bt_stride + (ok ? j / p.block_size : 0)];
-        ok = ok && bid >= 0 && bid < p.num_blocks;
-        kr = p.k_cache + (((int64_t)(ok ? bid : 0) * p.block_size + j % p.block_size) * HK + g) * kKwD;
-      }
-      counts |= (uint64_t)(uint32_t)__builtin_amdgcn_ballot_w64(ok) << (32 * kt);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const u32x4 v = ld_g16(kr + 16 * i + 8 * h);
-        kf[kt][i] = ok ? v : zero4();
-      }
-    }
-
     // ---- the part's rows that see a key of the item: token tq sees key j when j <= old + tq. Query wave qw takes tiles qw,
     // qw + QW, ... from row `begin` on; a tile is two halves of 32 rows.
     const int end = min(s.n, (x + 1) * k.part_rows);
@@ -286,6 +285,28 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
     f32x16 sa[KT], sb[KT];
     float la, lx = 0.f;
     load(0, C0{});
+
+    // ---- this wave's keys: key j = jb + 32 kt + col, dims 16 s + 8 h + [0, 8) in kf[kt][s]; keys that do not count are zeros
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int j = jb + 32 * kt + col;
+      bool ok = j < s.nk;
+      const uint16_t* kr;
+      if (!paged) {
+        kr = p.k_src + ((int64_t)s.k0 + (ok ? j : 0)) * p.k_row_stride + g * kKwD;
+      } else {
+        ok = ok && j < p.max_blocks * p.block_size;
+        const int bid = p.block_tables[(int64_t)b * p.bt_stride + (ok ? j / p.block_size : 0)];
+        ok = ok && bid >= 0 && bid < p.num_blocks;
+        kr = p.k_cache + (((int64_t)(ok ? bid : 0) * p.block_size + j % p.block_size) * HK + g) * kKwD;
+      }
+      counts |= (uint64_t)(uint32_t)__builtin_amdgcn_ballot_w64(ok) << (32 * kt);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32x4 v = ld_g16(kr + 16 * i + 8 * h);
+        kf[kt][i] = ok ? v : zero4();
+      }
+    }
     arrive();
     load(1, C1{});
     {
@@ -432,9 +453,10 @@ hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
       k.row0 = k0.row0 + b0;
     const int64_t blocks = ((int64_t)k.max_k + kKwKeys - 1) / kKwKeys;
     const int64_t items = blocks * k.max_parts * k.a.batch * k.a.num_kv_heads;
-    const int64_t most = 512;  // two workgroups a CU
-    const unsigned grid = (unsigned)(((items < most ? items : most) + kXcds - 1) / kXcds * kXcds);
-    key_weights_kernel<<<dim3(grid), dim3(256), 0, stream>>>(k);
+    if (items <= 512)
+      key_weights_kernel<true><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
+    else  // two workgroups a CU
+      key_weights_kernel<false><<<dim3(512), dim3(256), 0, stream>>>(k);
     if (k.max_parts > 1)
       key_weights_sum_kernel<<<dim3((unsigned)((k.max_k + 255) / 256), (unsigned)k.a.batch, (unsigned)k.a.num_kv_heads),
                                dim3(256), 0, stream>>>(k);
