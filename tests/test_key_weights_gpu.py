@@ -485,3 +485,43 @@ def test_evict_with_tables_wider_than_a_workgroup_holds():
         _evict_case(kv.clone(), weights.clone(), tables, [n, 40], budget, 3, 100)
         new = [rest[:-(-budget // bs)] + [-1] * (cols - -(-budget // bs)), [-1] * cols]
         _evict_case(kv, weights, tables, [n, 40], budget, 3, 100, None, new)
+
+
+@pytest.mark.parametrize("bs", [64, None])
+def test_chunk_lengths_past_what_the_call_says(bs):
+    """Queries past max_seqlen_q and keys past max_seqlen_k are left out: the weights are those of the others, the places of
+    keys that nothing saw as they were, and the memory around the scratch is not written."""
+    gen = torch.Generator().manual_seed(51)
+    h, hk, seqs, max_q, max_k = 16, 2, [(900, 900), (40, 40), (300, 500 if bs else 300)], 128, 400
+    cu_q, cu_k = [0], [0]
+    for n, m in seqs:
+        cu_q.append(cu_q[-1] + n)
+        cu_k.append(cu_k[-1] + m)
+    q = randn(gen, cu_q[-1], h, D)
+    w = _received(gen, 3, hk, 1024)
+    wd = w.to(DEV)
+    kw = dict(cu_seqlens_q=_i32(cu_q), cu_seqlens_k=_i32(cu_k), max_seqlen_q=max_q, max_seqlen_k=max_k, softmax_scale=SCALE)
+    if bs:
+        lens = [m for _, m in seqs]
+        kc, vc, tables = paged_pool(gen, lens, 40, bs, hk)
+        keys = [tuple(ref.keys_of(c, tables[b], m)[0] for c in (kc, vc)) for b, m in enumerate(lens)]
+        kd = vd = None
+        kw.update(block_table=tables.to(DEV), k_cache=kc.to(DEV), v_cache=vc.to(DEV))
+    else:
+        k, v = randn(gen, cu_k[-1], hk, D), randn(gen, cu_k[-1], hk, D)
+        keys = [(k[cu_k[b]:cu_k[b + 1]], v[cu_k[b]:cu_k[b + 1]]) for b in range(3)]
+        kd, vd = k.to(DEV), v.to(DEV)
+    o = varlen_attention_weights(q.to(DEV), kd, vd, wd, **kw).cpu().double()
+    want = Want(w)
+    for b, (n, m) in enumerate(seqs):
+        took, seen = min(n, max_q), m - n + min(n, max_q)
+        before = want.w[b].clone()
+        want.sequence(q[cu_q[b]:cu_q[b] + took], keys[b][0][:seen], keys[b][1][:seen], None, b, took)
+        want.w[b][:, min(seen, max_k):] = before[:, min(seen, max_k):]
+        assert ((o[cu_q[b]:cu_q[b] + took] - want.o[-1]).abs() <= want.otol[-1]).all()
+    off = (wd.cpu().double() - want.w).abs() - want.tol
+    assert (off <= 0).all()
+
+
+def test_chunk_of_a_group_of_128():
+    _varlen_case(52, [(70, 70), (3, 200), (1, 1)], 128, 1, 64)

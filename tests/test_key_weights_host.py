@@ -414,6 +414,7 @@ PAGED = dict(key=None, value=None, ks=0, vs=0, kc=P, vc=P, blocks=4, bs=64, bt=P
     (dict(batch=70000), "65535"), (dict(key=None), "null key"), (dict(h=24, qs=3200, outs=3200), "divide 128"), (dict(d=64), "head_dim"),
     (dict(PAGED, bs=32), "multiple of 64"), (dict(PAGED, bs=0), "multiple of 64"), (dict(PAGED, mb=1 << 25, bts=1 << 25), "too wide"),
     (dict(PAGED, kc=None), "without caches"), (dict(PAGED, bts=1), "bad block table"),
+    (dict(mq=1 << 28), "too large"), (dict(mk=(1 << 30) + 1), "too large"), (dict(mk=1 << 30, batch=100), "too large"),
     (dict(PAGED, ws=P, ws_bytes=10), "workspace"), (dict(PAGED, ws=P, ws_bytes=1 << 30, plan=5), "plan mode"),
     (dict(PAGED, ws=P, ws_bytes=1 << 30), "scores"),
     (dict(PAGED, ws=P, ws_bytes=1 << 30, scores=P, scores_bytes=2 * 8 * 16 * 16 * 4 - 1), "needed"),

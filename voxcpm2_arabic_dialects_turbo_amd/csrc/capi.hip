@@ -1165,6 +1165,11 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   k.a.out = (uint16_t*)out;
   k.a.out_row_stride = out_row_stride;
   k.a.row_limit = num_tokens;
+  // (rows, keys and work items are counted in 32 bits)
+  const int64_t slice = batch < vox::kMaxSeqPerLaunch ? batch : vox::kMaxSeqPerLaunch;
+  if ((int64_t)max_seqlen_q * k.a.group > (1 << 30) || max_seqlen_k > (1 << 30) ||
+      ((int64_t)max_seqlen_k / 128 + 1) * 8 * num_kv_heads * slice > INT32_MAX)
+    return fail(VOX_EINVAL, "%s: max_seqlen_q %d or max_seqlen_k %d too large", fn, max_seqlen_q, max_seqlen_k);
   const WeightsScratch ws = weights_scratch(num_tokens, batch, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads);
   if (!scratch || !aligned16(scratch) || scratch_bytes < ws.total)
     return fail(VOX_EINVAL, "%s: scratch of %zu bytes (16-byte aligned), %zu needed", fn, scratch_bytes, ws.total);
@@ -1173,6 +1178,7 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   k.rows = weight_rows;
   k.row_count = num_weight_rows;
   k.width = weight_width;
+  k.max_q = max_seqlen_q;
   k.max_k = max_seqlen_k;
   k.part_rows = ws.part_rows;
   k.max_parts = ws.parts;

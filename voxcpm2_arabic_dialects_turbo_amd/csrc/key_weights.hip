@@ -96,7 +96,7 @@ struct KwSeq {
   // key blocks that see a row of part x: those that start at or before the part's last token
   __device__ __forceinline__ int blocks(const KeyWeightsArgs& k, int x, int gsh) const {
     const int last = (min(n, (x + 1) * k.part_rows) - 1) >> gsh;
-    const int64_t end = min((int64_t)min(nk, old + last + 1), min(k.width, (int64_t)k.max_k));
+    const int64_t end = min((int64_t)min(nk, old + last + 1), k.width);
     return end <= 0 ? 0 : (int)((end + kKwKeys - 1) / kKwKeys);
   }
 };
@@ -110,7 +110,9 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
   s.old = s.nk - s.nq;
   s.row = k.rows ? (int64_t)k.rows[b] : b + k.row0;
   const bool mine = s.nq > 0 && s.nk > 0 && s.row >= 0 && s.row < k.row_count && !(p.skip_single && s.nq == 1);
-  if (p.row_limit > 0) s.nq = (int)max((int64_t)0, min((int64_t)s.nq, p.row_limit - s.q0));  // (rows that q holds)
+  // (the rows that the attention took, and the keys that those may see)
+  s.nq = (int)max((int64_t)0, min((int64_t)min(s.nq, k.max_q), p.row_limit - s.q0));
+  s.nk = min(min(s.nk, s.old + s.nq), k.max_k);
   s.n = mine ? s.nq << gsh : 0;
   s.parts = (s.n + k.part_rows - 1) / k.part_rows;
   return s;
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
       float got = sums[kw][lane] + sums[kw + KW][lane];
       got = (counts >> lane) & 1u ? got : 0.f;
       if (s.parts > 1) {
-        if (j < k.max_k) k.partials[(((int64_t)b * HK + g) * k.max_parts + x) * k.max_k + j] = got;
+        k.partials[(((int64_t)b * HK + g) * k.max_parts + x) * k.max_k + j] = got;
       } else {
         float* out = k.weights + (s.row * HK + g) * k.width + j;
         *out = j >= s.old ? got : *out + got;
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   const int b = blockIdx.y, g = blockIdx.z, j = (int)(blockIdx.x * 256 + threadIdx.x);
   const int gsh = __builtin_ctz(k.a.group);
   const KwSeq s = kw_seq(k, b, gsh);
-  if (s.parts <= 1 || j >= s.nk || j >= k.width || j >= k.max_k) return;
+  if (s.parts <= 1 || j >= s.nk || j >= k.width) return;
   const float* part = k.partials + ((int64_t)b * k.a.num_kv_heads + g) * k.max_parts * k.max_k + j;
   float got = 0.f;
   for (int x = 0; x < s.parts; ++x)
@@ -438,7 +440,7 @@ int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int m
 hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
   KeyWeightsArgs k = k0;
   if (k.max_k <= 0 || k.a.batch <= 0) return hipSuccess;
-  if (!k.a.lse || !k.weights || !k.a.cu_q || !k.a.cu_k || k.part_rows <= 0 || k.part_rows % 128 ||
+  if (!k.a.lse || !k.weights || !k.a.cu_q || !k.a.cu_k || k.a.row_limit <= 0 || k.max_q <= 0 || k.part_rows <= 0 || k.part_rows % 128 ||
       (k.max_parts > 1 && !k.partials))
     return hipErrorInvalidValue;
   const int batch = k0.a.batch;

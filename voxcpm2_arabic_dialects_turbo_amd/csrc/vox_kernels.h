@@ -139,7 +139,8 @@ struct KeyWeightsArgs {
   const int32_t* rows;        // int32 [batch], or null: row b + row0 (outside [0, row_count): none)
   int64_t row0;
   int64_t row_count;
-  int64_t width;              // keys at or past it, or at or past max_k: left out
+  int64_t width;              // keys at or past it, or at or past max_k: left out, as queries at or past max_q or a.row_limit
+  int max_q;
   int max_k;
   int part_rows;              // a sequence's query rows (tokens x group) in parts of so many; a multiple of 128
   int max_parts;              // of a sequence
