@@ -1168,7 +1168,7 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   // (rows, keys and work items are counted in 32 bits)
   const int64_t slice = batch < vox::kMaxSeqPerLaunch ? batch : vox::kMaxSeqPerLaunch;
   if ((int64_t)max_seqlen_q * k.a.group > (1 << 30) || max_seqlen_k > (1 << 30) ||
-      ((int64_t)max_seqlen_k / 128 + 1) * 8 * num_kv_heads * slice > INT32_MAX)
+      ((int64_t)max_seqlen_k / 128 + 1) * 16 * num_kv_heads * slice > INT32_MAX)
     return fail(VOX_EINVAL, "%s: max_seqlen_q %d or max_seqlen_k %d too large", fn, max_seqlen_q, max_seqlen_k);
   const WeightsScratch ws = weights_scratch(num_tokens, batch, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads);
   if (!scratch || !aligned16(scratch) || scratch_bytes < ws.total)

@@ -120,7 +120,7 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
 
 // Persistent: the items (128 keys, a part of the query rows, kv head, sequence), the key blocks of a part side by side, are
 // dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2. DIRECT, where the grid of
-// all there may be is at most two workgroups a CU: a workgroup for each, without the items' layout.
+// all there may be is small: a workgroup for each, without the items' layout.
 template <bool DIRECT>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   constexpr int KW = 2, QW = 2, KT = 2;
@@ -381,9 +381,16 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   const KwSeq s = kw_seq(k, b, gsh);
   if (s.parts <= 1 || j >= s.nk || j >= k.width) return;
   const float* part = k.partials + ((int64_t)b * k.a.num_kv_heads + g) * k.max_parts * k.max_k + j;
+  // the first part with a row that sees the key's block
+  const int from = (int)(((int64_t)max(0, j / kKwKeys * kKwKeys - s.old) << gsh) / k.part_rows);
   float got = 0.f;
-  for (int x = 0; x < s.parts; ++x)
-    if (j < (int64_t)s.blocks(k, x, gsh) * kKwKeys) got += part[(int64_t)x * k.max_k];
+  for (int x = from; x < s.parts; x += 8) {  // (eight loads in flight)
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = part[(int64_t)min(x + i, s.parts - 1) * k.max_k];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) got += x + i < s.parts ? v[i] : 0.f;
+  }
   float* out = k.weights + (s.row * k.a.num_kv_heads + g) * k.width + j;
   *out = j >= s.old ? got : *out + got;
 }
@@ -428,12 +435,17 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
 }
 
 int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {
-  // about three items for each workgroup slot (two a CU), but no part of less than 512 rows nor more than eight of them
+  // About three items for each workgroup slot (two a CU), of 256 to 4096 rows, and 16 parts at most; one part of up to 640
+  // rows, where a second launch costs what it saves. us, in parts of 512 rows and eight at most, against this: prompts of 64
+  // tokens 11.0 (in parts of 256 9.0 + 2.6 and a launch's gap), 100 11.5 + 3.9 and 9.5 + 3.3, 237 12.2 + 3.8 and 9.7 + 3.9,
+  // 1000 18.6 + 4.2 and 12.9 + 4.0.
   const int64_t blocks = ((int64_t)max_seqlen_k + kKwKeys - 1) / kKwKeys;
+  const int64_t longest = (int64_t)max_seqlen_q * group, least = (longest + 15) / 16;
   const int64_t want = num_tokens * group * num_kv_heads * blocks / 1536;
-  const int64_t least = ((int64_t)max_seqlen_q * group + 7) / 8;
-  const int64_t rows = want < 512 ? 512 : want > 4096 ? 4096 : want;
-  const int64_t r = ((rows > least ? rows : least) + 127) / 128 * 128;
+  int64_t r = want < 256 ? 256 : want > 4096 ? 4096 : want;
+  r = r > least ? r : least;
+  if (longest <= 640 && r < longest) r = longest;
+  r = (r + 127) / 128 * 128;
   return r > INT32_MAX / 2 ? INT32_MAX / 2 / 128 * 128 : (int)r;
 }
 
@@ -455,7 +467,7 @@ hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
       k.row0 = k0.row0 + b0;
     const int64_t blocks = ((int64_t)k.max_k + kKwKeys - 1) / kKwKeys;
     const int64_t items = blocks * k.max_parts * k.a.batch * k.a.num_kv_heads;
-    if (items <= 512)
+    if (items <= 1536)  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> KW_PROMPTS us)
       key_weights_kernel<true><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
     else  // two workgroups a CU
       key_weights_kernel<false><<<dim3(512), dim3(256), 0, stream>>>(k);
