@@ -271,6 +271,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
           const int kt = y >> 4, e = y & 15;
           const float pr = fast_exp2(fmaf(sc[kt][e], c, -lse));
           acc[kt][e] += !MASK || 32 * kt + 8 * (e >> 2) + (e & 3) <= last ? pr : 0.f;
+          asm volatile("" : "+v"(acc[kt][e]));  // (here: sunk behind the two forms of the step, the adds ran beside no MFMA)
         }
         __builtin_amdgcn_sched_barrier(0);
       }
