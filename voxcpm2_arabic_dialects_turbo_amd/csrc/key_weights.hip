@@ -468,7 +468,7 @@ hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
       k.row0 = k0.row0 + b0;
     const int64_t blocks = ((int64_t)k.max_k + kKwKeys - 1) / kKwKeys;
     const int64_t items = blocks * k.max_parts * k.a.batch * k.a.num_kv_heads;
-    if (items <= 1536)  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> KW_PROMPTS us)
+    if (items <= 1536)  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> 19.4 us)
       key_weights_kernel<true><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
     else  // two workgroups a CU
       key_weights_kernel<false><<<dim3(512), dim3(256), 0, stream>>>(k);
