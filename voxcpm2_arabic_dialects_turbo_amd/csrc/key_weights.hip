@@ -1,14 +1,21 @@
 // What every key of a causal varlen call receives: for sequence b, kv head g and key j
 //   got[g, j] = sum over b's queries i that see j and the query heads h of g of exp2(c q_ih . k_j - lse_ih),
 // c the log2-scaled softmax scale, lse_ih = log2 sum_j exp2(c q_ih . k_j): the column sums of the attention's probabilities.
-// Two launches. The attention (prefill_tile32.h) leaves every row's lse behind; then key_weights_kernel makes the scores
-// again, a key block at a time over all queries that see it, which needs neither atomics nor partial sums in memory: every
-// key's sum is one workgroup's, in a fixed order, fp32. A new key's weight is set, a cached one's grows.
+// The attention (prefill_tile32.h) leaves every row's lse behind, and key_weights_kernel makes the scores again: sums down
+// the columns inside the attention would be a cross-workgroup sum for every (row tile, key), this one's are registers. It has
+// neither atomics nor an order that changes: an item is (128 keys, a part of the query rows, kv head, sequence), one
+// workgroup's; key_weights_sum_kernel adds the parts where a sequence has several. fp32 throughout but for the scores' bf16
+// inputs. A new key's weight is set, a cached one's grows.
 //
-// A workgroup is (KW x 32 keys, sequence, kv head), as KW x QW waves: wave (kw, qw) holds its 32 keys' K rows in registers
-// (the A operand of the score MFMA) and takes the 32-row query tiles qw, qw + QW, ... from the first that sees its keys.
-// Rows are (token, query head of g), so S^T[32 keys x 32 rows] has a row's scores in one lane column and its lse in one
-// register; 16 fma, exp2 and adds a tile behind 8 MFMAs. The lanes' sums meet in LDS at the end.
+// A workgroup is KW x QW = 2 x 2 waves: wave (kw, qw) holds its 64 keys' K rows in registers (the A operand of the score MFMA)
+// and takes the 64-row query tiles qw, qw + 2, ... from the first that sees its keys, out of LDS (two buffers, filled by
+// loads straight into LDS while the other is read). Rows are (token, query head of g), so S^T[32 keys x 32 rows] has a row's
+// scores in one lane column and its lse in one register: fma, exp2, add, beside the next half tile's MFMAs in a fixed order.
+// The lanes' sums meet in LDS at the end.
+//
+// Bound by those fma, exp2 (quarter rate) and adds, about as many cycles as the MFMAs: 6 chunks of 1000-2000 tokens over
+// 1500-2500 (16 heads of 2, 107 GFLOP of scores) 139-160 us, beside 235-250 for the attention; small calls by latency
+// (44 chunks of 33-59 over 50: 9.8 us).
 #include <type_traits>
 
 #include "prefill_tile32.h"
@@ -86,7 +93,7 @@ __global__ __launch_bounds__(64 * RG * KS, 2) void prefill32_lse_kernel(PrefillA
   }
 }
 
-constexpr int kKwKeys = 128;  // keys of an item
+constexpr int kKwKeys = 128;  // keys of an item (DIRECT grids may halve it)
 constexpr int kKwRows = 64;   // query rows of a tile
 
 // A sequence's items: query rows [0, n) in parts of k.part_rows, the cached keys `old` before its own, key blocks.
@@ -97,7 +104,7 @@ struct KwSeq {
   __device__ __forceinline__ int blocks(const KeyWeightsArgs& k, int x, int gsh) const {
     const int last = (min(n, (x + 1) * k.part_rows) - 1) >> gsh;
     const int64_t end = min((int64_t)min(nk, old + last + 1), k.width);
-    return end <= 0 ? 0 : (int)((end + kKwKeys - 1) / kKwKeys);
+    return end <= 0 ? 0 : (int)((end + (1 << k.item_shift) - 1) >> k.item_shift);
   }
 };
 __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh) {
@@ -121,9 +128,9 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
 // Persistent: the items (128 keys, a part of the query rows, kv head, sequence), the key blocks of a part side by side, are
 // dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2. DIRECT, where the grid of
 // all there may be is small: a workgroup for each, without the items' layout.
-template <bool DIRECT>
+template <bool DIRECT, int KT>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
-  constexpr int KW = 2, QW = 2, KT = 2;
+  constexpr int KW = 2, QW = 2;
   constexpr int KEYS = 32 * KT;               // keys of a wave
   constexpr int TILE = kKwRows * 256;
   constexpr int BUF = QW * TILE + 4 * 256;    // a tile for each query wave, and each wave's copy of its rows' lse
@@ -172,13 +179,13 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
     int b, x, g, first;
     KwSeq s;
     if constexpr (DIRECT) {
-      const int blocks = (k.max_k + kKwKeys - 1) / kKwKeys;
-      first = item % blocks * kKwKeys;
+      const int blocks = (k.max_k + KW * KEYS - 1) / (KW * KEYS);
+      first = item % blocks * (KW * KEYS);
       x = item / blocks % k.max_parts;
       g = item / blocks / k.max_parts % HK;
       b = item / blocks / k.max_parts / HK;
       s = kw_seq(k, b, gsh);
-      if (x >= s.parts || first >= s.blocks(k, x, gsh) * kKwKeys) return;
+      if (x >= s.parts || first >= s.blocks(k, x, gsh) * (KW * KEYS)) return;
     } else {
       b = sequence_of(item, p.batch, starts);
       s = kw_seq(k, b, gsh);
@@ -192,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
       x = __builtin_amdgcn_readfirstlane(x);
       blocks = __builtin_amdgcn_readfirstlane(blocks);
       g = left / blocks;
-      first = left % blocks * kKwKeys;
+      first = left % blocks * (KW * KEYS);
     }
 
     const int jb = first + kw * KEYS;  // this wave's first key
@@ -361,7 +368,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
     wait_vmem_all();  // (tiles behind the last one)
     __syncthreads();
     const int j = jb + lane;
-    if (qw == 0 && j < s.nk && j < k.width) {
+    if (qw == 0 && lane < KEYS && j < s.nk && j < k.width) {
       float got = sums[kw][lane] + sums[kw + KW][lane];
       got = (counts >> lane) & 1u ? got : 0.f;
       if (s.parts > 1) {
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   if (s.parts <= 1 || j >= s.nk || j >= k.width) return;
   const float* part = k.partials + ((int64_t)b * k.a.num_kv_heads + g) * k.max_parts * k.max_k + j;
   // the first part with a row that sees the key's block
-  const int from = (int)(((int64_t)max(0, j / kKwKeys * kKwKeys - s.old) << gsh) / k.part_rows);
+  const int from = (int)(((int64_t)max(0, (j >> k.item_shift << k.item_shift) - s.old) << gsh) / k.part_rows);
   float got = 0.f;
   for (int x = from; x < s.parts; x += 8) {  // (eight loads in flight)
     float v[8];
@@ -467,11 +474,18 @@ hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
     else
       k.row0 = k0.row0 + b0;
     const int64_t blocks = ((int64_t)k.max_k + kKwKeys - 1) / kKwKeys;
-    const int64_t items = blocks * k.max_parts * k.a.batch * k.a.num_kv_heads;
-    if (items <= 1536)  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> 19.4 us)
-      key_weights_kernel<true><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
+    int64_t items = blocks * k.max_parts * k.a.batch * k.a.num_kv_heads;
+    // Grids of at most a workgroup a CU, which the exponentials of their own rows bound: half the keys each (us, whole and
+    // half key blocks: a prompt of 30 tokens 8.6 and 6.8, 64 11.0 and 8.6, 237 9.7 and 7.4, 44 of 33-59 over 50 13.2 and
+    // 9.8; past it 5 of 237-900 19.2 and 24.6, 4 of 300 over 700 21.4 and 22.8).
+    k.item_shift = items <= 256 ? 6 : 7;
+    if (items <= 256) {
+      items = ((int64_t)k.max_k + 63) / 64 * k.max_parts * k.a.batch * k.a.num_kv_heads;
+      key_weights_kernel<true, 1><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
+    } else if (items <= 1536)  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> 19.2 us)
+      key_weights_kernel<true, 2><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
     else  // two workgroups a CU
-      key_weights_kernel<false><<<dim3(512), dim3(256), 0, stream>>>(k);
+      key_weights_kernel<false, 2><<<dim3(512), dim3(256), 0, stream>>>(k);
     if (k.max_parts > 1)
       key_weights_sum_kernel<<<dim3((unsigned)((k.max_k + 255) / 256), (unsigned)k.a.batch, (unsigned)k.a.num_kv_heads),
                                dim3(256), 0, stream>>>(k);

@@ -145,6 +145,7 @@ struct KeyWeightsArgs {
   int part_rows;              // a sequence's query rows (tokens x group) in parts of so many; a multiple of 128
   int max_parts;              // of a sequence
   float* partials;            // max_parts > 1: fp32 [a launch's sequences, HK, max_parts, max_k]
+  int item_shift;             // a key block has 1 << item_shift keys
 };
 
 // Tokens dropped from a paged cache (kv_evict.hip): of every sequence longer than `budget` its first `sinks`, last `recent`
