@@ -525,3 +525,16 @@ def test_chunk_lengths_past_what_the_call_says(bs):
 
 def test_chunk_of_a_group_of_128():
     _varlen_case(52, [(70, 70), (3, 200), (1, 1)], 128, 1, 64)
+
+
+def test_bounds_past_32_bits():
+    """Budgets and numbers of queries that no sequence reaches, however large: nothing is dropped, nothing is left out."""
+    gen = torch.Generator().manual_seed(53)
+    for budget in (500, 2 ** 31, 2 ** 33 + 5):
+        kv, w = _kv(gen, 1, 8, 64, 2, "bf16"), torch.rand(1, 2, 2, 256, generator=gen)
+        _evict_case(kv, w, [[1, 2, 3, 0], [5, 6, -1, -1]], [256, 100], budget, 3, 90)
+    _, k, v, kw, _ = _varlen_case(54, [(70, 70), (9, 9)], 16, 2)
+    q, w = randn(gen, 79, 16, D).to(DEV), [torch.zeros(2, 2, 256, device=DEV) for _ in range(2)]
+    for x, n in zip(w, (70, 2 ** 33 + 1)):
+        o = varlen_attention_weights(q, k, v, x, **{**kw, "max_seqlen_q": n})
+    assert torch.equal(*w) and w[0].any() and o.isfinite().all()

@@ -215,12 +215,13 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {hk}")
     n_rows, width, rows = _weights(fn, key_weights, weight_rows, max(B, 0), hk, reach, q.get_device())
     q, q_stride, out = _query(fn, q, out, dev, False)
+    max_seqlen_q = min(int(max_seqlen_q), T)
     if T == 0 or B <= 0 or max_seqlen_q <= 0:
         return out
     cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
     lib = _lib.load()
     with _on(dev):
-        need = lib.vox_prefill_weights_bytes(T, B, int(max_seqlen_q), reach, H, hk)
+        need = lib.vox_prefill_weights_bytes(T, B, max_seqlen_q, reach, H, hk)
         scores_at = (need + 255) // 256 * 256
         ws, scores_bytes, mode, recorded = None, 0, _lib.PLAN_NONE, None
         if block_table is not None and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) \
@@ -230,7 +231,7 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         scratch = torch.empty((scores_at + scores_bytes,), dtype=torch.uint8, device=dev)
         at = scratch.data_ptr()
         _lib.check(lib.vox_prefill_attn_weights(
-            q.data_ptr(), q_stride, *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, int(max_seqlen_q), reach, T, H, hk, D,
+            q.data_ptr(), q_stride, *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, max_seqlen_q, reach, T, H, hk, D,
             scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), n_rows, width, at, need,
             at + scores_at if scores_bytes else None, scores_bytes, mode, None if ws is None else ws.data_ptr(),
             0 if ws is None else ws.numel(), out.data_ptr(), _row_stride(out), _lib.stream_handle(dev)), fn)
