@@ -941,12 +941,17 @@ __device__ __forceinline__ void merge_row(const DecodeArgs& p, int b, int part, 
 // N = 4 weight_wgs (decode_merge_kernel; `lse` is the wave's own LDS). A key's weight at kv head g grows by the sum over
 // g's query heads h of exp2(s c - lse_h), the probabilities of the attention: s are the scores that the split kernel left,
 // lse_h comes from the partials' m and l, the same sum that the output is divided by. The newest token's weight is set: its
-// place may hold anything. Lane = (token, one of four steps), so a head's scores and a kv head's weights are read and
-// written side by side.
+// place may hold anything. A lane reads four tokens of one head of a step, 16 bytes; two steps' sums over the heads then come
+// to a lane each, (token, step, kv head), by exchanges that halve what a lane holds.
 __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int N, float* lse) {
   const int lane = threadIdx.x & 63;
   const int r16 = lane & 15, sub = lane >> 4;
   const int H = p.num_heads, HK = H / p.group;
+  // this lane's head (two kv heads: the wave's halves) and tokens; the token, step of two and kv head of its weight
+  const int slot = HK == 2 ? (lane >> 2) & 7 : lane >> 2, head = HK == 2 ? (lane >> 5) * p.group + slot : slot;
+  const bool heads = slot < p.group, takes = HK == 2 || lane < 32;
+  const int in_step = min(head, H - 1) * kTile + 4 * (lane & 3);
+  const int wtok = 4 * (lane & 3) + 2 * ((lane >> 3) & 1) + ((lane >> 2) & 1), wstep = sub & 1;
   // lane k: sequence base + k's first and end steps, context and row
   int base = 0, st = 0, en = 0, len = 0, row = 0;
   auto window = [&](int at) {
@@ -982,21 +987,23 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
     const int n = __builtin_amdgcn_readlane(len, k);
     const int64_t wr = __builtin_amdgcn_readlane(row, k), reach = min((int64_t)n, p.weight_width);
     const bool mine = wr >= 0 && wr < p.weight_row_count;
-    float* const wb = p.weights + wr * HK * p.weight_width;
-    // steps u to u + 3: the scores of every head and the weights
-    float x[kMaxHeads], w0 = 0.f, w1 = 0.f;
-    auto live = [&](int u) { return mine && u + sub < te && (int64_t)(u + sub - sb) * kTile + r16 < reach; };
-    auto fetch = [&](int u) {
-      const int64_t tok = (int64_t)(u + sub - sb) * kTile + r16;
-      const float* s = p.scores + (int64_t)(u + sub) * H * kTile + r16;
-      if (live(u)) {
+    float* const wb = p.weights + ((mine ? wr : 0) * HK + (HK == 2 ? sub >> 1 : 0)) * p.weight_width;
+    // steps u to u + 3: the scores and the weights. (Every lane loads something that is there: loads behind branches would
+    // have every wait for one round wait for all.)
+    struct Round {
+      f32x4 x[4];
+      float w[2];
+    } ra, rb;
+    auto token = [&](int u) { return (int64_t)(u + wstep - sb) * kTile + wtok; };
+    auto fetch = [&](int u, Round& r) {
 #pragma unroll
-        for (int hh = 0; hh < kMaxHeads; ++hh) x[hh] = hh < H ? s[hh * kTile] : -INFINITY;
-        w0 = wb[tok];
-        w1 = HK == 2 ? wb[p.weight_width + tok] : 0.f;
-      }
+      for (int i = 0; i < 4; ++i)
+        r.x[i] = *reinterpret_cast<const f32x4*>(p.scores + (int64_t)min(u + i, te - 1) * H * kTile + in_step);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) r.w[i] = wb[min(token(min(u + 2 * i, te - 1)), p.weight_width - 1)];
     };
-    fetch(t);
+    fetch(t, ra);
+    fetch(t + 4, rb);
     // the sequence's pieces are those of merge_row; four at a time, head r16
     const int g_first = (int)muldiv(sb + 1, G, S - 1, S) - 1;
     const int g_last = (int)min(G - 1, muldiv(eb, G, S - 1, S) - 1);
@@ -1024,21 +1031,41 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
     // (a head without any key: exp2(s c - inf) = 0)
     lse[r16] = Lt == 0.f ? INFINITY : Mt + __builtin_amdgcn_logf(Lt);
     wave_lds_sync();
-    for (int u = t; u < te; u += 4) {
-      float a0 = 0.f, a1 = 0.f;
+    const float my_lse = lse[min(head, H - 1)];
+    auto add = [&](int u, const Round& r) {
 #pragma unroll
-      for (int hh = 0; hh < kMaxHeads; ++hh) {
-        const float e = hh < H ? fast_exp2(fmaf(x[hh], p.scale_log2, -lse[hh])) : 0.f;
-        a0 += hh < p.group ? e : 0.f;
-        a1 += hh < p.group ? 0.f : e;
+      for (int i = 0; i < 2; ++i) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = heads ? fast_exp2(fmaf(r.x[2 * i][j], p.scale_log2, -my_lse)) : 0.f;
+          const float z = heads ? fast_exp2(fmaf(r.x[2 * i + 1][j], p.scale_log2, -my_lse)) : 0.f;
+          // the even 16-lane rows keep the first step's, the odd ones the second's
+          const auto s2 = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(z), false, false);
+          v[j] = __uint_as_float(s2[0]) + __uint_as_float(s2[1]);
+        }
+        // lanes of bit 3 tokens 2 and 3 of the four, the others 0 and 1 (row_ror:8)
+        float y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float keep = lane & 8 ? v[2 + j] : v[j], give = lane & 8 ? v[j] : v[2 + j];
+          y[j] = keep + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0x128, 0xF, 0xF, false));
+        }
+        // bit 2: the second of these, or the first (lane ^ 4: row_half_mirror, then quad_perm 3 2 1 0)
+        const float keep = lane & 4 ? y[1] : y[0], give = lane & 4 ? y[0] : y[1];
+        int x4 = __builtin_amdgcn_update_dpp(0, __float_as_int(give), 0x141, 0xF, 0xF, false);
+        x4 = __builtin_amdgcn_update_dpp(0, x4, 0x1B, 0xF, 0xF, false);
+        float got = keep + __int_as_float(x4);
+        if (HK == 1) got = xhalf_sum(got);
+        const int64_t tok = token(u + 2 * i);
+        if (mine && takes && u + 2 * i + wstep < te && tok < reach) wb[tok] = tok == n - 1 ? got : r.w[i] + got;
       }
-      if (live(u)) {
-        const int64_t tok = (int64_t)(u + sub - sb) * kTile + r16;
-        const bool fresh = tok == n - 1;
-        wb[tok] = fresh ? a0 : w0 + a0;
-        if (HK == 2) wb[p.weight_width + tok] = fresh ? a1 : w1 + a1;
-      }
-      if (u + 4 < te) fetch(u + 4);
+    };
+    for (int u = t; u < te; u += 8) {
+      add(u, ra);
+      fetch(u + 8, ra);
+      add(u + 4, rb);
+      fetch(u + 12, rb);
     }
     wave_lds_sync();  // (lse is read before the next sequence's)
     t = te;
