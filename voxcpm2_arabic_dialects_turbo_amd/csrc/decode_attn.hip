@@ -198,8 +198,9 @@ hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stre
 hipError_t launch_decode_weights(const DecodeArgs& a0, int num_kv_heads, hipStream_t stream) {
   if (!a0.scores || !a0.weights) return hipErrorInvalidValue;
   DecodeArgs a = a0;
-  // a wave for every four steps that the tables allow, a round of add_key_weights, up to two workgroups per CU (one: 24 of
-  // 20000-32768 tokens 17.4 -> 24 us; four 16.4, 150 of 256-2048 12.0 -> 12.6)
+  // a wave for every four steps that the tables allow, a round of add_key_weights, up to two workgroups per CU (the kernel's us
+  // with up to one, two, four: 24 of 20000-32768 tokens 14.5, 13.4, 14.2; 150 of 256-2048 9.0, 8.9, 11.1; 120 such rows
+  // beside 6 prompts 7.4, 8.4, 10.4)
   const int64_t steps = (int64_t)a.batch * (((int64_t)a.max_blocks * a.block_size + kTile - 1) / kTile);
   a.weight_wgs = (int)min((int64_t)512, (steps + 15) / 16);
   const hipError_t e = launch_split<true>(a, num_kv_heads, stream);

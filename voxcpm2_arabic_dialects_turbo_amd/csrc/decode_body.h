@@ -1063,9 +1063,9 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
     };
     for (int u = t; u < te; u += 8) {
       add(u, ra);
-      fetch(u + 8, ra);
+      if (u + 8 < te) fetch(u + 8, ra);
       add(u + 4, rb);
-      fetch(u + 12, rb);
+      if (u + 12 < te) fetch(u + 12, rb);
     }
     wave_lds_sync();  // (lse is read before the next sequence's)
     t = te;
