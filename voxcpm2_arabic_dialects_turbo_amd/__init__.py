@@ -4,7 +4,8 @@ A drop-in for the reference engine's attention path (reference: nanovllm_voxcpm/
 context of nanovllm_voxcpm/engine/utils.py:25-99): ``Attention`` with the same constructor, attributes and
 ``forward(q, k, v)`` dispatch over the module-global ``Context``, backed by three HIP kernels in libvoxattn.so
 (KV slot scatter, varlen GQA prefill on bf16 MFMA, split-KV paged decode) reached through a C ABI
-(include/vox_attn.h). The caches are bf16 or held in 4 bits (ops_fp4). Build the library with ``python -m voxcpm2_arabic_dialects_turbo_amd.build``.
+(include/vox_attn.h). The caches are bf16 or held in 4 bits (ops_fp4); attention may add up what every cached token receives
+(ops_weights), for eviction by it. Build the library with ``python -m voxcpm2_arabic_dialects_turbo_amd.build``.
 """
 
 from .context import Context, get_context, reset_context, set_context

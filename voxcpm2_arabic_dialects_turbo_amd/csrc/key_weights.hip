@@ -14,7 +14,7 @@
 // The lanes' sums meet in LDS at the end.
 //
 // Bound by those fma, exp2 (quarter rate) and adds, about as many cycles as the MFMAs: 6 chunks of 1000-2000 tokens over
-// 1500-2500 (16 heads of 2, 107 GFLOP of scores) 139-160 us, beside 235-250 for the attention; small calls by latency
+// 1500-2500 (16 heads of 2, 107 GFLOP of scores) 144-159 us, beside 236-255 for the attention; small calls by latency
 // (44 chunks of 33-59 over 50: 9.8 us).
 #include <type_traits>
 
@@ -444,9 +444,9 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
 
 int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {
   // About three items for each workgroup slot (two a CU), of 256 to 4096 rows, and 16 parts at most; one part of up to 640
-  // rows, where a second launch costs what it saves. us, in parts of 512 rows and eight at most, against this: prompts of 64
-  // tokens 11.0 (in parts of 256 9.0 + 2.6 and a launch's gap), 100 11.5 + 3.9 and 9.5 + 3.3, 237 12.2 + 3.8 and 9.7 + 3.9,
-  // 1000 18.6 + 4.2 and 12.9 + 4.0.
+  // rows, where a second launch costs what it saves. us (with whole key blocks), in parts of 512 rows and eight at most,
+  // against this: prompts of 64 tokens 11.0 (in parts of 256 9.0 + 2.6 and a launch's gap), 100 11.5 + 3.9 and 9.5 + 3.3,
+  // 237 12.2 + 3.8 and 9.7 + 3.9, 1000 18.6 + 4.2 and 12.9 + 4.0.
   const int64_t blocks = ((int64_t)max_seqlen_k + kKwKeys - 1) / kKwKeys;
   const int64_t longest = (int64_t)max_seqlen_q * group, least = (longest + 15) / 16;
   const int64_t want = num_tokens * group * num_kv_heads * blocks / 1536;
