@@ -538,3 +538,44 @@ def test_bounds_past_32_bits():
     for x, n in zip(w, (70, 2 ** 33 + 1)):
         o = varlen_attention_weights(q, k, v, x, **{**kw, "max_seqlen_q": n})
     assert torch.equal(*w) and w[0].any() and o.isfinite().all()
+
+
+def test_caches_past_4_gib():
+    """Planes of 4.7 GiB: blocks at both ends, in decode steps, chunks and evictions; and a long prefix."""
+    gen = torch.Generator().manual_seed(55)
+    n, bs, h, hk, cols = 36000, 256, 16, 2, 5
+    lens, blocks = [1100, 300], [n - 1, 7, n - 2, 33000, 0, n - 3, 34001]
+    small = _kv(gen, 1, 7, bs, hk, "bf16")  # (the blocks in this order)
+    big = torch.empty(1, 2, n, bs, hk, D, dtype=torch.bfloat16, device=DEV)
+    for i, at in enumerate(blocks):
+        big[:, :, at] = small[:, :, i].to(DEV)
+    near = torch.tensor([[0, 1, 2, 3, 4], [5, 6, -1, -1, -1]], dtype=torch.int32)
+    far = torch.tensor([[blocks[i] if i >= 0 else -1 for i in row] for row in near.tolist()], dtype=torch.int32, device=DEV)
+    q, w = randn(gen, 2, h, D), _received(gen, 2, hk, cols * bs)
+    for chunk in (False, True):
+        wd, want = w.to(DEV), Want(w)
+        if chunk:
+            qs = randn(gen, 60, h, D)
+            o = varlen_attention_weights(qs.to(DEV), None, None, wd, cu_seqlens_q=_i32([0, 40, 60]), cu_seqlens_k=_i32([0, 1100, 1400]),
+                                         max_seqlen_q=40, max_seqlen_k=1100, softmax_scale=SCALE, block_table=far,
+                                         k_cache=big[0, 0], v_cache=big[0, 1])
+            rows = [qs[:40], qs[40:]]
+        else:
+            o = decode_attention_weights(q.to(DEV), big[0, 0], big[0, 1], _i32(lens), far, SCALE, wd)
+            rows = [q[:1], q[1:]]
+        for b in range(2):
+            k, v = (ref.keys_of(small[0, x], near[b], lens[b])[0] for x in (0, 1))
+            want.sequence(rows[b], k, v, None, b, rows[b].shape[0])
+        want.check(o, wd)
+    weights = torch.rand(1, 2, hk, cols * bs, generator=gen)
+    wd = weights.to(DEV)
+    t, left = evict_kv_tokens(big, wd, far, _i32(lens), 260, recent=20, sinks=3)
+    want_t, want_n = ref.evict(small, weights, near.tolist(), lens, 260, 3, 20, None, None)
+    assert left.tolist() == want_n and t.tolist() == [[blocks[i] if i >= 0 else -1 for i in row] for row in want_t]
+    assert torch.equal(wd.cpu(), weights)
+    for i, at in enumerate(blocks):
+        assert torch.equal(big[:, :, at].cpu(), small[:, :, i])
+
+
+def test_chunk_behind_a_long_prefix():
+    _varlen_case(56, [(40, 33000), (3, 9), (1, 20000)], 16, 2, 256)
