@@ -579,3 +579,25 @@ def test_caches_past_4_gib():
 
 def test_chunk_behind_a_long_prefix():
     _varlen_case(56, [(40, 33000), (3, 9), (1, 20000)], 16, 2, 256)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_not_finite_reaches_who_sees_it(bad):
+    """A new token's key: the outputs of the queries before it and the weights of another sequence. Its value: no weight."""
+    gen = torch.Generator().manual_seed(57)
+    q, k, v = randn(gen, 130, 16, D).to(DEV), randn(gen, 130, 2, D).to(DEV), randn(gen, 130, 2, D).to(DEV)
+    kw = dict(cu_seqlens_q=_i32([0, 100, 130]), cu_seqlens_k=_i32([0, 100, 130]), max_seqlen_q=100, max_seqlen_k=100,
+              softmax_scale=SCALE)
+
+    def run(k, v):
+        w = torch.zeros(2, 2, 128, device=DEV)
+        return varlen_attention_weights(q, k, v, w, **kw), w
+
+    o, w = run(k, v)
+    k2, v2 = k.clone(), v.clone()
+    k2[99], v2[99] = bad, bad
+    o2, w2 = run(k2, v)
+    assert torch.equal(o2[:99], o[:99]) and torch.equal(o2[100:], o[100:]) and torch.equal(w2[1], w[1])
+    assert w2[0, :, :100].isnan().all() and not w2[0, :, 100:].any() and o2[99].isnan().all()
+    o3, w3 = run(k, v2)
+    assert torch.equal(w3, w) and torch.equal(o3[100:], o[100:])

@@ -181,7 +181,9 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
 
     No sequence has more than max_seqlen_q queries or max_seqlen_k keys (further ones are left out). H / HK divides 128, and
     cache blocks are a multiple of 64 tokens. One-query sequences run on the decode kernels where a call is mostly those, as
-    varlen_attention's do; ``plan``: as decode_attention_weights's, for these."""
+    varlen_attention's do; ``plan``: as decode_attention_weights's, for these. A key that is not finite reaches the queries that
+    see it alone; a value that is not reaches, as in varlen_attention, outputs of earlier queries of its tile too (never
+    weights)."""
     fn = "varlen_attention_weights"
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"{fn}: q must be bf16 [T, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
