@@ -1107,8 +1107,8 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
 }
 
 namespace {
-// Scratch of a varlen call that adds to key weights, each part 256-byte aligned: lse [num_tokens, num_heads], then the parts'
-// sums [sequences of a launch, num_kv_heads, parts, max_k]
+// Scratch of a varlen call that adds to key weights, each part 256-byte aligned: lse [num_tokens, num_heads], then the sums of
+// the sequences that have several parts [places, num_kv_heads, max_k], at most twice as many places as parts fit the call's rows
 struct WeightsScratch {
   int part_rows, parts;
   size_t partials, total;
@@ -1119,8 +1119,8 @@ WeightsScratch weights_scratch(int64_t num_tokens, int batch, int max_q, int max
   s.part_rows = vox::key_weights_part_rows(num_tokens, batch, max_q, max_k, group, num_kv_heads);
   s.parts = (int)(((int64_t)max_q * group + s.part_rows - 1) / s.part_rows);
   s.partials = round256((size_t)num_tokens * num_heads * 4);
-  const size_t slice = batch < vox::kMaxSeqPerLaunch ? batch : vox::kMaxSeqPerLaunch;
-  s.total = s.partials + (s.parts > 1 ? round256(slice * num_kv_heads * s.parts * (size_t)max_k * 4) : 0);
+  const size_t places = 2 * (size_t)(num_tokens * group / s.part_rows);
+  s.total = s.partials + (s.parts > 1 ? round256(places * num_kv_heads * (size_t)max_k * 4) : 0);
   return s;
 }
 }  // namespace

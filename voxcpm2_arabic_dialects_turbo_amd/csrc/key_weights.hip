@@ -106,6 +106,11 @@ struct KwSeq {
     const int64_t end = min((int64_t)min(nk, old + last + 1), k.width);
     return end <= 0 ? 0 : (int)((end + (1 << k.item_shift) - 1) >> k.item_shift);
   }
+  // the place of its first part among the partials, where it has several: with r the call's rows before it over part_rows, two
+  // sequences' floor(r) are apart by at least the parts of the first less one, so twice that by at least its parts
+  __device__ __forceinline__ int64_t first_part(const KeyWeightsArgs& k, int gsh) const {
+    return (((int64_t)q0 << gsh) / k.part_rows) * 2;
+  }
 };
 __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh) {
   const PrefillArgs& p = k.a;
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
       float got = sums[kw][lane] + sums[kw + KW][lane];
       got = (counts >> lane) & 1u ? got : 0.f;
       if (s.parts > 1) {
-        k.partials[(((int64_t)b * HK + g) * k.max_parts + x) * k.max_k + j] = got;
+        k.partials[((s.first_part(k, gsh) + x) * HK + g) * k.max_k + j] = got;
       } else {
         float* out = k.weights + (s.row * HK + g) * k.width + j;
         *out = j >= s.old ? got : *out + got;
@@ -388,14 +393,15 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   const int gsh = __builtin_ctz(k.a.group);
   const KwSeq s = kw_seq(k, b, gsh);
   if (s.parts <= 1 || j >= s.nk || j >= k.width) return;
-  const float* part = k.partials + ((int64_t)b * k.a.num_kv_heads + g) * k.max_parts * k.max_k + j;
+  const int64_t apart = (int64_t)k.a.num_kv_heads * k.max_k;
+  const float* part = k.partials + s.first_part(k, gsh) * apart + (int64_t)g * k.max_k + j;
   // the first part with a row that sees the key's block
   const int from = (int)(((int64_t)max(0, (j >> k.item_shift << k.item_shift) - s.old) << gsh) / k.part_rows);
   float got = 0.f;
   for (int x = from; x < s.parts; x += 8) {  // (eight loads in flight)
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = part[(int64_t)min(x + i, s.parts - 1) * k.max_k];
+    for (int i = 0; i < 8; ++i) v[i] = part[min(x + i, s.parts - 1) * apart];
 #pragma unroll
     for (int i = 0; i < 8; ++i) got += x + i < s.parts ? v[i] : 0.f;
   }

@@ -144,7 +144,7 @@ struct KeyWeightsArgs {
   int max_k;
   int part_rows;              // a sequence's query rows (tokens x group) in parts of so many; a multiple of 128
   int max_parts;              // of a sequence
-  float* partials;            // max_parts > 1: fp32 [a launch's sequences, HK, max_parts, max_k]
+  float* partials;            // max_parts > 1: fp32 [2 floor(a.row_limit group / part_rows), HK, max_k]
   int item_shift;             // a key block has 1 << item_shift keys
 };
 
