@@ -1113,10 +1113,10 @@ struct WeightsScratch {
   int part_rows, parts;
   size_t partials, total;
 };
-WeightsScratch weights_scratch(int64_t num_tokens, int batch, int max_q, int max_k, int num_heads, int num_kv_heads) {
+WeightsScratch weights_scratch(int64_t num_tokens, int max_q, int max_k, int num_heads, int num_kv_heads) {
   WeightsScratch s;
   const int group = num_heads / num_kv_heads;
-  s.part_rows = vox::key_weights_part_rows(num_tokens, batch, max_q, max_k, group, num_kv_heads);
+  s.part_rows = vox::key_weights_part_rows(num_tokens, max_q, max_k, group, num_kv_heads);
   s.parts = (int)(((int64_t)max_q * group + s.part_rows - 1) / s.part_rows);
   s.partials = round256((size_t)num_tokens * num_heads * 4);
   const size_t places = 2 * (size_t)(num_tokens * group / s.part_rows);
@@ -1130,7 +1130,7 @@ size_t vox_prefill_weights_bytes(int64_t num_tokens, int batch, int max_seqlen_q
   if (num_tokens <= 0 || batch <= 0 || max_seqlen_q <= 0 || max_seqlen_k < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads)
     return 0;
-  return weights_scratch(num_tokens, batch, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads).total;
+  return weights_scratch(num_tokens, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads).total;
 }
 
 int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
@@ -1170,7 +1170,7 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   if ((int64_t)max_seqlen_q * k.a.group > (1 << 30) || max_seqlen_k > (1 << 30) ||
       ((int64_t)max_seqlen_k / 128 + 1) * 16 * num_kv_heads * slice > INT32_MAX)
     return fail(VOX_EINVAL, "%s: max_seqlen_q %d or max_seqlen_k %d too large", fn, max_seqlen_q, max_seqlen_k);
-  const WeightsScratch ws = weights_scratch(num_tokens, batch, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads);
+  const WeightsScratch ws = weights_scratch(num_tokens, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads);
   if (!scratch || !aligned16(scratch) || scratch_bytes < ws.total)
     return fail(VOX_EINVAL, "%s: scratch of %zu bytes (16-byte aligned), %zu needed", fn, scratch_bytes, ws.total);
   k.a.lse = (float*)scratch;

@@ -448,7 +448,7 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
   return launch_lse<4, 1, false>(a, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
 }
 
-int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {
+int key_weights_part_rows(int64_t num_tokens, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {
   // About three items for each workgroup slot (two a CU), of 256 to 4096 rows, and 16 parts at most; one part of up to 640
   // rows, where a second launch costs what it saves. us (with whole key blocks), in parts of 512 rows and eight at most,
   // against this: prompts of 64 tokens 11.0 (in parts of 256 9.0 + 2.6 and a launch's gap), 100 11.5 + 3.9 and 9.5 + 3.3,

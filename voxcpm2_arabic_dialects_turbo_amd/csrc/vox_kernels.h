@@ -264,7 +264,7 @@ hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t st
 // Causal varlen attention that also leaves every row's a.lse, then what the keys received (key_weights.hip).
 hipError_t launch_prefill_lse(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 hipError_t launch_key_weights(const KeyWeightsArgs& k, hipStream_t stream);
-int key_weights_part_rows(int64_t num_tokens, int batch, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads);
+int key_weights_part_rows(int64_t num_tokens, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads);
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 
