@@ -31,7 +31,7 @@ def attend(q, k, v, scale, counts=None):
 def add(row, p, new):
     """Adds p [H, n, m] to one sequence's row of weights [HK, width] in place; the last ``new`` tokens start with theirs."""
     hk, m = row.shape[0], p.shape[2]
-    got = p.sum(1).view(hk, -1, m).sum(1)
+    got = p.sum(1).view(hk, p.shape[0] // hk, m).sum(1)
     old = max(m - new, 0)
     row[:, :old] += got[:, :old]
     row[:, old:m] = got[:, old:]

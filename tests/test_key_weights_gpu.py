@@ -601,3 +601,70 @@ def test_what_is_not_finite_reaches_who_sees_it(bad):
     assert w2[0, :, :100].isnan().all() and not w2[0, :, 100:].any() and o2[99].isnan().all()
     o3, w3 = run(k, v2)
     assert torch.equal(w3, w) and torch.equal(o3[100:], o[100:])
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# seeded random calls
+
+
+def _draw(gen, lo, hi):
+    return int(torch.randint(lo, hi + 1, (1,), generator=gen))
+
+
+def _rows(gen, n):
+    if _draw(gen, 0, 1):
+        return None
+    rows = torch.randperm(n + 4, generator=gen)[:n].tolist()
+    return [-1 if _draw(gen, 0, 9) == 0 else r for r in rows]
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_random_decodes(seed):
+    gen = torch.Generator().manual_seed(1000 + seed)
+    h, hk = [(16, 2), (8, 1), (16, 1), (4, 2), (10, 2), (7, 1)][seed % 6]
+    top = [40, 400, 1500][seed % 3]
+    lens = [_draw(gen, 0, top) if _draw(gen, 0, 6) else 0 for _ in range(_draw(gen, 1, [180, 40, 12][seed % 3]))]
+    _decode_case(1000 + seed, lens, h, hk, [256, 64, 32, 160][_draw(gen, 0, 3)], _rows(gen, len(lens)),
+                 bool(_draw(gen, 0, 1)) and any(lens), extra_cols=_draw(gen, 0, 2))
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_random_chunks(seed):
+    """Few rows and many, short keys and long: every form of the two launches."""
+    gen = torch.Generator().manual_seed(2000 + seed)
+    h, hk = [(16, 2), (8, 1), (16, 1), (4, 4), (32, 4), (64, 1)][_draw(gen, 0, 5)]
+    packed, top = bool(_draw(gen, 0, 2) == 0), [20, 150, 700][seed % 3]
+    seqs = []
+    for _ in range(_draw(gen, 1, [90, 24, 5][seed % 3])):
+        n = [0, 1, 1, _draw(gen, 1, top), _draw(gen, 1, top)][_draw(gen, 0, 4)]
+        prefix = 0 if packed and _draw(gen, 0, 3) else _draw(gen, 0, [60, 500, 1500][_draw(gen, 0, 2)])
+        seqs.append((n, max(n + prefix - (_draw(gen, 0, 9) == 0) * 3, 0)))
+    if not any(n for n, _ in seqs):
+        seqs.append((3, 5))
+    _varlen_case(2000 + seed, seqs, h, hk, None if packed else [64, 256, 192][_draw(gen, 0, 2)], _rows(gen, len(seqs)),
+                 extra_cols=_draw(gen, 0, 2))
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_random_evictions(seed):
+    gen = torch.Generator().manual_seed(3000 + seed)
+    kind, hk, bs = ["bf16", "fp4", "narrow"][seed % 3], _draw(gen, 1, 3), [16, 64, 96, 256][_draw(gen, 0, 3)]
+    reach = _draw(gen, 1, [200, 1500, 3000][_draw(gen, 0, 2)])
+    cols = -(-reach // bs)
+    if kind == "fp4" and bs % 64:
+        bs, cols = 64, -(-reach // 64)
+    lens = [_draw(gen, 0, reach) for _ in range(_draw(gen, 1, 6))]
+    budget = _draw(gen, 1, reach)
+    sinks = _draw(gen, 0, budget)
+    recent = _draw(gen, 0, budget - sinks)
+    need, spare = sum(-(-n // bs) for n in lens), len(lens) * -(-budget // bs)
+    tables, rest = _tables(gen, lens, need + spare + 2, bs, cols)
+    new = None
+    if _draw(gen, 0, 1):
+        per = -(-budget // bs)
+        new = [[rest[b * per + c] if c < per and _draw(gen, 0, 2) else -1 for c in range(cols)] for b in range(len(lens))]
+    rows = _rows(gen, len(lens))
+    weights = torch.rand(2, len(lens) + 4, hk, cols * bs + _draw(gen, 0, 9), generator=gen)
+    if _draw(gen, 0, 1):
+        weights = torch.floor(weights * 8)
+    _evict_case(_kv(gen, 2, need + spare + 2, bs, hk, kind), weights, tables, lens, budget, sinks, recent, rows, new)

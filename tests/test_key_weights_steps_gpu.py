@@ -283,3 +283,32 @@ def test_a_planned_step_is_the_unplanned_one():
             y = decode_attention_weights(q, kc, vc, _i32(lens), tables, SCALE, b)
             assert torch.equal(x, y) and torch.equal(a, b)
     assert get_context().weight_rows is None
+
+
+def test_layers_with_and_without_weights_in_one_planned_step():
+    """Calls of both kinds, riding stores and varlen calls among them, under one plan key: each as without a plan."""
+    gen = torch.Generator().manual_seed(6)
+    kc, vc = randn(gen, 12, BS, HK, D).to(DEV), randn(gen, 12, BS, HK, D).to(DEV)
+    tables, lens = _i32([[0, 1, 2, 3], [4, 5, 6, 7], [8, 9, 10, 11]]), [700, 90, 1024]
+    slots = _i32([699, 4 * BS + 89, 8 * BS + 1023])
+    cu_k = _i32([0, 700, 790, 1814])
+    kw = dict(cu_seqlens_q=_i32([0, 1, 2, 3]), cu_seqlens_k=cu_k, max_seqlen_q=1, max_seqlen_k=1024, softmax_scale=SCALE,
+              block_table=tables, k_cache=kc, v_cache=vc)
+    new = dict(key=randn(gen, 3, HK, D).to(DEV), value=randn(gen, 3, HK, D).to(DEV), slot_mapping=slots)
+    decode_attention_weights(randn(gen, 3, H, D).to(DEV), kc, vc, _i32(lens), tables, SCALE,
+                             torch.ones(3, HK, 1024, device=DEV), **new)  # (the rows are there from here on)
+    for kind in "wdwwvdswsvvw":
+        q = randn(gen, 3, H, D).to(DEV)
+        got = []
+        for plan in (("one", 1), None) if kind != "d" else (("one", 1), ("other", kind)):
+            w = torch.ones(3, HK, 1024, device=DEV)
+            if kind == "d":
+                o = ops.decode_attention(q, kc, vc, _i32(lens), tables, SCALE, plan=plan)
+            elif kind == "v":
+                o = varlen_attention_weights(q, None, None, w, **kw, plan=plan)
+            else:
+                o = decode_attention_weights(q, kc, vc, _i32(lens), tables, SCALE, w, plan=plan,
+                                             **(new if kind == "s" else {}))
+            got.append((o, w))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+        assert got[0][0].isfinite().all() and (kind == "d" or (got[0][1] != 1).any())
