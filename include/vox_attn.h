@@ -400,7 +400,7 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
  *   into         int32 [batch, into_stride] or NULL: where into[b][c] is not negative, block c of what sequence b keeps is
  *                that one, which no table of the call names, in place of its own (which then stays as it was). Blocks that
  *                several rows name need it in every row that is over the budget.
- *   moves        int32 [num_layers, batch, num_kv_heads, min(budget, max_blocks * block_size), 2], 8-byte aligned: scratch
+ *   moves        int32 [num_layers, batch, num_kv_heads, min(budget, max_blocks * block_size) + 1, 2], 8-byte aligned: scratch
  *   new_tables   int32 [batch, max_blocks]: the blocks still in use, -1 behind them; new_lens int32 [batch]
  * A context past what max_blocks blocks hold counts as that. Tokens whose block, or whose new block, is not one of the cache
  * are not moved: their new slots keep what they held. */

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
   __shared__ int hist[kBins];
   __shared__ int scratch[NW][2];
   __shared__ int counts[E * NW][2];  // [round][wave]: tokens that stay for sure, and those equal to T
-  __shared__ int s_bin, s_want;
+  __shared__ int s_bin, s_want, s_first;
   __shared__ int s_from[kTable], s_to[kTable];  // the blocks of the sequence, and those that take what it keeps
   const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
   const int lane = tid & 63, wv = tid >> 6;
@@ -86,7 +86,8 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
   }
   if (!drops) return;
   float* w = p.weights + (((int64_t)layer * p.row_count + row) * p.num_heads + g) * p.width;
-  int2* moves = p.moves + (((int64_t)layer * p.batch + b) * p.num_heads + g) * p.kept;
+  int2* moves = p.moves + (((int64_t)layer * p.batch + b) * p.num_heads + g) * (p.kept + 1);
+  if (tid == 0) s_first = p.budget;  // (before the barriers below)
   const int lo = p.sinks, hi = n - p.recent;  // (n > budget >= sinks + recent)
   int want = p.budget - p.sinks - p.recent;
   const int chunks = (n + CHUNK - 1) / CHUNK;
@@ -163,6 +164,7 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
   }
   // `want`: how many of those equal to T stay
   int sure0 = 0, ties0 = 0;  // of the chunks before
+  int first = p.budget;      // the first place of this lane's whose row moves
   for (int c = 0; c < chunks; ++c) {
     if (c > 0) load(c);
     auto kind = [&](int e, bool& sure, bool& tie) {
@@ -210,6 +212,7 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
           const bool there = src >= 0 && src < p.num_blocks && dst >= 0 && dst < p.num_blocks;
           const int from = there ? src * bs + i - ci * bs : -1, to = there ? dst * bs + j - cj * bs : -1;
           moves[j] = make_int2(from == to ? -1 : from, to);
+          if (from != to) first = min(first, j);
         }
       }
     };
@@ -221,14 +224,18 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
     }
     __syncthreads();
   }
+  first = p.budget - wave_max_dpp(p.budget - first);
+  if (lane == 0 && first < p.budget) atomicMin(&s_first, first);
+  __syncthreads();
+  if (tid == 0) moves[p.kept] = make_int2(s_first, 0);
 }
 
 // The rows of one (plane, sequence, kv head) moved: units of V, `pieces` a row, from byte `at` of a block on, a slot's
-// `slot_run` bytes apart; idle: a slot of the sequence's. LINEAR: the cache's slots are evenly spaced (no scales behind a
-// block's slots).
+// `slot_run` bytes apart, from place `first` on; idle: a slot of the sequence's. LINEAR: the cache's slots are evenly spaced (no
+// scales behind a block's slots).
 template <typename V, bool LINEAR>
 __device__ __forceinline__ void move_rows(const EvictArgs& p, const int2* moves, uint8_t* plane, int64_t block_bytes, int64_t at,
-                                          int64_t slot_run, int pieces, int idle) {
+                                          int64_t slot_run, int pieces, int idle, int first) {
   const int per = kMoveThreads / pieces;  // rows a step of the workgroup moves
   const int r = (int)threadIdx.x / pieces, piece = (int)threadIdx.x % pieces;
   const bool on = r < per;
@@ -242,7 +249,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& p, const int2* moves,
   auto pairs = [&](int j0, int2 (&m)[kMoveRows]) {
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u) {
-      const int j = j0 + u * per + r;
+      const int j = first + j0 + u * per + r;
       m[u] = moves[min(j, left - 1)];
       if (!on || j >= left) m[u].x = -1;
     }
@@ -264,7 +271,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& p, const int2* moves,
   };
   int2 ma[kMoveRows], mb[kMoveRows];
   V va[kMoveRows], vb[kMoveRows];
-  const int rounds = (left + round - 1) / round;
+  const int rounds = (left - first + round - 1) / round;
   pairs(0, ma);
   rows(ma, va);
   pairs(round, mb);
@@ -293,7 +300,9 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs p) {
   const int n = max(0, min(p.context_lens[b], p.max_blocks * p.block_size));
   const int64_t row = p.rows ? (int64_t)p.rows[b] : b;
   if (n <= p.budget || row < 0 || row >= p.row_count) return;
-  const int2* moves = p.moves + (((int64_t)(plane >> 1) * p.batch + b) * p.num_heads + g) * p.kept;
+  const int2* moves = p.moves + (((int64_t)(plane >> 1) * p.batch + b) * p.num_heads + g) * (p.kept + 1);
+  const int first = moves[p.kept].x;  // (the rows before the first dropped token are where they belong)
+  if (first >= p.budget) return;
   const int64_t block_bytes = (int64_t)p.block_size * p.num_heads * (p.head_bytes + p.scale_bytes);
   const int64_t run = (int64_t)p.num_heads * p.head_bytes;
   uint8_t* base = p.kv + (int64_t)plane * p.num_blocks * block_bytes;
@@ -301,12 +310,12 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs p) {
   const int bytes = p.head_bytes / p.parts;
   const int64_t at = (int64_t)g * p.head_bytes + x * bytes;
   if (!p.scale_bytes)
-    move_rows<u32x4, true>(p, moves, base, block_bytes, at, run, bytes / 16, idle);
+    move_rows<u32x4, true>(p, moves, base, block_bytes, at, run, bytes / 16, idle, first);
   else if (x < p.parts)
-    move_rows<u32x4, false>(p, moves, base, block_bytes, at, run, bytes / 16, idle);
+    move_rows<u32x4, false>(p, moves, base, block_bytes, at, run, bytes / 16, idle, first);
   else
     move_rows<uint32_t, false>(p, moves, base, block_bytes, (int64_t)p.block_size * run + (int64_t)g * p.scale_bytes,
-                               (int64_t)p.num_heads * p.scale_bytes, p.scale_bytes / 4, idle);
+                               (int64_t)p.num_heads * p.scale_bytes, p.scale_bytes / 4, idle, first);
 }
 
 }  // namespace

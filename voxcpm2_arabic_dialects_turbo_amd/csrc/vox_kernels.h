@@ -170,8 +170,8 @@ struct EvictArgs {
   int budget, sinks, recent;    // budget > 0, sinks + recent <= budget
   const int32_t* into;          // int32 [batch, into_stride], first max_blocks columns, or null: blocks that take the kept
   int64_t into_stride;          // tokens in place of the table's own (-1: those)
-  int2* moves;                  // [layers, batch, num_heads, kept]: the slots that place j's token comes from (-1: it stays) and
-  int64_t kept;                 // goes to; kept = min(budget, max_blocks * block_size); 8-byte aligned
+  int2* moves;                  // [layers, batch, num_heads, kept + 1]: the slots that place j's token comes from (-1: it stays)
+  int64_t kept;                 // and goes to, then the first place that one moves to; kept = min(budget, max_blocks * block_size)
   int parts;                    // set by the launcher: slices of a row's bytes
   int32_t* new_tables;          // int32 [batch, max_blocks]
   int32_t* new_lens;            // int32 [batch]

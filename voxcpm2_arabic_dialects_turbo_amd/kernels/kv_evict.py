@@ -71,7 +71,7 @@ def evict_kv_tokens(kv: torch.Tensor, key_weights: torch.Tensor, block_tables: t
         budget, sinks, recent = mb * bs, 0, 0
     lib = _lib.load()
     with _on(dev):
-        moves = torch.empty(layers, batch, hk, budget, 2, dtype=torch.int32, device=dev)
+        moves = torch.empty(layers, batch, hk, budget + 1, 2, dtype=torch.int32, device=dev)
         _lib.check(lib.vox_evict_kv_tokens(kv.data_ptr(), layers, blocks, bs, hk, slot // hk, scale // hk, bt.data_ptr(),
                                            bt_stride, mb, lens.data_ptr(), batch, key_weights.data_ptr(),
                                            None if rows is None else rows.data_ptr(), key_weights.shape[1],
