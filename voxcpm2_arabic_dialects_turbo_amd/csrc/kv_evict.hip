@@ -7,8 +7,9 @@
 // those equal to T the first ones that are still wanted. Place j of a kept token at i is how many kept ones lie before it:
 // (those above T or protected before i) + min(those equal to T before i, still wanted), from ballots and one scan. Its weight
 // moves there, and move_kernel gets the pair of slots. Weights are held in registers (lane-contiguous rounds of the
-// workgroup); rows longer than those are read again. Bound by the chain of three histograms and scans: 8 us for one sequence
-// of 28 layers, 41 us for 8 of 20000-32768 tokens.
+// workgroup); rows longer than those are read again. Bound by the chain of three histograms and scans (8 us for one sequence
+// of 28 layers), for long rows by a workgroup's instructions (39 us for 8 sequences of 20000-32768 tokens, 12 layers; eight
+// histograms side by side, against lanes that meet in a bin: 38.5).
 //
 // Both kernels work in place: place j takes token i_j >= j, a round's reads are done before its writes, and a later round
 // reads only behind them. So a sequence's tokens of one kv head (and of one slice of a row's bytes) are one workgroup's.
