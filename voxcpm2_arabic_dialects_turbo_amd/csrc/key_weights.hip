@@ -14,7 +14,7 @@
 // The lanes' sums meet in LDS at the end.
 //
 // Bound by those fma, exp2 (quarter rate) and adds, about as many cycles as the MFMAs: 6 chunks of 1000-2000 tokens over
-// 1500-2500 (16 heads of 2, 107 GFLOP of scores) 144-159 us, beside 236-255 for the attention; small calls by latency
+// 1500-2500 (16 heads of 2, 107 GFLOP of scores) 143-160 us, beside 223-245 for the attention; small calls by latency
 // (44 chunks of 33-59 over 50: 9.8 us).
 #include <type_traits>
 
@@ -62,8 +62,9 @@ __device__ __forceinline__ int sequence_of(int item, int batch, const int* start
   return __builtin_amdgcn_readfirstlane(b);
 }
 
-// WALK: for calls whose (q tile, sequence) grid would be mostly empty: a fixed grid walks the q tiles that there are, a
-// sequence's heaviest first.
+// Heavy q tiles, which see most keys, first: one that starts late is the launch's end. WALK: a workgroup for each of the q tiles
+// that there are, sequence by sequence, where the (q tile, sequence) grid would be mostly empty, or so large that its empty
+// ones cost more than the items' layout.
 template <int SRC, int RG, int KS, bool WALK>
 __global__ __launch_bounds__(64 * RG * KS, 2) void prefill32_lse_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t kt0[pf32::kTB];
@@ -80,16 +81,13 @@ __global__ __launch_bounds__(64 * RG * KS, 2) void prefill32_lse_kernel(PrefillA
       const int nq = p.cu_q[b + 1] - p.cu_q[b];
       return nq <= 0 || (p.skip_single && nq == 1) ? 0 : (nq + BQ - 1) / BQ * HK;
     });
-    for (int item = blockIdx.x; item < total; item += gridDim.x) {
-      const int b = sequence_of(item, p.batch, starts);
-      const int from = __builtin_amdgcn_readfirstlane(starts[b]), n = __builtin_amdgcn_readfirstlane(starts[b + 1]) - from;
-      pf32::tile<SRC, RG, KS, true>(p, (n - 1 - (item - from)) / HK, b, (item - from) % HK, bufs);
-      __syncthreads();  // the tiles are free
-    }
+    const int item = blockIdx.x;
+    if (item >= total) return;
+    const int b = sequence_of(item, p.batch, starts);
+    const int from = __builtin_amdgcn_readfirstlane(starts[b]), n = __builtin_amdgcn_readfirstlane(starts[b + 1]) - from;
+    pf32::tile<SRC, RG, KS, true>(p, (n - 1 - (item - from)) / HK, b, (item - from) % HK, bufs);
   } else {
-    int qt, b, g;
-    grid_item(p, qt, b, g);
-    pf32::tile<SRC, RG, KS, true>(p, qt, b, g, bufs);
+    pf32::tile<SRC, RG, KS, true>(p, (int)(gridDim.x - 1 - blockIdx.x), (int)blockIdx.y, (int)blockIdx.z, bufs);
   }
 }
 
@@ -427,24 +425,30 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
     return hipErrorInvalidValue;
   PrefillArgs a = a0;
   const int64_t tiles = ((int64_t)max_seqlen_q + 128 / a.group - 1) / (128 / a.group);
-  // T rows against the grid's: (row_limit is the rows that there are)
-  if (4 * a.row_limit <= (int64_t)max_seqlen_q * a.batch) {
+  const int64_t grid = tiles * a.batch * a.num_kv_heads;
+  // WALK (6 x 1000-2000 over 1500-2500: 245 us, the plain grid heavy tiles first 248, in XCD order 255; 44 x 33-59 over 50 13.2
+  // against the plain grid's 12.3, 5 x 237-900 27.2 against 25.1)
+  if (grid >= 1024 || 4 * a.row_limit <= (int64_t)max_seqlen_q * a.batch) {
     for (int b0 = 0; b0 < a0.batch; b0 += kMaxSeqPerLaunch) {
       a.batch = a0.batch - b0 < kMaxSeqPerLaunch ? a0.batch - b0 : kMaxSeqPerLaunch;
       a.cu_q = a0.cu_q + b0;
       a.cu_k = a0.cu_k + b0;
       if (a.block_tables) a.block_tables = a0.block_tables + (int64_t)b0 * a0.bt_stride;
-      const int64_t items = tiles * a.batch * a.num_kv_heads;
-      const hipError_t e = launch_lse<4, 1, true>(a, dim3((unsigned)(items < 512 ? items : 512)), stream);
+      // no more tiles than fit the call's rows, and one more a sequence
+      const int64_t items = (a.row_limit * a.group / 128 + a.batch) * a.num_kv_heads;
+      if (items > INT32_MAX) return hipErrorInvalidValue;
+      const hipError_t e = launch_lse<4, 1, true>(a, dim3((unsigned)items), stream);
       if (e != hipSuccess) return e;
     }
     return hipSuccess;
   }
-  const bool small = 64 % a.group == 0;
-  const int64_t tiles64 = small ? ((int64_t)max_seqlen_q + 64 / a.group - 1) / (64 / a.group) : 0;
-  if (small && tiles64 * a.batch * a.num_kv_heads <= 512)
+  // 64 rows a workgroup, two waves on the same ones: halves the chain of key tiles. Two workgroups a CU at once, or two rounds of
+  // them where the chains are long (1 x 3000 tokens: 50 us, in 128 rows 59; 44 x 33-59 over 50 15.3 and 12.4)
+  const bool fits64 = 64 % a.group == 0;
+  const int64_t tiles64 = fits64 ? ((int64_t)max_seqlen_q + 64 / a.group - 1) / (64 / a.group) : 0;
+  const int64_t grid64 = tiles64 * a.batch * a.num_kv_heads;
+  if (fits64 && (grid64 <= 512 || (grid64 <= 1024 && tiles64 >= 16)))
     return launch_lse<2, 2, false>(a, dim3((unsigned)tiles64, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
-  a.xcd_order = tiles * a.batch * a.num_kv_heads >= 1024;
   return launch_lse<4, 1, false>(a, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
 }
 

@@ -1019,6 +1019,23 @@ __device__ __forceinline__ void store_rows(const PrefillArgs& p, int wid) {
   }
 }
 
+// The plain grid's work item of this workgroup (with xcd_order, its XCD's next one)
+__device__ __forceinline__ void grid_item(const PrefillArgs& p, int& qt, int& b, int& g) {
+  qt = blockIdx.x;
+  b = blockIdx.y;
+  g = blockIdx.z;
+  if (p.xcd_order) {
+    const unsigned nwg = gridDim.x * gridDim.y * gridDim.z;
+    const unsigned id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+    const unsigned xq = nwg / kXcds, xr = nwg % kXcds, xcd = id % kXcds, loc = id / kXcds;
+    const unsigned work = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + loc;
+    qt = (int)(work % gridDim.x);
+    b = (int)((work / gridDim.x) % gridDim.y);
+    g = (int)(work / (gridDim.x * gridDim.y));
+    if (p.causal) qt = (int)gridDim.x - 1 - qt;  // heavy query tiles first
+  }
+}
+
 // Waves per SIMD the registers must allow: two 4-wave workgroups per CU (their 64 KB of LDS each fits twice), two
 // 8-wave ones (block sizes that are no multiple of 64; at most 128 VGPRs), one int8 workgroup (128 KB of LDS).
 constexpr int prefill_waves_per_simd(bool quant, int nw) { return quant ? 1 : (nw == 8 ? 4 : 2); }

@@ -619,23 +619,6 @@ __device__ __forceinline__ void tile(const PrefillArgs& p, const int qt, const i
 
 constexpr unsigned kXcds = 8;  // MI355X: workgroups are dealt round-robin over 8 XCDs
 
-// The plain grid's work item of this workgroup (with xcd_order, its XCD's next one)
-__device__ __forceinline__ void grid_item(const PrefillArgs& p, int& qt, int& b, int& g) {
-  qt = blockIdx.x;
-  b = blockIdx.y;
-  g = blockIdx.z;
-  if (p.xcd_order) {
-    const unsigned nwg = gridDim.x * gridDim.y * gridDim.z;
-    const unsigned id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
-    const unsigned xq = nwg / kXcds, xr = nwg % kXcds, xcd = id % kXcds, loc = id / kXcds;
-    const unsigned work = (xcd < xr ? xcd * (xq + 1) : xr * (xq + 1) + (xcd - xr) * xq) + loc;
-    qt = (int)(work % gridDim.x);
-    b = (int)((work / gridDim.x) % gridDim.y);
-    g = (int)(work / (gridDim.x * gridDim.y));
-    if (p.causal) qt = (int)gridDim.x - 1 - qt;  // heavy query tiles first
-  }
-}
-
 }  // namespace
 
 }  // namespace vox
