@@ -371,6 +371,17 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
                             size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
                             void* stream);
 
+/* The same over 4-bit caches, as vox_decode_attn_fp4 and vox_decode_attn_store_fp4: a score is off by at most 2^-13 of
+ * softmax_scale sum |q||k|, a probability by that many parts twice. */
+int vox_decode_attn_weights_fp4(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                                int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping,
+                                void* k_cache, void* v_cache, int64_t num_blocks, int block_size,
+                                const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                                const int32_t* context_lens, int batch, int num_heads, int num_kv_heads, int head_dim,
+                                float softmax_scale, float* key_weights, const int32_t* weight_rows,
+                                int64_t num_weight_rows, int64_t weight_width, void* scores, size_t scores_bytes, int plan,
+                                void* workspace, size_t workspace_bytes, void* out, void* stream);
+
 /* vox_prefill_attn with cu_seqlens, causal, that also adds what every key received: the last cu_seqlens_q[b + 1] -
  * cu_seqlens_q[b] tokens of a sequence are the step's own, and their weights become it, the earlier ones' grow by it. A
  * sequence without queries keeps its weights. max_seqlen_k: no sequence has more keys (further ones are left out of the

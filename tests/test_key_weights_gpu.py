@@ -12,6 +12,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from oracle import fp4
 from oracle import key_weights as ref
 from tests._util import paged_pool, randn
 from voxcpm2_arabic_dialects_turbo_amd.kernels.kv_evict import evict_kv_tokens
@@ -41,9 +42,9 @@ class Want:
         self.w, self.tol = weights.double(), torch.zeros_like(weights, dtype=torch.float64)
         self.o, self.otol = [], []
 
-    def sequence(self, q, k, v, counts, row, new, scale=SCALE):
+    def sequence(self, q, k, v, counts, row, new, scale=SCALE, more=0.0):
         o, p, pv, size = ref.attend(q, k, v, scale, counts)
-        rel = _p_tolerance(size, k.shape[0])
+        rel = _p_tolerance(size, k.shape[0]) + more
         self.o.append(o)
         self.otol.append((2 ** -8 + 2 * rel) * pv + 2 ** -8 * (o.abs() + 2 ** -8 * pv) + 1e-30)
         if row is not None and 0 <= row < self.w.shape[0] and q.shape[0]:
@@ -668,3 +669,90 @@ def test_random_evictions(seed):
     if _draw(gen, 0, 1):
         weights = torch.floor(weights * 8)
     _evict_case(_kv(gen, 2, need + spare + 2, bs, hk, kind), weights, tables, lens, budget, sinks, recent, rows, new)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# decode over 4-bit caches
+
+
+def _decode_fp4_case(seed, lens, h, hk, bs, rows=None, store=False, plan=None):
+    """As _decode_case. A score is off by at most 2^-13 of its magnitude (the scaled MFMA's sum) and by what the query's two
+    fp8 parts leave, 2^-18 of the row's largest magnitude a channel; a probability takes its own score's error x and its
+    row's: e^2x - 1 <= 2 x (1 + 2 x) of it."""
+    gen = torch.Generator().manual_seed(seed)
+    B, need = len(lens), sum(-(-n // bs) for n in lens) + 2
+    _, _, tables = paged_pool(gen, lens, need, bs, 1, 1, 1)
+    planes, live, slots = [], torch.zeros(need * bs, dtype=torch.bool), []
+    for b, n in enumerate(lens):
+        at = [int(tables[b, j // bs]) * bs + j % bs for j in range(n)]
+        live[at] = True
+        slots.append(at[-1] if at else -1)
+    for _ in range(2):  # what no context reaches is not a number
+        scales = torch.randint(123, 128, (need * bs, hk, 4), generator=gen, dtype=torch.uint8)
+        scales[~live] = 255
+        planes.append(fp4.plane(torch.randint(0, 256, (need, bs, hk, 64), generator=gen, dtype=torch.uint8),
+                                scales.view(need, bs, hk, 4)))
+    n_rows = B if rows is None else max([*rows, 0]) + 2
+    w = _received(gen, n_rows, hk, tables.shape[1] * bs + 5)
+    q, key, value = randn(gen, B, h, D), randn(gen, B, hk, D), randn(gen, B, hk, D)
+    for b, n in enumerate(lens):
+        r = b if rows is None else rows[b]
+        if n and 0 <= r < n_rows:
+            w[r, :, n - 1] = float("nan")
+    kd, vd, wd = planes[0].to(DEV), planes[1].to(DEV), w.to(DEV)
+    kw = dict(key=key.to(DEV), value=value.to(DEV), slot_mapping=_i32(slots)) if store else {}
+    o = decode_attention_weights(q.to(DEV), kd, vd, _i32(lens), tables.to(DEV), SCALE, wd, plan=plan,
+                                 weight_rows=None if rows is None else _i32(rows), **kw)
+    if store:
+        fp4.store(key, value, planes[0], planes[1], torch.tensor(slots, dtype=torch.int32))
+        assert torch.equal(kd.cpu(), planes[0]) and torch.equal(vd.cpu(), planes[1])
+    kv, vv = (fp4.cache_values(c) for c in planes)
+    want = Want(w)
+    for b, n in enumerate(lens):
+        if n == 0:
+            want.o.append(torch.zeros(1, h, D, dtype=torch.float64))
+            want.otol.append(torch.zeros(1, h, D, dtype=torch.float64))
+            continue
+        k, v = ref.keys_of(kv, tables[b], n)[0], ref.keys_of(vv, tables[b], n)[0]
+        size = (q[b].double().abs().view(hk, -1, D) @ k.abs().permute(1, 2, 0)).max()
+        x = SCALE * float(2.0 ** -13 * size + 2.0 ** -18 * q[b].abs().max() * k.abs().sum(-1).max())
+        want.sequence(q[b:b + 1], k, v, None, b if rows is None else rows[b], 1, more=2 * x * (1 + 2 * x))
+    want.check(o, wd)
+
+
+@pytest.mark.parametrize("store", [False, True])
+@pytest.mark.parametrize("h,hk,bs", [(16, 2, 256), (8, 1, 64), (16, 1, 128), (6, 2, 192), (3, 1, 64), (2, 2, 256)])
+def test_decode_fp4_lengths(h, hk, bs, store):
+    """Lengths around the steps, the chunks of two and the blocks, padded rows, rows in any order and none."""
+    lens = [1, 2, 0, 15, 16, 17, 31, 32, 33, 47, 63, 64, 65, bs - 1, bs, bs + 1, 0, 500, 3 * bs + 7]
+    gen = torch.Generator().manual_seed(h)
+    rows = torch.randperm(len(lens) + 3, generator=gen)[:len(lens)].tolist()
+    rows[4] = -1
+    _decode_fp4_case(60 + h + bs, lens, h, hk, bs, rows, store)
+    _decode_fp4_case(61 + h + bs, lens, h, hk, bs, None, store, plan=("fp4", h, bs, store))
+
+
+@pytest.mark.parametrize("lens,h,hk", [([420], 16, 2), ([33000], 16, 2), ([2, 9000, 5], 8, 1), ([40 + 7 * i for i in range(150)], 16, 2),
+                                       ([20] * 600, 16, 1), ([20000] * 3 + [17000], 16, 2)])
+def test_decode_fp4_batches(lens, h, hk):
+    """Four waves a workgroup and eight, sequences in many ranges, more than a launch lays out."""
+    _decode_fp4_case(len(lens), lens, h, hk, 256, None, len(lens) > 1)
+
+
+def test_decode_fp4_blocks_that_are_none_take_no_weight():
+    gen = torch.Generator().manual_seed(71)
+    n, bs, h, hk = 500, 64, 16, 2
+    planes = [fp4.plane(torch.randint(0, 256, (12, bs, hk, 64), generator=gen, dtype=torch.uint8),
+                        torch.randint(123, 128, (12, bs, hk, 4), generator=gen, dtype=torch.uint8)) for _ in range(2)]
+    table = torch.tensor([[3, -1, 5, 900, 7, 1, 0, 11]], dtype=torch.int32)
+    q, w = randn(gen, 1, h, D), _received(gen, 1, hk, 512)
+    before = w.clone().double()
+    o = decode_attention_weights(q.to(DEV), planes[0].to(DEV), planes[1].to(DEV), _i32([n]), table.to(DEV), SCALE,
+                                 wd := w.to(DEV))
+    (k, ok), (v, _) = (ref.keys_of(fp4.cache_values(c), table[0], n) for c in planes)
+    size = (q[0].double().abs().view(hk, -1, D) @ k.abs().permute(1, 2, 0)).max()
+    x = SCALE * float(2.0 ** -13 * size + 2.0 ** -18 * q.abs().max() * k.abs().sum(-1).max())
+    want = Want(w)
+    want.sequence(q, k, v, ok, 0, 1, more=2 * x * (1 + 2 * x))
+    want.check(o, wd)
+    assert not ok[64:128].any() and torch.equal(wd[0, :, 64:128].cpu().double(), before[0, :, 64:128])

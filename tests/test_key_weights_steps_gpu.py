@@ -312,3 +312,41 @@ def test_layers_with_and_without_weights_in_one_planned_step():
             got.append((o, w))
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
         assert got[0][0].isfinite().all() and (kind == "d" or (got[0][1] != 1).any())
+
+
+def test_a_text_over_4_bit_caches():
+    """Prompts, decode steps and evictions through the module over 4-bit caches: the calls' own outputs and weights, and tokens
+    that go on from what an eviction left."""
+    gen = torch.Generator().manual_seed(7)
+    layers = [Attention(H, D, SCALE, HK) for _ in range(2)]
+    kv = runner.allocate_kv_cache(layers, 12, BS, dtype=torch.uint8 if not hasattr(torch, "float4_e2m1fn_x2")
+                                  else torch.float4_e2m1fn_x2, device=DEV)
+    weights = runner.allocate_key_weights(layers, 4, 1024, device=DEV)
+    weights.fill_(float("nan"))
+    tasks, rows = [runner.RunnerTask([0, 1], 300, 0), runner.RunnerTask([2], 30, 0)], [3, 1]
+    runner.prepare_prefill_context(tasks, BS, device=DEV, weight_rows=rows)
+    for layer in layers:
+        layer(randn(gen, 330, H, D).to(DEV), randn(gen, 330, HK, D).to(DEV), randn(gen, 330, HK, D).to(DEV))
+    spare = list(range(3, 12))
+    for step in range(6):
+        for t in tasks:
+            _next(t, spare)
+        runner.prepare_decode_context(tasks, BS, device=DEV, weight_rows=rows)
+        ctx = get_context()
+        for i, layer in enumerate(layers):
+            q, k, v = randn(gen, 2, H, D).to(DEV), randn(gen, 2, HK, D).to(DEV), randn(gen, 2, HK, D).to(DEV)
+            kv2, w2 = kv[i].clone(), weights[i].clone()
+            o = layer(q, k, v)
+            o2 = decode_attention_weights(q, kv2[0], kv2[1], ctx.context_lens, ctx.block_tables, SCALE, w2, ctx.weight_rows,
+                                          key=k, value=v, slot_mapping=ctx.slot_mapping)
+            assert torch.equal(o.reshape(o2.shape), o2) and torch.equal(kv[i], kv2)
+            assert torch.equal(weights[i].view(torch.int32), w2.view(torch.int32))
+            for t, r in zip(tasks, rows):
+                assert weights[i, r, :, :t.seq_length].isfinite().all() and weights[i, r, :, t.seq_length].isnan().all() \
+                    or step > 3
+        if step == 3:
+            lens = [t.seq_length for t in tasks]
+            tables = [tasks[0].block_table, tasks[1].block_table + [-1]]
+            new, left = evict_kv_tokens(kv, weights, _i32(tables), _i32(lens), 100, recent=20, sinks=4, weight_rows=_i32(rows))
+            assert left.tolist() == [100, lens[1]]
+            tasks[0].block_table, tasks[0].seq_length = [b for b in new[0].tolist() if b >= 0], 100

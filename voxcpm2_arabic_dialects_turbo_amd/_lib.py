@@ -51,6 +51,7 @@ EXPORTS = (
     "vox_compact_kv_blocks",
     "vox_decode_scores_bytes",
     "vox_decode_attn_weights",
+    "vox_decode_attn_weights_fp4",
     "vox_prefill_weights_bytes",
     "vox_prefill_attn_weights",
     "vox_evict_kv_tokens",
@@ -118,6 +119,10 @@ _SIGNATURES = {
                                        _c_void_p, _i64, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32, _i32, _i32, _i32,
                                        _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _i32, _c_void_p, _size,
                                        _c_void_p, _c_void_p]),
+    "vox_decode_attn_weights_fp4": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                           _c_void_p, _i64, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32, _i32, _i32, _i32,
+                                           _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _i32, _c_void_p, _size,
+                                           _c_void_p, _c_void_p]),
     "vox_prefill_weights_bytes": (_size, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "vox_prefill_attn_weights": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
                                         _i32, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _i64,

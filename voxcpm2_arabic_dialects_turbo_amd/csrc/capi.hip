@@ -1061,7 +1061,10 @@ size_t vox_decode_scores_bytes(int batch, int max_blocks, int block_size, int nu
   return (size_t)slice * steps * num_heads * 16 * 4;
 }
 
-int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+}  // extern "C"
+
+namespace {
+int decode_attn_weights(const char* fn, bool fp4, const void* q, int64_t q_row_stride, const void* key, const void* value,
                             int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping, void* k_cache,
                             void* v_cache, int64_t num_blocks, int block_size, const int32_t* block_tables,
                             int64_t bt_stride, int max_blocks, const int32_t* context_lens, int batch, int num_heads,
@@ -1069,12 +1072,13 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
                             const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width, void* scores,
                             size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
                             void* stream) {
-  const char* fn = "decode_attn_weights";
   if (batch < 0) return fail(VOX_EINVAL, "%s: batch < 0", fn);
   if (plan != VOX_PLAN_NONE && plan != VOX_PLAN_RECORD && plan != VOX_PLAN_REUSE)
     return fail(VOX_EINVAL, "%s: plan mode %d", fn, plan);
   if (batch == 0) return VOX_OK;
   int st = weights_setup(fn, key_weights, num_weight_rows, weight_width, softmax_scale);
+  if (st == VOX_OK && fp4) st = fp4_cache(fn, k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+  if (st == VOX_OK && fp4) st = fp4_softmax(fn, softmax_scale);
   if (st != VOX_OK) return st;
   if ((key == nullptr) != (value == nullptr) || (key == nullptr) != (slot_mapping == nullptr))
     return fail(VOX_EINVAL, "%s: key, value and slot_mapping go together", fn);
@@ -1103,7 +1107,39 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
   a.weight_rows = weight_rows;
   a.weight_row_count = num_weight_rows;
   a.weight_width = weight_width;
-  return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream, vox::launch_decode_weights);
+  return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream,
+                              fp4 ? vox::launch_decode_weights_fp4 : vox::launch_decode_weights);
+}
+}  // namespace
+
+extern "C" {
+
+int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                            int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping, void* k_cache,
+                            void* v_cache, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                            int64_t bt_stride, int max_blocks, const int32_t* context_lens, int batch, int num_heads,
+                            int num_kv_heads, int head_dim, float softmax_scale, float* key_weights,
+                            const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width, void* scores,
+                            size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
+                            void* stream) {
+  return decode_attn_weights("decode_attn_weights", false, q, q_row_stride, key, value, key_row_stride, value_row_stride, slot_mapping, k_cache, v_cache,
+                             num_blocks, block_size, block_tables, bt_stride, max_blocks, context_lens, batch, num_heads,
+                             num_kv_heads, head_dim, softmax_scale, key_weights, weight_rows, num_weight_rows, weight_width,
+                             scores, scores_bytes, plan, workspace, workspace_bytes, out, stream);
+}
+
+int vox_decode_attn_weights_fp4(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                            int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping, void* k_cache,
+                            void* v_cache, int64_t num_blocks, int block_size, const int32_t* block_tables,
+                            int64_t bt_stride, int max_blocks, const int32_t* context_lens, int batch, int num_heads,
+                            int num_kv_heads, int head_dim, float softmax_scale, float* key_weights,
+                            const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width, void* scores,
+                            size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
+                            void* stream) {
+  return decode_attn_weights("decode_attn_weights_fp4", true, q, q_row_stride, key, value, key_row_stride, value_row_stride, slot_mapping, k_cache, v_cache,
+                             num_blocks, block_size, block_tables, bt_stride, max_blocks, context_lens, batch, num_heads,
+                             num_kv_heads, head_dim, softmax_scale, key_weights, weight_rows, num_weight_rows, weight_width,
+                             scores, scores_bytes, plan, workspace, workspace_bytes, out, stream);
 }
 
 namespace {

@@ -195,21 +195,34 @@ hipError_t launch_decode(const DecodeArgs& a, int num_kv_heads, hipStream_t stre
   return launch_decode_merge(a, stream);
 }
 
-hipError_t launch_decode_weights(const DecodeArgs& a0, int num_kv_heads, hipStream_t stream) {
-  if (!a0.scores || !a0.weights) return hipErrorInvalidValue;
+namespace {
+
+template <bool FP4>
+hipError_t launch_merge_weights(const DecodeArgs& a, hipStream_t stream) {
+  if (a.batch <= kMergeSplitBatch)
+    decode_merge_kernel<4, FP4, true><<<dim3((unsigned)(4 * a.batch + a.weight_wgs)), dim3(256), 0, stream>>>(a);
+  else
+    decode_merge_kernel<1, FP4, true><<<dim3((unsigned)(a.batch + a.weight_wgs)), dim3(256), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_decode_merge_weights(const DecodeArgs& a0, bool fp4, hipStream_t stream) {
   DecodeArgs a = a0;
   // a wave for every four steps that the tables allow, a round of add_key_weights, up to two workgroups per CU (the kernel's us
   // with up to one, two, four: 24 of 20000-32768 tokens 14.5, 13.4, 14.2; 150 of 256-2048 9.0, 8.9, 11.1; 120 such rows
   // beside 6 prompts 7.4, 8.4, 10.4)
   const int64_t steps = (int64_t)a.batch * (((int64_t)a.max_blocks * a.block_size + kTile - 1) / kTile);
   a.weight_wgs = (int)min((int64_t)512, (steps + 15) / 16);
+  return fp4 && a.slot_mapping ? launch_merge_weights<true>(a, stream) : launch_merge_weights<false>(a, stream);
+}
+
+hipError_t launch_decode_weights(const DecodeArgs& a, int num_kv_heads, hipStream_t stream) {
+  if (!a.scores || !a.weights) return hipErrorInvalidValue;
   const hipError_t e = launch_split<true>(a, num_kv_heads, stream);
   if (e != hipSuccess) return e;
-  if (a.batch <= kMergeSplitBatch)
-    decode_merge_kernel<4, false, true><<<dim3((unsigned)(4 * a.batch + a.weight_wgs)), dim3(256), 0, stream>>>(a);
-  else
-    decode_merge_kernel<1, false, true><<<dim3((unsigned)(a.batch + a.weight_wgs)), dim3(256), 0, stream>>>(a);
-  return hipGetLastError();
+  return launch_decode_merge_weights(a, false, stream);
 }
 
 }  // namespace vox

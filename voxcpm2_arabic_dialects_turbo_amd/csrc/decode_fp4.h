@@ -47,7 +47,7 @@ struct Chunk {
   u32x4 piece;              // 8 channels: lanes [0, 16 HK) of its key row, [16 HK, 32 HK) of its value row
 };
 
-template <int HK, bool BTL, int NW, int SEGS = 6>
+template <int HK, bool BTL, int NW, int SEGS = 6, bool SCORES = false>
 struct LdsFp4 {
   static constexpr bool kOwnWalk = true;
   static constexpr int kNW = NW;
@@ -256,8 +256,9 @@ struct LdsFp4 {
 
     // A chunk whose first token is t0, of a sequence that ends at tok_end: scores, online softmax (the running max moves
     // when the chunk's exceeds it by more than 8 in log2 units, as in decode_body.h) and P V, one kv head after the other.
-    // `between`: called when the chunk's registers are free.
-    auto compute = [&](Chunk<HK>& T, int t0, int tok_end, auto&& between) {
+    // `between`: called when the chunk's registers are free. SCORES: the scores of its steps, from step t on and below `en`, go
+    // to p.scores as decode_split's do, behind the next chunk's loads.
+    auto compute = [&](Chunk<HK>& T, int t, int en, int t0, int tok_end, auto&& between) {
       if (T.fresh >= 0) take_fresh(T);
       int lim[kSteps];  // tokens of each step that count
 #pragma unroll
@@ -310,6 +311,11 @@ struct LdsFp4 {
         wave_lds_sync();
       };
       store_v(0);
+      float raw[SCORES ? kSteps * 4 : 1];
+      if constexpr (SCORES) {
+#pragma unroll
+        for (int i = 0; i < kSteps * 4; ++i) raw[i] = x[i];
+      }
 
       float tm = x[0];
 #pragma unroll
@@ -336,7 +342,16 @@ struct LdsFp4 {
 #pragma unroll
       for (int g = 0; g < HK; ++g) {
         if (g > 0) store_v(g);
-        if (g == HK - 1) between();
+        if (g == HK - 1) {
+          between();
+          if constexpr (SCORES) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+              if (head_ok && t + s < en)
+                *reinterpret_cast<f32x4*>(p.scores + ((int64_t)(t + s) * p.num_heads + head) * kTile + jq * 4) =
+                    f32x4{raw[4 * s], raw[4 * s + 1], raw[4 * s + 2], raw[4 * s + 3]};
+          }
+        }
         const u32x4 pb = HK == 1 || hg == g ? pv : zero4();
 #pragma unroll
         for (int a = 0; a < 8; ++a) {
@@ -363,7 +378,7 @@ struct LdsFp4 {
         kn = next_seg(k);
         load_q(qv, kn);
       }
-      compute(T, (t - win.st(k)) * kTile, win.ctx(k), [&]() { issue(T); });
+      compute(T, t, en, (t - win.st(k)) * kTile, win.ctx(k), [&]() { issue(T); });
       t += kSteps;
       if (!last) continue;
       const float l = col_sum4(lsum);

@@ -256,8 +256,10 @@ hipError_t launch_decode_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t 
 hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t stream);
 hipError_t launch_decode_merge_fp4(const DecodeArgs& a, hipStream_t stream);
 
-// Decode in weights mode.
+// Decode in weights mode, over bf16 caches and 4-bit ones, and its merge kernel alone.
 hipError_t launch_decode_weights(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
+hipError_t launch_decode_weights_fp4(const DecodeArgs& a, int num_kv_heads, hipStream_t stream);
+hipError_t launch_decode_merge_weights(const DecodeArgs& a, bool fp4, hipStream_t stream);
 
 hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 

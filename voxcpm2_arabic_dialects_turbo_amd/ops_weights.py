@@ -10,9 +10,9 @@ A token that is new in a call starts with what it gets there, whatever its place
 row needs no clearing between the sequences that have it in turn. ``runner.allocate_key_weights`` makes the planes, and
 ``Attention.forward`` adds to its layer's.
 
-The attention itself is that of ``ops`` over bf16 caches. Like its operators these run on torch's current stream of the
-tensors' device, allocate with torch, never synchronize and can be captured into HIP graphs. head_dim 128, softmax_scale
-positive. No reference counterpart.
+The attention itself is that of ``ops`` and, for decode steps, ``ops_fp4``; chunks through a block table take bf16 caches.
+Like their operators these run on torch's current stream of the tensors' device, allocate with torch, never synchronize and
+can be captured into HIP graphs. head_dim 128, softmax_scale positive. No reference counterpart.
 """
 
 from __future__ import annotations
@@ -22,7 +22,7 @@ import torch
 from . import _lib
 from .ops import (HEAD_DIM, MAX_DECODE_HEADS, _as_i32, _check_cuda, _flat, _plan_recorded, _takes_decode_rows,
                   store_kvcache)
-from .ops_fp4 import _ids, _on, _row_stride, _table, _workspace
+from .ops_fp4 import _cache_shape, _ids, _on, _row_stride, _table, _workspace, is_fp4_cache, store_kvcache_fp4
 
 
 def _weights(fn: str, key_weights: torch.Tensor, weight_rows: torch.Tensor | None, batch: int, hk: int, reach: int,
@@ -107,12 +107,16 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     and kv head g the sum of g's query heads' probabilities, on top of the weight for j < context_lens[b] - 1, in its place
     for the newest. Returns o [B, H, 128] bf16, zeros where context_lens[b] is 0 (whose row is left alone).
 
+    Over 4-bit caches (``decode_attention_fp4``'s attention) a score is off by at most 2^-13 of softmax_scale sum |q||k|, so a
+    probability by twice that many parts.
+
     The call takes scratch for the scores of every token that the tables reach, 4 H bytes a token. ``plan``: as
     decode_attention's; planned calls share the device's decode workspace and must not overlap other calls on it."""
     fn = "decode_attention_weights"
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise TypeError(f"{fn}: q must be bf16 [B, H, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
-    blocks, bs, hk = _caches(fn, k_cache, v_cache)
+    fp4 = is_fp4_cache(k_cache) and is_fp4_cache(v_cache)
+    blocks, bs, hk = _cache_shape(k_cache, v_cache) if fp4 else _caches(fn, k_cache, v_cache)
     B, H, D = q.shape
     if hk not in (1, 2) or H == 0 or H % hk or H > MAX_DECODE_HEADS:
         raise ValueError(f"decode supports H <= {MAX_DECODE_HEADS} query heads over 1 or 2 KV heads, got {H}/{hk}")
@@ -144,7 +148,7 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     lib = _lib.load()
     with _on(dev):
         if key is not None and ride[0] is None:
-            store_kvcache(key, value, k_cache, v_cache, slots)
+            (store_kvcache_fp4 if fp4 else store_kvcache)(key, value, k_cache, v_cache, slots)
         need = lib.vox_decode_scores_bytes(B, mb, bs, H)
         mode, recorded = _lib.PLAN_NONE, None
         if plan is None:  # all scratch in one piece: the call's own
@@ -155,10 +159,11 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         else:
             scratch = torch.empty((need,), dtype=torch.uint8, device=dev)
             scores = scratch.data_ptr()
-            kept, mode, recorded = _workspace(lib, dev, B, plan, "decode_weights", ride[0] is not None, B, mb, bt_stride, H,
-                                              hk, bs)
+            kept, mode, recorded = _workspace(lib, dev, B, plan, "decode_weights", fp4, ride[0] is not None, B, mb,
+                                              bt_stride, H, hk, bs)
             ws, ws_bytes = kept.data_ptr(), kept.numel()
-        _lib.check(lib.vox_decode_attn_weights(
+        call = lib.vox_decode_attn_weights_fp4 if fp4 else lib.vox_decode_attn_weights
+        _lib.check(call(
             q.data_ptr(), q_stride, *ride, k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, mb,
             lens.data_ptr(), B, H, hk, D, scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), n_rows,
             width, scores, need, mode, ws, ws_bytes, out.data_ptr(), _lib.stream_handle(dev)), fn)
