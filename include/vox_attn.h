@@ -401,6 +401,17 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
                              size_t scratch_bytes, void* scores, size_t scores_bytes, int plan, void* workspace,
                              size_t workspace_bytes, void* out, int64_t out_row_stride, void* stream);
 
+/* The same over 4-bit caches through a block table, as vox_prefill_attn_fp4; scores as vox_decode_attn_weights_fp4's. */
+int vox_prefill_attn_weights_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                 int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                                 int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                                 int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads,
+                                 int num_kv_heads, int head_dim, float softmax_scale, float* key_weights,
+                                 const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width,
+                                 void* scratch, size_t scratch_bytes, void* scores, size_t scores_bytes, int plan,
+                                 void* workspace, size_t workspace_bytes, void* out, int64_t out_row_stride,
+                                 void* stream);
+
 /* Drops tokens from sequences longer than `budget`: their first `sinks` and last `recent` tokens stay and, in every layer
  * and kv head apart, the budget - sinks - recent heaviest of the others by key_weights (fp32 [num_layers, num_weight_rows,
  * num_kv_heads, weight_width], weight_width >= max_blocks * block_size; of equal ones the earliest, NaN above every number).

@@ -756,3 +756,83 @@ def test_decode_fp4_blocks_that_are_none_take_no_weight():
     want.sequence(q, k, v, ok, 0, 1, more=2 * x * (1 + 2 * x))
     want.check(o, wd)
     assert not ok[64:128].any() and torch.equal(wd[0, :, 64:128].cpu().double(), before[0, :, 64:128])
+
+
+def _varlen_fp4_case(seed, seqs, h, hk, bs, rows=None, drop=(), plan=None):
+    """As _varlen_case through block tables, the tolerances as _decode_fp4_case's."""
+    gen = torch.Generator().manual_seed(seed)
+    lens, T, cu_q, cu_k = [m for _, m in seqs], sum(n for n, _ in seqs), [0], [0]
+    for n, m in seqs:
+        cu_q.append(cu_q[-1] + n)
+        cu_k.append(cu_k[-1] + m)
+    need = sum(-(-n // bs) for n in lens) + 2
+    _, _, tables = paged_pool(gen, lens, need, bs, 1, 1, 1)
+    for b, c in drop:
+        tables[b, c] = -1
+    live = torch.zeros(need * bs, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        live[[int(tables[b, j // bs]) * bs + j % bs for j in range(n) if tables[b, j // bs] >= 0]] = True
+    planes = []
+    for _ in range(2):
+        scales = torch.randint(123, 128, (need * bs, hk, 4), generator=gen, dtype=torch.uint8)
+        scales[~live] = 255
+        planes.append(fp4.plane(torch.randint(0, 256, (need, bs, hk, 64), generator=gen, dtype=torch.uint8),
+                                scales.view(need, bs, hk, 4)))
+    n_rows = len(seqs) if rows is None else max([*rows, 0]) + 2
+    w, q = _received(gen, n_rows, hk, tables.shape[1] * bs + 3), randn(gen, T, h, D)
+    for b, (n, m) in enumerate(seqs):
+        r = b if rows is None else rows[b]
+        if n and 0 <= r < n_rows:
+            w[r, :, max(m - n, 0):m] = float("nan")
+    wd = w.to(DEV)
+    o = varlen_attention_weights(q.to(DEV), None, None, wd, None if rows is None else _i32(rows), cu_seqlens_q=_i32(cu_q),
+                                 cu_seqlens_k=_i32(cu_k), max_seqlen_q=max(n for n, _ in seqs), max_seqlen_k=max(lens),
+                                 softmax_scale=SCALE, block_table=tables.to(DEV), k_cache=planes[0].to(DEV),
+                                 v_cache=planes[1].to(DEV), plan=plan)
+    kv, vv = (fp4.cache_values(c) for c in planes)
+    want = Want(w)
+    for b, (n, m) in enumerate(seqs):
+        (k, ok), (v, _) = (ref.keys_of(c, tables[b], m) for c in (kv, vv))
+        x, qb = 0.0, q[cu_q[b]:cu_q[b + 1]]
+        if n and m:
+            size = (qb.double().abs().view(n, hk, -1, D).transpose(0, 1).reshape(hk, -1, D) @ k.abs().permute(1, 2, 0)).max()
+            x = SCALE * float(2.0 ** -13 * size + 2.0 ** -18 * qb.abs().max() * k.abs().sum(-1).max())
+        want.sequence(qb, k, v, ok, b if rows is None else rows[b], n, more=2 * x * (1 + 2 * x))
+    want.check(o, wd)
+
+
+@pytest.mark.parametrize("h,hk", [(16, 2), (8, 1), (4, 4), (32, 4), (16, 1), (64, 1)])
+@pytest.mark.parametrize("bs", [64, 256, 192])
+def test_chunks_over_fp4_prefixes(h, hk, bs):
+    """Chunks over prefixes of none to several blocks, a sequence without queries, one with fewer keys than queries, rows of
+    any order, one of them none, blocks that are none."""
+    seqs = [(5, 55), (1, 1), (1, 300), (0, 130), (33, 33), (64, 257), (17, 11), (100, 420), (3, 64)]
+    gen = torch.Generator().manual_seed(h + bs)
+    rows = torch.randperm(len(seqs) + 3, generator=gen)[:len(seqs)].tolist()
+    rows[1] = -1
+    _varlen_fp4_case(80 + h + hk + bs, seqs, h, hk, bs, rows, drop=[(7, 0)] if bs < 256 else [])
+
+
+@pytest.mark.parametrize("seqs,h,hk", [
+    ([(700, 2300), (1, 1801)], 16, 2), ([(44, 94)] * 44, 16, 2), ([(1100, 1100)] * 3 + [(513, 700)], 16, 2), ([(1, 1)], 8, 1),
+    ([(1, 5 + 37 * i) for i in range(20)] + [(90, 90), (0, 50), (130, 400), (1, 1)], 16, 2),
+    ([(1, 5 + 37 * i) for i in range(20)] + [(90, 90), (0, 50), (130, 400), (1, 1)], 8, 1),
+    ([(1, 1 + i % 70) for i in range(600)], 8, 1), ([(40, 20000)], 16, 2), ([(1300, 1300)], 8, 1)])
+def test_chunk_fp4_sizes(seqs, h, hk):
+    _varlen_fp4_case(len(seqs) + h, seqs, h, hk, 256)
+    _varlen_fp4_case(len(seqs) + h, seqs, h, hk, 64, plan=("fp4 chunk", len(seqs), h))
+
+
+def test_chunk_fp4_groups_that_are_not_numbers():
+    """A key's group without a number, at a cached token: NaN wherever a query sees it, and nowhere else."""
+    gen = torch.Generator().manual_seed(91)
+    codes = torch.randint(0, 256, (2, 4, 64, 2, 64), generator=gen, dtype=torch.uint8)
+    scales = torch.randint(123, 128, (2, 4, 64, 2, 4), generator=gen, dtype=torch.uint8)
+    scales[0, 0, 50, 1, 2] = 255  # token 50's key, kv head 1
+    planes = [fp4.plane(c, s) for c, s in zip(codes, scales)]
+    w = torch.zeros(1, 2, 256, device=DEV)
+    o = varlen_attention_weights(randn(gen, 60, 16, D).to(DEV), None, None, w, cu_seqlens_q=_i32([0, 60]),
+                                 cu_seqlens_k=_i32([0, 60]), max_seqlen_q=60, max_seqlen_k=60, softmax_scale=SCALE,
+                                 block_table=_i32([[0, 1]]), k_cache=planes[0].to(DEV), v_cache=planes[1].to(DEV))
+    assert w[0, 0, :60].isfinite().all() and o[:, :8].isfinite().all() and o[:50, 8:].isfinite().all()
+    assert o[50:, 8:].isnan().all() and w[0, 1, :51].isnan().all()

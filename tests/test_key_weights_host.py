@@ -192,7 +192,7 @@ def test_attention_adds_where_the_layer_has_weights_and_the_step_rows(calls):
     assert calls[0][1][-2] is layer.key_weights and calls[0][2]["slot_mapping"].tolist() == [0, 256]
 
 
-def test_attention_over_4_bit_caches_adds_only_over_the_steps_own_rows(calls):
+def test_attention_over_4_bit_caches_adds_too(calls):
     i32 = lambda *x: torch.tensor(x, dtype=I32)  # noqa: E731
     layer = _layer(fp4=True)
     layer.key_weights = torch.zeros(1, 2, 256)
@@ -201,9 +201,9 @@ def test_attention_over_4_bit_caches_adds_only_over_the_steps_own_rows(calls):
     assert [c[0] for c in calls] == ["store_kvcache", "varlen_attention_weights"]
     calls.clear()
     set_context(True, i32(0, 3), i32(0, 3), 3, 3, i32(0, 1, 2), None, i32(0).view(1, 1), i32(0))
-    with pytest.raises(TypeError, match="bf16 caches"):
-        layer(*_rows(3))
-    assert not calls  # (nothing stored)
+    layer(*_rows(3))
+    assert [c[0] for c in calls] == ["store_kvcache", "varlen_attention_weights"]
+    assert calls[1][2]["k_cache"] is layer.k_cache and calls[1][2]["block_table"] is not None
 
 
 def test_eviction_violations():
@@ -309,8 +309,8 @@ def test_decode_rows_refusals(monkeypatch):
      "multiple of 64"),
     (dict(block_table=torch.zeros(1, 1, dtype=I32), k_cache=torch.zeros(4, 64, 2, 128, dtype=BF16)), ValueError,
      "block_table must be"),
-    (dict(block_table=torch.zeros(2, 1, dtype=I32), k_cache=torch.zeros(4, 64, 2, 68, dtype=torch.uint8)), TypeError,
-     "bf16 caches"),
+    (dict(block_table=torch.zeros(2, 1, dtype=I32), k_cache=torch.zeros(4, 64, 2, 68, dtype=torch.uint8),
+          v_cache=torch.zeros(4, 64, 2, 128, dtype=BF16)), TypeError, "bf16 caches"),
     (dict(max_seqlen_k=129), ValueError, "the keys may be 129"),
     (dict(key_weights=torch.zeros(1, 2, 128)), ValueError, "1 rows for 2"),
     (dict(out=torch.zeros(4, 16, 128)), ValueError, "out must be"),
@@ -322,7 +322,7 @@ def test_varlen_refusals(monkeypatch, kw, error, match):
              cu_seqlens_k=torch.zeros(3, dtype=I32), max_seqlen_q=3, max_seqlen_k=3, softmax_scale=0.1)
     a.update(kw)
     if "k_cache" in a:
-        a["v_cache"] = a["k_cache"]
+        a.setdefault("v_cache", a["k_cache"])
     with pytest.raises(error, match=match):
         varlen_attention_weights(**a)
 
@@ -421,6 +421,27 @@ PAGED = dict(key=None, value=None, ks=0, vs=0, kc=P, vc=P, blocks=4, bs=64, bt=P
 ])
 def test_c_prefill_refusals(kw, match):
     _einval(_lib.load().vox_prefill_attn_weights(*{**PREFILL_C, **kw}.values()), match)
+
+
+FP4 = [(dict(bs=96), "multiple of 64"), (dict(d=64), "head_dim"), (dict(kc=None), "null pointer"), (dict(vc=P + 8), "aligned"),
+       (dict(blocks=0), "empty cache"), (dict(blocks=1 << 26), "int32 slots"), (dict(scale=1e-45), "positive"),
+       (dict(w=None), "key_weights"), (dict(batch=-1), "batch")]
+
+
+@pytest.mark.parametrize("kw,match", FP4 + [(dict(scores=None), "scores"), (dict(plan=7), "plan mode"),
+                                            (dict(key=P), "go together"), (dict(hk=3, h=3), "num_kv_heads")])
+def test_c_decode_fp4_refusals(kw, match):
+    _einval(_lib.load().vox_decode_attn_weights_fp4(*{**DECODE_C, **kw}.values()), match)
+
+
+@pytest.mark.parametrize("kw,match", FP4 + [
+    (dict(bt=None), "null pointer"), (dict(scratch_bytes=8 * 16 * 4 - 1), "needed"), (dict(mk=-1), "negative"),
+    (dict(ws=P, ws_bytes=10), "workspace"), (dict(ws=P, ws_bytes=1 << 30), "scores"), (dict(outs=100), "out row stride")])
+def test_c_prefill_fp4_refusals(kw, match):
+    args = {**PREFILL_C, **PAGED, **kw}
+    for name in ("key", "value", "ks", "vs"):
+        del args[name]
+    _einval(_lib.load().vox_prefill_attn_weights_fp4(*args.values()), match)
 
 
 def test_c_prefill_of_nothing():

@@ -350,3 +350,32 @@ def test_a_text_over_4_bit_caches():
             new, left = evict_kv_tokens(kv, weights, _i32(tables), _i32(lens), 100, recent=20, sinks=4, weight_rows=_i32(rows))
             assert left.tolist() == [100, lens[1]]
             tasks[0].block_table, tasks[0].seq_length = [b for b in new[0].tolist() if b >= 0], 100
+
+
+def test_a_chunk_over_what_an_eviction_left_in_a_4_bit_cache():
+    """A prompt, an eviction, a chunk and a mixed step behind it through the module: as the calls over the same cache."""
+    gen = torch.Generator().manual_seed(8)
+    layer = Attention(H, D, SCALE, HK)
+    kv = runner.allocate_kv_cache([layer], 12, BS, dtype=getattr(torch, "float4_e2m1fn_x2", torch.uint8), device=DEV)
+    weights = runner.allocate_key_weights([layer], 5, 1024, device=DEV)
+    rows = lambda n: (randn(gen, n, H, D).to(DEV), randn(gen, n, HK, D).to(DEV), randn(gen, n, HK, D).to(DEV))  # noqa: E731
+    runner.prepare_prefill_context([runner.RunnerTask([0, 1, 2], 700, 0)], BS, device=DEV, weight_rows=[2])
+    layer(*rows(700))
+    new, left = evict_kv_tokens(kv, weights, _i32([[0, 1, 2]]), _i32([700]), 300, recent=50, sinks=4, weight_rows=_i32([2]))
+    assert new.tolist() == [[0, 1, -1]] and left.tolist() == [300]
+    steps = [([runner.RunnerTask([0, 1], 380, 300)], [2]),
+             ([runner.RunnerTask([0, 1], 381, 380)] + [runner.RunnerTask([3 + i], 1, 0) for i in range(6)] +
+              [runner.RunnerTask([9], 60, 0)], [2, 0, 1, -1, -1, -1, -1, 4])]
+    for tasks, where in steps:
+        runner.prepare_prefill_context(tasks, BS, device=DEV, weight_rows=where, evicted=[400] + [0] * (len(tasks) - 1),
+                                       graphs=True)
+        ctx, (q, k, v) = get_context(), rows(sum(t.seq_length - t.num_cached_tokens for t in tasks))
+        kv2, w2 = kv[0].clone(), weights[0].clone()
+        o = layer(q, k, v)
+        ops.store_kvcache(k, v, kv2[0], kv2[1], ctx.slot_mapping)
+        o2 = varlen_attention_weights(q, None, None, w2, ctx.weight_rows, cu_seqlens_q=ctx.cu_seqlens_q,
+                                      cu_seqlens_k=ctx.cu_seqlens_k, max_seqlen_q=ctx.max_seqlen_q,
+                                      max_seqlen_k=ctx.max_seqlen_k, softmax_scale=SCALE, block_table=ctx.block_tables,
+                                      k_cache=kv2[0], v_cache=kv2[1])
+        assert torch.equal(o.reshape(o2.shape), o2) and torch.equal(kv[0], kv2) and torch.equal(weights[0], w2)
+        assert o2.isfinite().all() and weights[0, 2, :, :380].isfinite().all() and (weights[0, 2, :, 300:380] > 0).all()

@@ -54,6 +54,7 @@ EXPORTS = (
     "vox_decode_attn_weights_fp4",
     "vox_prefill_weights_bytes",
     "vox_prefill_attn_weights",
+    "vox_prefill_attn_weights_fp4",
     "vox_evict_kv_tokens",
 )
 
@@ -128,6 +129,10 @@ _SIGNATURES = {
                                         _i32, _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _i64,
                                         _i32, _i32, _i32, _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size,
                                         _c_void_p, _size, _i32, _c_void_p, _size, _c_void_p, _i64, _c_void_p]),
+    "vox_prefill_attn_weights_fp4": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64, _i32,
+                                            _c_void_p, _c_void_p, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _f32,
+                                            _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p, _size, _i32,
+                                            _c_void_p, _size, _c_void_p, _i64, _c_void_p]),
     "vox_evict_kv_tokens": (_i32, [_c_void_p, _i64, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32,
                                    _c_void_p, _c_void_p, _i64, _i64, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p,
                                    _c_void_p, _c_void_p, _c_void_p]),

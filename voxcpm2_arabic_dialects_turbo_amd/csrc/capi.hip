@@ -1169,7 +1169,10 @@ size_t vox_prefill_weights_bytes(int64_t num_tokens, int batch, int max_seqlen_q
   return weights_scratch(num_tokens, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads).total;
 }
 
-int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+}  // extern "C"
+
+namespace {
+int prefill_attn_weights(const char* fn, bool fp4, const void* q, int64_t q_row_stride, const void* key, const void* value,
                              int64_t key_row_stride, int64_t value_row_stride, const void* k_cache, const void* v_cache,
                              int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                              int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
@@ -1178,7 +1181,6 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
                              int64_t num_weight_rows, int64_t weight_width, void* scratch,
                              size_t scratch_bytes, void* scores, size_t scores_bytes, int plan, void* workspace,
                              size_t workspace_bytes, void* out, int64_t out_row_stride, void* stream) {
-  const char* fn = "prefill_attn_weights";
   if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_tokens < 0)
     return fail(VOX_EINVAL, "%s: negative batch, max_seqlen_q, max_seqlen_k or num_tokens", fn);
   if (batch == 0 || max_seqlen_q == 0 || num_tokens == 0) return VOX_OK;
@@ -1193,6 +1195,12 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
     return fail(VOX_EINVAL, "%s: block_size %d must be a positive multiple of 64", fn, block_size);
   if (block_tables && (int64_t)max_blocks * block_size > (1 << 30))
     return fail(VOX_EINVAL, "%s: block table too wide", fn);
+  if (fp4) {
+    if (!block_tables) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+    st = fp4_cache(fn, k_cache, v_cache, num_blocks, block_size, num_kv_heads, head_dim);
+    if (st == VOX_OK) st = fp4_softmax(fn, softmax_scale);
+    if (st != VOX_OK) return st;
+  }
   vox::KeyWeightsArgs k{};
   st = prefill_setup(fn, q, q_row_stride, key, value, key_row_stride, value_row_stride, k_cache, v_cache, num_blocks,
                      block_size, block_tables, bt_stride, max_blocks, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, 0, 0,
@@ -1209,6 +1217,7 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   const WeightsScratch ws = weights_scratch(num_tokens, max_seqlen_q, max_seqlen_k, num_heads, num_kv_heads);
   if (!scratch || !aligned16(scratch) || scratch_bytes < ws.total)
     return fail(VOX_EINVAL, "%s: scratch of %zu bytes (16-byte aligned), %zu needed", fn, scratch_bytes, ws.total);
+  k.fp4 = fp4;
   k.a.lse = (float*)scratch;
   k.weights = key_weights;
   k.rows = weight_rows;
@@ -1238,11 +1247,51 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
   }
   const hipStream_t s = (hipStream_t)stream;
   if (!decodes || max_seqlen_q > 1) {
-    st = hip_status(vox::launch_prefill_lse(k.a, max_seqlen_q, s), "prefill_attn_weights launch");
+    st = hip_status((fp4 ? vox::launch_prefill_lse_fp4 : vox::launch_prefill_lse)(k.a, max_seqlen_q, s),
+                    "prefill_attn_weights launch");
     if (st == VOX_OK) st = hip_status(vox::launch_key_weights(k, s), "prefill_attn_weights sums launch");
     if (st != VOX_OK) return st;
   }
-  return decodes ? launch_decode_slices(d, batch, num_kv_heads, plan, workspace, s, vox::launch_decode_weights) : VOX_OK;
+  return decodes ? launch_decode_slices(d, batch, num_kv_heads, plan, workspace, s,
+                                        fp4 ? vox::launch_decode_weights_fp4 : vox::launch_decode_weights)
+                 : VOX_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* key, const void* value,
+                             int64_t key_row_stride, int64_t value_row_stride, const void* k_cache, const void* v_cache,
+                             int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                             int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                             int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads, int num_kv_heads,
+                             int head_dim, float softmax_scale, float* key_weights, const int32_t* weight_rows,
+                             int64_t num_weight_rows, int64_t weight_width, void* scratch,
+                             size_t scratch_bytes, void* scores, size_t scores_bytes, int plan, void* workspace,
+                             size_t workspace_bytes, void* out, int64_t out_row_stride, void* stream) {
+  return prefill_attn_weights("prefill_attn_weights", false, q, q_row_stride, key, value, key_row_stride,
+                              value_row_stride, k_cache, v_cache, num_blocks, block_size, block_tables, bt_stride,
+                              max_blocks, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, max_seqlen_k, num_tokens,
+                              num_heads, num_kv_heads, head_dim, softmax_scale, key_weights, weight_rows,
+                              num_weight_rows, weight_width, scratch, scratch_bytes, scores, scores_bytes, plan,
+                              workspace, workspace_bytes, out, out_row_stride, stream);
+}
+
+int vox_prefill_attn_weights_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                 int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                                 int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                                 int max_seqlen_q, int max_seqlen_k, int64_t num_tokens, int num_heads,
+                                 int num_kv_heads, int head_dim, float softmax_scale, float* key_weights,
+                                 const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width,
+                                 void* scratch, size_t scratch_bytes, void* scores, size_t scores_bytes, int plan,
+                                 void* workspace, size_t workspace_bytes, void* out, int64_t out_row_stride,
+                                 void* stream) {
+  return prefill_attn_weights("prefill_attn_weights_fp4", true, q, q_row_stride, nullptr, nullptr, 0, 0, k_cache,
+                              v_cache, num_blocks, block_size, block_tables, bt_stride, max_blocks, cu_seqlens_q,
+                              cu_seqlens_k, batch, max_seqlen_q, max_seqlen_k, num_tokens, num_heads, num_kv_heads,
+                              head_dim, softmax_scale, key_weights, weight_rows, num_weight_rows, weight_width,
+                              scratch, scratch_bytes, scores, scores_bytes, plan, workspace, workspace_bytes, out,
+                              out_row_stride, stream);
 }
 
 int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_bytes,

@@ -18,6 +18,7 @@
 // (44 chunks of 33-59 over 50: 9.8 us).
 #include <type_traits>
 
+#include "fp4_common.h"
 #include "prefill_tile32.h"
 #include "vox_common.h"
 #include "vox_kernels.h"
@@ -130,8 +131,9 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
 
 // Persistent: the items (128 keys, a part of the query rows, kv head, sequence), the key blocks of a part side by side, are
 // dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2. DIRECT, where the grid of
-// all there may be is small: a workgroup for each, without the items' layout.
-template <bool DIRECT, int KT>
+// all there may be is small: a workgroup for each, without the items' layout. FP4: the keys come from a 4-bit cache, as bf16,
+// which holds their values exactly.
+template <bool DIRECT, int KT, bool FP4>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   constexpr int KW = 2, QW = 2;
   constexpr int KEYS = 32 * KT;               // keys of a wave
@@ -304,20 +306,42 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
     for (int kt = 0; kt < KT; ++kt) {
       const int j = jb + 32 * kt + col;
       bool ok = j < s.nk;
-      const uint16_t* kr;
+      const uint16_t* kr = nullptr;
+      const uint8_t *block = nullptr, *code = nullptr;
+      int in = 0;
       if (!paged) {
         kr = p.k_src + ((int64_t)s.k0 + (ok ? j : 0)) * p.k_row_stride + g * kKwD;
       } else {
         ok = ok && j < p.max_blocks * p.block_size;
         const int bid = p.block_tables[(int64_t)b * p.bt_stride + (ok ? j / p.block_size : 0)];
         ok = ok && bid >= 0 && bid < p.num_blocks;
-        kr = p.k_cache + (((int64_t)(ok ? bid : 0) * p.block_size + j % p.block_size) * HK + g) * kKwD;
+        if constexpr (FP4) {
+          in = j % p.block_size;
+          block = reinterpret_cast<const uint8_t*>(p.k_cache) + (ok ? bid : 0) * fp4::block_bytes(p.block_size, HK);
+          code = block + (int64_t)(in * HK + g) * fp4::kHeadCodes;
+        } else {
+          kr = p.k_cache + (((int64_t)(ok ? bid : 0) * p.block_size + j % p.block_size) * HK + g) * kKwD;
+        }
       }
       counts |= (uint64_t)(uint32_t)__builtin_amdgcn_ballot_w64(ok) << (32 * kt);
+      if constexpr (FP4) {  // chunk i's 4 bytes: word 2 (i % 2) + h of the 32 channels i / 2
+        u32x4 codes[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const u32x4 v = ld_g16(kr + 16 * i + 8 * h);
-        kf[kt][i] = ok ? v : zero4();
+        for (int i = 0; i < 4; ++i) codes[i] = *reinterpret_cast<const u32x4*>(code + 16 * i);
+        const uint32_t scale = *reinterpret_cast<const uint32_t*>(block + (int64_t)p.block_size * HK * fp4::kHeadCodes +
+                                                                  (in * HK + g) * fp4::kHeadScales);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const u32x4 c4 = codes[i / 2];
+          const u32x4 v = fp4::values8(h ? c4[2 * (i & 1) + 1] : c4[2 * (i & 1)], fp4::scale_float((scale >> (8 * (i / 2))) & 0xffu));
+          kf[kt][i] = ok ? v : zero4();
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const u32x4 v = ld_g16(kr + 16 * i + 8 * h);
+          kf[kt][i] = ok ? v : zero4();
+        }
       }
     }
     arrive();
@@ -407,6 +431,14 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   *out = j >= s.old ? got : *out + got;
 }
 
+template <bool DIRECT, int KT>
+void launch_sums(const KeyWeightsArgs& k, int64_t grid, hipStream_t stream) {
+  if (k.fp4)
+    key_weights_kernel<DIRECT, KT, true><<<dim3((unsigned)grid), dim3(256), 0, stream>>>(k);
+  else
+    key_weights_kernel<DIRECT, KT, false><<<dim3((unsigned)grid), dim3(256), 0, stream>>>(k);
+}
+
 template <int RG, int KS, bool WALK>
 hipError_t launch_lse(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
   const dim3 block(64 * RG * KS);
@@ -471,7 +503,7 @@ hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
   KeyWeightsArgs k = k0;
   if (k.max_k <= 0 || k.a.batch <= 0) return hipSuccess;
   if (!k.a.lse || !k.weights || !k.a.cu_q || !k.a.cu_k || k.a.row_limit <= 0 || k.max_q <= 0 || k.part_rows <= 0 || k.part_rows % 128 ||
-      (k.max_parts > 1 && !k.partials))
+      (k.max_parts > 1 && !k.partials) || (k.fp4 && !k.a.block_tables))
     return hipErrorInvalidValue;
   const int batch = k0.a.batch;
   for (int b0 = 0; b0 < batch; b0 += kMaxSeqPerLaunch) {  // (the sequences' items are laid out in LDS)
@@ -491,11 +523,12 @@ hipError_t launch_key_weights(const KeyWeightsArgs& k0, hipStream_t stream) {
     k.item_shift = items <= 256 ? 6 : 7;
     if (items <= 256) {
       items = ((int64_t)k.max_k + 63) / 64 * k.max_parts * k.a.batch * k.a.num_kv_heads;
-      key_weights_kernel<true, 1><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
-    } else if (items <= 1536)  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> 19.2 us)
-      key_weights_kernel<true, 2><<<dim3((unsigned)items), dim3(256), 0, stream>>>(k);
-    else  // two workgroups a CU
-      key_weights_kernel<false, 2><<<dim3(512), dim3(256), 0, stream>>>(k);
+      launch_sums<true, 1>(k, items, stream);
+    } else if (items <= 1536) {  // (5 prompts of 237-900 tokens, 1200 of them: 23.2 -> 19.2 us)
+      launch_sums<true, 2>(k, items, stream);
+    } else {  // two workgroups a CU
+      launch_sums<false, 2>(k, 512, stream);
+    }
     if (k.max_parts > 1)
       key_weights_sum_kernel<<<dim3((unsigned)((k.max_k + 255) / 256), (unsigned)k.a.batch, (unsigned)k.a.num_kv_heads),
                                dim3(256), 0, stream>>>(k);

@@ -58,8 +58,8 @@ struct Lds {
   int* nan_at;    // [2]: the first key of the last tile that held any
 };
 
-// Query tile qt of sequence b and kv head g.
-template <int KS>
+// Query tile qt of sequence b and kv head g. LSE: every row's log2 of the sum its output is divided by goes to p.lse.
+template <int KS, bool LSE = false>
 __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g, int qt, const Lds& L) {
   uint8_t* const s_t0 = L.t0;
   uint8_t* const s_t1 = L.t1;
@@ -396,6 +396,7 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
     const float top = fmaxf(m, x[0]), mu = top == -INFINITY ? 0.f : top;
     const float a0 = fast_exp2(m - mu), a1 = fast_exp2(x[0] - mu);
     l = l * a0 + x[1] * a1;
+    if constexpr (LSE) m = top;
     nan_groups |= __float_as_uint(x[2]);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
@@ -407,6 +408,10 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
           acc[dt][4 * i + j] = (kh == 0 ? acc[dt][4 * i + j] : acc[2 + dt][4 * i + j]) * a0 + y[j] * a1;
       }
     __syncthreads();
+  }
+  if constexpr (LSE) {
+    if (h == 0 && kh == 0 && tq < nq && row >= 0 && row < p.row_limit)
+      p.lse[row * p.num_heads + head] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row that sees no key: zeros
   uint16_t* const so = L.v + rg * 32 * kORow;
@@ -434,15 +439,15 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& p, int b, int g,
   }
 }
 
-template <int KS>
+template <int KS, bool LSE>
 __global__ __launch_bounds__(256, 2) void prefill_fp4_kernel(PrefillArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t s_v[2 * kBK * kVRow];
   __shared__ __attribute__((aligned(16))) uint8_t s_t0[2 * kTileBytes], s_t1[2 * kTileBytes];
   __shared__ __attribute__((aligned(4))) uint8_t s_nan[2 * kBK * 4];
   __shared__ int s_nan_at[2];
   // the last tile has the most keys: first
-  prefill_item<KS>(p, (int)blockIdx.y, (int)blockIdx.z, (int)gridDim.x - 1 - (int)blockIdx.x,
-                   Lds{s_v, s_t0, s_t1, s_nan, s_nan_at});
+  prefill_item<KS, LSE>(p, (int)blockIdx.y, (int)blockIdx.z, (int)gridDim.x - 1 - (int)blockIdx.x,
+                        Lds{s_v, s_t0, s_t1, s_nan, s_nan_at});
 }
 
 // ---- steps that mix prompts with decode rows, in one launch: workgroups [0, da.grid) are the decode split of the one-query
@@ -548,7 +553,8 @@ hipError_t launch_mixed_fp4(const PrefillArgs& a, int max_seqlen_q, const Decode
   return launch_decode_merge_fp4(d, stream);
 }
 
-hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream) {
+template <bool LSE>
+static hipError_t launch_prefill_fp4_form(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream) {
   // Two waves on the same rows where the launch is at most half a workgroup a compute unit: the chain of tiles is then the
   // time (16 query heads of 2 kv heads, KS = 1 | 2: 1000 tokens over 2000 cached, 126 workgroups of 128 rows, 58.6 | 47.6 us;
   // 4 x 200 over 2000, 104: 44.9 | 36.8; 100 over 300, 14: 13.4 | 11.9). From there on 64-row workgroups stage and convert
@@ -558,10 +564,20 @@ hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_
   const int bq_ks = (two ? 64 : 128) / a.group;
   const dim3 grid((unsigned)((max_seqlen_q + bq_ks - 1) / bq_ks), (unsigned)a.batch, (unsigned)a.num_kv_heads);
   if (two)
-    pf4::prefill_fp4_kernel<2><<<grid, dim3(256), 0, stream>>>(a);
+    pf4::prefill_fp4_kernel<2, LSE><<<grid, dim3(256), 0, stream>>>(a);
   else
-    pf4::prefill_fp4_kernel<1><<<grid, dim3(256), 0, stream>>>(a);
+    pf4::prefill_fp4_kernel<1, LSE><<<grid, dim3(256), 0, stream>>>(a);
   return hipGetLastError();
+}
+
+hipError_t launch_prefill_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream) {
+  return launch_prefill_fp4_form<false>(a, max_seqlen_q, stream);
+}
+
+hipError_t launch_prefill_lse_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream) {
+  if (max_seqlen_q <= 0 || a.batch <= 0) return hipSuccess;
+  if (!a.lse || !a.causal) return hipErrorInvalidValue;
+  return launch_prefill_fp4_form<true>(a, max_seqlen_q, stream);
 }
 
 }  // namespace vox

@@ -135,6 +135,7 @@ struct PrefillArgs {
 // What the keys of a varlen call received (launch_key_weights), after launch_prefill_lse of the same call has left a.lse.
 struct KeyWeightsArgs {
   PrefillArgs a;              // cu_q, cu_k; packed keys or paged ones
+  bool fp4;                   // paged keys: of a 4-bit cache
   float* weights;             // fp32 [row_count, HK, width]
   const int32_t* rows;        // int32 [batch], or null: row b + row0 (outside [0, row_count): none)
   int64_t row0;
@@ -265,6 +266,7 @@ hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t st
 
 // Causal varlen attention that also leaves every row's a.lse, then what the keys received (key_weights.hip).
 hipError_t launch_prefill_lse(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
+hipError_t launch_prefill_lse_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 hipError_t launch_key_weights(const KeyWeightsArgs& k, hipStream_t stream);
 int key_weights_part_rows(int64_t num_tokens, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads);
 

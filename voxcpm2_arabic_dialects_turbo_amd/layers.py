@@ -18,8 +18,8 @@ decode steps and prefills through block tables attend over what the caches then 
 the step's own rows).
 
 A layer with ``key_weights`` (fp32 [rows, HK, width], see ops_weights; ``runner.allocate_key_weights`` sets them) adds to
-them what the step's attention gives every key, in every step whose context has ``weight_rows``; its bf16 caches and outputs
-are those of the step without (a step over 4-bit caches adds only in a prefill over its own rows, and is refused else).
+them what the step's attention gives every key, in every step whose context has ``weight_rows``; its caches are those of the
+step without, its outputs too but for the order of a prefill's sums.
 
 Every branch runs a HIP kernel of libvoxattn.so; nothing here synchronizes or allocates outside torch, so the
 module can be captured into HIP graphs exactly where the reference captures its decode step.
@@ -195,8 +195,6 @@ class Attention(nn.Module):
             return decode_attention_weights(q, k_cache, v_cache, context.context_lens, tables, self.scale,
                                             self.key_weights, context.weight_rows, key=k, value=v,
                                             slot_mapping=context.slot_mapping, plan=_plan_key(context)).unsqueeze(1)
-        if tables is not None and is_fp4_cache(k_cache):  # (refused before anything is stored)
-            raise TypeError("key_weights: attention through block tables takes bf16 caches")
         store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
         return varlen_attention_weights(q, k, v, self.key_weights, context.weight_rows, cu_seqlens_q=context.cu_seqlens_q,
                                         cu_seqlens_k=context.cu_seqlens_k, max_seqlen_q=context.max_seqlen_q,

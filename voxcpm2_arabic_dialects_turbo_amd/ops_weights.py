@@ -10,9 +10,10 @@ A token that is new in a call starts with what it gets there, whatever its place
 row needs no clearing between the sequences that have it in turn. ``runner.allocate_key_weights`` makes the planes, and
 ``Attention.forward`` adds to its layer's.
 
-The attention itself is that of ``ops`` and, for decode steps, ``ops_fp4``; chunks through a block table take bf16 caches.
-Like their operators these run on torch's current stream of the tensors' device, allocate with torch, never synchronize and
-can be captured into HIP graphs. head_dim 128, softmax_scale positive. No reference counterpart.
+The attention itself is that of ``ops``, or over 4-bit caches of ``ops_fp4``. There a score is off by at most 2^-13 of
+softmax_scale sum |q||k|, so a probability by at most twice that many parts of it. Like their operators these run on torch's
+current stream of the tensors' device, allocate with torch, never synchronize and can be captured into HIP graphs. head_dim
+128, softmax_scale positive. No reference counterpart.
 """
 
 from __future__ import annotations
@@ -72,7 +73,7 @@ def _caches(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int,
     """(num_blocks, block_size, HK) of a pair of bf16 caches."""
     shape = k_cache.shape
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
-        raise TypeError(f"{fn} takes bf16 caches, got {k_cache.dtype} and {v_cache.dtype}")
+        raise TypeError(f"{fn} takes bf16 caches or 4-bit ones, got {k_cache.dtype} and {v_cache.dtype}")
     if len(shape) != 4 or shape[3] != HEAD_DIM or v_cache.shape != shape or not (k_cache.is_contiguous()
                                                                                 and v_cache.is_contiguous()):
         raise ValueError(f"{fn}: caches must be contiguous [num_blocks, block_size, HK, {HEAD_DIM}] of one shape")
@@ -106,9 +107,6 @@ def decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     slot_mapping the step's rows stored in the same call), adding to ``key_weights`` what every key received: for token j
     and kv head g the sum of g's query heads' probabilities, on top of the weight for j < context_lens[b] - 1, in its place
     for the newest. Returns o [B, H, 128] bf16, zeros where context_lens[b] is 0 (whose row is left alone).
-
-    Over 4-bit caches (``decode_attention_fp4``'s attention) a score is off by at most 2^-13 of softmax_scale sum |q||k|, so a
-    probability by twice that many parts.
 
     The call takes scratch for the scores of every token that the tables reach, 4 H bytes a token. ``plan``: as
     decode_attention's; planned calls share the device's decode workspace and must not overlap other calls on it."""
@@ -201,7 +199,8 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
     if block_table is not None:
         if k_cache is None or v_cache is None:
             raise ValueError(f"{fn}: block_table given without caches")
-        blocks, bs, hk = _caches(fn, k_cache, v_cache)
+        fp4 = is_fp4_cache(k_cache) and is_fp4_cache(v_cache)
+        blocks, bs, hk = _cache_shape(k_cache, v_cache) if fp4 else _caches(fn, k_cache, v_cache)
         if bs % 64:
             raise ValueError(f"{fn}: cache blocks must be a multiple of 64 tokens, got {bs}")
         if block_table.dim() != 2 or block_table.shape[0] < B:
@@ -209,7 +208,9 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         _check_cuda(q, k_cache, v_cache, block_table)
         bt, bt_stride = _table(block_table)
         reach = min(int(max_seqlen_k), bt.shape[1] * bs)
-        keys = (None, None, 0, 0, k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, bt.shape[1])
+        keys = (k_cache.data_ptr(), v_cache.data_ptr(), blocks, bs, bt.data_ptr(), bt_stride, bt.shape[1])
+        if not fp4:
+            keys = (None, None, 0, 0, *keys)
     else:
         if k is None or v is None:
             raise ValueError(f"{fn}: packed keys and values required without a block table")
@@ -217,6 +218,7 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         hk = k.shape[1] if k.dim() == 3 else 0
         k, v = _new_rows(fn, k, v, hk)
         reach = int(max_seqlen_k)
+        fp4 = False
         keys = (k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), None, None, 0, 0, None, 0, 0)
     if hk == 0 or H == 0 or H % hk:
         raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {hk}")
@@ -233,11 +235,12 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         ws, scores_bytes, mode, recorded = None, 0, _lib.PLAN_NONE, None
         if block_table is not None and (max_seqlen_q == 1 or 4 * T <= B * max_seqlen_q) \
                 and _takes_decode_rows(H, hk, bs, bt.shape[1], out, _row_stride(out)):
-            ws, mode, recorded = _workspace(lib, dev, B, plan, "varlen_weights", B, bt.shape[1], bt_stride, H, hk, bs)
+            ws, mode, recorded = _workspace(lib, dev, B, plan, "varlen_weights", fp4, B, bt.shape[1], bt_stride, H, hk, bs)
             scores_bytes = lib.vox_decode_scores_bytes(B, bt.shape[1], bs, H)
         scratch = torch.empty((scores_at + scores_bytes,), dtype=torch.uint8, device=dev)
         at = scratch.data_ptr()
-        _lib.check(lib.vox_prefill_attn_weights(
+        call = lib.vox_prefill_attn_weights_fp4 if fp4 else lib.vox_prefill_attn_weights
+        _lib.check(call(
             q.data_ptr(), q_stride, *keys, cu_q.data_ptr(), cu_k.data_ptr(), B, max_seqlen_q, reach, T, H, hk, D,
             scale, key_weights.data_ptr(), None if rows is None else rows.data_ptr(), n_rows, width, at, need,
             at + scores_at if scores_bytes else None, scores_bytes, mode, None if ws is None else ws.data_ptr(),
