@@ -73,12 +73,31 @@ __device__ __forceinline__ void quantise8(u32x4 x, uint32_t& codes, uint32_t& b)
   codes = b == 255u ? 0u : codes8(x, scale_float(b));
 }
 
-// 8 codes to 8 bf16 (packed): exact, a 2-bit significand and the scale's exponent.
+// 8 codes to 8 bf16 (packed): exact, a 2-bit significand and the scale's exponent, but for those from 2^128 on, which become
+// infinities (a 4 at 2^126, a 2 at 2^127).
 __device__ __forceinline__ u32x4 values8(uint32_t codes, float scale) {
   return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
+
+// The same under scale byte b, a quarter of it: exact at every byte (2^-130, three steps of bf16's least one, to 1.5 x 2^127), where
+// values8 has infinities from 2^128 on. 255 gives NaN.
+__device__ __forceinline__ u32x4 quarter_values8(uint32_t codes, uint32_t b) {
+  u32x4 v = values8(codes, scale_float(b == 255u ? 255u : 127u));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float lo = __builtin_ldexpf(__uint_as_float(v[i] << 16), (int)b - 129);
+    const float hi = __builtin_ldexpf(__uint_as_float(v[i] & 0xffff0000u), (int)b - 129);
+    v[i] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
+  }
+  return v;
+}
+
+// Whether one of a head's four scale bytes is 253 or more: its codes may stand for more than bf16 holds.
+__device__ __forceinline__ bool past_bf16(uint32_t scales) {
+  return (scales & 0xffu) >= 253u || (scales >> 8 & 0xffu) >= 253u || (scales >> 16 & 0xffu) >= 253u || scales >> 24 >= 253u;
 }
 
 // The scale byte b of 32 codes as V's conversion to bf16 takes it: 255 too where they stand for more than bf16 holds, from

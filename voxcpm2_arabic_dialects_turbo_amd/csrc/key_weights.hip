@@ -16,6 +16,7 @@
 // Bound by those fma, exp2 (quarter rate) and adds, about as many cycles as the MFMAs: 6 chunks of 1000-2000 tokens over
 // 1500-2500 (16 heads of 2, 107 GFLOP of scores) 143-160 us, beside 223-245 for the attention; small calls by latency
 // (44 chunks of 33-59 over 50: 9.8 us).
+#include <cfloat>
 #include <type_traits>
 
 #include "fp4_common.h"
@@ -132,7 +133,8 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
 // Persistent: the items (128 keys, a part of the query rows, kv head, sequence), the key blocks of a part side by side, are
 // dealt to the XCDs in contiguous ranges, whose workgroups read the part's rows from that XCD's L2. DIRECT, where the grid of
 // all there may be is small: a workgroup for each, without the items' layout. FP4: the keys come from a 4-bit cache, as bf16,
-// which holds their values exactly.
+// which holds their values exactly; where 32 keys have a scale past which it does not, a quarter of them all, at four times the
+// softmax scale.
 template <bool DIRECT, int KT, bool FP4>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
   constexpr int KW = 2, QW = 2;
@@ -248,12 +250,14 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
       wait_vmem_all();
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
-    const float c = p.scale_log2;
+    float c[KT];  // (wave-uniform)
     float acc[KT][16];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int kt = 0; kt < KT; ++kt) {
+      c[kt] = p.scale_log2;
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+    }
     constexpr int NM = 8 * KT, NE = 16 * KT;
     // the scores (into sn) of half `hn` of the tile in buffer `buf` beside the probabilities of the half before it, whose first
     // row is r0
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
 #pragma unroll
         for (int y = i * NE / NM; y < (i + 1) * NE / NM; ++y) {
           const int kt = y >> 4, e = y & 15;
-          const float pr = fast_exp2(fmaf(sc[kt][e], c, -lse));
+          const float pr = fast_exp2(fmaf(sc[kt][e], c[kt], -lse));
           acc[kt][e] += !MASK || 32 * kt + 8 * (e >> 2) + (e & 3) <= last ? pr : 0.f;
           asm volatile("" : "+v"(acc[kt][e]));  // (here: sunk behind the two forms of the step, the adds ran beside no MFMA)
         }
@@ -330,11 +334,19 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs k) {
         for (int i = 0; i < 4; ++i) codes[i] = *reinterpret_cast<const u32x4*>(code + 16 * i);
         const uint32_t scale = *reinterpret_cast<const uint32_t*>(block + (int64_t)p.block_size * HK * fp4::kHeadCodes +
                                                                   (in * HK + g) * fp4::kHeadScales);
+        auto convert = [&](auto&& values) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const u32x4 c4 = codes[i / 2];
-          const u32x4 v = fp4::values8(h ? c4[2 * (i & 1) + 1] : c4[2 * (i & 1)], fp4::scale_float((scale >> (8 * (i / 2))) & 0xffu));
-          kf[kt][i] = ok ? v : zero4();
+          for (int i = 0; i < 8; ++i) {
+            const u32x4 c4 = codes[i / 2];
+            const u32x4 v = values(h ? c4[2 * (i & 1) + 1] : c4[2 * (i & 1)], (scale >> (8 * (i / 2))) & 0xffu);
+            kf[kt][i] = ok ? v : zero4();
+          }
+        };
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(ok && fp4::past_bf16(scale)) != 0, 0)) {
+          convert([](uint32_t codes8, uint32_t b) { return fp4::quarter_values8(codes8, b); });
+          c[kt] = fminf(4.f * p.scale_log2, FLT_MAX);  // (an infinity would make NaN of a score of 0)
+        } else {
+          convert([](uint32_t codes8, uint32_t b) { return fp4::values8(codes8, fp4::scale_float(b)); });
         }
       } else {
 #pragma unroll
