@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define VOX_ABI_VERSION 15
+#define VOX_ABI_VERSION 16
 
 #define VOX_OK 0
 #define VOX_EINVAL 1 /* bad argument: shape, stride, alignment or null pointer (reference: the asserts of
@@ -411,6 +411,14 @@ int vox_prefill_attn_weights_fp4(const void* q, int64_t q_row_stride, const void
                                  void* scratch, size_t scratch_bytes, void* scores, size_t scores_bytes, int plan,
                                  void* workspace, size_t workspace_bytes, void* out, int64_t out_row_stride,
                                  void* stream);
+
+/* For a step with fewer queries than new tokens, ahead of its vox_prefill_attn_weights (which takes as many tokens of a sequence
+ * as it has queries for the step's own): sets the weights of the last cu_seqlens_new[b + 1] - cu_seqlens_new[b] (int32 [batch +
+ * 1]) tokens of sequence b's cu_seqlens_k[b + 1] - cu_seqlens_k[b] to 0. max_keys: what the block tables reach (a longer
+ * sequence ends there; packed keys: INT32_MAX); tokens at or past max_tokens are left alone. */
+int vox_clear_key_weights(float* key_weights, const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width,
+                          int num_kv_heads, const int32_t* cu_seqlens_new, const int32_t* cu_seqlens_k, int batch,
+                          int max_keys, int max_tokens, void* stream);
 
 /* Drops tokens from sequences longer than `budget`: their first `sinks` and last `recent` tokens stay and, in every layer
  * and kv head apart, the budget - sinks - recent heaviest of the others by key_weights (fp32 [num_layers, num_weight_rows,

@@ -1,0 +1,82 @@
+"""Calls around the key weights on the CPU: steps that the module takes, looks at a step from the host (nothing is launched)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_key_weights_host import P, _einval, _layer, _rows, calls  # noqa: F401
+from voxcpm2_arabic_dialects_turbo_amd import _lib, ops_weights
+from voxcpm2_arabic_dialects_turbo_amd.context import get_context, set_context
+from voxcpm2_arabic_dialects_turbo_amd.ops_weights import varlen_attention_weights
+
+BF16, I32 = torch.bfloat16, torch.int32
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=I32)
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("paged", [False, True])
+def test_last_rows_say_which_tokens_are_new(calls, paged, fp4):  # noqa: F811
+    """cu_seqlens_q swapped on the live context: the operator gets the step's own beside it."""
+    layer = _layer(fp4)
+    layer.key_weights = torch.zeros(2, 2, 256)
+    cu, tables = _i32(0, 2, 5), _i32(0, 1).view(2, 1) if paged else None
+    set_context(True, cu, cu, 3, 3, _i32(0, 1, 256, 257, 258), None, tables, _i32(0, 1))
+    (q, _, _), (_, k, v) = _rows(2), _rows(5)
+    ctx = get_context()
+    ctx.cu_seqlens_q, ctx.max_seqlen_q = _i32(0, 1, 2), 1
+    layer(q, k, v)
+    assert [c[0] for c in calls] == ["store_kvcache", "varlen_attention_weights"]
+    kw = calls[1][2]
+    assert kw["cu_seqlens_new"] is cu and kw["cu_seqlens_q"].tolist() == [0, 1, 2] and kw["max_seqlen_q"] == 1
+    assert calls[0][1][3].numel() == 5
+    ctx.cu_seqlens_q, ctx.max_seqlen_q = cu, 3
+    layer(_rows(5)[0], k, v)
+    assert calls[-1][2]["cu_seqlens_new"] is None
+
+
+def test_fewer_queries_than_rows_need_the_new_tokens(calls):  # noqa: F811
+    """Nothing is stored or added where the context does not say which tokens are new."""
+    layer = _layer()
+    layer.key_weights = torch.zeros(2, 2, 256)
+    set_context(True, _i32(0, 1, 2), _i32(0, 2, 5), 1, 3, _i32(0, 1, 256, 257, 258), None, None, _i32(0, 1))
+    with pytest.raises(ValueError, match="2 queries for 5 new tokens"):
+        layer(_rows(2)[0], *_rows(5)[1:])
+    get_context().cu_seqlens_new = None
+    with pytest.raises(ValueError, match="2 queries for 5 new tokens"):
+        layer(_rows(2)[0], *_rows(5)[1:])
+    assert calls == []
+
+
+def test_new_tokens_refusals(monkeypatch):
+    monkeypatch.setattr(ops_weights, "_check_cuda", lambda *t: torch.device("cpu"))
+    a = dict(q=torch.zeros(4, 16, 128, dtype=BF16), k=torch.zeros(4, 2, 128, dtype=BF16), v=torch.zeros(4, 2, 128, dtype=BF16),
+             key_weights=torch.zeros(2, 2, 128), cu_seqlens_q=torch.zeros(3, dtype=I32), cu_seqlens_k=torch.zeros(3, dtype=I32),
+             max_seqlen_q=3, max_seqlen_k=3, softmax_scale=0.1)
+    with pytest.raises(ValueError, match="as many entries"):
+        varlen_attention_weights(**a, cu_seqlens_new=torch.zeros(2, dtype=I32))
+    with pytest.raises(TypeError, match="integer"):
+        varlen_attention_weights(**a, cu_seqlens_new=torch.zeros(3))
+    monkeypatch.undo()
+    with pytest.raises(ValueError, match="same GPU"):
+        varlen_attention_weights(**a, cu_seqlens_new=torch.zeros(3, dtype=I32))
+
+
+CLEAR_C = dict(w=P, rows=None, n_rows=2, width=128, hk=2, cu_new=P, cu_k=P, batch=2, max_keys=128, max_tokens=128, stream=None)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(batch=-1), "negative"), (dict(max_keys=-1), "negative"), (dict(max_tokens=-1), "negative"), (dict(w=None), "key_weights"),
+    (dict(w=P + 2), "key_weights"), (dict(n_rows=0), "empty key_weights"), (dict(width=0), "empty key_weights"),
+    (dict(cu_new=None), "null"), (dict(cu_k=None), "null"), (dict(hk=0), "65535"), (dict(hk=70000), "65535"),
+    (dict(batch=70000), "65535")])
+def test_c_clear_refusals(kw, match):
+    _einval(_lib.load().vox_clear_key_weights(*{**CLEAR_C, **kw}.values()), match)
+
+
+def test_c_clear_of_nothing():
+    for kw in (dict(batch=0), dict(max_keys=0), dict(max_tokens=0)):
+        assert _lib.load().vox_clear_key_weights(*{**CLEAR_C, "w": None, **kw}.values()) == _lib.VOX_OK

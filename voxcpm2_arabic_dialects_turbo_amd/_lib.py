@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must be loaded before the library: shared HIP runti
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvoxattn.so")
 
 VOX_OK, VOX_EINVAL, VOX_EHIP = 0, 1, 2
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 PLAN_NONE, PLAN_RECORD, PLAN_REUSE = 0, 1, 2
 
@@ -55,6 +55,7 @@ EXPORTS = (
     "vox_prefill_weights_bytes",
     "vox_prefill_attn_weights",
     "vox_prefill_attn_weights_fp4",
+    "vox_clear_key_weights",
     "vox_evict_kv_tokens",
 )
 
@@ -133,6 +134,8 @@ _SIGNATURES = {
                                             _c_void_p, _c_void_p, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _f32,
                                             _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p, _size, _i32,
                                             _c_void_p, _size, _c_void_p, _i64, _c_void_p]),
+    "vox_clear_key_weights": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32,
+                                     _c_void_p]),
     "vox_evict_kv_tokens": (_i32, [_c_void_p, _i64, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i64, _i32, _c_void_p, _i32,
                                    _c_void_p, _c_void_p, _i64, _i64, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p,
                                    _c_void_p, _c_void_p, _c_void_p]),

@@ -9,6 +9,8 @@ reset_context), so a runner that sets the context for the reference's Attention 
   (-1 padded);
 - ``weight_rows`` int32 [B] (no reference counterpart): the sequences' rows in the layers' ``key_weights``, None where the
   step adds nothing to them;
+- ``cu_seqlens_new`` int32 [B + 1] (no reference counterpart): the step's own tokens, cu_seqlens_q as the step was set up; it
+  stays where a caller swaps cu_seqlens_q for one layer, whose ``key_weights`` go by it;
 - ``first_patch``: carried for the reference's runner, not read by attention.
 
 The context is a module global read when ``Attention.forward`` runs: callers such as the reference's ``last_rows``
@@ -35,6 +37,7 @@ class Context:
     block_tables: torch.Tensor | None = None
     first_patch: bool = True
     weight_rows: torch.Tensor | None = None
+    cu_seqlens_new: torch.Tensor | None = None
 
 
 _CONTEXT = Context()
@@ -66,6 +69,7 @@ def set_context(
         context_lens,
         block_tables,
         weight_rows=weight_rows,
+        cu_seqlens_new=cu_seqlens_q,
     )
 
 

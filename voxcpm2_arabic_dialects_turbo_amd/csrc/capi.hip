@@ -1294,6 +1294,31 @@ int vox_prefill_attn_weights_fp4(const void* q, int64_t q_row_stride, const void
                               out_row_stride, stream);
 }
 
+int vox_clear_key_weights(float* key_weights, const int32_t* weight_rows, int64_t num_weight_rows, int64_t weight_width,
+                          int num_kv_heads, const int32_t* cu_seqlens_new, const int32_t* cu_seqlens_k, int batch,
+                          int max_keys, int max_tokens, void* stream) {
+  const char* fn = "clear_key_weights";
+  if (batch < 0 || max_keys < 0 || max_tokens < 0) return fail(VOX_EINVAL, "%s: negative batch, max_keys or max_tokens", fn);
+  if (batch == 0 || max_keys == 0 || max_tokens == 0) return VOX_OK;
+  if (!key_weights || ((uintptr_t)key_weights & 3u)) return fail(VOX_EINVAL, "%s: null or unaligned key_weights", fn);
+  if (num_weight_rows <= 0 || weight_width <= 0) return fail(VOX_EINVAL, "%s: empty key_weights", fn);
+  if (!cu_seqlens_new || !cu_seqlens_k) return fail(VOX_EINVAL, "%s: null pointer argument", fn);
+  if (num_kv_heads <= 0 || num_kv_heads > 65535 || batch > 65535)
+    return fail(VOX_EINVAL, "%s: at most 65535 sequences and kv heads", fn);
+  vox::ClearWeightsArgs a{};
+  a.weights = key_weights;
+  a.rows = weight_rows;
+  a.row_count = num_weight_rows;
+  a.width = weight_width;
+  a.num_heads = num_kv_heads;
+  a.cu_new = cu_seqlens_new;
+  a.cu_k = cu_seqlens_k;
+  a.batch = batch;
+  a.max_keys = max_keys;
+  a.max_tokens = max_tokens;
+  return hip_status(vox::launch_clear_new_weights(a, (hipStream_t)stream), "clear_key_weights launch");
+}
+
 int vox_evict_kv_tokens(void* kv, int64_t num_layers, int64_t num_blocks, int block_size, int num_kv_heads, int head_bytes,
                         int scale_bytes, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
                         const int32_t* context_lens, int batch, float* key_weights, const int32_t* weight_rows,

@@ -85,6 +85,7 @@ struct Entry<R (*)(A...)> {
   X(vox_prefill_weights_bytes)      \
   X(vox_prefill_attn_weights)       \
   X(vox_prefill_attn_weights_fp4)   \
+  X(vox_clear_key_weights)          \
   X(vox_evict_kv_tokens)
 
 #define VOX_DEFINE(name)                                                              \

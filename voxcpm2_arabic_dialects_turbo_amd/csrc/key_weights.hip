@@ -443,6 +443,21 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
   *out = j >= s.old ? got : *out + got;
 }
 
+// A step with fewer queries than new tokens (a layer that takes the last row of each sequence): the sums above and the decode
+// kernels set the queries' own places and add to all before them, so the others of the step start at 0 here. A launch of its
+// own ahead of them, for those layers alone; bound by its start.
+__global__ __launch_bounds__(256) void clear_new_weights_kernel(ClearWeightsArgs a) {
+  const int b = blockIdx.y, g = blockIdx.z;
+  const int64_t row = a.rows ? (int64_t)a.rows[b] : b;
+  const int64_t nk = min((int64_t)a.cu_k[b + 1] - a.cu_k[b], (int64_t)a.max_keys);
+  const int64_t fresh = (int64_t)a.cu_new[b + 1] - a.cu_new[b];
+  if (row < 0 || row >= a.row_count) return;
+  const int64_t to = min(min(nk, (int64_t)a.max_tokens), a.width);
+  float* const w = a.weights + (row * a.num_heads + g) * a.width;
+  for (int64_t j = max((int64_t)0, nk - max((int64_t)0, fresh)) + blockIdx.x * 256 + threadIdx.x; j < to; j += (int64_t)gridDim.x * 256)
+    w[j] = 0.f;
+}
+
 template <bool DIRECT, int KT>
 void launch_sums(const KeyWeightsArgs& k, int64_t grid, hipStream_t stream) {
   if (k.fp4)
@@ -494,6 +509,13 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
   if (fits64 && (grid64 <= 512 || (grid64 <= 1024 && tiles64 >= 16)))
     return launch_lse<2, 2, false>(a, dim3((unsigned)tiles64, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
   return launch_lse<4, 1, false>(a, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)a.num_kv_heads), stream);
+}
+
+hipError_t launch_clear_new_weights(const ClearWeightsArgs& a, hipStream_t stream) {
+  if (a.batch <= 0 || a.max_tokens <= 0 || a.num_heads <= 0) return hipSuccess;
+  const int64_t wgs = ((int64_t)a.max_tokens + 1023) / 1024;
+  clear_new_weights_kernel<<<dim3((unsigned)(wgs < 64 ? wgs : 64), (unsigned)a.batch, (unsigned)a.num_heads), dim3(256), 0, stream>>>(a);
+  return hipGetLastError();
 }
 
 int key_weights_part_rows(int64_t num_tokens, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {

@@ -149,6 +149,20 @@ struct KeyWeightsArgs {
   int item_shift;             // a key block has 1 << item_shift keys
 };
 
+// The weights of the tokens that are new in a step, set to 0 (launch_clear_new_weights): sequence b's last cu_new[b + 1] - cu_new[b].
+struct ClearWeightsArgs {
+  float* weights;             // as KeyWeightsArgs', these four
+  const int32_t* rows;
+  int64_t row_count;
+  int64_t width;
+  int num_heads;              // kv heads
+  const int32_t* cu_new;      // int32 [batch + 1], as cu_k
+  const int32_t* cu_k;
+  int batch;
+  int max_keys;               // what the block tables reach: a longer context ends there
+  int max_tokens;             // places at or past it are left alone
+};
+
 // Tokens dropped from a paged cache (kv_evict.hip): of every sequence longer than `budget` its first `sinks`, last `recent`
 // and, for every layer and kv head, the budget - sinks - recent heaviest others, moved to the front in their order.
 struct EvictArgs {
@@ -268,6 +282,7 @@ hipError_t launch_prefill(const PrefillArgs& a, int max_seqlen_q, hipStream_t st
 hipError_t launch_prefill_lse(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 hipError_t launch_prefill_lse_fp4(const PrefillArgs& a, int max_seqlen_q, hipStream_t stream);
 hipError_t launch_key_weights(const KeyWeightsArgs& k, hipStream_t stream);
+hipError_t launch_clear_new_weights(const ClearWeightsArgs& a, hipStream_t stream);
 int key_weights_part_rows(int64_t num_tokens, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads);
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);

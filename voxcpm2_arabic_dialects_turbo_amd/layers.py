@@ -19,7 +19,8 @@ the step's own rows).
 
 A layer with ``key_weights`` (fp32 [rows, HK, width], see ops_weights; ``runner.allocate_key_weights`` sets them) adds to
 them what the step's attention gives every key, in every step whose context has ``weight_rows``; its caches are those of the
-step without, its outputs too but for the order of a prefill's sums.
+step without, its outputs too but for the order of a prefill's sums. In a layer run for the last row of each sequence alone, with
+cu_seqlens_q swapped on the live context, every token of the step starts with what those queries give it.
 
 Every branch runs a HIP kernel of libvoxattn.so; nothing here synchronizes or allocates outside torch, so the
 module can be captured into HIP graphs exactly where the reference captures its decode step.
@@ -195,9 +196,15 @@ class Attention(nn.Module):
             return decode_attention_weights(q, k_cache, v_cache, context.context_lens, tables, self.scale,
                                             self.key_weights, context.weight_rows, key=k, value=v,
                                             slot_mapping=context.slot_mapping, plan=_plan_key(context)).unsqueeze(1)
+        new = None
+        if k.shape[0] != q.shape[0]:  # fewer queries than new tokens
+            new = context.cu_seqlens_new
+            if new is None or new is context.cu_seqlens_q:
+                raise ValueError(f"key weights: {q.shape[0]} queries for {k.shape[0]} new tokens, and the context does not say "
+                                 "whose these are: set it up with the step's own cu_seqlens_q, and swap that for the layer's")
         store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
         return varlen_attention_weights(q, k, v, self.key_weights, context.weight_rows, cu_seqlens_q=context.cu_seqlens_q,
                                         cu_seqlens_k=context.cu_seqlens_k, max_seqlen_q=context.max_seqlen_q,
                                         max_seqlen_k=context.max_seqlen_k, softmax_scale=self.scale, block_table=tables,
                                         k_cache=k_cache, v_cache=v_cache,
-                                        plan=_plan_key(context) if tables is not None else None)
+                                        plan=_plan_key(context) if tables is not None else None, cu_seqlens_new=new)

@@ -174,13 +174,17 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
                              weight_rows: torch.Tensor | None = None, *, cu_seqlens_q: torch.Tensor,
                              cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float,
                              block_table: torch.Tensor | None = None, k_cache: torch.Tensor | None = None,
-                             v_cache: torch.Tensor | None = None, out: torch.Tensor | None = None, plan=None
-                             ) -> torch.Tensor:
+                             v_cache: torch.Tensor | None = None, out: torch.Tensor | None = None, plan=None,
+                             cu_seqlens_new: torch.Tensor | None = None) -> torch.Tensor:
     """``ops.varlen_attention`` (causal: sequence b's queries q [T, H, 128] are the last of its keys, from packed rows k / v
     [Tk, HK, 128] or, with block_table, from the caches), adding to ``key_weights`` what every key received: for token j and
     kv head g the sum of the probabilities of b's queries at g's query heads, in place of the weight for the step's own
     tokens, the last cu_seqlens_q[b + 1] - cu_seqlens_q[b], on top of it for the earlier ones. Returns o [T, H, 128] bf16,
     zeros for a query that sees no key. A sequence without queries keeps its weights.
+
+    ``cu_seqlens_new`` (int [B + 1], as cu_seqlens_k): the step's own tokens, where there are fewer queries than those (a layer
+    that takes the last row of each sequence): the last cu_seqlens_new[b + 1] - cu_seqlens_new[b] of sequence b's keys start with
+    what the queries give them, with 0 where it has none.
 
     No sequence has more than max_seqlen_q queries or max_seqlen_k keys (further ones are left out). H / HK divides 128, and
     cache blocks are a multiple of 64 tokens. One-query sequences run on the decode kernels where a call is mostly those, as
@@ -224,11 +228,22 @@ def varlen_attention_weights(q: torch.Tensor, k: torch.Tensor | None, v: torch.T
         raise ValueError(f"num_heads {H} is not a multiple of num_kv_heads {hk}")
     n_rows, width, rows = _weights(fn, key_weights, weight_rows, max(B, 0), hk, reach, q.get_device())
     q, q_stride, out = _query(fn, q, out, dev, False)
+    cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
+    lib = _lib.load()
+    if cu_seqlens_new is not None:
+        if cu_seqlens_new.numel() != B + 1:
+            raise ValueError("cu_seqlens_new must have as many entries as cu_seqlens_q")
+        _check_cuda(q, cu_seqlens_new)
+        cu_new = _as_i32(_flat(cu_seqlens_new), "cu_seqlens_new")
+        if B > 0 and reach > 0:
+            with _on(dev):
+                _lib.check(lib.vox_clear_key_weights(
+                    key_weights.data_ptr(), None if rows is None else rows.data_ptr(), n_rows, width, hk, cu_new.data_ptr(),
+                    cu_k.data_ptr(), B, 2 ** 31 - 1 if block_table is None else bt.shape[1] * bs, reach,
+                    _lib.stream_handle(dev)), fn)
     max_seqlen_q = min(int(max_seqlen_q), T)
     if T == 0 or B <= 0 or max_seqlen_q <= 0:
         return out
-    cu_q, cu_k = _as_i32(cu_seqlens_q, "cu_seqlens_q"), _as_i32(cu_seqlens_k, "cu_seqlens_k")
-    lib = _lib.load()
     with _on(dev):
         need = lib.vox_prefill_weights_bytes(T, B, max_seqlen_q, reach, H, hk)
         scores_at = (need + 255) // 256 * 256
