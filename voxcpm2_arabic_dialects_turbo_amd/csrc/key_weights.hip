@@ -119,6 +119,7 @@ __device__ __forceinline__ KwSeq kw_seq(const KeyWeightsArgs& k, int b, int gsh)
   s.nq = p.cu_q[b + 1] - s.q0;
   s.k0 = p.cu_k[b];
   s.nk = p.cu_k[b + 1] - s.k0;
+  if (p.block_tables) s.nk = min(s.nk, p.max_blocks * p.block_size);  // (the attention ends, and aligns the queries, there)
   s.old = s.nk - s.nq;
   s.row = k.rows ? (int64_t)k.rows[b] : b + k.row0;
   const bool mine = s.nq > 0 && s.nk > 0 && s.row >= 0 && s.row < k.row_count && !(p.skip_single && s.nq == 1);
