@@ -10,7 +10,7 @@ from oracle import fp4
 from oracle import key_weights as ref
 from tests._util import paged_pool, randn
 from tests.test_key_weights_gpu import D, DEV, SCALE, Want, _i32, _received
-from voxcpm2_arabic_dialects_turbo_amd.ops_weights import varlen_attention_weights
+from voxcpm2_arabic_dialects_turbo_amd.ops_weights import decode_attention_weights, varlen_attention_weights
 
 pytestmark = pytest.mark.gpu
 H, HK, BS = 16, 2, 64
@@ -67,3 +67,29 @@ def _varlen(seed, seqs, reach, max_k, four_bit):
     [(20, 250), (40, 192), (30, 100), (1, 300), (3, 192)], [(100, 1000), (150, 193)]])
 def test_chunks_past_their_tables(seqs, four_bit):
     _varlen(len(seqs), seqs, 192, 1000, four_bit)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("seqs", [
+    [(1, 250), (1, 192), (1, 193), (1, 100), (1, 1000)], [(1, 200 + i) for i in range(20)] + [(60, 230)]])
+def test_decode_rows_past_their_tables(seqs, four_bit):
+    """Decode rows alone, and beside a chunk."""
+    _varlen(10 + len(seqs), seqs, 192, 1000, four_bit)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_decode_contexts_past_their_tables(four_bit):
+    """The last token that the table reaches is the newest one."""
+    gen = torch.Generator().manual_seed(40)
+    caches, values, tables = _caches(gen, 192, 4, four_bit)
+    lens = [193, 192, 50, 100000]
+    q, w = randn(gen, 4, H, D), _received(gen, 4, HK, 192)
+    for b, n in enumerate(lens):
+        w[b, :, min(n, 192) - 1] = float("nan")
+    wd = w.to(DEV)
+    o = decode_attention_weights(q.to(DEV), *caches, _i32(lens), tables.to(DEV), SCALE, wd)
+    want = Want(w)
+    for b, n in enumerate(lens):
+        k, v = (ref.keys_of(c, tables[b], min(n, 192))[0] for c in values)
+        want.sequence(q[b:b + 1], k, v, None, b, 1, more=_more(q[b:b + 1], k, four_bit))
+    want.check(o, wd)

@@ -959,7 +959,8 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
     const int b = min(at + lane, p.batch - 1);
     st = p.steps[b];
     en = p.steps[b + 1];
-    len = p.cu_q ? p.cu_k[b + 1] - p.cu_k[b] : p.context_lens[b];
+    // (ended where the split kernel ends it: its newest token is the last one that the table reaches)
+    len = min(p.cu_q ? p.cu_k[b + 1] - p.cu_k[b] : p.context_lens[b], p.max_blocks * p.block_size);
     row = p.weight_rows ? p.weight_rows[b] : (int)p.weight_row0 + b;
   };
   int s_tot = p.steps[p.batch], s_g = p.steps[p.batch + 1];
