@@ -93,3 +93,13 @@ def test_decode_contexts_past_their_tables(four_bit):
         k, v = (ref.keys_of(c, tables[b], min(n, 192))[0] for c in values)
         want.sequence(q[b:b + 1], k, v, None, b, 1, more=_more(q[b:b + 1], k, four_bit))
     want.check(o, wd)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("seqs", [
+    [(1, 150), (1, 90), (1, 100), (1, 101), (1, 192)],
+    [(1, 80 + 5 * i) for i in range(20)] + [(60, 150)],
+    [(20, 150), (40, 192), (1, 150)]])
+def test_keys_past_what_the_call_says(seqs, four_bit):
+    """The same on the decode kernels as on the chunk's."""
+    _varlen(30 + len(seqs), seqs, 192, 100, four_bit)

@@ -1107,6 +1107,7 @@ int decode_attn_weights(const char* fn, bool fp4, const void* q, int64_t q_row_s
   a.weight_rows = weight_rows;
   a.weight_row_count = num_weight_rows;
   a.weight_width = weight_width;
+  a.weight_reach = weight_width;
   return launch_decode_slices(a, batch, num_kv_heads, plan, workspace, (hipStream_t)stream,
                               fp4 ? vox::launch_decode_weights_fp4 : vox::launch_decode_weights);
 }
@@ -1244,6 +1245,7 @@ int prefill_attn_weights(const char* fn, bool fp4, const void* q, int64_t q_row_
     d.weight_rows = weight_rows;
     d.weight_row_count = num_weight_rows;
     d.weight_width = weight_width;
+    d.weight_reach = weight_width < max_seqlen_k ? weight_width : max_seqlen_k;  // (as the chunk's kernels leave them out)
   }
   const hipStream_t s = (hipStream_t)stream;
   if (!decodes || max_seqlen_q > 1) {

@@ -986,7 +986,7 @@ __device__ __forceinline__ void add_key_weights(const DecodeArgs& p, int W, int 
     if (eb <= t) continue;
     const int te = min(r1, eb);
     const int n = __builtin_amdgcn_readlane(len, k);
-    const int64_t wr = __builtin_amdgcn_readlane(row, k), reach = min((int64_t)n, p.weight_width);
+    const int64_t wr = __builtin_amdgcn_readlane(row, k), reach = min((int64_t)n, p.weight_reach);
     const bool mine = wr >= 0 && wr < p.weight_row_count;
     float* const wb = p.weights + ((mine ? wr : 0) * HK + (HK == 2 ? sub >> 1 : 0)) * p.weight_width;
     // steps u to u + 3: the scores and the weights. (Every lane loads something that is there: loads behind branches would

@@ -63,13 +63,14 @@ struct DecodeArgs {
   int copy_wgs;
   // Weights mode (launch_decode_weights): what every key receives is added to row weight_rows[b] (weight_row0 + b where that
   // is null; rows outside [0, weight_row_count): none) of weights fp32 [weight_row_count, HK, weight_width], by merge
-  // workgroups [merges, merges + weight_wgs); keys at or past weight_width: left out. scores: fp32 [steps, H, 16].
+  // workgroups [merges, merges + weight_wgs); keys at or past weight_reach (<= weight_width): left out. scores: fp32 [steps, H, 16].
   float* scores;
   float* weights;
   const int32_t* weight_rows;
   int64_t weight_row0;
   int64_t weight_row_count;
   int64_t weight_width;
+  int64_t weight_reach;
   int weight_wgs;
 };
 
