@@ -51,6 +51,26 @@ def test_fewer_queries_than_rows_need_the_new_tokens(calls):  # noqa: F811
     assert calls == []
 
 
+@pytest.mark.parametrize("fp4", [False, True])
+def test_decode_steps_with_more_rows_than_queries_store_then_attend(calls, fp4):  # noqa: F811
+    """As a layer without weights takes them."""
+    layer = _layer(fp4)
+    layer.key_weights = torch.zeros(3, 2, 256)
+    for rows, want in ((5, ["store_kvcache", "decode_attention_weights"]), (3, ["decode_attention_weights"])):
+        calls.clear()
+        slots = torch.arange(rows, dtype=I32) * 256
+        set_context(False, slot_mapping=slots, context_lens=_i32(1, 1, 1), block_tables=_i32(0, 1, 2).view(3, 1),
+                    weight_rows=_i32(0, 1, 2))
+        (q, _, _), (_, k, v) = _rows(3), _rows(rows)
+        layer(q, k, v)
+        assert [c[0] for c in calls] == want
+        if rows == 5:  # (the recorded store drops its first argument)
+            assert calls[0][1][0] is v and calls[0][1][3] is slots
+            assert calls[1][2].get("key") is None and calls[1][2].get("slot_mapping") is None
+        else:
+            assert calls[0][2]["key"] is k and calls[0][2]["slot_mapping"] is slots
+
+
 def test_new_tokens_refusals(monkeypatch):
     monkeypatch.setattr(ops_weights, "_check_cuda", lambda *t: torch.device("cpu"))
     a = dict(q=torch.zeros(4, 16, 128, dtype=BF16), k=torch.zeros(4, 2, 128, dtype=BF16), v=torch.zeros(4, 2, 128, dtype=BF16),

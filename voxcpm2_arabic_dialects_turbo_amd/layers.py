@@ -192,10 +192,15 @@ class Attention(nn.Module):
         """A step that adds to key_weights."""
         k_cache, v_cache, tables = self.k_cache, self.v_cache, context.block_tables
         if not context.is_prefill:
-            _check_riding_store(context, k_cache.shape[1], decode=True)
+            rows = dict(key=k, value=v, slot_mapping=context.slot_mapping)
+            if context.slot_mapping is not None and k.dim() == 3 and k.shape[0] == q.shape[0]:
+                _check_riding_store(context, k_cache.shape[1], decode=True)
+            else:  # (more rows than queries: each goes to its slot, then the queries attend)
+                store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
+                rows = {}
             return decode_attention_weights(q, k_cache, v_cache, context.context_lens, tables, self.scale,
-                                            self.key_weights, context.weight_rows, key=k, value=v,
-                                            slot_mapping=context.slot_mapping, plan=_plan_key(context)).unsqueeze(1)
+                                            self.key_weights, context.weight_rows, **rows,
+                                            plan=_plan_key(context)).unsqueeze(1)
         new = None
         if k.shape[0] != q.shape[0]:  # fewer queries than new tokens
             new = context.cu_seqlens_new
