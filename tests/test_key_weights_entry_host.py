@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_key_weights_host import P, _einval, _layer, _rows, calls  # noqa: F401
-from voxcpm2_arabic_dialects_turbo_amd import _lib, ops_weights
+from voxcpm2_arabic_dialects_turbo_amd import _lib, checks, ops_weights
 from voxcpm2_arabic_dialects_turbo_amd.context import get_context, set_context
 from voxcpm2_arabic_dialects_turbo_amd.ops_weights import varlen_attention_weights
 
@@ -69,6 +69,38 @@ def test_decode_steps_with_more_rows_than_queries_store_then_attend(calls, fp4):
             assert calls[1][2].get("key") is None and calls[1][2].get("slot_mapping") is None
         else:
             assert calls[0][2]["key"] is k and calls[0][2]["slot_mapping"] is slots
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_steps_whose_sequences_share_a_row_are_found(calls, monkeypatch, prefill):  # noqa: F811
+    layer = _layer()
+    layer.key_weights = torch.zeros(3, 2, 256)
+
+    def step(*rows):
+        calls.clear()
+        slots = torch.arange(3, dtype=I32) * 256
+        if prefill:
+            set_context(True, _i32(0, 1, 2, 3), _i32(0, 1, 2, 3), 1, 1, slots, None, None, _i32(*rows))
+        else:
+            set_context(False, slot_mapping=slots, context_lens=_i32(1, 1, 1), block_tables=_i32(0, 1, 2).view(3, 1),
+                        weight_rows=_i32(*rows))
+        layer(*_rows(3))
+
+    step(1, 0, 1)  # (not looked for by default)
+    monkeypatch.setenv("VOX_CHECK_STORE", "1")
+    for rows in ((0, 1, 2), (-1, 2, -1)):
+        step(*rows)
+        assert calls
+    with pytest.raises(ValueError, match="sequences 0 and 2 share row 1"):
+        step(1, 0, 1)
+    assert calls == []
+
+
+def test_weight_row_violations():
+    assert checks.weight_row_violations(_i32(3, -1, 0, -1, 7)) == []
+    assert checks.weight_row_violations(_i32(3, 3, 3)) == ["sequences 0 and 1 share row 3 of the weights",
+                                                         "sequences 1 and 2 share row 3 of the weights"]
+    assert len(checks.weight_row_violations(torch.zeros(50, dtype=torch.int64), limit=4)) == 4
 
 
 def test_new_tokens_refusals(monkeypatch):

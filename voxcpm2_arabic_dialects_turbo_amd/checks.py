@@ -15,7 +15,8 @@ which the reference engine guarantees: its runner computes the slots from the ta
 (nanovllm_voxcpm/engine/model_runner.py:880-883 for prefill, :919 for decode) and its block manager gives every
 sequence's last block to that sequence alone. `riding_store_violations` checks both on the host for one step's
 context, so an integration that builds its own contexts can verify them; ``Attention.forward`` runs it before every
-riding store when the environment sets ``VOX_CHECK_STORE=1`` (it copies the context to the host and synchronizes).
+riding store when the environment sets ``VOX_CHECK_STORE=1`` (it copies the context to the host and synchronizes), and
+`weight_row_violations` before every step that adds to key weights.
 """
 
 from __future__ import annotations
@@ -23,7 +24,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-__all__ = ["riding_store_violations", "eviction_violations"]
+__all__ = ["riding_store_violations", "eviction_violations", "weight_row_violations"]
 
 
 def _host(t: torch.Tensor | None) -> np.ndarray | None:
@@ -93,6 +94,18 @@ def riding_store_violations(slot_mapping: torch.Tensor, block_tables: torch.Tens
     return out
 
 
+def weight_row_violations(weight_rows: torch.Tensor, limit: int = 10) -> list[str]:
+    """The sequences of one step that share a row of key weights, which both would write at once (at most `limit` messages;
+    empty when each has its own; rows below 0 keep no weights and may be several)."""
+    out: list[str] = []
+    seen: dict[int, int] = {}
+    for b, r in enumerate(_host(weight_rows).reshape(-1).tolist()):
+        if r >= 0 and r in seen:
+            out.append(f"sequences {seen[r]} and {b} share row {r} of the weights")
+        seen[r] = b
+    return out[:limit]
+
+
 def eviction_violations(block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int, budget: int, *,
                         weight_rows: torch.Tensor | None = None, new_blocks: torch.Tensor | None = None,
                         limit: int = 10) -> list[str]:
@@ -104,12 +117,7 @@ def eviction_violations(block_tables: torch.Tensor, context_lens: torch.Tensor, 
         return ["block_tables must be [B, max_blocks]"]
     fresh = _host(new_blocks)
     rows = np.arange(lens.size) if weight_rows is None else _host(weight_rows).reshape(-1)
-    out: list[str] = []
-    seen: dict[int, int] = {}
-    for b, r in enumerate(rows.tolist()):
-        if r >= 0 and r in seen:
-            out.append(f"sequences {seen[r]} and {b} share row {r} of the weights")
-        seen[r] = b
+    out = weight_row_violations(torch.from_numpy(rows), limit)
     named: dict[int, set[int]] = {}
     written: dict[int, int] = {}
     for b, n in enumerate(lens.tolist()):
