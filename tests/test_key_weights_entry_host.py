@@ -103,6 +103,20 @@ def test_weight_row_violations():
     assert len(checks.weight_row_violations(torch.zeros(50, dtype=torch.int64), limit=4)) == 4
 
 
+def test_eviction_violations_finds_blocks_that_keep_their_hash():
+    tables, lens = torch.tensor([[3, 0, 7], [6, 4, 5], [1, -1, -1]]), _i32(180, 150, 60)
+    look = lambda hashed, **kw: checks.eviction_violations(tables, lens, 64, 100, hashed_blocks=hashed, **kw)  # noqa: E731
+    assert look([]) == [] and look([1, 5, 7]) == []  # (blocks of a sequence within the budget, and those behind it)
+    assert look({0}) == ["sequence 0 is brought down into block 0, which is still handed out by its hash"]
+    assert look(torch.tensor([3, 4])) == [f"sequence {b} is brought down into block {v}, which is still handed out by its hash"
+                                          for b, v in ((0, 3), (1, 4))]
+    new = torch.tensor([[8, 9, -1], [-1, -1, -1], [-1, -1, -1]])
+    assert look([3, 0], new_blocks=new) == []
+    assert look([3, 0, 9], new_blocks=new) == ["sequence 0 is brought down into block 9, which is still handed out by its hash"]
+    assert look([3, 4], weight_rows=_i32(-1, 0, 1)) == ["sequence 1 is brought down into block 4, which is still handed out by "
+                                                       "its hash"]
+
+
 def test_new_tokens_refusals(monkeypatch):
     monkeypatch.setattr(ops_weights, "_check_cuda", lambda *t: torch.device("cpu"))
     a = dict(q=torch.zeros(4, 16, 128, dtype=BF16), k=torch.zeros(4, 2, 128, dtype=BF16), v=torch.zeros(4, 2, 128, dtype=BF16),

@@ -21,6 +21,8 @@ riding store when the environment sets ``VOX_CHECK_STORE=1`` (it copies the cont
 
 from __future__ import annotations
 
+from collections.abc import Iterable
+
 import numpy as np
 import torch
 
@@ -108,10 +110,11 @@ def weight_row_violations(weight_rows: torch.Tensor, limit: int = 10) -> list[st
 
 def eviction_violations(block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int, budget: int, *,
                         weight_rows: torch.Tensor | None = None, new_blocks: torch.Tensor | None = None,
-                        limit: int = 10) -> list[str]:
+                        hashed_blocks: Iterable[int] = (), limit: int = 10) -> list[str]:
     """What kernels.kv_evict.evict_kv_tokens assumes about a call and cannot see from the host (at most `limit` messages;
     empty when all of it holds): no two sequences share a row of weights, and a block that a sequence over the budget is
-    brought down into is named by no other sequence and is no other's new block."""
+    brought down into is named by no other sequence, is no other's new block, and is none of ``hashed_blocks``, those that the
+    block manager would hand to a later request by the text they held (its prefix hashes, as they stand behind the call)."""
     tables, lens = _host(block_tables), _host(context_lens).reshape(-1)
     if tables is None or tables.ndim != 2 or tables.shape[0] < lens.size:
         return ["block_tables must be [B, max_blocks]"]
@@ -120,6 +123,7 @@ def eviction_violations(block_tables: torch.Tensor, context_lens: torch.Tensor, 
     out = weight_row_violations(torch.from_numpy(rows), limit)
     named: dict[int, set[int]] = {}
     written: dict[int, int] = {}
+    hashed = {int(v) for v in hashed_blocks}
     for b, n in enumerate(lens.tolist()):
         need = -(-min(max(n, 0), tables.shape[1] * block_size) // block_size)
         for v in tables[b, :need].tolist():
@@ -137,6 +141,8 @@ def eviction_violations(block_tables: torch.Tensor, context_lens: torch.Tensor, 
             if others:
                 what = "new block" if given else "block"
                 out.append(f"sequence {b} is brought down into {what} {v}, which sequence {min(others)} names")
+            if v in hashed:
+                out.append(f"sequence {b} is brought down into block {v}, which is still handed out by its hash")
             if v in written:
                 out.append(f"sequences {written[v]} and {b} are both brought down into block {v}")
             written[v] = b

@@ -32,7 +32,12 @@ def evict_kv_tokens(kv: torch.Tensor, key_weights: torch.Tensor, block_tables: t
     A block that several rows name (a forked prefix) must not be written: ``new_blocks`` int [B, max_blocks] names blocks,
     which no row names, that take the place of the sequence's own as it is brought down (-1: its own). Every row over the
     budget needs one for each block among its first ceil(budget / block_size) that another row names too;
-    ``checks.eviction_violations`` looks a step over."""
+    ``checks.eviction_violations`` looks a step over.
+
+    A block that was written no longer holds the text that it was filled from: its tokens are others in every layer and kv head.
+    Where blocks are found again by their text (a prefix cache's hashes), those written in place and the new ones lose their
+    hash, a sequence that was brought down registers none for its further blocks, and a block whose hash is to stay needs a new
+    one in its place."""
     planes, blocks, bs, slot, scale = pages_of(kv)
     layers, hk = planes // 2, kv.shape[4]
     if slot % hk or (slot // hk) % 16 or slot // hk > 4096:
