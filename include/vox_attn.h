@@ -371,8 +371,9 @@ int vox_decode_attn_weights(const void* q, int64_t q_row_stride, const void* key
                             size_t scores_bytes, int plan, void* workspace, size_t workspace_bytes, void* out,
                             void* stream);
 
-/* The same over 4-bit caches, as vox_decode_attn_fp4 and vox_decode_attn_store_fp4: a score is off by at most 2^-13 of
- * softmax_scale sum |q||k|, a probability by that many parts twice. */
+/* The same over 4-bit caches, as vox_decode_attn_fp4 and vox_decode_attn_store_fp4: a row's scores are off by at most x =
+ * softmax_scale (2^-13 sum |q||k| + 2^-18 max |q| sum |k|), a probability by at most e^(2x) - 1 of it beside the roundings in 32
+ * bits. */
 int vox_decode_attn_weights_fp4(const void* q, int64_t q_row_stride, const void* key, const void* value,
                                 int64_t key_row_stride, int64_t value_row_stride, const int32_t* slot_mapping,
                                 void* k_cache, void* v_cache, int64_t num_blocks, int block_size,
@@ -401,7 +402,8 @@ int vox_prefill_attn_weights(const void* q, int64_t q_row_stride, const void* ke
                              size_t scratch_bytes, void* scores, size_t scores_bytes, int plan, void* workspace,
                              size_t workspace_bytes, void* out, int64_t out_row_stride, void* stream);
 
-/* The same over 4-bit caches through a block table, as vox_prefill_attn_fp4; scores as vox_decode_attn_weights_fp4's. */
+/* The same over 4-bit caches through a block table, as vox_prefill_attn_fp4; scores as vox_decode_attn_weights_fp4's, in the
+ * sums that a chunk's probabilities are divided by: those of one query add up to 1 within e^x - 1. */
 int vox_prefill_attn_weights_fp4(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                                  int64_t num_blocks, int block_size, const int32_t* block_tables, int64_t bt_stride,
                                  int max_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,

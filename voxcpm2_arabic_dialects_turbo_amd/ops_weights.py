@@ -10,10 +10,14 @@ A token that is new in a call starts with what it gets there, whatever its place
 row needs no clearing between the sequences that have it in turn. ``runner.allocate_key_weights`` makes the planes, and
 ``Attention.forward`` adds to its layer's.
 
-The attention itself is that of ``ops``, or over 4-bit caches of ``ops_fp4``. There a score is off by at most 2^-13 of
-softmax_scale sum |q||k|, so a probability by at most twice that many parts of it. Like their operators these run on torch's
-current stream of the tensors' device, allocate with torch, never synchronize and can be captured into HIP graphs. head_dim
-128, softmax_scale positive. No reference counterpart.
+The attention itself is that of ``ops``, or over 4-bit caches of ``ops_fp4``. There a score is off by at most x =
+softmax_scale (2^-13 sum |q||k| + 2^-18 max |q| sum |k|), the largest of its row: the scaled MFMA's sum, and what the query's two
+8-bit parts leave. A probability is off by at most e^(2x) - 1 of it, beside the roundings in 32 bits. A chunk's are made from
+scores in bf16 products over a sum from the scaled MFMA, so those of one query add up to 1 within e^x - 1 only; a decode step's
+come from one arithmetic and add up to 1.
+
+Like their operators these run on torch's current stream of the tensors' device, allocate with torch, never synchronize and
+can be captured into HIP graphs. head_dim 128, softmax_scale positive. No reference counterpart.
 """
 
 from __future__ import annotations
