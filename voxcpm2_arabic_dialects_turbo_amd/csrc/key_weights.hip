@@ -446,7 +446,7 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(KeyWeightsArgs k) 
 
 // A step with fewer queries than new tokens (a layer that takes the last row of each sequence): the sums above and the decode
 // kernels set the queries' own places and add to all before them, so the others of the step start at 0 here. A launch of its
-// own ahead of them, for those layers alone; bound by its start.
+// own ahead of them, for those layers alone; bound by its start (44 sequences of 83-109 tokens 2.7 us).
 __global__ __launch_bounds__(256) void clear_new_weights_kernel(ClearWeightsArgs a) {
   const int b = blockIdx.y, g = blockIdx.z;
   const int64_t row = a.rows ? (int64_t)a.rows[b] : b;
@@ -503,7 +503,8 @@ hipError_t launch_prefill_lse(const PrefillArgs& a0, int max_seqlen_q, hipStream
     return hipSuccess;
   }
   // 64 rows a workgroup, two waves on the same ones: halves the chain of key tiles. Two workgroups a CU at once, or two rounds of
-  // them where the chains are long (1 x 3000 tokens: 50 us, in 128 rows 59; 44 x 33-59 over 50 15.3 and 12.4)
+  // them where the chains are long (1 x 3000 tokens: 50 us, in 128 rows 59; 44 x 33-59 over 50 15.3 and 12.4). Counted as the call
+  // says it, sequences shorter than max_seqlen_q at their full length.
   const bool fits64 = 64 % a.group == 0;
   const int64_t tiles64 = fits64 ? ((int64_t)max_seqlen_q + 64 / a.group - 1) / (64 / a.group) : 0;
   const int64_t grid64 = tiles64 * a.batch * a.num_kv_heads;
@@ -522,7 +523,7 @@ hipError_t launch_clear_new_weights(const ClearWeightsArgs& a, hipStream_t strea
 int key_weights_part_rows(int64_t num_tokens, int max_seqlen_q, int max_seqlen_k, int group, int num_kv_heads) {
   // About three items for each workgroup slot (two a CU), of 256 to 4096 rows, and 16 parts at most; one part of up to 640
   // rows, where a second launch costs what it saves. us (with whole key blocks), in parts of 512 rows and eight at most,
-  // against this: prompts of 64 tokens 11.0 (in parts of 256 9.0 + 2.6 and a launch's gap), 100 11.5 + 3.9 and 9.5 + 3.3,
+  // against this (max_seqlen_k counts a mixed step's decode rows too): prompts of 64 tokens 11.0 (in parts of 256 9.0 + 2.6 and a launch's gap), 100 11.5 + 3.9 and 9.5 + 3.3,
   // 237 12.2 + 3.8 and 9.7 + 3.9, 1000 18.6 + 4.2 and 12.9 + 4.0.
   const int64_t blocks = ((int64_t)max_seqlen_k + kKwKeys - 1) / kKwKeys;
   const int64_t longest = (int64_t)max_seqlen_q * group, least = (longest + 15) / 16;

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(NT) void select_kernel(EvictArgs p) {
 
 // The rows of one (plane, sequence, kv head) moved: units of V, `pieces` a row, from byte `at` of a block on, a slot's
 // `slot_run` bytes apart, from place `first` on; idle: a slot of the sequence's. LINEAR: the cache's slots are evenly spaced (no
-// scales behind a block's slots).
+// scales behind a block's slots); else a place takes a division (30 x 700-1500 tokens of a 4-bit cache: 4.0 TB/s).
 template <typename V, bool LINEAR>
 __device__ __forceinline__ void move_rows(const EvictArgs& p, const int2* moves, uint8_t* plane, int64_t block_bytes, int64_t at,
                                           int64_t slot_run, int pieces, int idle, int first) {
