@@ -85,9 +85,7 @@ def _check_riding_store(context, block_size: int, decode: bool) -> None:
 
 
 def _check_weight_rows(weight_rows: torch.Tensor) -> None:
-    """With VOX_CHECK_STORE=1: raise ValueError where two sequences of the step share a row of key weights."""
-    if os.environ.get("VOX_CHECK_STORE") != "1":
-        return
+    """Raises ValueError where two sequences of the step share a row of key weights."""
     from .checks import weight_row_violations
 
     v = weight_row_violations(weight_rows)
@@ -202,11 +200,14 @@ class Attention(nn.Module):
     def _forward_weights(self, context, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
         """A step that adds to key_weights."""
         k_cache, v_cache, tables = self.k_cache, self.v_cache, context.block_tables
-        _check_weight_rows(context.weight_rows)
+        check = os.environ.get("VOX_CHECK_STORE") == "1"
+        if check:
+            _check_weight_rows(context.weight_rows)
         if not context.is_prefill:
             rows = dict(key=k, value=v, slot_mapping=context.slot_mapping)
             if context.slot_mapping is not None and k.dim() == 3 and k.shape[0] == q.shape[0]:
-                _check_riding_store(context, k_cache.shape[1], decode=True)
+                if check:
+                    _check_riding_store(context, k_cache.shape[1], decode=True)
             else:  # (more rows than queries: each goes to its slot, then the queries attend)
                 store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
                 rows = {}
